@@ -29,6 +29,7 @@ ERROR_NAMES = {
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 8, 12, 14
 MOE_NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024  # FM_MOE_NOALLOC_SCRATCH_BYTES
 X_F32, X_BF16 = 0, 1
+X_F16, X_E4M3 = 2, 3  # the attention side only
 ORDER_ANY, ORDER_SCALAR, ORDER_AVX2 = 0, 1, 2
 
 # {block_size, block_bytes} (src/gguf.cpp:58-106 of the reference)
@@ -156,6 +157,114 @@ class RecordLoadStats(C.Structure):
                 ("elapsed_ms", C.c_double)]
 
 
+class RmsNormArgs(C.Structure):
+    """fmcuda_rms_norm_args (include/freemoe_b200.h)."""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("y", C.c_void_p),
+        ("residual_out", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("residual_stride", C.c_int64),
+        ("y_stride", C.c_int64),
+        ("x_dtype", C.c_int32),
+        ("residual_dtype", C.c_int32),
+        ("weight_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("tokens", C.c_uint32),
+        ("d_model", C.c_uint32),
+        ("epsilon", C.c_float),
+    ]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP, ROPE_BANDS = range(5)
+
+
+class RopeScaling(C.Structure):
+    """fmcuda_rope_scaling."""
+    _fields_ = [
+        ("kind", C.c_int32),
+        ("factor", C.c_double),
+        ("trained_context", C.c_double),
+        ("fast", C.c_double),
+        ("slow", C.c_double),
+    ]
+
+
+class RopeAppendArgs(C.Structure):
+    """fmcuda_rope_append_args."""
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("q_out_token_stride", C.c_int64),
+        ("q_out_head_stride", C.c_int64),
+        ("cache_page_stride", C.c_int64),
+        ("cache_head_stride", C.c_int64),
+        ("cache_row_stride", C.c_int64),
+        ("in_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("tokens", C.c_uint32),
+        ("heads", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("rot_dim", C.c_uint32),
+        ("interleaved", C.c_int32),
+        ("attention_factor", C.c_float),
+        ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    """fmcuda_paged_attention_args."""
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("q_start", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("cache_page_stride", C.c_int64),
+        ("cache_head_stride", C.c_int64),
+        ("cache_row_stride", C.c_int64),
+        ("page_table_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("seqs", C.c_uint32),
+        ("tokens", C.c_uint32),
+        ("heads", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("max_q_len", C.c_uint32),
+        ("max_kv_len", C.c_uint32),
+        ("causal", C.c_int32),
+        ("window", C.c_uint32),
+        ("scale", C.c_float),
+    ]
+
+
 READER_BUFFERED, READER_DIRECT = 1, 3  # fm::ReaderMode ordinals
 
 MOE_STAGES = ("router", "grouping", "x_planes", "gate_up", "act_planes", "down", "combine")
@@ -242,6 +351,12 @@ SIGNATURES = [
     ("fmcuda_record_load_workspace_bytes", _U64, [_U64]),
     ("fmcuda_record_load", C.c_int, [_P, C.POINTER(Extent), _U32, _P, _U64, C.c_int, _U64, _P, _U64, _P, _U32,
                                      C.POINTER(RecordLoadStats)]),
+    ("fmcuda_add_rms_norm", C.c_int, [C.POINTER(RmsNormArgs), _P]),
+    ("fmcuda_rope_frequencies", C.c_int, [_U32, _D, C.POINTER(RopeScaling), C.POINTER(C.c_float),
+                                          C.POINTER(C.c_float)]),
+    ("fmcuda_rope_append", C.c_int, [C.POINTER(RopeAppendArgs), _P]),
+    ("fmcuda_paged_attention_workspace_bytes", C.c_int, [C.POINTER(PagedAttentionArgs), C.POINTER(C.c_uint64)]),
+    ("fmcuda_paged_attention", C.c_int, [C.POINTER(PagedAttentionArgs), _P, _U64, _P]),
     ("fmcuda_synth_weights", C.c_int, [_U32, _P, _U64, _U32, _U64, _F, _P]),
 ]
 

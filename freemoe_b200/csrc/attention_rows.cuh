@@ -1,0 +1,467 @@
+// attention_rows.cuh -- attention of few rows (decoding, short chunks) over a
+// paged cache: one read of the keys and values, limited by HBM.
+//
+// The rows of a key head -- tokens x the query heads that share it -- make
+// 16-row tiles, the M of mma.sync.m16n8k16; a step is 16 keys: S = Q K^T (keys
+// are the N), the running maximum and sum of the softmax, O += P V (keys are
+// the K, P's accumulator fragments are its A fragments).  The contraction is
+// far below what mma.sync does; the point is the stream of keys, so each warp
+// has its own ring of 16-byte asynchronous copies in shared memory and waits
+// for no other warp.
+//
+// Work split: all (sequence, key head, row tile) units laid end to end, in
+// steps of 16 keys, are cut into equal ranges, one a warp; whatever the lengths,
+// every warp reads the same number of bytes.  A unit inside one range is written
+// out at once; the fragments of a cut unit leave (O, max, sum) in f32 and
+// attn_combine_kernel joins them, in order, so that the result does not depend
+// on timing.  A warp has at most two fragments: of the unit that began before
+// its range, and of the unit that goes on after it.
+#pragma once
+
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace fmb {
+
+constexpr uint32_t AR_WARPS = 8, AR_THREADS = AR_WARPS * 32;
+constexpr uint32_t AR_ROWS = 16, AR_KEYS = 16;
+
+template <int DP> struct ARows {
+    static constexpr uint32_t ROW_BYTES = DP * 2;
+    static constexpr uint32_t HALF = AR_KEYS * ROW_BYTES; // K or V of a step
+    static constexpr uint32_t STAGE = 2 * HALF;
+    static constexpr uint32_t STAGES = 24576 / STAGE; // 24 KB a warp
+    static constexpr uint32_t SMEM = AR_WARPS * STAGES * STAGE;
+};
+
+// Row tiles and steps a unit of sequence s in the rows kernel (no tiles: not its work).
+struct ARShape {
+    uint32_t tiles, step0, steps;
+};
+__device__ __forceinline__ ARShape ar_shape(const AttnParams &p, const AttnSeq &s) {
+    ARShape r;
+    const uint64_t rows = static_cast<uint64_t>(s.ql) * p.group;
+    r.tiles = rows <= p.row_limit ? static_cast<uint32_t>((rows + AR_ROWS - 1) / AR_ROWS) : 0;
+    r.step0 = s.lo / AR_KEYS;
+    const uint32_t last = (s.kl + AR_KEYS - 1) / AR_KEYS;
+    r.steps = last > r.step0 ? last - r.step0 : 1; // a unit without keys still writes its zeros
+    return r;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, "
+                     "%9}, {%0, %1, %2, %3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, "
+                     "%9}, {%0, %1, %2, %3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A place in the laid-out work.
+struct ARCursor {
+    uint32_t b, tile, step; // tile: key head * row tiles + row tile
+    AttnSeq s;
+    ARShape sh;
+};
+
+__device__ __forceinline__ void ar_enter(const AttnParams &p, ARCursor &c) {
+    // the next sequence that has tiles; the caller stops at the range's end before there is none
+    while (c.b < p.seqs) {
+        c.s = attn_seq(p, c.b, false);
+        c.sh = ar_shape(p, c.s);
+        if (c.sh.tiles) return;
+        ++c.b;
+    }
+}
+
+__device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
+    if (++c.step < c.sh.steps) return;
+    c.step = 0;
+    if (++c.tile < c.sh.tiles * p.kv_heads) return;
+    c.tile = 0;
+    ++c.b;
+    ar_enter(p, c);
+}
+
+// Element offset in the caches of the key of lane & 15, or -1 (not to be read).
+__device__ __forceinline__ int64_t ar_key_offset(const AttnParams &p, const ARCursor &c, uint32_t lane) {
+    const uint32_t key = (c.sh.step0 + c.step) * AR_KEYS + (lane & 15u);
+    if (key < c.s.lo || key >= c.s.kl) return -1;
+    const uint32_t page = key / p.page_size;
+    const int32_t id = __ldg(p.table + c.b * p.tb + page);
+    if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
+        raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
+        return -1;
+    }
+    return id * p.cp + static_cast<int64_t>(key - page * p.page_size) * p.cr + (c.tile / c.sh.tiles) * p.ch;
+}
+
+// Queues the copies of a step's 16 keys and values; what is not to be read becomes zeros.
+template <int DP>
+__device__ __forceinline__ void ar_fetch(const AttnParams &p, uint32_t stage, int64_t offset, uint32_t lane) {
+    constexpr uint32_t CH = DP / 8, PER = 32 / CH; // 16-byte pieces a row, rows a round
+    const uint32_t piece = lane % CH;
+#pragma unroll
+    for (uint32_t i = 0; i < AR_KEYS / PER; ++i) {
+        const uint32_t row = i * PER + lane / CH;
+        const int64_t at = __shfl_sync(0xFFFFFFFFu, offset, row);
+        const bool live = at >= 0 && piece * 8 < p.dim;
+        const int64_t from = live ? at + piece * 8 : 0;
+        const uint32_t dst = stage + row * ARows<DP>::ROW_BYTES + ((piece ^ (row & 7u)) << 4);
+        const uint32_t n = live ? 16u : 0u;
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst),
+                     "l"(static_cast<const uint16_t *>(p.kc) + from), "r"(n)
+                     : "memory");
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst + ARows<DP>::HALF),
+                     "l"(static_cast<const uint16_t *>(p.vc) + from), "r"(n)
+                     : "memory");
+    }
+}
+
+// Exclusive sum over the CTA of one 64-bit value a thread; *total: of all.
+__device__ __forceinline__ uint64_t ar_block_scan(uint64_t v, uint64_t *s_part, uint64_t *total) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    uint64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += t;
+    }
+    __syncthreads();
+    if (lane == 31) s_part[warp] = inc;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < AR_WARPS; ++w) {
+        if (w < warp) before += s_part[w];
+        all += s_part[w];
+    }
+    *total = all;
+    return before + inc - v;
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnParams p) {
+    using L = ARows<DP>;
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    __shared__ uint64_t s_part[AR_WARPS], s_first[AR_WARPS];
+    __shared__ uint32_t s_seq[AR_WARPS];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+
+    // ---- this warp's range, and the sequence that it begins in -------------------
+    uint64_t total = 0, mine = 0, before = 0;
+    const bool few = p.seqs <= AR_THREADS;
+    for (uint32_t b0 = 0; b0 < p.seqs; b0 += AR_THREADS) {
+        const uint32_t b = b0 + threadIdx.x;
+        mine = 0;
+        if (b < p.seqs) {
+            const AttnSeq s = attn_seq(p, b, blockIdx.x == 0);
+            const ARShape sh = ar_shape(p, s);
+            mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
+        }
+        uint64_t sum;
+        before = ar_block_scan(mine, s_part, &sum);
+        if (blockIdx.x == 0 && b < p.seqs) p.prefix[b] = total + before;
+        total += sum;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.seqs] = total;
+    const uint64_t even = (total + p.workers - 1) / p.workers;
+    const uint64_t per = even > p.least ? even : p.least;
+    uint64_t running = 0;
+    for (uint32_t b0 = 0; b0 < p.seqs; b0 += AR_THREADS) {
+        const uint32_t b = b0 + threadIdx.x;
+        if (!few) {
+            mine = 0;
+            if (b < p.seqs) {
+                const AttnSeq s = attn_seq(p, b, false);
+                const ARShape sh = ar_shape(p, s);
+                mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
+            }
+            uint64_t sum;
+            before = running + ar_block_scan(mine, s_part, &sum);
+            running += sum;
+        }
+        if (mine) {
+#pragma unroll
+            for (uint32_t w = 0; w < AR_WARPS; ++w) {
+                const uint64_t at = (static_cast<uint64_t>(w) * gridDim.x + blockIdx.x) * per;
+                if (at >= before && at < before + mine) {
+                    s_seq[w] = b;
+                    s_first[w] = before;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
+    const uint64_t begin = worker * per;
+    if (begin >= total) return;
+    const uint32_t count = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
+
+    ARCursor c;
+    c.b = s_seq[warp];
+    c.s = attn_seq(p, c.b, false);
+    c.sh = ar_shape(p, c.s);
+    const uint64_t inside = begin - s_first[warp];
+    c.tile = static_cast<uint32_t>(inside / c.sh.steps);
+    c.step = static_cast<uint32_t>(inside - static_cast<uint64_t>(c.tile) * c.sh.steps);
+
+    // ---- the stream of keys -------------------------------------------------------
+    const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
+    ARCursor f = c;
+    uint32_t fetched = 0;
+    int64_t next = ar_key_offset(p, f, lane); // one step ahead of the copies: hides the table's latency
+    auto fetch = [&] {
+        if (fetched < count) {
+            ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
+            if (++fetched < count) {
+                ar_advance(p, f);
+                next = ar_key_offset(p, f, lane);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
+
+    uint32_t qf[DP / 16][4];
+    float o[DP / 8][4];
+    float m[2], l[2];           // of rows lane / 4 and lane / 4 + 8; m in log2
+    uint32_t key_lo[2], key_hi[2];
+    bool fresh = true;
+    uint32_t first_step = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (fresh) {
+            fresh = false;
+            first_step = c.step;
+            const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
+            const uint16_t *rows[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t row = rt * AR_ROWS + lane / 4 + r * 8;
+                const uint32_t t = row / p.group, g = row - t * p.group;
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
+                key_lo[r] = key_hi[r] = 0;
+                rows[r] = nullptr;
+                if (t < c.s.ql) {
+                    const int64_t pos = static_cast<int64_t>(c.s.kl) - c.s.ql + t;
+                    const int64_t hi = p.causal ? pos + 1 : c.s.kl;
+                    const int64_t lo = p.window ? pos - p.window + 1 : 0;
+                    key_hi[r] = hi > 0 ? static_cast<uint32_t>(hi) : 0;
+                    key_lo[r] = lo > 0 ? static_cast<uint32_t>(lo) : 0;
+                    rows[r] = static_cast<const uint16_t *>(p.q) + (c.s.q0 + t) * p.qt +
+                              static_cast<int64_t>(head * p.group + g) * p.qh;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t col = k * 16 + (x >> 1) * 8 + (lane & 3u) * 2;
+                    const uint16_t *row = rows[x & 1];
+                    qf[k][x] = row && col < p.dim ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
+                }
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[n][x] = 0.0f;
+        }
+        cp_async_wait<L::STAGES - 2>();
+        __syncwarp();
+        const uint32_t st = ring + (i % L::STAGES) * L::STAGE;
+        // S = Q K^T: two 8-key tiles
+        float sc[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t b[4];
+            const uint32_t row = ((lane >> 4) << 3) + (lane & 7u), piece = k * 2 + ((lane >> 3) & 1u);
+            ldsm4(st + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+            mma_16816<BF16>(sc[0], qf[k], b[0], b[1]);
+            mma_16816<BF16>(sc[1], qf[k], b[2], b[3]);
+        }
+        const uint32_t key0 = (c.sh.step0 + c.step) * AR_KEYS + (lane & 3u) * 2;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int r = x >> 1;
+                const uint32_t key = key0 + n * 8 + (x & 1);
+                sc[n][x] = key >= key_lo[r] && key < key_hi[r] ? sc[n][x] * p.scale_log2 : -INFINITY;
+                top[r] = fmaxf(top[r], sc[n][x]);
+            }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+        }
+        // the reference exponent moves only when it is over 2^8 too small: the weights
+        // stay in range of f32 sums and of 16-bit products, and O is rarely rescaled
+        if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
+            float f2[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float to = fmaxf(m[r], top[r]);
+                f2[r] = m[r] == -INFINITY ? 0.0f : exp2_approx(m[r] - to);
+                m[r] = to;
+                l[r] *= f2[r];
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[n][x] *= f2[x >> 1];
+        }
+        float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        uint32_t pf[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                sc[n][x] = exp2_approx(sc[n][x] - base[x >> 1]);
+                l[x >> 1] += sc[n][x];
+            }
+            pf[2 * n] = pack_pair<BF16>(sc[n][0], sc[n][1]);
+            pf[2 * n + 1] = pack_pair<BF16>(sc[n][2], sc[n][3]);
+        }
+        // O += P V
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+            uint32_t b[4];
+            const uint32_t row = (((lane >> 3) & 1u) << 3) + (lane & 7u), piece = n * 2 + (lane >> 4);
+            ldsm4_t(st + L::HALF + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+            mma_16816<BF16>(o[2 * n], pf, b[0], b[1]);
+            mma_16816<BF16>(o[2 * n + 1], pf, b[2], b[3]);
+        }
+        __syncwarp(); // every lane has read the stage that the next copies fill
+        fetch();
+
+        if (c.step + 1 == c.sh.steps || i + 1 == count) {
+            fresh = true;
+            const bool whole = first_step == 0 && c.step + 1 == c.sh.steps;
+            const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
+            const uint64_t slot = worker * 2 + (first_step == 0 ? 1 : 0);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float sum = l[r];
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                const uint32_t in = lane / 4 + r * 8, row = rt * AR_ROWS + in;
+                const uint32_t t = row / p.group, g = row - t * p.group;
+                if (t >= c.s.ql) continue;
+                if (whole) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const uint64_t h = head * p.group + g;
+                    uint16_t *dst = static_cast<uint16_t *>(p.out) + (c.s.q0 + t) * p.ot + h * p.oh;
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n) {
+                        const uint32_t col = n * 8 + (lane & 3u) * 2;
+                        if (col < p.dim)
+                            *reinterpret_cast<uint32_t *>(dst + col) =
+                                pack_pair<BF16>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
+                    }
+                    if (p.lse && (lane & 3u) == 0)
+                        p.lse[static_cast<uint64_t>(c.s.q0 + t) * p.heads + h] =
+                            sum == 0.0f ? -INFINITY : m[r] * 0.6931471805599453f + logf(sum);
+                } else {
+                    float *dst = p.part + (slot * AR_ROWS + in) * DP;
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n)
+                        *reinterpret_cast<float2 *>(dst + n * 8 + (lane & 3u) * 2) =
+                            make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                    if ((lane & 3u) == 0) p.part_ml[slot * AR_ROWS + in] = make_float2(m[r], sum);
+                }
+            }
+        }
+        if (i + 1 < count) ar_advance(p, c);
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the fragments of the units that were cut: a CTA a unit and row.  Its
+// warps take every eighth fragment each, a lane four (two) values of the head.
+constexpr uint32_t AC_THREADS = 256;
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AC_THREADS) attn_combine_kernel(const AttnParams p) {
+    constexpr int V = DP / 32;
+    __shared__ float s_o[AC_THREADS / 32][DP];
+    __shared__ float s_m[AC_THREADS / 32], s_l[AC_THREADS / 32];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t b = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
+    const AttnSeq s = attn_seq(p, b, false);
+    const ARShape sh = ar_shape(p, s);
+    if (sh.tiles == 0) return;
+    const uint64_t total = p.prefix[p.seqs];
+    const uint64_t even = (total + p.workers - 1) / p.workers;
+    const uint64_t per = even > p.least ? even : p.least;
+    for (uint32_t row = blockIdx.y; row < s.ql * p.group; row += gridDim.y) {
+        const uint32_t t = row / p.group, g = row % p.group, in = row % AR_ROWS;
+        const uint64_t first = p.prefix[b] + static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * sh.steps;
+        const uint64_t w0 = first / per, w1 = (first + sh.steps - 1) / per;
+        if (w0 == w1) continue; // written by its one warp
+        float acc[V] = {}, m = -INFINITY, l = 0.0f;
+        for (uint64_t w = w0 + warp; w <= w1; w += AC_THREADS / 32) {
+            const uint64_t slot = (w * 2 + (w == w0 ? 1 : 0)) * AR_ROWS + in;
+            const float2 ml = p.part_ml[slot];
+            const float *src = p.part + slot * DP + lane * V;
+            float v[V];
+#pragma unroll
+            for (int x = 0; x < V; ++x) v[x] = src[x];
+            if (ml.x == -INFINITY) continue;
+            const float to = fmaxf(m, ml.x);
+            const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to), fb = exp2_approx(ml.x - to);
+            m = to;
+            l = l * fa + ml.y * fb;
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[x] = acc[x] * fa + v[x] * fb;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < V; ++x) s_o[warp][lane * V + x] = acc[x];
+        if (lane == 0) {
+            s_m[warp] = m;
+            s_l[warp] = l;
+        }
+        __syncthreads();
+        const uint32_t col = threadIdx.x * 2;
+        if (col >= p.dim) continue;
+        float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < AC_THREADS / 32; ++w) top = fmaxf(top, s_m[w]);
+#pragma unroll
+        for (uint32_t w = 0; w < AC_THREADS / 32; ++w) {
+            const float f = s_m[w] == -INFINITY ? 0.0f : exp2_approx(s_m[w] - top);
+            sum += s_l[w] * f;
+            a0 += s_o[w][col] * f;
+            a1 += s_o[w][col + 1] * f;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint64_t h = head * p.group + g;
+        uint16_t *dst = static_cast<uint16_t *>(p.out) + (s.q0 + t) * p.ot + h * p.oh;
+        *reinterpret_cast<uint32_t *>(dst + col) = pack_pair<BF16>(a0 * inv, a1 * inv);
+        if (p.lse && col == 0)
+            p.lse[static_cast<uint64_t>(s.q0 + t) * p.heads + h] =
+                sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
+    }
+}
+
+} // namespace fmb

@@ -32,6 +32,9 @@ inline int check_launch(const char *what) {
     return FM_STATUS_OK;
 }
 
+// Streaming multiprocessors of the current device (148 where the query fails).
+int device_sm_count();
+
 // Geometry of the GGUF block types on the path (src/gguf.cpp:58-106).
 inline bool block_geometry(uint32_t type_id, uint32_t *bs, uint32_t *bb) {
     switch (type_id) {

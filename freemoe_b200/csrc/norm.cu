@@ -1,0 +1,269 @@
+// norm.cu -- root-mean-square norm of rows with the residual's addition, to
+// f32 / bf16 / f16 or to e4m3 codes with one scale for each 128 values.
+//
+//   h = x + residual,  y = h * w / sqrt(mean(h^2) + eps)
+//
+// (the RMSNorm of Engine::forward_token, src/engine.cpp, whose sum is a double
+// over one token; here f32 partial sums of at most 32 values a thread joined
+// pairwise).  The operator is one read of x and residual and one write of y and
+// h; the weight stays in registers over the rows of a CTA.
+#include <string>
+
+#include "vec8.cuh"
+
+namespace fmb {
+
+namespace {
+
+struct NormParams {
+    const void *x, *res, *w;
+    void *y, *res_out;
+    float *scales;
+    int64_t xs, rs, ys;
+    int32_t xt, rt, wt, yt;
+    uint32_t tokens, d;
+    float eps;
+};
+
+template <int NT> __device__ __forceinline__ float team_sum(float v, float *s_part) {
+    v = warp_sum(v);
+    if constexpr (NT > 32) {
+        const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+        if (lane == 0) s_part[warp] = v;
+        __syncthreads();
+        v = lane < NT / 32 ? s_part[lane] : 0.0f;
+        v = warp_sum(v);
+    }
+    return v;
+}
+
+// A team of NT threads (a warp, or the CTA) takes a row; thread c of the team
+// holds chunks c, c + NT, ... of 8 values.  VEC: a chunk is 8 consecutive
+// values (16-byte accesses).  Otherwise the chunks of a group of 128 values are
+// dealt out value by value over 16 lanes, so that the accesses of the lanes
+// still lie side by side.  Either way 16 neighbouring lanes hold a scale's group.
+template <bool VEC> __device__ __forceinline__ uint32_t value_at(uint32_t c, int j) {
+    return VEC ? c * 8 + j : (c >> 4) * 128 + j * 16 + (c & 15u);
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_chunk(const void *p, int32_t t, int64_t row, uint32_t c, uint32_t d,
+                                           float (&v)[8]) {
+    if constexpr (VEC) {
+        if (c * 8 < d) {
+            raw8_unpack(raw8_load(p, t, row + c * 8), t, v);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t e = value_at<VEC>(c, j);
+            v[j] = e < d ? load1(p, t, row + e) : 0.0f;
+        }
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_chunk(void *p, int32_t t, int64_t row, uint32_t c, uint32_t d,
+                                            const float (&v)[8]) {
+    if constexpr (VEC) {
+        if (c * 8 < d) store8(p, t, row + c * 8, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t e = value_at<VEC>(c, j);
+            if (e < d) store1(p, t, row + e, v[j]);
+        }
+    }
+}
+
+// The 16 lanes of a group call this together; lanes past the row's end hold zeros.
+template <bool VEC>
+__device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, uint32_t c, const float (&v)[8]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float scale = fmaxf(top, 1e-10f) / 448.0f;
+    const float inv = 1.0f / scale;
+    uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
+    const uint32_t groups = (p.d + 127) / 128;
+    if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;
+    if constexpr (VEC) {
+        if (c * 8 < p.d) {
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[i] = e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) | e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16;
+            *reinterpret_cast<uint2 *>(y + c * 8) = make_uint2(w[0], w[1]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t e = value_at<VEC>(c, j);
+            if (e < p.d) y[e] = static_cast<uint8_t>(e4m3x2(v[j] * inv, 0.0f));
+        }
+    }
+}
+
+// ITER chunks a thread, held in registers from the read to the write.
+template <bool VEC, int NT, int ITER>
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const NormParams p) {
+    constexpr uint32_t TEAMS = NT < 128 ? 128 / NT : 1;
+    __shared__ float s_part[2][32];
+    const uint32_t c0 = NT < 128 ? threadIdx.x % NT : threadIdx.x;
+    const uint32_t team = blockIdx.x * TEAMS + (NT < 128 ? threadIdx.x / NT : 0);
+    float w[ITER][8];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) load_chunk<VEC>(p.w, p.wt, 0, c0 + i * NT, p.d, w[i]);
+    uint32_t turn = 0;
+    for (uint64_t row = team; row < p.tokens; row += static_cast<uint64_t>(gridDim.x) * TEAMS, turn ^= 1u) {
+        float h[ITER][8];
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) load_chunk<VEC>(p.x, p.xt, row * p.xs, c0 + i * NT, p.d, h[i]);
+        if (p.res) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                float r[8];
+                load_chunk<VEC>(p.res, p.rt, row * p.rs, c0 + i * NT, p.d, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] += r[j];
+            }
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+        // two buffers of partial sums: a thread that is ahead by a row writes the other one
+        sum = team_sum<NT>(sum, s_part[turn]);
+        const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+        if (p.res_out) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) store_chunk<VEC>(p.res_out, p.rt, row * p.rs, c0 + i * NT, p.d, h[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * root * w[i][j];
+            if (p.yt == FM_X_E4M3)
+                store_e4m3<VEC>(p, row, c0 + i * NT, h[i]);
+            else
+                store_chunk<VEC>(p.y, p.yt, row * p.ys, c0 + i * NT, p.d, h[i]);
+        }
+    }
+}
+
+// Rows longer than the registers of a CTA hold: read twice, the second time from L2.
+template <bool VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(const NormParams p) {
+    __shared__ float s_part[2][32];
+    const uint32_t chunks = ((p.d + 127) / 128) * 16;
+    uint32_t turn = 0;
+    for (uint64_t row = blockIdx.x; row < p.tokens; row += gridDim.x, turn ^= 1u) {
+        float sum = 0.0f;
+        for (uint32_t c = threadIdx.x; c < chunks; c += 1024) {
+            float h[8], r[8];
+            load_chunk<VEC>(p.x, p.xt, row * p.xs, c, p.d, h);
+            if (p.res) {
+                load_chunk<VEC>(p.res, p.rt, row * p.rs, c, p.d, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] += r[j];
+            }
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) part = fmaf(h[j], h[j], part);
+            sum += part;
+        }
+        sum = team_sum<1024>(sum, s_part[turn]);
+        const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+        // whole warps go round together: a scale's 16 lanes exchange inside
+        for (uint32_t c0 = threadIdx.x & ~31u; c0 < chunks; c0 += 1024) {
+            const uint32_t c = c0 + (threadIdx.x & 31u);
+            float h[8], r[8], w[8];
+            load_chunk<VEC>(p.x, p.xt, row * p.xs, c, p.d, h);
+            load_chunk<VEC>(p.w, p.wt, 0, c, p.d, w);
+            if (p.res) {
+                load_chunk<VEC>(p.res, p.rt, row * p.rs, c, p.d, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] += r[j];
+            }
+            if (p.res_out) store_chunk<VEC>(p.res_out, p.rt, row * p.rs, c, p.d, h);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = h[j] * root * w[j];
+            if (p.yt == FM_X_E4M3)
+                store_e4m3<VEC>(p, row, c, h);
+            else
+                store_chunk<VEC>(p.y, p.yt, row * p.ys, c, p.d, h);
+        }
+    }
+}
+
+template <bool VEC, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
+    constexpr uint32_t threads = NT < 128 ? 128 : NT, teams = threads / NT;
+    const uint32_t want = (p.tokens + teams - 1) / teams;
+    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * (2048 / threads);
+    add_rms_norm_kernel<VEC, NT, ITER><<<want < most ? want : most, threads, 0, s>>>(p);
+}
+
+template <bool VEC> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+    if (p.d <= 256)
+        launch_norm<VEC, 32, 1>(p, s);
+    else if (p.d <= 1024)
+        launch_norm<VEC, 32, 4>(p, s);
+    else if (p.d <= 2048)
+        launch_norm<VEC, 128, 2>(p, s);
+    else if (p.d <= 4096)
+        launch_norm<VEC, 256, 2>(p, s);
+    else if (p.d <= 8192)
+        launch_norm<VEC, 512, 2>(p, s);
+    else if (p.d <= 16384)
+        launch_norm<VEC, 1024, 2>(p, s);
+    else {
+        const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
+        add_rms_norm_long_kernel<VEC><<<p.tokens < most ? p.tokens : most, 1024, 0, s>>>(p);
+    }
+}
+
+} // namespace
+} // namespace fmb
+
+using namespace fmb;
+
+extern "C" int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *a, void *stream) {
+    if (!a) return set_error(FM_STATUS_INVALID_ARGUMENT, "null norm arguments");
+    if (a->d_model == 0 || a->d_model > (1u << 24))
+        return set_error(FM_STATUS_SHAPE_MISMATCH, "norm width must be 1 to 2^24");
+    if (!is_float_x(a->x_dtype) || !is_float_x(a->weight_dtype) ||
+        ((a->residual || a->residual_out) && !is_float_x(a->residual_dtype)))
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "norm inputs must be float32, bfloat16 or float16");
+    if (!is_float_x(a->y_dtype) && a->y_dtype != FM_X_E4M3)
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "norm output must be float32, bfloat16, float16 or e4m3");
+    if (!(a->epsilon >= 0.0f)) return set_error(FM_STATUS_INVALID_ARGUMENT, "norm epsilon must not be negative");
+    if (a->tokens == 0) return FM_STATUS_OK;
+    if (!a->x || !a->weight || !a->y) return set_error(FM_STATUS_INVALID_ARGUMENT, "null norm buffer");
+    if (a->y_dtype == FM_X_E4M3 && !a->scales)
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "an e4m3 output needs scales");
+    if (!aligned_to_value(a->x, a->x_dtype) || !aligned_to_value(a->residual, a->residual_dtype) ||
+        !aligned_to_value(a->residual_out, a->residual_dtype) || !aligned_to_value(a->weight, a->weight_dtype) ||
+        !aligned_to_value(a->y, a->y_dtype) || !aligned_to_value(a->scales, FM_X_F32))
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "norm buffer is not aligned to its values");
+    const int64_t d = a->d_model;
+    if (a->tokens > 1 && (a->x_stride < d || a->y_stride < d ||
+                          ((a->residual || a->residual_out) && a->residual_stride < d)))
+        return set_error(FM_STATUS_SHAPE_MISMATCH, "norm row stride is smaller than the row");
+    const NormParams p{a->x,        a->residual,        a->weight,   a->y,       a->residual_out,  a->scales,
+                       a->x_stride, a->residual_stride, a->y_stride, a->x_dtype, a->residual_dtype, a->weight_dtype,
+                       a->y_dtype,  a->tokens,          a->d_model,  a->epsilon};
+    const bool vec = d % 8 == 0 && a->x_stride % 8 == 0 && a->y_stride % 8 == 0 && a->residual_stride % 8 == 0 &&
+                     aligned16(a->x) && aligned16(a->residual) && aligned16(a->weight) && aligned16(a->y) &&
+                     aligned16(a->residual_out);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (vec)
+        dispatch_norm<true>(p, s);
+    else
+        dispatch_norm<false>(p, s);
+    return check_launch("add_rms_norm_kernel");
+}

@@ -28,6 +28,16 @@ int *device_status_word() {
     return addr[dev];
 }
 
+int device_sm_count() {
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!n[dev] &&
+        (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] <= 0))
+        n[dev] = 148;
+    return n[dev];
+}
+
 namespace {
 thread_local std::string g_last_error;
 }

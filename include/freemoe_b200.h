@@ -49,6 +49,8 @@ enum { FM_TYPE_F32 = 0, FM_TYPE_Q8_0 = 8, FM_TYPE_Q4_K = 12, FM_TYPE_Q6_K = 14 }
 
 /* ---- activation dtypes ---- */
 enum { FM_X_F32 = 0, FM_X_BF16 = 1 };
+/* taken by the attention side of the layer only (fmcuda_add_rms_norm and after) */
+enum { FM_X_F16 = 2, FM_X_E4M3 = 3 };
 
 /* ---- summation order of the F32 matvec (fmcuda_matvec_f32) ---- */
 enum {
@@ -586,6 +588,143 @@ int fmcuda_record_load(fmcuda_record_loader *loader, const fmcuda_extent *extent
                        void *slot, uint64_t slot_bytes, int checksum_known, uint64_t expected_checksum,
                        void *workspace, uint64_t workspace_bytes, void *stream, uint32_t timeout_ms,
                        fmcuda_record_load_stats *stats);
+
+/* ==================== the attention side of a decoder layer ==================== *
+ * What stands between two MoE blocks of a decoder layer, on device memory: the
+ * norm with the residual's addition, rotary positions with the write of the new
+ * keys and values into a paged cache, and attention over that cache.  In the
+ * reference these are the scalar loops of Engine::forward_token (src/engine.cpp)
+ * and src/rope.cpp, one token and one sequence at a time over a private cache;
+ * here a call takes all tokens of a batch of sequences.
+ *
+ * Element strides are counted in elements; the innermost dimension (a row of
+ * d_model values, a head of head_dim values) is contiguous. */
+
+/* y = h * w / sqrt(mean(h^2) + epsilon) row by row, h = x + residual.
+ * Sums are held in f32 and each result is rounded once to its type; the norm
+ * reads h before any rounding.  y_dtype FM_X_E4M3 writes 8-bit codes and one f32
+ * scale for each 128 consecutive values of a row (the last group may be shorter):
+ *   scale = max(largest |y| of the group, 1e-10) / 448,  y ~ code * scale;
+ * a NaN is coded as NaN and does not count for the largest.
+ * y may be x and residual_out may be residual where type and stride are the same. */
+typedef struct fmcuda_rms_norm_args {
+    const void *x;              /* [tokens][d_model] */
+    const void *residual;       /* optional [tokens][d_model]; NULL: h = x */
+    const void *weight;         /* [d_model] */
+    void *y;                    /* [tokens][d_model] */
+    void *residual_out;         /* optional: h, in residual_dtype */
+    float *scales;              /* [tokens][ceil(d_model / 128)] with FM_X_E4M3, else unused */
+    int64_t x_stride;           /* from row to row, at least d_model */
+    int64_t residual_stride;    /* of residual and of residual_out */
+    int64_t y_stride;
+    int32_t x_dtype;            /* FM_X_F32, FM_X_BF16, FM_X_F16 */
+    int32_t residual_dtype;     /* the same three */
+    int32_t weight_dtype;       /* the same three */
+    int32_t y_dtype;            /* the same three, or FM_X_E4M3 */
+    uint32_t tokens;
+    uint32_t d_model;           /* 1 .. 2^24 */
+    float epsilon;              /* >= 0 */
+} fmcuda_rms_norm_args;
+int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *args, void *stream);
+
+/* Rotary frequencies f_i = base^(-2i / rot_dim), i < rot_dim / 2, and their
+ * scalings for contexts longer than the trained one (host arithmetic in double,
+ * rounded once).  *attention_factor is what cos and sin are multiplied by. */
+enum {
+    FM_ROPE_PLAIN = 0,  /* f_i; factor 1 */
+    FM_ROPE_LINEAR = 1, /* f_i / factor (positions interpolated) */
+    FM_ROPE_BASE = 2,   /* base' = base * factor^(rot_dim / (rot_dim - 2)) */
+    FM_ROPE_RAMP = 3,   /* f_i where a pair turns more than `fast` times in the trained context, f_i / factor
+                           where less than `slow` times, a linear ramp over i between; cos and sin grow by
+                           0.1 ln(factor) + 1 */
+    FM_ROPE_BANDS = 4   /* the same three bands, the ramp linear in the number of turns; factor 1 */
+};
+typedef struct fmcuda_rope_scaling {
+    int32_t kind;              /* FM_ROPE_* */
+    double factor;             /* > 0; context stretched by this much */
+    double trained_context;    /* FM_ROPE_RAMP, FM_ROPE_BANDS */
+    double fast, slow;         /* turns in the trained context, fast > slow > 0 */
+} fmcuda_rope_scaling;
+int fmcuda_rope_frequencies(uint32_t rot_dim, double base, const fmcuda_rope_scaling *scaling, float *inv_freq,
+                            float *attention_factor);
+
+/* Rotates q and k by their positions and writes k and v into the cache's pages.
+ * Pair i of a head, at (i, i + rot_dim/2) or, interleaved, at (2i, 2i + 1), turns
+ * by position * inv_freq[i]; the angle is reduced in 64 bits, cos and sin are
+ * f32; values from rot_dim on are copied.  Token t goes to slot = slots[t]:
+ * page slot / page_size, row slot % page_size; a negative slot writes nothing
+ * (padding), one past the cache sets the device status to INVALID_ARGUMENT.
+ * Two tokens of a call must not share a slot.  k, v and the caches may be NULL
+ * together (rotate q alone); q_out may be q where type and strides are equal. */
+typedef struct fmcuda_rope_append_args {
+    const void *q, *k, *v;      /* [tokens][heads or kv_heads][head_dim], in_dtype */
+    void *q_out;                /* [tokens][heads][head_dim], out_dtype */
+    void *k_cache, *v_cache;    /* [n_pages][..page_size, kv_heads..][head_dim], out_dtype */
+    const int32_t *positions;   /* device [tokens] */
+    const int64_t *slots;       /* device [tokens] */
+    const float *inv_freq;      /* device [rot_dim / 2] */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t q_out_token_stride, q_out_head_stride;
+    int64_t cache_page_stride, cache_head_stride, cache_row_stride; /* of both caches */
+    int32_t in_dtype, out_dtype; /* FM_X_F32, FM_X_BF16, FM_X_F16 */
+    uint32_t tokens, heads, kv_heads, head_dim;
+    uint32_t rot_dim;           /* even, <= head_dim; 0 copies */
+    int32_t interleaved;
+    float attention_factor;
+    uint32_t n_pages, page_size;
+} fmcuda_rope_append_args;
+int fmcuda_rope_append(const fmcuda_rope_append_args *args, void *stream);
+
+/* Attention of new tokens over a paged cache: for row t of sequence b and query
+ * head j, over the keys i that the row sees,
+ *   out[t, j] = sum_i softmax_i(scale * q[t, j] . k_i) v_i ,  k, v of head j / (heads / kv_heads).
+ * Sequence b has the rows q_start[b] .. q_start[b + 1) of q and kv_len[b] keys in
+ * the cache, its new tokens' own keys (fmcuda_rope_append) being the last of
+ * them: key i lies on page page_table[b][i / page_size], row i % page_size.  Its
+ * row r stands at position kv_len - rows + r; causal rows see the keys up to
+ * their position, with a window w only the last w of those; without causal
+ * every row sees all keys.  A row that sees no key gives zeros and lse = -inf.
+ * A row a sequence is decoding, more are a chunk of a prompt; one call takes both.
+ *
+ * Products of f16 or bf16 values with f32 sums, softmax in f32, its weights
+ * rounded to `dtype` for the product with v, the result rounded once.
+ *
+ * Rows of the cache that no row of the call sees (past kv_len, before the
+ * window, other pages) may hold anything, NaN included, and their table entries
+ * are not followed.  A key that some row of the call sees and another does not
+ * must be finite, or the other row may get NaN.
+ *
+ * max_q_len and max_kv_len bound the sequences' rows and keys (they set the
+ * launch; the lengths themselves stay on the device).  A length past its bound,
+ * rows past `tokens`, or a page of a visible key outside [0, n_pages) sets the
+ * device status to INVALID_ARGUMENT; the rows concerned are then undefined and
+ * no memory outside the arguments is touched.
+ *
+ * head_dim: multiple of 8, at most 128; page_size: multiple of 8; heads a
+ * multiple of kv_heads; strides multiples of 8 and pointers 16-byte aligned. */
+typedef struct fmcuda_paged_attention_args {
+    const void *q;                /* [tokens][heads][head_dim] */
+    const void *k_cache, *v_cache; /* [n_pages][..page_size, kv_heads..][head_dim] */
+    void *out;                    /* [tokens][heads][head_dim] */
+    float *lse;                   /* optional [tokens][heads]: log of the sum of exp(scale * q . k) */
+    const int32_t *page_table;    /* device [seqs][page_table_stride] */
+    const int32_t *q_start;       /* device [seqs + 1], ascending, from 0 to tokens */
+    const int32_t *kv_len;        /* device [seqs] */
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int64_t cache_page_stride, cache_head_stride, cache_row_stride; /* of both caches */
+    int64_t page_table_stride;    /* entries a sequence, at least ceil(max_kv_len / page_size) */
+    int32_t dtype;                /* FM_X_BF16 or FM_X_F16: q, caches and out */
+    uint32_t seqs, tokens, heads, kv_heads, head_dim;
+    uint32_t n_pages, page_size;
+    uint32_t max_q_len, max_kv_len;
+    int32_t causal;
+    uint32_t window;              /* 0: none; needs causal */
+    float scale;
+} fmcuda_paged_attention_args;
+int fmcuda_paged_attention_workspace_bytes(const fmcuda_paged_attention_args *args, uint64_t *bytes);
+/* `workspace`: device memory of that many bytes, 256-byte aligned; calls that overlap need one each. */
+int fmcuda_paged_attention(const fmcuda_paged_attention_args *args, void *workspace, uint64_t workspace_bytes,
+                           void *stream);
 
 /* ====================== synthetic weights (bench/test) ====================== */
 
