@@ -719,7 +719,7 @@ typedef struct fmcuda_paged_attention_args {
     uint32_t max_q_len, max_kv_len;
     int32_t causal;
     uint32_t window;              /* 0: none; needs causal */
-    float scale;
+    float scale;                  /* > 0 */
 } fmcuda_paged_attention_args;
 int fmcuda_paged_attention_workspace_bytes(const fmcuda_paged_attention_args *args, uint64_t *bytes);
 /* `workspace`: device memory of that many bytes, 256-byte aligned; calls that overlap need one each. */
