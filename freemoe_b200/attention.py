@@ -10,70 +10,69 @@ head_dim]`` with any strides but the last (token-major pages are its
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 import math
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from ._lib import (ROPE_BANDS, ROPE_BASE, ROPE_LINEAR, ROPE_PLAIN, ROPE_RAMP, X_BF16, X_E4M3, X_F16, X_F32, FmError,
-                   PagedAttentionArgs, RmsNormArgs, RopeAppendArgs, RopeScaling, check, load)
+                   PagedAttentionArgs, RmsNormArgs, RopeAppendArgs, RopeScaling, check, load, packed_entry, packer)
 
 FP8_GROUP = 128
 _DTYPES = {torch.float32: X_F32, torch.bfloat16: X_BF16, torch.float16: X_F16}
+_NO_DTYPE = -1  # refused by the C entry
 _ROPE_KINDS = {"plain": ROPE_PLAIN, "linear": ROPE_LINEAR, "base": ROPE_BASE, "ramp": ROPE_RAMP, "bands": ROPE_BANDS}
 INVALID_ARGUMENT, SHAPE_MISMATCH = 26, 8
 
-
-def _dtype(t: torch.dtype) -> int:
-    code = _DTYPES.get(t)
-    if code is None:
-        raise FmError(INVALID_ARGUMENT, f"{t} is not float32, bfloat16 or float16")
-    return code
-
-
-def _need(ok: bool, message: str, code: int = SHAPE_MISMATCH) -> None:
-    if not ok:
-        raise FmError(code, message)
+# A decoding step makes these calls for every layer with a few microseconds of GPU work
+# each, so the wrappers test what the C entry cannot see in one expression, pack the
+# arguments into bytes, and leave types, strides and alignment to the C entry's checks.
+_pack_norm = packer(RmsNormArgs).pack
+_pack_rope = packer(RopeAppendArgs).pack
+_pack_attention = packer(PagedAttentionArgs).pack
 
 
-def _on_device(*tensors) -> None:
-    """Device memory of the current device, rows contiguous."""
-    device = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != device):
-            raise FmError(INVALID_ARGUMENT, f"tensor on {t.device}: the current device is cuda:{device}")
+@functools.cache
+def _entry(name: str, *argtypes):
+    return packed_entry(name, *argtypes)
 
 
-def _dense(what: str, *tensors) -> None:
-    """The innermost dimension is contiguous."""
-    for t in tensors:
-        if t is not None and t.stride(-1) != 1 and t.shape[-1] != 1:
-            raise FmError(SHAPE_MISMATCH, f"{what} must be contiguous in its last dimension")
+def _refuse(message: str, code: int = SHAPE_MISMATCH):
+    raise FmError(code, message)
 
 
-def _stream(stream):
-    """The stream's handle, and a context in which torch allocates on it."""
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream, contextlib.nullcontext()
-    return stream.cuda_stream, torch.cuda.stream(stream)
+def _check_device(device: int, *tensors) -> None:
+    current = torch.cuda.current_device()
+    for t in (device, *(t.get_device() for t in tensors if t is not None)):
+        if t != current:
+            _refuse(f"a tensor is not on the current device, cuda:{current}", INVALID_ARGUMENT)
 
 
-def _norm(x, weight, residual, epsilon, y, scales, stream):
-    _need(x.dim() == 2 and weight.dim() == 1 and weight.shape[0] == x.shape[1],
-          "norm takes [tokens, d_model] and a weight of d_model")
-    _need(residual is None or residual.shape == x.shape, "residual and x differ in shape")
-    _on_device(x, weight, residual)
-    _dense("norm input", x, weight, residual)
-    h = None
+def _norm(x, weight, residual, epsilon, y, y_dtype, scales):
+    device = x.get_device()
+    _check_device(device, weight, residual)
+    tokens, dim = x.shape
+    if weight.shape != (dim,) or (residual is not None and residual.shape != x.shape):
+        _refuse("norm takes [tokens, d_model], a weight of d_model and a residual like x")
+    xs, ys = x.stride(), y.stride()
+    dense = (xs[1] == 1 or dim == 1) and (weight.stride(0) == 1 or dim == 1)
+    h, rs, r_at, h_at, r_dtype = None, 0, 0, 0, 0
     if residual is not None:
-        h = torch.empty_strided(residual.shape, residual.stride(), dtype=residual.dtype, device=x.device)
-    a = RmsNormArgs(x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), y.data_ptr(),
-                    None if h is None else h.data_ptr(), None if scales is None else scales.data_ptr(),
-                    x.stride(0), 0 if residual is None else residual.stride(0), y.stride(0), _dtype(x.dtype),
-                    0 if residual is None else _dtype(residual.dtype), _dtype(weight.dtype),
-                    X_E4M3 if scales is not None else _dtype(y.dtype), x.shape[0], x.shape[1], epsilon)
-    check(load().fmcuda_add_rms_norm(C.byref(a), stream))
+        # h like the residual in memory too: the C entry takes one stride for both
+        rs = residual.stride()
+        h = torch.empty_strided(residual.shape, rs, dtype=residual.dtype, device=residual.device)
+        dense = dense and (rs[1] == 1 or dim == 1)
+        rs, r_at, h_at, r_dtype = rs[0], residual.data_ptr(), h.data_ptr(), _DTYPES.get(residual.dtype, _NO_DTYPE)
+    if not dense:
+        _refuse("norm inputs must be contiguous in their rows")
+    rc = _entry("fmcuda_add_rms_norm", C.c_void_p)(
+        _pack_norm(x.data_ptr(), r_at, weight.data_ptr(), y.data_ptr(), h_at, 0 if scales is None else scales.data_ptr(),
+                   xs[0], rs, ys[0], _DTYPES.get(x.dtype, _NO_DTYPE), r_dtype, _DTYPES.get(weight.dtype, _NO_DTYPE),
+                   y_dtype, tokens, dim, epsilon), _raw_stream(device))
+    if rc:
+        check(rc)
     return h
 
 
@@ -83,10 +82,13 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tenso
 
     ``x`` is [tokens, d_model]; returns ``(y, h)``, ``h`` in the residual's type
     and None without one."""
-    handle, on_stream = _stream(stream)
-    with on_stream:
-        y = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
-        return y, _norm(x, weight, residual, epsilon, y, None, handle)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return add_rms_norm(x, weight, residual=residual, epsilon=epsilon, out_dtype=out_dtype)
+    if x.dim() != 2:
+        _refuse("norm takes [tokens, d_model]")
+    y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
+    return y, _norm(x, weight, residual, epsilon, y, _DTYPES.get(y.dtype, _NO_DTYPE), None)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
@@ -94,12 +96,14 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.T
     """The norm with an 8-bit output: ``(codes, scales, h)``, codes
     ``float8_e4m3fn`` [tokens, d_model] and one f32 scale for each 128 values
     of a row: ``y ~ codes * scales``."""
-    handle, on_stream = _stream(stream)
-    _need(x.dim() == 2, "norm takes [tokens, d_model]")
-    with on_stream:
-        codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((x.shape[0], -(-x.shape[1] // FP8_GROUP)), dtype=torch.float32, device=x.device)
-        return codes, scales, _norm(x, weight, residual, epsilon, codes, scales, handle)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return add_rms_norm_fp8(x, weight, residual=residual, epsilon=epsilon)
+    if x.dim() != 2:
+        _refuse("norm takes [tokens, d_model]")
+    codes = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scales = x.new_empty((x.shape[0], -(-x.shape[1] // FP8_GROUP)), dtype=torch.float32)
+    return codes, scales, _norm(x, weight, residual, epsilon, codes, X_E4M3, scales)
 
 
 def rope_frequencies(rot_dim: int, base: float = 10000.0, *, kind: str = "plain", factor: float = 1.0,
@@ -109,7 +113,9 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, *, kind: str = "plain"
 
     ``kind``: "plain", "linear", "base", "ramp" or "bands"."""
     if kind not in _ROPE_KINDS:
-        raise FmError(INVALID_ARGUMENT, f"unknown rotary scaling {kind!r}")
+        _refuse(f"unknown rotary scaling {kind!r}", INVALID_ARGUMENT)
+    if rot_dim < 0:
+        _refuse("rotary width must be even, 2 to 1024")
     scaling = RopeScaling(_ROPE_KINDS[kind], factor, trained_context, fast, slow)
     host = (C.c_float * max(1, rot_dim // 2))()
     attention_factor = C.c_float(1.0)
@@ -127,50 +133,53 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
     rotated q in the caches' type (``out_dtype`` without caches).
 
     ``positions`` int32 [tokens]; ``inv_freq`` f32, one per rotated pair."""
-    handle, on_stream = _stream(stream)
-    _need(q.dim() == 3, "q is [tokens, heads, head_dim]")
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved=interleaved,
+                               attention_factor=attention_factor, out_dtype=out_dtype)
+    if q.dim() != 3:
+        _refuse("q is [tokens, heads, head_dim]")
+    device = q.get_device()
+    _check_device(device, k, v, positions, inv_freq, k_cache, v_cache, slots)
     tokens, heads, dim = q.shape
-    _need(positions.shape == (tokens,) and positions.dtype == torch.int32 and positions.is_contiguous(),
-          "positions are int32 [tokens]")
-    _need(inv_freq.dim() == 1 and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(),
-          "inv_freq is float32 [rot_dim / 2]")
-    _on_device(q, k, v, positions, inv_freq, k_cache, v_cache, slots)
-    _dense("q, k, v and caches", q, k, v, k_cache, v_cache)
-    cached = (k, v, k_cache, v_cache, slots)
-    if any(t is not None for t in cached):
-        _need(all(t is not None for t in cached), "k, v, their caches and slots come together", INVALID_ARGUMENT)
-        _need(k.dim() == 3 and k.shape == v.shape and k.shape[0] == tokens and k.shape[2] == dim,
-              "k and v are [tokens, kv_heads, head_dim]")
-        kv_heads = k.shape[1]
-        _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride() and
-              k_cache.shape[1] == kv_heads and k_cache.shape[3] == dim,
-              "caches are [pages, kv_heads, page_size, head_dim], of one layout")
-        _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v have one type", INVALID_ARGUMENT)
-        _need(k_cache.dtype == v_cache.dtype and out_dtype in (None, k_cache.dtype),
-              "the output and the caches have one type", INVALID_ARGUMENT)
-        _need(slots.shape == (tokens,) and slots.dtype == torch.int64 and slots.is_contiguous(),
-              "slots are int64 [tokens]")
-        out_dtype = k_cache.dtype
-        cache = (k_cache.stride(0), k_cache.stride(1), k_cache.stride(2))
-        pages, page_size = k_cache.shape[0], k_cache.shape[2]
-        strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    qs = q.stride()
+    if (positions.shape != (tokens,) or positions.dtype != torch.int32 or not positions.is_contiguous() or
+            inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous()):
+        _refuse("positions are int32 [tokens], inv_freq is float32 [rot_dim / 2]")
+    dense = qs[2] == 1 or dim == 1
+    if k is not None or v is not None or k_cache is not None or v_cache is not None or slots is not None:
+        if k is None or v is None or k_cache is None or v_cache is None or slots is None:
+            _refuse("k, v, their caches and slots come together", INVALID_ARGUMENT)
+        kv_heads = k.shape[1] if k.dim() == 3 else -1
+        if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
+            _refuse("k and v are [tokens, kv_heads, head_dim]")
+        cache, ks, vs, cs = k_cache.shape, k.stride(), v.stride(), k_cache.stride()
+        if (len(cache) != 4 or v_cache.shape != cache or v_cache.stride() != cs or cache[1] != kv_heads or
+                cache[3] != dim):
+            _refuse("caches are [pages, kv_heads, page_size, head_dim], of one layout")
+        if slots.shape != (tokens,) or slots.dtype != torch.int64 or not slots.is_contiguous():
+            _refuse("slots are int64 [tokens]")
+        kind = k_cache.dtype
+        if k.dtype != q.dtype or v.dtype != q.dtype or v_cache.dtype != kind or out_dtype not in (None, kind):
+            _refuse("q, k and v have one type, the output and the caches have one", INVALID_ARGUMENT)
+        dense = dense and (dim == 1 or ks[2] == vs[2] == cs[3] == 1)
+        at = (k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr())
+        strides = (ks[0], ks[1], vs[0], vs[1])
+        pages, page_size, cs = cache[0], cache[2], cs[:3]
     else:
-        kv_heads, pages, page_size, cache, strides = 0, 0, 0, (0, 0, 0), (0, 0, 0, 0)
-    with on_stream:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
-    at = [None if t is None else t.data_ptr() for t in (k, v, k_cache, v_cache, slots)]
-    a = RopeAppendArgs(q.data_ptr(), at[0], at[1], out.data_ptr(), at[2], at[3], positions.data_ptr(), at[4],
-                       inv_freq.data_ptr(), q.stride(0), q.stride(1), *strides, out.stride(0), out.stride(1), *cache,
-                       _dtype(q.dtype), _dtype(out.dtype), tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0],
-                       1 if interleaved else 0, attention_factor, pages, page_size)
-    check(load().fmcuda_rope_append(C.byref(a), handle))
+        kind = q.dtype if out_dtype is None else out_dtype
+        at, strides, kv_heads, pages, page_size, cs = (0,) * 5, (0,) * 4, 0, 0, 0, (0, 0, 0)
+    if not dense:
+        _refuse("q, k, v and caches must be contiguous in their heads")
+    out = torch.empty_like(q, dtype=kind, memory_format=torch.contiguous_format)
+    rc = _entry("fmcuda_rope_append", C.c_void_p)(
+        _pack_rope(q.data_ptr(), at[0], at[1], out.data_ptr(), at[2], at[3], positions.data_ptr(), at[4],
+                   inv_freq.data_ptr(), qs[0], qs[1], *strides, heads * dim, dim, *cs, _DTYPES.get(q.dtype, _NO_DTYPE),
+                   _DTYPES.get(kind, _NO_DTYPE), tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0],
+                   1 if interleaved else 0, attention_factor, pages, page_size), _raw_stream(device))
+    if rc:
+        check(rc)
     return out
-
-
-def paged_attention_workspace_bytes(args: PagedAttentionArgs) -> int:
-    v = C.c_uint64(0)
-    check(load().fmcuda_paged_attention_workspace_bytes(C.byref(args), C.byref(v)))
-    return v.value
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -186,33 +195,52 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_kv_len`` bound the lengths.  ``workspace``: device bytes to use instead
     of allocating (256-byte aligned, not shared with a call that overlaps).
     Returns the output, and with ``return_lse`` the f32 [tokens, heads] log-sum-exp."""
-    handle, on_stream = _stream(stream)
-    _need(q.dim() == 3, "q is [tokens, heads, head_dim]")
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, max_q_len=max_q_len,
+                                   max_kv_len=max_kv_len, scale=scale, causal=causal, window=window,
+                                   return_lse=return_lse, workspace=workspace)
+    if q.dim() != 3 or k_cache.dim() != 4:
+        _refuse("q is [tokens, heads, head_dim], caches are [pages, kv_heads, page_size, head_dim]")
+    device = q.get_device()
+    _check_device(device, k_cache, v_cache, page_table, q_start, kv_len, workspace)
     tokens, heads, dim = q.shape
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride() and
-          k_cache.shape[3] == dim, "caches are [pages, kv_heads, page_size, head_dim], of one layout")
-    _need(q.dtype == k_cache.dtype == v_cache.dtype, "q and the caches have one type", INVALID_ARGUMENT)
-    seqs = kv_len.shape[0]
-    _need(page_table.dim() == 2 and page_table.shape[0] == seqs and q_start.shape == (seqs + 1,) and kv_len.dim() == 1,
-          "page_table is [seqs, pages], q_start [seqs + 1], kv_len [seqs]")
-    _need(page_table.dtype == q_start.dtype == kv_len.dtype == torch.int32 and q_start.is_contiguous() and
-          kv_len.is_contiguous(), "page_table, q_start and kv_len are int32", INVALID_ARGUMENT)
-    _need(page_table.shape[1] * k_cache.shape[2] >= max_kv_len, "page table is shorter than max_kv_len")
-    _need(max_q_len >= 0 and max_kv_len >= 0 and window >= 0, "lengths must not be negative", INVALID_ARGUMENT)
-    _on_device(q, k_cache, v_cache, page_table, q_start, kv_len, workspace)
-    _dense("q, caches and page_table", q, k_cache, v_cache, page_table)
-    with on_stream:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
-        a = PagedAttentionArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-                               None if lse is None else lse.data_ptr(), page_table.data_ptr(), q_start.data_ptr(),
-                               kv_len.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                               k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), page_table.stride(0),
-                               _dtype(q.dtype), seqs, tokens, heads, k_cache.shape[1], dim, k_cache.shape[0],
-                               k_cache.shape[2], min(max_q_len, tokens), max_kv_len, 1 if causal else 0, window,
-                               1.0 / math.sqrt(dim) if scale is None else scale)
-        if workspace is None:
-            workspace = torch.empty(paged_attention_workspace_bytes(a), dtype=torch.uint8, device=q.device)
-        check(load().fmcuda_paged_attention(C.byref(a), workspace.data_ptr(),
-                                            workspace.numel() * workspace.element_size(), handle))
+    pages, kv_heads, page_size, cache_dim = k_cache.shape
+    qs, cs, ts = q.stride(), k_cache.stride(), page_table.stride()
+    if v_cache.shape != k_cache.shape or v_cache.stride() != cs or cache_dim != dim:
+        _refuse("caches are [pages, kv_heads, page_size, head_dim], of one layout")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        _refuse("q and the caches have one type", INVALID_ARGUMENT)
+    seqs = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or q_start.shape != (seqs + 1,):
+        _refuse("page_table is [seqs, pages], q_start [seqs + 1], kv_len [seqs]")
+    if (page_table.dtype != torch.int32 or q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or
+            not q_start.is_contiguous() or not kv_len.is_contiguous()):
+        _refuse("page_table, q_start and kv_len are int32", INVALID_ARGUMENT)
+    if max_q_len < 0 or max_kv_len < 0 or window < 0:
+        _refuse("lengths must not be negative", INVALID_ARGUMENT)
+    if page_table.shape[1] * page_size < max_kv_len:
+        _refuse("page table is shorter than max_kv_len")
+    if qs[2] != 1 or cs[3] != 1 or (ts[1] != 1 and page_table.shape[1] > 1):
+        _refuse("q, caches and page_table must be contiguous in their last dimension")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    args = _pack_attention(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+        page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), qs[0], qs[1], heads * dim, dim, cs[0], cs[1], cs[2],
+        ts[0], _DTYPES.get(q.dtype, _NO_DTYPE), seqs, tokens, heads, kv_heads, dim, pages, page_size,
+        min(max_q_len, tokens), max_kv_len, 1 if causal else 0, window, 1.0 / math.sqrt(dim) if scale is None else scale)
+    if workspace is None:
+        need = C.c_uint64()
+        rc = _entry("fmcuda_paged_attention_workspace_bytes", C.POINTER(C.c_uint64))(args, need)
+        if rc:
+            check(rc)
+        workspace = q.new_empty(need.value, dtype=torch.uint8)
+        size = need.value
+    else:
+        size = workspace.numel() * workspace.element_size()
+    rc = _entry("fmcuda_paged_attention", C.c_void_p, C.c_uint64, C.c_void_p)(args, workspace.data_ptr(), size,
+                                                                            _raw_stream(device))
+    if rc:
+        check(rc)
     return (out, lse) if return_lse else out

@@ -5,17 +5,19 @@
 // into tiles of 128; a CTA holds two such tiles, so that a block of 128 keys
 // and values, once in shared memory, serves 256 rows.  For each block and tile
 //   S = Q K^T        tcgen05.mma, Q and K in shared memory, S in tensor memory
-//   P = exp2(S - m)  one thread a row: read S, running maximum m and sum, P back
-//                    over S as 16-bit values
+//   P = exp2(S - m)  one thread a row: read S, running maximum m and sum, P as
+//                    16-bit values into tensor memory
 //   O += P V         tcgen05.mma, P in tensor memory, V in shared memory
 // Roles: warps 0-3 and 4-7 the softmax of tile 0 and 1 (and its Q, and its
 // result), warp 8 copies keys and values page by page (TMA boxes of as many
-// rows as divide a page), warps 9 and 10 issue the products of tile 0 and 1.
-// While one tile is in its softmax the other has the tensor cores.  S_{j+1} is
-// written over P_j only after the commit of P_j V; so when a softmax warp sees
-// S_{j+1}, O is at rest, and it can rescale O in place -- which it does only
-// when the maximum has grown by more than 2^8, since any reference exponent in
-// that range gives the same P / sum.
+// rows as divide a page), warp 9 issues Q K^T and warp 10 P V.  P has a place of
+// its own, so that the next S is computed while the softmax still works on this
+// block; heads of 128 then leave room for a single S, which the tiles use in
+// turn: a softmax moves it to registers at once, and the turns keep the tiles
+// half a block apart, one in its softmax while the other has the tensor cores
+// (left to themselves they fall into step).  A softmax thread rescales O in
+// place, and only when the maximum has grown by more than 2^8, since any
+// reference exponent in that range gives the same P / sum.
 //
 // A tile's keys end at its last row's position; only blocks that some row sees
 // in part are masked.  In the first and last block V's rows outside the
@@ -39,6 +41,12 @@ template <int DP> struct APrompt {
     static constexpr uint32_t HALF = AP_KEYS * 128;        // 128 rows of 64 values
     static constexpr uint32_t BLOCK = HALVES * HALF;       // a Q tile, a K block, a V block
     static constexpr uint32_t STAGES = DP == 128 ? 5 : 8;
+    // Tensor memory, 512 columns: P (64) and O (DP) of each tile, and S (128): one of each
+    // tile where there is room, else one that the tiles use in turn.
+    static constexpr bool ONE_S = DP == 128;
+    __host__ __device__ static constexpr uint32_t o_col(uint32_t t) { return t * DP; }
+    __host__ __device__ static constexpr uint32_t p_col(uint32_t t) { return 2 * DP + t * 64; }
+    __host__ __device__ static constexpr uint32_t s_col(uint32_t t) { return 2 * DP + 128 + (ONE_S ? 0 : t * 128); }
     static constexpr uint32_t OFF_KV = 2 * BLOCK;
     static constexpr uint32_t OFF_BAR = OFF_KV + STAGES * BLOCK;
     static constexpr uint32_t SMEM = OFF_BAR + 512 + 1024; // and the alignment to 1024
@@ -115,6 +123,12 @@ __device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -196,7 +210,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ap_smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
     uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_done = bars + 6, *edge = bars + 8;
-    uint64_t *drain = bars + 9, *kv_full = bars + 11, *kv_empty = kv_full + L::STAGES;
+    uint64_t *s_free = bars + 9, *drain = bars + 11, *kv_full = bars + 13, *kv_empty = kv_full + L::STAGES;
     // TMEM base, abort, the pair's sequence, the pair in it and among all
     uint32_t *misc = reinterpret_cast<uint32_t *>(kv_empty + L::STAGES);
     volatile uint32_t *abort_flag = misc + 1;
@@ -241,12 +255,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
             mbar_init(&o_done[i], 1);
+            mbar_init(&s_free[i], 128);
             mbar_init(&drain[i], 1);
         }
         mbar_init(edge, 1);
         for (uint32_t i = 0; i < L::STAGES; ++i) {
             mbar_init(&kv_full[i], 1);
-            mbar_init(&kv_empty[i], 2);
+            mbar_init(&kv_empty[i], 1);
         }
         misc[1] = 0;
         fence_barrier_init();
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const uint32_t tmem = misc[0];
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
         if (warp == 8) {
             // ---- keys and values ----------------------------------------------------
             const uint32_t R = pp.box_rows, n_boxes = AP_KEYS / R;
@@ -335,64 +350,66 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (!going)
                 for (uint32_t i = it > L::STAGES ? it - L::STAGES : 0; i < it; ++i)
                     (void)mbar_wait(&kv_full[i % L::STAGES], (i / L::STAGES) & 1u);
-        } else if (warp < 11 && lane == 0) {
-            // ---- the products of one tile -------------------------------------------
-            const uint32_t t = warp - 9;
-            const APTile tile = t ? tile1 : tile0;
-            const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * DP;
-            const uint32_t q_addr = smem_u32(smem + t * L::BLOCK);
+        } else if ((warp == 9 || warp == 10) && lane == 0) {
+            // ---- the products: warp 9 S = Q K^T, warp 10 O += P V -----------------------
+            // S is asked for as soon as its place is free, so that it waits for its softmax
+            // and not the other way round; the tensor cores take what is ready.
+            const bool scores = warp == 9;
             constexpr uint32_t id_s = ap_idesc<BF16>(AP_KEYS, false), id_o = ap_idesc<BF16>(DP, true);
-            uint32_t it = 0, n = 0;
+            uint32_t it = scores ? 0 : 1; // load of block jb's keys, or values
+            uint32_t n0 = 0, n1 = 0, s_used = 0;
             bool ok = true;
             for (uint32_t j = jb; j < je && ok; ++j, it += 2) {
-                const uint32_t sk = it % L::STAGES, sv = (it + 1) % L::STAGES;
-                const bool active = j >= tile.j0 && j < tile.j1;
-                ok = ap_wait(&kv_full[sk], (it / L::STAGES) & 1u, abort_flag, p.status);
-                if (!ok) break;
-                if (active) {
-                    ok = n ? ap_wait(&o_done[t], (n - 1) & 1u, abort_flag, p.status)
-                           : ap_wait(&q_full[t], 0, abort_flag, p.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t k_addr = smem_u32(smem + L::OFF_KV + sk * L::BLOCK);
+                const uint32_t st = it % L::STAGES;
+                const uint32_t kv = smem_u32(smem + L::OFF_KV + st * L::BLOCK);
+                ok = ap_wait(&kv_full[st], (it / L::STAGES) & 1u, abort_flag, p.status);
 #pragma unroll
-                    for (uint32_t k = 0; k < DP / 16; ++k) {
-                        const uint32_t off = (k >> 2) * L::HALF + (k & 3u) * 32;
-                        mma_f16_ss(s_tmem, smem_desc_sw128(q_addr + off), smem_desc_sw128(k_addr + off), id_s, k != 0);
+                for (uint32_t t = 0; t < 2; ++t) {
+                    const APTile &tile = t ? tile1 : tile0;
+                    uint32_t &n = t ? n1 : n0;
+                    if (!ok || j < tile.j0 || j >= tile.j1) continue;
+                    if (scores) {
+                        if (n == 0) ok = ap_wait(&q_full[t], 0, abort_flag, p.status);
+                        const uint32_t used = L::ONE_S ? s_used : n;
+                        if (ok && used) ok = ap_wait(&s_free[L::ONE_S ? 0 : t], (used - 1) & 1u, abort_flag, p.status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t q_addr = smem_u32(smem + t * L::BLOCK);
+#pragma unroll
+                        for (uint32_t k = 0; k < DP / 16; ++k) {
+                            const uint32_t off = (k >> 2) * L::HALF + (k & 3u) * 32;
+                            mma_f16_ss(tmem + L::s_col(t), smem_desc_sw128(q_addr + off), smem_desc_sw128(kv + off),
+                                       id_s, k != 0);
+                        }
+                        tc_commit(&s_full[t]);
+                        ++s_used;
+                    } else {
+                        ok = ap_wait(&p_full[t], n & 1u, abort_flag, p.status);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (uint32_t k = 0; k < AP_KEYS / 16; ++k)
+                            mma_f16_ts(tmem + L::o_col(t), tmem + L::p_col(t) + k * 8,
+                                       ap_desc_v(kv + k * 2048, L::HALF), id_o, (n | k) != 0);
+                        tc_commit(&o_done[t]);
                     }
-                    tc_commit(&s_full[t]);
-                    tc_commit(&kv_empty[sk]);
-                } else {
-                    mbar_arrive(&kv_empty[sk]);
-                }
-                ok = ap_wait(&kv_full[sv], ((it + 1) / L::STAGES) & 1u, abort_flag, p.status);
-                if (!ok) break;
-                if (active) {
-                    ok = ap_wait(&p_full[t], n & 1u, abort_flag, p.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v_addr = smem_u32(smem + L::OFF_KV + sv * L::BLOCK);
-#pragma unroll
-                    for (uint32_t k = 0; k < AP_KEYS / 16; ++k)
-                        mma_f16_ts(o_tmem, s_tmem + k * 8, ap_desc_v(v_addr + k * 2048, L::HALF), id_o, (n | k) != 0);
-                    tc_commit(&o_done[t]);
-                    tc_commit(&kv_empty[sv]);
                     ++n;
-                } else {
-                    mbar_arrive(&kv_empty[sv]);
                 }
+                if (ok) tc_commit(&kv_empty[st]);
             }
             // every product and commit must have ended before tensor and shared memory go away
-            tc_commit(&drain[t]);
-            (void)mbar_wait(&drain[t], 0);
+            tc_commit(&drain[scores ? 0 : 1]);
+            (void)mbar_wait(&drain[scores ? 0 : 1], 0);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
         // ---- softmax: one thread a row ------------------------------------------------
         const uint32_t t = warp >> 2, r = threadIdx.x & 127u;
         const APTile tile = t ? tile1 : tile0;
         const uint32_t lane_addr = ((warp & 3u) * 32u) << 16;
-        const uint32_t s_tmem = tmem + t * 128 + lane_addr, o_tmem = tmem + 256 + t * DP + lane_addr;
+        const uint32_t s_tmem = tmem + (t ? L::s_col(1) : L::s_col(0)) + lane_addr;
+        const uint32_t p_tmem = tmem + (t ? L::p_col(1) : L::p_col(0)) + lane_addr;
+        const uint32_t o_tmem = tmem + (t ? L::o_col(1) : L::o_col(0)) + lane_addr;
         const uint32_t row = pair * AP_PAIR + t * AP_TILE + r;
         const uint32_t tok = row / p.group, g = row - tok * p.group;
         const bool valid = r < tile.rows;
@@ -436,6 +453,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 4; ++c) pin32(x[c]);
+            tc_fence_before();
+            mbar_arrive(&s_free[L::ONE_S ? 0 : t]);
             const uint32_t key0 = (tb + n) * AP_KEYS;
             if (key0 + AP_KEYS > tile.whole_hi || key0 < tile.whole_lo) {
 #pragma unroll
@@ -451,9 +470,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             for (int c = 0; c < 4; ++c) {
                 top[c] = __uint_as_float(x[c][0]);
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(x[c][i]));
+                for (int i = 1; i < 31; i += 2)
+                    top[c] = max3(top[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                top[c] = fmaxf(top[c], __uint_as_float(x[c][31]));
             }
             const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+            if (n) { // the last block's product has read P and written O
+                ok = ap_wait(&o_done[t], (n - 1) & 1u, abort_flag, p.status);
+                if (!ok) break;
+                tc_fence_after();
+            }
             if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
                 const float to = fmaxf(m, high);
                 const float f = m == -INFINITY ? 0.0f : exp2_approx(m - to);
@@ -490,7 +516,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                     sum2 = add_f32x2(sum2, pack_f32x2(a, c2));
                     w[i] = pack_pair<BF16>(a, c2);
                 }
-                tmem_st32(s_tmem + h * 32, w);
+                tmem_st32(p_tmem + h * 32, w);
             }
             tmem_wait_st();
             tc_fence_before();
