@@ -100,9 +100,9 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
 // Uses of v stay behind this point (a wait for tensor-memory loads does not name their registers).
-__device__ __forceinline__ void pin32(uint32_t (&v)[32]) {
+template <int N> __device__ __forceinline__ void pin(uint32_t (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
+    for (int i = 0; i < N; i += 8)
         asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]),
                           "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
@@ -160,7 +160,7 @@ __device__ __forceinline__ uint32_t ap_pairs(const AttnParams &p, const AttnSeq 
 // blocks that every row of the tile sees whole: those inside [whole_lo, whole_hi).
 struct APTile {
     uint32_t rows, j0, j1;
-    int64_t whole_lo, whole_hi;
+    uint32_t whole_lo, whole_hi;
 };
 __device__ __forceinline__ APTile ap_tile(const AttnParams &p, const AttnSeq &s, uint32_t row0) {
     APTile t{};
@@ -172,13 +172,25 @@ __device__ __forceinline__ APTile ap_tile(const AttnParams &p, const AttnSeq &s,
     const int64_t hi = p.causal ? last + 1 : s.kl;
     int64_t lo = p.window ? first - p.window + 1 : 0;
     if (lo < 0) lo = 0;
-    t.whole_hi = p.causal ? first + 1 : s.kl;
-    t.whole_lo = p.window ? last - p.window + 1 : 0;
+    const int64_t whole_hi = p.causal ? first + 1 : s.kl, whole_lo = p.window ? last - p.window + 1 : 0;
+    t.whole_hi = whole_hi > 0 ? static_cast<uint32_t>(whole_hi) : 0;
+    t.whole_lo = whole_lo > 0 ? static_cast<uint32_t>(whole_lo) : 0;
     if (hi > lo) {
         t.j0 = static_cast<uint32_t>(lo / AP_KEYS);
         t.j1 = static_cast<uint32_t>((hi + AP_KEYS - 1) / AP_KEYS);
     }
     return t;
+}
+
+// Row r of tile t of a pair: its token and query head.
+struct APRow {
+    uint64_t token, qhead;
+    bool valid;
+};
+__device__ __forceinline__ APRow ap_row(const AttnParams &p, const AttnSeq &s, uint32_t head, uint32_t pair, uint32_t t,
+                                        uint32_t r) {
+    const uint32_t row = pair * AP_PAIR + t * AP_TILE + r, tok = row / p.group;
+    return {static_cast<uint64_t>(s.q0) + tok, static_cast<uint64_t>(head) * p.group + (row - tok * p.group), tok < s.ql};
 }
 
 // The blocks of a pair, and how many parts they are split into.
@@ -285,7 +297,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const uint32_t tmem = misc[0];
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 8) {
             // ---- keys and values ----------------------------------------------------
             const uint32_t R = pp.box_rows, n_boxes = AP_KEYS / R;
@@ -402,7 +414,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             (void)mbar_wait(&drain[scores ? 0 : 1], 0);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
         // ---- softmax: one thread a row ------------------------------------------------
         const uint32_t t = warp >> 2, r = threadIdx.x & 127u;
         const APTile tile = t ? tile1 : tile0;
@@ -410,18 +422,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const uint32_t s_tmem = tmem + (t ? L::s_col(1) : L::s_col(0)) + lane_addr;
         const uint32_t p_tmem = tmem + (t ? L::p_col(1) : L::p_col(0)) + lane_addr;
         const uint32_t o_tmem = tmem + (t ? L::o_col(1) : L::o_col(0)) + lane_addr;
-        const uint32_t row = pair * AP_PAIR + t * AP_TILE + r;
-        const uint32_t tok = row / p.group, g = row - tok * p.group;
-        const bool valid = r < tile.rows;
-        const uint64_t qhead = static_cast<uint64_t>(head) * p.group + g;
         // Q, rows past the end as zeros
         {
-            const uint16_t *src = static_cast<const uint16_t *>(p.q) + (s.q0 + tok) * p.qt + qhead * p.qh;
+            const APRow w = ap_row(p, s, head, pair, t, r);
+            const uint16_t *src = static_cast<const uint16_t *>(p.q) + w.token * p.qt + w.qhead * p.qh;
             const uint32_t dst = smem_u32(smem + t * L::BLOCK) + r * 128;
 #pragma unroll
             for (uint32_t c = 0; c < DP / 8; ++c) {
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (valid && c * 8 < p.dim) v = *reinterpret_cast<const uint4 *>(src + c * 8);
+                if (w.valid && c * 8 < p.dim) v = *reinterpret_cast<const uint4 *>(src + c * 8);
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (c >> 3) * L::HALF +
                                                                               (((c & 7u) ^ (r & 7u)) << 4)),
                              "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
@@ -431,8 +440,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_arrive(&q_full[t]);
         }
         uint32_t key_lo = 0, key_hi = s.kl;
-        if (valid) {
-            const int64_t pos = static_cast<int64_t>(s.kl) - s.ql + tok;
+        if (r < tile.rows) {
+            const int64_t pos = static_cast<int64_t>(s.kl) - s.ql + (pair * AP_PAIR + t * AP_TILE + r) / p.group;
             const int64_t hi = p.causal ? pos + 1 : s.kl, lo = p.window ? pos - p.window + 1 : 0;
             key_hi = hi > 0 ? static_cast<uint32_t>(hi) : 0;
             key_lo = lo > 0 ? static_cast<uint32_t>(lo) : 0;
@@ -452,7 +461,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, x[c]);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) pin32(x[c]);
+            for (int c = 0; c < 4; ++c) pin(x[c]);
             tc_fence_before();
             mbar_arrive(&s_free[L::ONE_S ? 0 : t]);
             const uint32_t key0 = (tb + n) * AP_KEYS;
@@ -475,49 +484,53 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 top[c] = fmaxf(top[c], __uint_as_float(x[c][31]));
             }
             const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-            if (n) { // the last block's product has read P and written O
-                ok = ap_wait(&o_done[t], (n - 1) & 1u, abort_flag, p.status);
-                if (!ok) break;
-                tc_fence_after();
-            }
             if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
                 const float to = fmaxf(m, high);
                 const float f = m == -INFINITY ? 0.0f : exp2_approx(m - to);
                 m = to;
-                if (n) {
+                if (n) { // the last block's product has written O
+                    ok = ap_wait(&o_done[t], (n - 1) & 1u, abort_flag, p.status);
+                    if (!ok) break;
+                    tc_fence_after();
                     float a, c2;
                     unpack_f32x2(sum2, a, c2);
                     sum2 = pack_f32x2(a * f, c2 * f);
 #pragma unroll
-                    for (int c = 0; c < DP / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(o_tmem + c * 32, o);
+                    for (int c = 0; c < DP / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(o_tmem + c * 16, o);
                         tmem_wait_ld();
-                        pin32(o);
+                        pin(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(o_tmem + c * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(o_tmem + c * 16, o);
                     }
                 }
             }
             const float base = m == -INFINITY ? 0.0f : -m;
             const uint64_t base2 = pack_f32x2(base, base);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[32];
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint32_t *e = &x[2 * h + (i >> 4)][(i & 15) * 2];
+                for (int i = 0; i < 16; ++i) {
                     float a, c2;
-                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, base2), a,
-                                 c2);
+                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])),
+                                           scale2, base2),
+                                 a, c2);
                     a = exp2_approx(a);
                     c2 = exp2_approx(c2);
                     sum2 = add_f32x2(sum2, pack_f32x2(a, c2));
                     w[i] = pack_pair<BF16>(a, c2);
                 }
-                tmem_st32(p_tmem + h * 32, w);
+                if (c == 0 && n) { // the last block's product has read P
+                    ok = ap_wait(&o_done[t], (n - 1) & 1u, abort_flag, p.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                tmem_st16(p_tmem + c * 16, w);
             }
+            if (!ok) break;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&p_full[t]);
@@ -530,6 +543,12 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             unpack_f32x2(sum2, a, c2);
             const float sum = blocks ? a + c2 : 0.0f;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            // where the row goes is worked out again: kept over the loop it would cost registers
+            uint32_t again = r;
+            asm volatile("" : "+r"(again));
+            const AttnSeq s2 = attn_seq(p, misc[2], false);
+            const APRow w = ap_row(p, s2, head, misc[3], t, again);
+            uint16_t *out = static_cast<uint16_t *>(p.out) + w.token * p.ot + w.qhead * p.oh;
             const uint64_t slot =
                 ((static_cast<uint64_t>(misc[4]) * p.kv_heads + head) * pp.splits + part) * AP_PAIR + t * AP_TILE + r;
 #pragma unroll
@@ -538,23 +557,23 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 if (blocks) {
                     tmem_ld32(o_tmem + c * 32, o);
                     tmem_wait_ld();
-                    pin32(o);
+                    pin(o);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                if (!valid) continue;
+                if (!w.valid) continue;
                 if (span.parts == 1) {
-                    uint16_t *dst = static_cast<uint16_t *>(p.out) + (s.q0 + tok) * p.ot + qhead * p.oh + c * 32;
+                    uint16_t *dst = out + c * 32;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        uint32_t w[4];
+                        uint32_t v[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            w[k] = pack_pair<BF16>(__uint_as_float(o[i * 8 + 2 * k]) * inv,
+                            v[k] = pack_pair<BF16>(__uint_as_float(o[i * 8 + 2 * k]) * inv,
                                                    __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
                         if (c * 32u + i * 8u < p.dim)
-                            *reinterpret_cast<uint4 *>(dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4 *>(dst + i * 8) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 } else {
                     uint4 *dst = reinterpret_cast<uint4 *>(pp.part + slot * DP + c * 32);
@@ -563,11 +582,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                         dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
             }
-            if (valid) {
+            if (w.valid) {
                 if (span.parts > 1)
                     pp.part_ml[slot] = make_float2(m, sum);
                 else if (p.lse)
-                    p.lse[static_cast<uint64_t>(s.q0 + tok) * p.heads + qhead] =
+                    p.lse[w.token * p.heads + w.qhead] =
                         sum == 0.0f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
             }
         }
