@@ -22,11 +22,18 @@ inline uint64_t a256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
 // Rows (tokens x group) up to which a sequence is the rows kernel's.
 constexpr uint32_t ROW_LIMIT = 32;
 
+// The prompt kernel's work is dealt out by blocks where whole items would leave
+// CTAs idle: with fewer than DEAL_ITEMS items a CTA, or one a CTA where one
+// prompt without context brings its own small items.  Items of up to WHOLE_BLOCKS
+// blocks are not worth the fragments and the kernel that joins them.
+constexpr uint32_t DEAL_ITEMS = 6, WHOLE_BLOCKS = 10;
+
 struct AttnPlan {
     uint32_t dp, workers, group;
     bool rows, prompt;       // which kernels have work
-    uint32_t pairs, splits;  // prompt kernel: bound on its tile pairs, parts of a pair
-    uint64_t prefix, part, part_ml, ppart, ppart_ml, total; // workspace offsets
+    bool deal;               // prompt kernel: blocks are dealt out, not items
+    uint32_t pairs, ctas;    // its pairs of tiles (a bound), and its grid
+    uint64_t prefix, part, part_ml, ppart, ppart_ml, tail, total; // workspace offsets
 };
 
 AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
@@ -52,20 +59,23 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         n.part = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * n.dp * 4);
         n.part_ml = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * 8);
     }
-    n.splits = 1;
     if (n.prompt) {
         const uint64_t big = all / ((n.rows ? ROW_LIMIT : 0) + 1);
         n.pairs = static_cast<uint32_t>(all / AP_PAIR + (big < a.seqs ? big : a.seqs));
-        // fewer pairs than SMs: split their keys until every SM has a part
-        const uint64_t want = (all + AP_PAIR - 1) / AP_PAIR * a.kv_heads;
-        const uint64_t most = a.max_kv_len / (AP_KEYS * AP_LEAST_BLOCKS);
-        uint64_t splits = want < sms ? sms / want : 1;
-        splits = splits < most ? splits : most;
-        n.splits = splits < 1 ? 1 : static_cast<uint32_t>(splits);
-        if (n.splits > 1) {
-            const uint64_t slots = static_cast<uint64_t>(n.pairs) * a.kv_heads * n.splits * AP_PAIR;
-            n.ppart = take(slots * n.dp * 4);
-            n.ppart_ml = take(slots * 8);
+        const uint64_t items = static_cast<uint64_t>(n.pairs) * a.kv_heads;
+        const bool prompt = a.seqs == 1 && a.causal && !a.window && a.max_q_len == a.max_kv_len;
+        uint64_t keys = a.max_kv_len;
+        if (a.window) {
+            const uint64_t seen = static_cast<uint64_t>(a.window) + AP_PAIR / n.group + 1;
+            keys = seen < keys ? seen : keys;
+        }
+        n.deal = items < static_cast<uint64_t>(sms) * (prompt ? 1 : DEAL_ITEMS) && n.pairs <= AP_MAX_PAIRS &&
+                 keys > AP_KEYS * WHOLE_BLOCKS;
+        n.ctas = !n.deal && items < sms ? static_cast<uint32_t>(items) : sms;
+        if (n.deal) {
+            n.ppart = take(static_cast<uint64_t>(n.ctas) * 2 * AP_PAIR * n.dp * 4);
+            n.ppart_ml = take(static_cast<uint64_t>(n.ctas) * 2 * AP_PAIR * 8);
+            n.tail = take(static_cast<uint64_t>(n.ctas) * 16);
         }
     }
     n.total = o;
@@ -100,6 +110,27 @@ int check_attention(const fmcuda_paged_attention_args *a) {
     return FM_STATUS_OK;
 }
 
+// A launch that may begin while the kernel before it on the stream ends (the kernel itself
+// waits, griddepcontrol.wait, before it reads what that one wrote).
+template <typename P>
+int launch_after(void (*kernel)(P), dim3 grid, uint32_t threads, cudaStream_t s, const P &p, const char *what) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
+    if (err != cudaSuccess) {
+        (void)cudaGetLastError();
+        return cuda_status(err, what);
+    }
+    return FM_STATUS_OK;
+}
+
 template <int DP, bool BF16> int launch_rows(const AttnParams &p, uint32_t rows, cudaStream_t s) {
     static bool ready[64] = {};
     auto kfn = attn_rows_kernel<DP, BF16>;
@@ -114,8 +145,8 @@ template <int DP, bool BF16> int launch_rows(const AttnParams &p, uint32_t rows,
     kfn<<<p.workers / AR_WARPS, AR_THREADS, ARows<DP>::SMEM, s>>>(p);
     int rc = check_launch("attn_rows_kernel");
     if (rc) return rc;
-    attn_combine_kernel<DP, BF16><<<dim3(p.seqs * p.kv_heads, rows), AC_THREADS, 0, s>>>(p);
-    return check_launch("attn_combine_kernel");
+    return launch_after(attn_combine_kernel<DP, BF16>, dim3(p.seqs * p.kv_heads, rows), AC_THREADS, s, p,
+                        "attn_combine_kernel");
 }
 
 // The cache as boxes of 64 values x box_rows rows of one head of one page, the
@@ -173,21 +204,21 @@ int launch_prompt(const fmcuda_paged_attention_args &a, const AttnPlan &n, const
     p.box_rows = a.page_size & (~a.page_size + 1u); // its lowest set bit
     if (p.box_rows > AP_KEYS) p.box_rows = AP_KEYS;
     p.heads_first = a.cache_head_stride < a.cache_row_stride;
-    p.splits = n.splits;
+    p.wide = a.head_dim % 16 == 0 && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(a.out) % 32 == 0;
+    p.deal = n.deal;
+    p.max_pairs = n.pairs;
     p.part = reinterpret_cast<float *>(ws + n.ppart);
     p.part_ml = reinterpret_cast<float2 *>(ws + n.ppart_ml);
+    p.tail = reinterpret_cast<int4 *>(ws + n.tail);
     CUtensorMap map_k, map_v;
     int rc = make_cache_map(&map_k, a, a.k_cache, p.box_rows, p.heads_first);
     if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, p.box_rows, p.heads_first);
     if (rc) return rc;
-    const uint64_t grid = static_cast<uint64_t>(n.pairs) * a.kv_heads * n.splits;
-    if (grid > 0x7FFFFFFFu) return set_error(FM_STATUS_SHAPE_MISMATCH, "too many rows in a call");
-    kfn<<<static_cast<uint32_t>(grid), AP_THREADS, L::SMEM, s>>>(map_k, map_v, p);
+    kfn<<<n.ctas, AP_THREADS, L::SMEM, s>>>(map_k, map_v, p);
     rc = check_launch("attn_prompt_kernel");
-    if (rc || n.splits == 1) return rc;
-    const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
-    attn_join_kernel<DP, BF16><<<static_cast<uint32_t>((rows + 7) / 8), 256, 0, s>>>(p);
-    return check_launch("attn_join_kernel");
+    if (rc || !n.deal) return rc;
+    return launch_after(attn_join_kernel<DP, BF16>, dim3(n.ctas, AJ_SLICES), 256, s, p, "attn_join_kernel");
 }
 
 template <int DP, bool BF16>

@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         }
     }
     __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;\n");
     const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
     const uint64_t begin = worker * per;
     if (begin >= total) return;
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(AC_THREADS) attn_combine_kernel(const AttnPara
     const AttnSeq s = attn_seq(p, b, false);
     const ARShape sh = ar_shape(p, s);
     if (sh.tiles == 0) return;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const uint64_t total = p.prefix[p.seqs];
     const uint64_t even = (total + p.workers - 1) / p.workers;
     const uint64_t per = even > p.least ? even : p.least;
