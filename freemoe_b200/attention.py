@@ -11,11 +11,11 @@ head_dim]`` with any strides but the last (token-major pages are its
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import math
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch._C import _cuda_getDevice as _current_device
 
 from ._lib import (ROPE_BANDS, ROPE_BASE, ROPE_LINEAR, ROPE_PLAIN, ROPE_RAMP, X_BF16, X_E4M3, X_F16, X_F32, FmError,
                    PagedAttentionArgs, RmsNormArgs, RopeAppendArgs, RopeScaling, check, load, packed_entry, packer)
@@ -34,25 +34,34 @@ _pack_rope = packer(RopeAppendArgs).pack
 _pack_attention = packer(PagedAttentionArgs).pack
 
 
-@functools.cache
-def _entry(name: str, *argtypes):
-    return packed_entry(name, *argtypes)
+class _Entries:
+    """The C entries taking packed arguments, bound at their first use."""
+
+    def __getattr__(self, name: str):
+        argtypes = {"norm": ("fmcuda_add_rms_norm", C.c_void_p), "rope": ("fmcuda_rope_append", C.c_void_p),
+                    "attention_bytes": ("fmcuda_paged_attention_workspace_bytes", C.c_void_p),
+                    "attention": ("fmcuda_paged_attention", C.c_void_p, C.c_uint64, C.c_void_p)}[name]
+        fn = packed_entry(*argtypes)
+        setattr(self, name, fn)
+        return fn
+
+
+_entries = _Entries()
 
 
 def _refuse(message: str, code: int = SHAPE_MISMATCH):
     raise FmError(code, message)
 
 
-def _check_device(device: int, *tensors) -> None:
-    current = torch.cuda.current_device()
-    for t in (device, *(t.get_device() for t in tensors if t is not None)):
-        if t != current:
-            _refuse(f"a tensor is not on the current device, cuda:{current}", INVALID_ARGUMENT)
+def _elsewhere():
+    _refuse(f"a tensor is not on the current device, cuda:{torch.cuda.current_device()}", INVALID_ARGUMENT)
 
 
 def _norm(x, weight, residual, epsilon, y, y_dtype, scales):
     device = x.get_device()
-    _check_device(device, weight, residual)
+    if device != _current_device() or weight.get_device() != device or (
+            residual is not None and residual.get_device() != device):
+        _elsewhere()
     tokens, dim = x.shape
     if weight.shape != (dim,) or (residual is not None and residual.shape != x.shape):
         _refuse("norm takes [tokens, d_model], a weight of d_model and a residual like x")
@@ -67,7 +76,7 @@ def _norm(x, weight, residual, epsilon, y, y_dtype, scales):
         rs, r_at, h_at, r_dtype = rs[0], residual.data_ptr(), h.data_ptr(), _DTYPES.get(residual.dtype, _NO_DTYPE)
     if not dense:
         _refuse("norm inputs must be contiguous in their rows")
-    rc = _entry("fmcuda_add_rms_norm", C.c_void_p)(
+    rc = _entries.norm(
         _pack_norm(x.data_ptr(), r_at, weight.data_ptr(), y.data_ptr(), h_at, 0 if scales is None else scales.data_ptr(),
                    xs[0], rs, ys[0], _DTYPES.get(x.dtype, _NO_DTYPE), r_dtype, _DTYPES.get(weight.dtype, _NO_DTYPE),
                    y_dtype, tokens, dim, epsilon), _raw_stream(device))
@@ -140,7 +149,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
     if q.dim() != 3:
         _refuse("q is [tokens, heads, head_dim]")
     device = q.get_device()
-    _check_device(device, k, v, positions, inv_freq, k_cache, v_cache, slots)
+    if device != _current_device() or positions.get_device() != device or inv_freq.get_device() != device:
+        _elsewhere()
     tokens, heads, dim = q.shape
     qs = q.stride()
     if (positions.shape != (tokens,) or positions.dtype != torch.int32 or not positions.is_contiguous() or
@@ -150,8 +160,12 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
     if k is not None or v is not None or k_cache is not None or v_cache is not None or slots is not None:
         if k is None or v is None or k_cache is None or v_cache is None or slots is None:
             _refuse("k, v, their caches and slots come together", INVALID_ARGUMENT)
-        kv_heads = k.shape[1] if k.dim() == 3 else -1
-        if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
+        if (k.get_device() != device or v.get_device() != device or k_cache.get_device() != device or
+                v_cache.get_device() != device or slots.get_device() != device):
+            _elsewhere()
+        shape = k.shape
+        kv_heads = shape[1] if len(shape) == 3 else -1
+        if shape != (tokens, kv_heads, dim) or v.shape != shape:
             _refuse("k and v are [tokens, kv_heads, head_dim]")
         cache, ks, vs, cs = k_cache.shape, k.stride(), v.stride(), k_cache.stride()
         if (len(cache) != 4 or v_cache.shape != cache or v_cache.stride() != cs or cache[1] != kv_heads or
@@ -172,7 +186,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
     if not dense:
         _refuse("q, k, v and caches must be contiguous in their heads")
     out = torch.empty_like(q, dtype=kind, memory_format=torch.contiguous_format)
-    rc = _entry("fmcuda_rope_append", C.c_void_p)(
+    rc = _entries.rope(
         _pack_rope(q.data_ptr(), at[0], at[1], out.data_ptr(), at[2], at[3], positions.data_ptr(), at[4],
                    inv_freq.data_ptr(), qs[0], qs[1], *strides, heads * dim, dim, *cs, _DTYPES.get(q.dtype, _NO_DTYPE),
                    _DTYPES.get(kind, _NO_DTYPE), tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0],
@@ -203,44 +217,48 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q.dim() != 3 or k_cache.dim() != 4:
         _refuse("q is [tokens, heads, head_dim], caches are [pages, kv_heads, page_size, head_dim]")
     device = q.get_device()
-    _check_device(device, k_cache, v_cache, page_table, q_start, kv_len, workspace)
+    if (device != _current_device() or k_cache.get_device() != device or v_cache.get_device() != device or
+            page_table.get_device() != device or q_start.get_device() != device or kv_len.get_device() != device or
+            (workspace is not None and workspace.get_device() != device)):
+        _elsewhere()
     tokens, heads, dim = q.shape
-    pages, kv_heads, page_size, cache_dim = k_cache.shape
+    cache, table = k_cache.shape, page_table.shape
+    pages, kv_heads, page_size, cache_dim = cache
     qs, cs, ts = q.stride(), k_cache.stride(), page_table.stride()
-    if v_cache.shape != k_cache.shape or v_cache.stride() != cs or cache_dim != dim:
+    if v_cache.shape != cache or v_cache.stride() != cs or cache_dim != dim:
         _refuse("caches are [pages, kv_heads, page_size, head_dim], of one layout")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    kind = q.dtype
+    if k_cache.dtype != kind or v_cache.dtype != kind:
         _refuse("q and the caches have one type", INVALID_ARGUMENT)
     seqs = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or q_start.shape != (seqs + 1,):
+    if len(table) != 2 or table[0] != seqs or q_start.shape != (seqs + 1,):
         _refuse("page_table is [seqs, pages], q_start [seqs + 1], kv_len [seqs]")
     if (page_table.dtype != torch.int32 or q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or
             not q_start.is_contiguous() or not kv_len.is_contiguous()):
         _refuse("page_table, q_start and kv_len are int32", INVALID_ARGUMENT)
     if max_q_len < 0 or max_kv_len < 0 or window < 0:
         _refuse("lengths must not be negative", INVALID_ARGUMENT)
-    if page_table.shape[1] * page_size < max_kv_len:
+    if table[1] * page_size < max_kv_len:
         _refuse("page table is shorter than max_kv_len")
-    if qs[2] != 1 or cs[3] != 1 or (ts[1] != 1 and page_table.shape[1] > 1):
+    if qs[2] != 1 or cs[3] != 1 or (ts[1] != 1 and table[1] > 1):
         _refuse("q, caches and page_table must be contiguous in their last dimension")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     args = _pack_attention(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
         page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), qs[0], qs[1], heads * dim, dim, cs[0], cs[1], cs[2],
-        ts[0], _DTYPES.get(q.dtype, _NO_DTYPE), seqs, tokens, heads, kv_heads, dim, pages, page_size,
+        ts[0], _DTYPES.get(kind, _NO_DTYPE), seqs, tokens, heads, kv_heads, dim, pages, page_size,
         min(max_q_len, tokens), max_kv_len, 1 if causal else 0, window, 1.0 / math.sqrt(dim) if scale is None else scale)
     if workspace is None:
         need = C.c_uint64()
-        rc = _entry("fmcuda_paged_attention_workspace_bytes", C.POINTER(C.c_uint64))(args, need)
+        rc = _entries.attention_bytes(args, C.addressof(need))
         if rc:
             check(rc)
-        workspace = q.new_empty(need.value, dtype=torch.uint8)
         size = need.value
+        at = (workspace := q.new_empty(size, dtype=torch.uint8)).data_ptr() if size else 0
     else:
-        size = workspace.numel() * workspace.element_size()
-    rc = _entry("fmcuda_paged_attention", C.c_void_p, C.c_uint64, C.c_void_p)(args, workspace.data_ptr(), size,
-                                                                            _raw_stream(device))
+        at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    rc = _entries.attention(args, at, size, _raw_stream(device))
     if rc:
         check(rc)
     return (out, lse) if return_lse else out

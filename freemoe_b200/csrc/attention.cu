@@ -19,6 +19,10 @@ namespace {
 
 inline uint64_t a256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
 
+// Steps a warp up to which the cluster form is taken: beyond, a wave of all SMs and the
+// kernel that joins the fragments cost less than the SMs that the clusters leave idle.
+constexpr uint32_t CLUSTER_STEPS = 16;
+
 // Rows (tokens x group) up to which a sequence is the rows kernel's.
 constexpr uint32_t ROW_LIMIT = 32;
 
@@ -31,10 +35,18 @@ constexpr uint32_t DEAL_ITEMS = 6, WHOLE_BLOCKS = 10;
 struct AttnPlan {
     uint32_t dp, workers, group;
     bool rows, prompt;       // which kernels have work
+    uint32_t cluster;        // CTAs a unit of the cluster form of the rows kernel; 0: the other form
+    uint32_t tiles;          // row tiles of a unit's sequence and head, at most
     bool deal;               // prompt kernel: blocks are dealt out, not items
     uint32_t pairs, ctas;    // its pairs of tiles (a bound), and its grid
     uint64_t prefix, part, part_ml, ppart, ppart_ml, tail, total; // workspace offsets
 };
+
+// Keys that `rows` packed rows of a sequence see together, at most.
+uint64_t keys_seen(const fmcuda_paged_attention_args &a, uint32_t rows) {
+    const uint64_t seen = static_cast<uint64_t>(a.window) + rows / (a.heads / a.kv_heads) + 1;
+    return a.window && seen < a.max_kv_len ? seen : a.max_kv_len;
+}
 
 AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
     AttnPlan n{};
@@ -54,7 +66,18 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         o += a256(bytes);
         return at;
     };
-    if (n.rows) {
+    const uint64_t most_rows = static_cast<uint64_t>(a.max_q_len) * n.group;
+    n.tiles = static_cast<uint32_t>((most_rows < ROW_LIMIT ? most_rows + AR_ROWS - 1 : ROW_LIMIT) / AR_ROWS);
+    const uint64_t keys = keys_seen(a, ROW_LIMIT);
+    const uint64_t units = static_cast<uint64_t>(a.seqs) * a.kv_heads * n.tiles;
+    if (n.rows && units && units <= sms) {
+        // the largest cluster that one wave holds and that has a step for each warp
+        const uint64_t steps = keys / AR_KEYS + 1;
+        uint32_t c = 8;
+        while (c > 1 && (units * c > sms || steps < c * AR_WARPS)) c /= 2;
+        if (steps <= static_cast<uint64_t>(c) * AR_WARPS * CLUSTER_STEPS) n.cluster = c;
+    }
+    if (n.rows && !n.cluster) {
         n.prefix = take((static_cast<uint64_t>(a.seqs) + 1) * 8);
         n.part = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * n.dp * 4);
         n.part_ml = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * 8);
@@ -64,13 +87,8 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         n.pairs = static_cast<uint32_t>(all / AP_PAIR + (big < a.seqs ? big : a.seqs));
         const uint64_t items = static_cast<uint64_t>(n.pairs) * a.kv_heads;
         const bool prompt = a.seqs == 1 && a.causal && !a.window && a.max_q_len == a.max_kv_len;
-        uint64_t keys = a.max_kv_len;
-        if (a.window) {
-            const uint64_t seen = static_cast<uint64_t>(a.window) + AP_PAIR / n.group + 1;
-            keys = seen < keys ? seen : keys;
-        }
         n.deal = items < static_cast<uint64_t>(sms) * (prompt ? 1 : DEAL_ITEMS) && n.pairs <= AP_MAX_PAIRS &&
-                 keys > AP_KEYS * WHOLE_BLOCKS;
+                 keys_seen(a, AP_PAIR) > AP_KEYS * WHOLE_BLOCKS;
         n.ctas = !n.deal && items < sms ? static_cast<uint32_t>(items) : sms;
         if (n.deal) {
             n.ppart = take(static_cast<uint64_t>(n.ctas) * 2 * AP_PAIR * n.dp * 4);
@@ -127,6 +145,37 @@ int launch_after(void (*kernel)(P), dim3 grid, uint32_t threads, cudaStream_t s,
     if (err != cudaSuccess) {
         (void)cudaGetLastError();
         return cuda_status(err, what);
+    }
+    return FM_STATUS_OK;
+}
+
+template <int DP, bool BF16>
+int launch_cluster(const AttnParams &p, const AttnPlan &n, cudaStream_t s) {
+    static bool ready[64] = {};
+    auto kfn = attn_cluster_kernel<DP, BF16>;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, ARows<DP>::SMEM);
+        if (e != cudaSuccess) return cuda_status(e, "attention shared memory");
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    cudaLaunchAttribute size{};
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = n.cluster;
+    size.val.clusterDim.y = size.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(p.seqs * p.kv_heads * n.tiles * n.cluster);
+    config.blockDim = dim3(AR_THREADS);
+    config.dynamicSmemBytes = ARows<DP>::SMEM;
+    config.stream = s;
+    config.attrs = &size;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kfn, p, n.tiles);
+    if (err != cudaSuccess) {
+        (void)cudaGetLastError();
+        return cuda_status(err, "attn_cluster_kernel");
     }
     return FM_STATUS_OK;
 }
@@ -227,6 +276,7 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
     int rc = FM_STATUS_OK;
     if (n.prompt) rc = launch_prompt<DP, BF16>(a, n, p, ws, s);
     if (rc || !n.rows) return rc;
+    if (n.cluster) return launch_cluster<DP, BF16>(p, n, s);
     const uint64_t rows = static_cast<uint64_t>(a.max_q_len) * n.group;
     return launch_rows<DP, BF16>(p, rows < ROW_LIMIT ? static_cast<uint32_t>(rows) : ROW_LIMIT, s);
 }

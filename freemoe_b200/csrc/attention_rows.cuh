@@ -101,19 +101,6 @@ __device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
     ar_enter(p, c);
 }
 
-// Element offset in the caches of the key of lane & 15, or -1 (not to be read).
-__device__ __forceinline__ int64_t ar_key_offset(const AttnParams &p, const ARCursor &c, uint32_t lane) {
-    const uint32_t key = (c.sh.step0 + c.step) * AR_KEYS + (lane & 15u);
-    if (key < c.s.lo || key >= c.s.kl) return -1;
-    const uint32_t page = key / p.page_size;
-    const int32_t id = __ldg(p.table + c.b * p.tb + page);
-    if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
-        raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
-        return -1;
-    }
-    return id * p.cp + static_cast<int64_t>(key - page * p.page_size) * p.cr + (c.tile / c.sh.tiles) * p.ch;
-}
-
 // Queues the copies of a step's 16 keys and values; what is not to be read becomes zeros.
 template <int DP>
 __device__ __forceinline__ void ar_fetch(const AttnParams &p, uint32_t stage, int64_t offset, uint32_t lane) {
@@ -156,6 +143,139 @@ __device__ __forceinline__ uint64_t ar_block_scan(uint64_t v, uint64_t *s_part, 
     }
     *total = all;
     return before + inc - v;
+}
+
+// A warp's 16 rows of a unit: Q fragments, O, and of rows lane / 4 and lane / 4 + 8 the
+// reference exponent (in log2), the lane's part of the sum, and the keys that the row sees.
+template <int DP, bool BF16> struct ARState {
+    uint32_t qf[DP / 16][4];
+    float o[DP / 8][4];
+    float m[2], l[2];
+    uint32_t key_lo[2], key_hi[2];
+
+    __device__ __forceinline__ void begin(const AttnParams &p, const AttnSeq &s, uint32_t head, uint32_t rt,
+                                          uint32_t lane) {
+        const uint16_t *rows[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t row = rt * AR_ROWS + lane / 4 + r * 8;
+            const uint32_t t = row / p.group, g = row - t * p.group;
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+            key_lo[r] = key_hi[r] = 0;
+            rows[r] = nullptr;
+            if (t < s.ql) {
+                const int64_t pos = static_cast<int64_t>(s.kl) - s.ql + t;
+                const int64_t hi = p.causal ? pos + 1 : s.kl;
+                const int64_t lo = p.window ? pos - p.window + 1 : 0;
+                key_hi[r] = hi > 0 ? static_cast<uint32_t>(hi) : 0;
+                key_lo[r] = lo > 0 ? static_cast<uint32_t>(lo) : 0;
+                rows[r] = static_cast<const uint16_t *>(p.q) + (static_cast<uint64_t>(s.q0) + t) * p.qt +
+                          static_cast<int64_t>(head * p.group + g) * p.qh;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t col = k * 16 + (x >> 1) * 8 + (lane & 3u) * 2;
+                const uint16_t *row = rows[x & 1];
+                qf[k][x] = row && col < p.dim ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
+            }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[n][x] = 0.0f;
+    }
+
+    // The 16 keys and values of stage `st`, the first of them key `key`.
+    __device__ __forceinline__ void step(const AttnParams &p, uint32_t st, uint32_t key_first, uint32_t lane) {
+        using L = ARows<DP>;
+        // S = Q K^T: two 8-key tiles
+        float sc[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t b[4];
+            const uint32_t row = ((lane >> 4) << 3) + (lane & 7u), piece = k * 2 + ((lane >> 3) & 1u);
+            ldsm4(st + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+            mma_16816<BF16>(sc[0], qf[k], b[0], b[1]);
+            mma_16816<BF16>(sc[1], qf[k], b[2], b[3]);
+        }
+        const uint32_t key0 = key_first + (lane & 3u) * 2;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int r = x >> 1;
+                const uint32_t key = key0 + n * 8 + (x & 1);
+                sc[n][x] = key >= key_lo[r] && key < key_hi[r] ? sc[n][x] * p.scale_log2 : -INFINITY;
+                top[r] = fmaxf(top[r], sc[n][x]);
+            }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+        }
+        // the reference exponent moves only when it is over 2^8 too small: the weights
+        // stay in range of f32 sums and of 16-bit products, and O is rarely rescaled
+        if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
+            float f2[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float to = fmaxf(m[r], top[r]);
+                f2[r] = m[r] == -INFINITY ? 0.0f : exp2_approx(m[r] - to);
+                m[r] = to;
+                l[r] *= f2[r];
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[n][x] *= f2[x >> 1];
+        }
+        const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        uint32_t pf[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                sc[n][x] = exp2_approx(sc[n][x] - base[x >> 1]);
+                l[x >> 1] += sc[n][x];
+            }
+            pf[2 * n] = pack_pair<BF16>(sc[n][0], sc[n][1]);
+            pf[2 * n + 1] = pack_pair<BF16>(sc[n][2], sc[n][3]);
+        }
+        // O += P V
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+            uint32_t b[4];
+            const uint32_t row = (((lane >> 3) & 1u) << 3) + (lane & 7u), piece = n * 2 + (lane >> 4);
+            ldsm4_t(st + L::HALF + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+            mma_16816<BF16>(o[2 * n], pf, b[0], b[1]);
+            mma_16816<BF16>(o[2 * n + 1], pf, b[2], b[3]);
+        }
+    }
+
+    // The rows' sums, in every lane of a row's four.
+    __device__ __forceinline__ float sum(int r) const {
+        float v = l[r];
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+        return v + __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+    }
+};
+
+// A cache row's place: the offset of the key of lane & 15 among 16 from `key_first` on.
+__device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq &s, uint32_t b, uint32_t head,
+                                             uint32_t key_first, uint32_t lane) {
+    const uint32_t key = key_first + (lane & 15u);
+    if (key < s.lo || key >= s.kl) return -1;
+    const uint32_t page = key / p.page_size;
+    const int32_t id = __ldg(p.table + b * p.tb + page);
+    if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
+        raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
+        return -1;
+    }
+    return id * p.cp + static_cast<int64_t>(key - page * p.page_size) * p.cr + head * p.ch;
 }
 
 template <int DP, bool BF16>
@@ -229,13 +349,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
     uint32_t fetched = 0;
-    int64_t next = ar_key_offset(p, f, lane); // one step ahead of the copies: hides the table's latency
+    auto place = [&] { return ar_key_at(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * AR_KEYS, lane); };
+    int64_t next = place(); // one step ahead of the copies: hides the table's latency
     auto fetch = [&] {
         if (fetched < count) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
             if (++fetched < count) {
                 ar_advance(p, f);
-                next = ar_key_offset(p, f, lane);
+                next = place();
             }
         }
         cp_async_commit();
@@ -243,158 +364,190 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
 #pragma unroll
     for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
 
-    uint32_t qf[DP / 16][4];
-    float o[DP / 8][4];
-    float m[2], l[2];           // of rows lane / 4 and lane / 4 + 8; m in log2
-    uint32_t key_lo[2], key_hi[2];
+    ARState<DP, BF16> u;
     bool fresh = true;
     uint32_t first_step = 0;
     for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
         if (fresh) {
             fresh = false;
             first_step = c.step;
-            const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
-            const uint16_t *rows[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t row = rt * AR_ROWS + lane / 4 + r * 8;
-                const uint32_t t = row / p.group, g = row - t * p.group;
-                m[r] = -INFINITY;
-                l[r] = 0.0f;
-                key_lo[r] = key_hi[r] = 0;
-                rows[r] = nullptr;
-                if (t < c.s.ql) {
-                    const int64_t pos = static_cast<int64_t>(c.s.kl) - c.s.ql + t;
-                    const int64_t hi = p.causal ? pos + 1 : c.s.kl;
-                    const int64_t lo = p.window ? pos - p.window + 1 : 0;
-                    key_hi[r] = hi > 0 ? static_cast<uint32_t>(hi) : 0;
-                    key_lo[r] = lo > 0 ? static_cast<uint32_t>(lo) : 0;
-                    rows[r] = static_cast<const uint16_t *>(p.q) + (c.s.q0 + t) * p.qt +
-                              static_cast<int64_t>(head * p.group + g) * p.qh;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t col = k * 16 + (x >> 1) * 8 + (lane & 3u) * 2;
-                    const uint16_t *row = rows[x & 1];
-                    qf[k][x] = row && col < p.dim ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
-                }
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][x] = 0.0f;
+            u.begin(p, c.s, head, rt, lane);
         }
         cp_async_wait<L::STAGES - 2>();
         __syncwarp();
-        const uint32_t st = ring + (i % L::STAGES) * L::STAGE;
-        // S = Q K^T: two 8-key tiles
-        float sc[2][4] = {};
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            uint32_t b[4];
-            const uint32_t row = ((lane >> 4) << 3) + (lane & 7u), piece = k * 2 + ((lane >> 3) & 1u);
-            ldsm4(st + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
-            mma_16816<BF16>(sc[0], qf[k], b[0], b[1]);
-            mma_16816<BF16>(sc[1], qf[k], b[2], b[3]);
-        }
-        const uint32_t key0 = (c.sh.step0 + c.step) * AR_KEYS + (lane & 3u) * 2;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int r = x >> 1;
-                const uint32_t key = key0 + n * 8 + (x & 1);
-                sc[n][x] = key >= key_lo[r] && key < key_hi[r] ? sc[n][x] * p.scale_log2 : -INFINITY;
-                top[r] = fmaxf(top[r], sc[n][x]);
-            }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
-        }
-        // the reference exponent moves only when it is over 2^8 too small: the weights
-        // stay in range of f32 sums and of 16-bit products, and O is rarely rescaled
-        if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
-            float f2[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float to = fmaxf(m[r], top[r]);
-                f2[r] = m[r] == -INFINITY ? 0.0f : exp2_approx(m[r] - to);
-                m[r] = to;
-                l[r] *= f2[r];
-            }
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][x] *= f2[x >> 1];
-        }
-        float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-        uint32_t pf[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                sc[n][x] = exp2_approx(sc[n][x] - base[x >> 1]);
-                l[x >> 1] += sc[n][x];
-            }
-            pf[2 * n] = pack_pair<BF16>(sc[n][0], sc[n][1]);
-            pf[2 * n + 1] = pack_pair<BF16>(sc[n][2], sc[n][3]);
-        }
-        // O += P V
-#pragma unroll
-        for (int n = 0; n < DP / 16; ++n) {
-            uint32_t b[4];
-            const uint32_t row = (((lane >> 3) & 1u) << 3) + (lane & 7u), piece = n * 2 + (lane >> 4);
-            ldsm4_t(st + L::HALF + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
-            mma_16816<BF16>(o[2 * n], pf, b[0], b[1]);
-            mma_16816<BF16>(o[2 * n + 1], pf, b[2], b[3]);
-        }
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, (c.sh.step0 + c.step) * AR_KEYS, lane);
         __syncwarp(); // every lane has read the stage that the next copies fill
         fetch();
 
         if (c.step + 1 == c.sh.steps || i + 1 == count) {
             fresh = true;
             const bool whole = first_step == 0 && c.step + 1 == c.sh.steps;
-            const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
             const uint64_t slot = worker * 2 + (first_step == 0 ? 1 : 0);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float sum = l[r];
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                const float sum = u.sum(r);
                 const uint32_t in = lane / 4 + r * 8, row = rt * AR_ROWS + in;
                 const uint32_t t = row / p.group, g = row - t * p.group;
                 if (t >= c.s.ql) continue;
                 if (whole) {
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const uint64_t h = head * p.group + g;
-                    uint16_t *dst = static_cast<uint16_t *>(p.out) + (c.s.q0 + t) * p.ot + h * p.oh;
+                    const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(c.s.q0) + t;
+                    uint16_t *dst = static_cast<uint16_t *>(p.out) + token * p.ot + h * p.oh;
 #pragma unroll
                     for (int n = 0; n < DP / 8; ++n) {
                         const uint32_t col = n * 8 + (lane & 3u) * 2;
                         if (col < p.dim)
                             *reinterpret_cast<uint32_t *>(dst + col) =
-                                pack_pair<BF16>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
+                                pack_pair<BF16>(u.o[n][2 * r] * inv, u.o[n][2 * r + 1] * inv);
                     }
                     if (p.lse && (lane & 3u) == 0)
-                        p.lse[static_cast<uint64_t>(c.s.q0 + t) * p.heads + h] =
-                            sum == 0.0f ? -INFINITY : m[r] * 0.6931471805599453f + logf(sum);
+                        p.lse[token * p.heads + h] =
+                            sum == 0.0f ? -INFINITY : u.m[r] * 0.6931471805599453f + logf(sum);
                 } else {
                     float *dst = p.part + (slot * AR_ROWS + in) * DP;
 #pragma unroll
                     for (int n = 0; n < DP / 8; ++n)
                         *reinterpret_cast<float2 *>(dst + n * 8 + (lane & 3u) * 2) =
-                            make_float2(o[n][2 * r], o[n][2 * r + 1]);
-                    if ((lane & 3u) == 0) p.part_ml[slot * AR_ROWS + in] = make_float2(m[r], sum);
+                            make_float2(u.o[n][2 * r], u.o[n][2 * r + 1]);
+                    if ((lane & 3u) == 0) p.part_ml[slot * AR_ROWS + in] = make_float2(u.m[r], sum);
                 }
             }
         }
         if (i + 1 < count) ar_advance(p, c);
     }
     cp_async_wait<0>();
+}
+
+// ---- few units of short sequences: a cluster each ----------------------------------
+//
+// Where a cluster of CTAs a unit is all the GPU can do with the work (one short
+// sequence, say), the unit's steps are cut over the cluster's warps, a CTA's
+// warps are joined in its shared memory and the CTAs through each other's: one
+// launch, no fragments in global memory.  blockIdx.x / cluster size: (sequence,
+// key head, row tile), `unit_tiles` row tiles a sequence and head.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// A value of CTA `rank`'s shared memory, at the address that `addr` has in this one's.
+__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnParams p, uint32_t unit_tiles) {
+    using L = ARows<DP>;
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    __shared__ float s_m[AR_WARPS][AR_ROWS], s_l[AR_WARPS][AR_ROWS]; // of the warps
+    __shared__ float s_top[AR_ROWS], s_sum[AR_ROWS];                 // of the CTA
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = cluster_rank(), ranks = cluster_size();
+    const uint32_t unit = blockIdx.x / ranks, rt = unit % unit_tiles;
+    const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
+    const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
+    const ARShape sh = ar_shape(p, s);
+    if (rt >= sh.tiles) return; // the whole cluster
+
+    const uint32_t part = rank * AR_WARPS + warp, parts = ranks * AR_WARPS;
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * part / parts);
+    const uint32_t count = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * (part + 1) / parts) - begin;
+    const uint32_t key_first = (sh.step0 + begin) * AR_KEYS;
+    const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
+    uint32_t fetched = 0;
+    int64_t next = count ? ar_key_at(p, s, b, head, key_first, lane) : -1;
+    auto fetch = [&] {
+        if (fetched < count) {
+            ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
+            if (++fetched < count) next = ar_key_at(p, s, b, head, key_first + fetched * AR_KEYS, lane);
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
+    ARState<DP, BF16> u;
+    u.begin(p, s, head, rt, lane);
+    for (uint32_t i = 0; i < count; ++i) {
+        cp_async_wait<L::STAGES - 2>();
+        __syncwarp();
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * AR_KEYS, lane);
+        __syncwarp();
+        fetch();
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    // the warp's O over its ring, 16 rows of DP
+    float *mine = reinterpret_cast<float *>(ar_smem + warp * (L::STAGES * L::STAGE));
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const float sum = u.sum(r);
+        const uint32_t in = lane / 4 + r * 8;
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+            *reinterpret_cast<float2 *>(mine + in * DP + n * 8 + (lane & 3u) * 2) =
+                make_float2(u.o[n][2 * r], u.o[n][2 * r + 1]);
+        if ((lane & 3u) == 0) {
+            s_m[warp][in] = u.m[r];
+            s_l[warp][in] = sum;
+        }
+    }
+    __syncthreads();
+    // the CTA's O behind warp 0's
+    float *joined = reinterpret_cast<float *>(ar_smem) + AR_ROWS * DP;
+    for (uint32_t i = threadIdx.x; i < AR_ROWS * DP; i += AR_THREADS) {
+        const uint32_t in = i / DP;
+        float top = -INFINITY, acc = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < AR_WARPS; ++w) top = fmaxf(top, s_m[w][in]);
+#pragma unroll
+        for (uint32_t w = 0; w < AR_WARPS; ++w) {
+            const float f = s_m[w][in] == -INFINITY ? 0.0f : exp2_approx(s_m[w][in] - top);
+            sum += s_l[w][in] * f;
+            acc += reinterpret_cast<const float *>(ar_smem + w * (L::STAGES * L::STAGE))[i] * f;
+        }
+        joined[i] = acc;
+        if (i % DP == 0) {
+            s_top[in] = top;
+            s_sum[in] = sum;
+        }
+    }
+    cluster_sync();
+    // rows rank, rank + ranks, ... of the unit
+    const uint32_t top_at = smem_u32(s_top), sum_at = smem_u32(s_sum), o_at = smem_u32(joined);
+    for (uint32_t i = threadIdx.x; i < AR_ROWS / ranks * (DP / 2); i += AR_THREADS) {
+        const uint32_t in = i / (DP / 2) * ranks + rank, col = i % (DP / 2) * 2;
+        const uint32_t row = rt * AR_ROWS + in, t = row / p.group, g = row - t * p.group;
+        if (t >= s.ql || col >= p.dim) continue;
+        float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
+        for (uint32_t k = 0; k < ranks; ++k) top = fmaxf(top, cluster_load(top_at + in * 4, k));
+        for (uint32_t k = 0; k < ranks; ++k) {
+            const float m = cluster_load(top_at + in * 4, k);
+            const float f = m == -INFINITY ? 0.0f : exp2_approx(m - top);
+            sum += cluster_load(sum_at + in * 4, k) * f;
+            a0 += cluster_load(o_at + (in * DP + col) * 4, k) * f;
+            a1 += cluster_load(o_at + (in * DP + col) * 4 + 4, k) * f;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
+        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + token * p.ot + h * p.oh + col) =
+            pack_pair<BF16>(a0 * inv, a1 * inv);
+        if (p.lse && col == 0)
+            p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
+    }
+    cluster_sync(); // nobody leaves while its shared memory is read
 }
 
 // Joins the fragments of the units that were cut: a CTA a unit and row.  Its

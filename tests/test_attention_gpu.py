@@ -333,7 +333,9 @@ def test_refusals(cuda):
     refused(8, max_kv_len=1000)
     refused(26, window=3, causal=False)
     refused(26, scale=float("nan"))
-    refused(26, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(FmError) as e:  # a long sequence: its work is cut, and the fragments need room
+        Batch([(1, 40000)], 8, 2, 64, 16).run(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    assert e.value.code == 26
     refused(8, set_("q", lambda c: torch.zeros(1, 8, 65, dtype=c.dtype, device="cuda")[:, :, :64]))
     refused(26, set_("q", lambda c: torch.zeros(8 * 64 + 1, dtype=c.dtype, device="cuda")[1:].view(1, 8, 64)))
     odd = torch.zeros(4, 2, 12, 64, dtype=b.dtype, device="cuda")
