@@ -194,8 +194,11 @@ template <int DP, bool BF16> int launch_rows(const AttnParams &p, uint32_t rows,
     kfn<<<p.workers / AR_WARPS, AR_THREADS, ARows<DP>::SMEM, s>>>(p);
     int rc = check_launch("attn_rows_kernel");
     if (rc) return rc;
-    return launch_after(attn_combine_kernel<DP, BF16>, dim3(p.seqs * p.kv_heads, rows), AC_THREADS, s, p,
-                        "attn_combine_kernel");
+    // few units are cut into many fragments each
+    const dim3 grid(p.seqs * p.kv_heads, rows);
+    if (p.seqs * p.kv_heads * 16 <= p.workers)
+        return launch_after(attn_combine_kernel<DP, BF16, 16>, grid, 16 * 32, s, p, "attn_combine_kernel");
+    return launch_after(attn_combine_kernel<DP, BF16, 4>, grid, 4 * 32, s, p, "attn_combine_kernel");
 }
 
 // The cache as boxes of 64 values x box_rows rows of one head of one page, the

@@ -550,73 +550,79 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     cluster_sync(); // nobody leaves while its shared memory is read
 }
 
-// Joins the fragments of the units that were cut: a CTA a unit and row.  Its
-// warps take every eighth fragment each, a lane four (two) values of the head.
-constexpr uint32_t AC_THREADS = 256;
-
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(AC_THREADS) attn_combine_kernel(const AttnParams p) {
+// Joins the fragments of the units that were cut: a CTA of W warps a unit and row.
+// Warp i takes fragments i, i + W, ..., a lane four (two) values of the head, with the
+// loads of four fragments under way together.
+template <int DP, bool BF16, int W> __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p) {
     constexpr int V = DP / 32;
-    __shared__ float s_o[AC_THREADS / 32][DP];
-    __shared__ float s_m[AC_THREADS / 32], s_l[AC_THREADS / 32];
+    __shared__ float s_o[W][DP];
+    __shared__ float s_m[W], s_l[W];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t b = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
     const AttnSeq s = attn_seq(p, b, false);
     const ARShape sh = ar_shape(p, s);
-    if (sh.tiles == 0) return;
+    const uint32_t row = blockIdx.y;
+    if (sh.tiles == 0 || row >= s.ql * p.group) return;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const uint64_t total = p.prefix[p.seqs];
     const uint64_t even = (total + p.workers - 1) / p.workers;
     const uint64_t per = even > p.least ? even : p.least;
-    for (uint32_t row = blockIdx.y; row < s.ql * p.group; row += gridDim.y) {
-        const uint32_t t = row / p.group, g = row % p.group, in = row % AR_ROWS;
-        const uint64_t first = p.prefix[b] + static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * sh.steps;
-        const uint64_t w0 = first / per, w1 = (first + sh.steps - 1) / per;
-        if (w0 == w1) continue; // written by its one warp
-        float acc[V] = {}, m = -INFINITY, l = 0.0f;
-        for (uint64_t w = w0 + warp; w <= w1; w += AC_THREADS / 32) {
-            const uint64_t slot = (w * 2 + (w == w0 ? 1 : 0)) * AR_ROWS + in;
-            const float2 ml = p.part_ml[slot];
-            const float *src = p.part + slot * DP + lane * V;
-            float v[V];
+    const uint32_t t = row / p.group, g = row % p.group, in = row % AR_ROWS;
+    const uint64_t first = p.prefix[b] + static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * sh.steps;
+    const uint64_t w0 = first / per;
+    const uint32_t n = static_cast<uint32_t>((first + sh.steps - 1) / per - w0) + 1;
+    if (n == 1) return; // written by its one warp
+    float acc[V] = {}, m = -INFINITY, l = 0.0f;
+    for (uint32_t f0 = warp; f0 < n; f0 += 4 * W) {
+        float2 ml[4];
+        float v[4][V];
 #pragma unroll
-            for (int x = 0; x < V; ++x) v[x] = src[x];
-            if (ml.x == -INFINITY) continue;
-            const float to = fmaxf(m, ml.x);
-            const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to), fb = exp2_approx(ml.x - to);
+        for (uint32_t x = 0; x < 4; ++x) {
+            const uint32_t f = f0 + x * W;
+            ml[x] = make_float2(-INFINITY, 0.0f);
+            if (f < n) {
+                const uint64_t slot = ((w0 + f) * 2 + (f == 0 ? 1 : 0)) * AR_ROWS + in;
+                ml[x] = p.part_ml[slot];
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[x][i] = p.part[slot * DP + lane * V + i];
+            }
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) {
+            if (ml[x].x == -INFINITY) continue;
+            const float to = fmaxf(m, ml[x].x);
+            const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to), fb = exp2_approx(ml[x].x - to);
             m = to;
-            l = l * fa + ml.y * fb;
+            l = l * fa + ml[x].y * fb;
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] = acc[x] * fa + v[x] * fb;
+            for (int i = 0; i < V; ++i) acc[i] = acc[i] * fa + v[x][i] * fb;
         }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < V; ++x) s_o[warp][lane * V + x] = acc[x];
-        if (lane == 0) {
-            s_m[warp] = m;
-            s_l[warp] = l;
-        }
-        __syncthreads();
-        const uint32_t col = threadIdx.x * 2;
-        if (col >= p.dim) continue;
-        float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < AC_THREADS / 32; ++w) top = fmaxf(top, s_m[w]);
-#pragma unroll
-        for (uint32_t w = 0; w < AC_THREADS / 32; ++w) {
-            const float f = s_m[w] == -INFINITY ? 0.0f : exp2_approx(s_m[w] - top);
-            sum += s_l[w] * f;
-            a0 += s_o[w][col] * f;
-            a1 += s_o[w][col + 1] * f;
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const uint64_t h = head * p.group + g;
-        uint16_t *dst = static_cast<uint16_t *>(p.out) + (s.q0 + t) * p.ot + h * p.oh;
-        *reinterpret_cast<uint32_t *>(dst + col) = pack_pair<BF16>(a0 * inv, a1 * inv);
-        if (p.lse && col == 0)
-            p.lse[static_cast<uint64_t>(s.q0 + t) * p.heads + h] =
-                sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = acc[i];
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
+    __syncthreads();
+    const uint32_t col = threadIdx.x * 2;
+    if (col >= p.dim) return;
+    float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) top = fmaxf(top, s_m[w]);
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+        const float f = s_m[w] == -INFINITY ? 0.0f : exp2_approx(s_m[w] - top);
+        sum += s_l[w] * f;
+        a0 += s_o[w][col] * f;
+        a1 += s_o[w][col + 1] * f;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
+    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + token * p.ot + h * p.oh + col) =
+        pack_pair<BF16>(a0 * inv, a1 * inv);
+    if (p.lse && col == 0)
+        p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
 }
 
 } // namespace fmb
