@@ -6,7 +6,7 @@
 // (the RMSNorm of Engine::forward_token, src/engine.cpp, whose sum is a double
 // over one token; here f32 partial sums of at most 32 values a thread joined
 // pairwise).  The operator is one read of x and residual and one write of y and
-// h; the weight stays in registers over the rows of a CTA.
+// h; the weight stays on the SM over the rows of a CTA.
 #include <string>
 
 #include "vec8.cuh"
@@ -89,6 +89,12 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float scale = fmaxf(top, 1e-10f) / 448.0f;
     const float inv = 1.0f / scale;
+    // v / scale, correctly rounded but for rare cases: the product's error, from one fused
+    // operation, corrects it (a code is a rounding of it: an error in its last bit flips codes)
+    auto code = [&](float x) {
+        const float q = x * inv;
+        return fmaf(fmaf(-q, scale, x), inv, q);
+    };
     uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
     const uint32_t groups = (p.d + 127) / 128;
     if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;
@@ -97,42 +103,103 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
             uint32_t w[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                w[i] = e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) | e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16;
+                w[i] = e4m3x2(code(v[4 * i]), code(v[4 * i + 1])) | e4m3x2(code(v[4 * i + 2]), code(v[4 * i + 3])) << 16;
             *reinterpret_cast<uint2 *>(y + c * 8) = make_uint2(w[0], w[1]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t e = value_at<VEC>(c, j);
-            if (e < p.d) y[e] = static_cast<uint8_t>(e4m3x2(v[j] * inv, 0.0f));
+            if (e < p.d) y[e] = static_cast<uint8_t>(e4m3x2(code(v[j]), 0.0f));
         }
     }
 }
 
-// ITER chunks a thread, held in registers from the read to the write.
-template <bool VEC, int NT, int ITER>
+// ITER chunks a thread, held in registers from the read to the write; the next row's
+// are on their way while this one is summed and written.  The weight waits in shared
+// memory, as f32 in the chunks' order.
+// WIDE: x or the residual is f32, whose eights take two accesses.
+template <bool VEC, bool WIDE, int ITER> struct NormRow {
+    uint4 x[ITER], r[ITER];                       // VEC
+    uint4 x2[WIDE ? ITER : 1], r2[WIDE ? ITER : 1];
+    float h[ITER][8];                             // otherwise: already h
+
+    __device__ __forceinline__ void load(const NormParams &p, uint64_t row, uint32_t c0, uint32_t step) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const uint32_t c = c0 + i * step;
+            if constexpr (VEC) {
+                x[i] = r[i] = make_uint4(0, 0, 0, 0);
+                if (WIDE) x2[i] = r2[i] = make_uint4(0, 0, 0, 0);
+                if (c * 8 < p.d) {
+                    if constexpr (WIDE) {
+                        const Raw8 a = raw8_load(p.x, p.xt, row * p.xs + c * 8);
+                        x[i] = a.a;
+                        x2[i] = a.b;
+                        if (p.res) {
+                            const Raw8 b = raw8_load(p.res, p.rt, row * p.rs + c * 8);
+                            r[i] = b.a;
+                            r2[i] = b.b;
+                        }
+                    } else {
+                        x[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.x) + row * p.xs + c * 8);
+                        if (p.res)
+                            r[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.res) + row * p.rs +
+                                                                    c * 8);
+                    }
+                }
+            } else {
+                load_chunk<false>(p.x, p.xt, row * p.xs, c, p.d, h[i]);
+                if (p.res) {
+                    float v[8];
+                    load_chunk<false>(p.res, p.rt, row * p.rs, c, p.d, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[i][j] += v[j];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void get(const NormParams &p, float (&out)[ITER][8]) const {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            if constexpr (VEC) {
+                raw8_unpack(Raw8{x[i], x2[WIDE ? i : 0]}, p.xt, out[i]);
+                if (p.res) {
+                    float v[8];
+                    raw8_unpack(Raw8{r[i], r2[WIDE ? i : 0]}, p.rt, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) out[i][j] += v[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) out[i][j] = h[i][j];
+            }
+        }
+    }
+};
+
+template <bool VEC, bool WIDE, int NT, int ITER>
 __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const NormParams p) {
-    constexpr uint32_t TEAMS = NT < 128 ? 128 / NT : 1;
+    constexpr uint32_t THREADS = NT < 128 ? 128 : NT, TEAMS = THREADS / NT;
+    extern __shared__ float4 s_w[]; // chunk c: s_w[2 c], s_w[2 c + 1]
     __shared__ float s_part[2][32];
     const uint32_t c0 = NT < 128 ? threadIdx.x % NT : threadIdx.x;
     const uint32_t team = blockIdx.x * TEAMS + (NT < 128 ? threadIdx.x / NT : 0);
-    float w[ITER][8];
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) load_chunk<VEC>(p.w, p.wt, 0, c0 + i * NT, p.d, w[i]);
-    uint32_t turn = 0;
-    for (uint64_t row = team; row < p.tokens; row += static_cast<uint64_t>(gridDim.x) * TEAMS, turn ^= 1u) {
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * TEAMS;
+    uint64_t row = team;
+    NormRow<VEC, WIDE, ITER> next;
+    if (row < p.tokens) next.load(p, row, c0, NT);
+    for (uint32_t c = threadIdx.x; c < NT * ITER; c += THREADS) {
+        float w[8];
+        load_chunk<VEC>(p.w, p.wt, 0, c, p.d, w);
+        s_w[2 * c] = make_float4(w[0], w[1], w[2], w[3]);
+        s_w[2 * c + 1] = make_float4(w[4], w[5], w[6], w[7]);
+    }
+    __syncthreads();
+    for (uint32_t turn = 0; row < p.tokens; row += step, turn ^= 1u) {
         float h[ITER][8];
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) load_chunk<VEC>(p.x, p.xt, row * p.xs, c0 + i * NT, p.d, h[i]);
-        if (p.res) {
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                float r[8];
-                load_chunk<VEC>(p.res, p.rt, row * p.rs, c0 + i * NT, p.d, r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] += r[j];
-            }
-        }
+        next.get(p, h);
+        if (row + step < p.tokens) next.load(p, row + step, c0, NT);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i)
@@ -147,12 +214,15 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const
         }
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
+            const uint32_t c = c0 + i * NT;
+            const float4 wa = s_w[2 * c], wb = s_w[2 * c + 1];
+            const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * root * w[i][j];
+            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * root * w[j];
             if (p.yt == FM_X_E4M3)
-                store_e4m3<VEC>(p, row, c0 + i * NT, h[i]);
+                store_e4m3<VEC>(p, row, c, h[i]);
             else
-                store_chunk<VEC>(p.y, p.yt, row * p.ys, c0 + i * NT, p.d, h[i]);
+                store_chunk<VEC>(p.y, p.yt, row * p.ys, c, p.d, h[i]);
         }
     }
 }
@@ -201,26 +271,35 @@ template <bool VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ke
     }
 }
 
-template <bool VEC, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
-    constexpr uint32_t threads = NT < 128 ? 128 : NT, teams = threads / NT;
+template <bool VEC, bool WIDE, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
+    constexpr uint32_t threads = NT < 128 ? 128 : NT, teams = threads / NT, smem = NT * ITER * 32;
+    auto kfn = add_rms_norm_kernel<VEC, WIDE, NT, ITER>;
     const uint32_t want = (p.tokens + teams - 1) / teams;
-    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * (2048 / threads);
-    add_rms_norm_kernel<VEC, NT, ITER><<<want < most ? want : most, threads, 0, s>>>(p);
+    static int per_sm = 0; // CTAs that an SM holds: the same on every device of this library's architecture
+    if (!per_sm) {
+        cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
+            (void)cudaGetLastError();
+            per_sm = 1;
+        }
+    }
+    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * per_sm;
+    kfn<<<want < most ? want : most, threads, smem, s>>>(p);
 }
 
-template <bool VEC> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+template <bool VEC, bool WIDE> void dispatch_norm(const NormParams &p, cudaStream_t s) {
     if (p.d <= 256)
-        launch_norm<VEC, 32, 1>(p, s);
+        launch_norm<VEC, WIDE, 32, 1>(p, s);
     else if (p.d <= 1024)
-        launch_norm<VEC, 32, 4>(p, s);
+        launch_norm<VEC, WIDE, 32, 4>(p, s);
     else if (p.d <= 2048)
-        launch_norm<VEC, 128, 2>(p, s);
+        launch_norm<VEC, WIDE, 128, 2>(p, s);
     else if (p.d <= 4096)
-        launch_norm<VEC, 256, 2>(p, s);
+        launch_norm<VEC, WIDE, 256, 2>(p, s);
     else if (p.d <= 8192)
-        launch_norm<VEC, 512, 2>(p, s);
+        launch_norm<VEC, WIDE, 512, 2>(p, s);
     else if (p.d <= 16384)
-        launch_norm<VEC, 1024, 2>(p, s);
+        launch_norm<VEC, WIDE, 1024, 2>(p, s);
     else {
         const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
         add_rms_norm_long_kernel<VEC><<<p.tokens < most ? p.tokens : most, 1024, 0, s>>>(p);
@@ -261,9 +340,11 @@ extern "C" int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *a, void *stream) 
                      aligned16(a->x) && aligned16(a->residual) && aligned16(a->weight) && aligned16(a->y) &&
                      aligned16(a->residual_out);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (vec)
-        dispatch_norm<true>(p, s);
+    if (!vec)
+        dispatch_norm<false, true>(p, s);
+    else if (p.xt == FM_X_F32 || (p.res && p.rt == FM_X_F32))
+        dispatch_norm<true, true>(p, s);
     else
-        dispatch_norm<false>(p, s);
+        dispatch_norm<true, false>(p, s);
     return check_launch("add_rms_norm_kernel");
 }

@@ -6,7 +6,8 @@
 // (src/rope.cpp of the reference turns one head at a time on the host).  The
 // operator is one read of q, k and v and one write of q and of two cache rows a
 // token; the cosines of a token are shared by all of its heads.  A CTA takes a
-// token, or a part of its heads when there are too few tokens to fill the GPU.
+// few tokens, whose cosines its threads work out together before the barrier, or
+// a part of one token's heads when there are too few tokens to fill the GPU.
 //
 // The angle of a far position does not fit f32 (at position 2^17 its last bit
 // is 2^-7 radians), so the product is taken in turns in 64 bits, its whole part
@@ -21,7 +22,7 @@ namespace fmb {
 namespace {
 
 constexpr uint32_t ROPE_THREADS = 256;
-constexpr uint32_t ROPE_MAX_DIM = 1024;
+constexpr uint32_t ROPE_MAX_DIM = 1024, ROPE_TURNS = ROPE_MAX_DIM / 2, ROPE_BATCH = 8;
 
 struct RopeParams {
     const void *q, *k, *v;
@@ -35,130 +36,217 @@ struct RopeParams {
     float factor;
     uint32_t page_size;
     uint64_t n_slots;
-    uint32_t head_items, value_items, items; // work items of a rotated head, of a value head, of a token
+    uint32_t head_items, value_items; // eights (or pairs of eights) of a rotated head, of a value head
+    uint32_t tokens, batch;                  // tokens a CTA takes together
     int *status;
 };
 
-struct Place {
-    const void *src;
-    void *dst;
-    int64_t from, to;
-    uint32_t item;
-    bool turns, live;
-};
-
-// Where item `it` of token `t` reads and writes: the heads of q, of k, of v in turn.
-__device__ __forceinline__ Place rope_place(const RopeParams &p, uint32_t it, int64_t t, int64_t cache_row) {
-    Place w;
-    const uint32_t turned = (p.heads + p.kv_heads) * p.head_items;
-    w.turns = it < turned;
-    w.live = true;
-    if (w.turns) {
-        uint32_t h = it / p.head_items;
-        w.item = it - h * p.head_items;
-        if (h < p.heads) {
-            w.src = p.q;
-            w.dst = p.q_out;
-            w.from = t * p.qt + h * p.qh;
-            w.to = t * p.ot + h * p.oh;
-            return w;
-        }
-        h -= p.heads;
-        w.src = p.k;
-        w.dst = p.kc;
-        w.from = t * p.kt + h * p.kh;
-        w.to = cache_row + h * p.ch;
-    } else {
-        const uint32_t h = (it - turned) / p.value_items;
-        w.item = it - turned - h * p.value_items;
-        w.src = p.v;
-        w.dst = p.vc;
-        w.from = t * p.vt + h * p.vh;
-        w.to = cache_row + h * p.ch;
-    }
-    w.live = cache_row >= 0;
-    return w;
-}
-
-// VEC: an item is 8 values and, for pairs at (i, i + rot/2), their 8 partners
-// (heads, strides and rot/2 in whole eights).  Otherwise it is one pair or one
-// value; consecutive lanes then take consecutive pairs.
-template <bool VEC, bool INTER>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const RopeParams p) {
-    __shared__ float2 s_turn[ROPE_MAX_DIM / 2];
-    const int64_t t = blockIdx.x;
+// The cosines of the CTA's tokens, and their rows of the cache (-1: a slot below zero or,
+// reported, past the cache); ends with the CTA's barrier.
+__device__ __forceinline__ void rope_tokens(const RopeParams &p, uint32_t t0, uint32_t n, float2 *s_turns,
+                                            int64_t *s_row) {
     const uint32_t half = p.rot / 2;
-    for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
-        const double turns = static_cast<double>(p.positions[t]) * static_cast<double>(p.inv_freq[i]) *
-                             0.15915494309189533577; // 1 / (2 pi)
+    for (uint32_t i = threadIdx.x; i < n * half; i += blockDim.x) {
+        const uint32_t k = i / half;
+        const double turns = static_cast<double>(p.positions[t0 + k]) *
+                             static_cast<double>(p.inv_freq[i - k * half]) * 0.15915494309189533577; // 1 / (2 pi)
         float sn, cs;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-        s_turn[i] = make_float2(cs * p.factor, sn * p.factor);
+        s_turns[i] = make_float2(cs * p.factor, sn * p.factor);
     }
-    int64_t cache_row = -1;
-    if (p.kc) {
-        const int64_t slot = p.slots[t];
-        if (slot >= 0 && static_cast<uint64_t>(slot) < p.n_slots) {
-            const int64_t page = slot / p.page_size;
-            cache_row = page * p.cp + (slot - page * p.page_size) * p.cr;
-        } else if (slot >= 0 && threadIdx.x == 0 && blockIdx.y == 0) {
-            raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
+    if (threadIdx.x < n) {
+        int64_t row = -1;
+        if (p.kc) {
+            const int64_t slot = p.slots[t0 + threadIdx.x];
+            if (slot >= 0 && static_cast<uint64_t>(slot) < p.n_slots) {
+                const int64_t page = slot / p.page_size;
+                row = page * p.cp + (slot - page * p.page_size) * p.cr;
+            } else if (slot >= 0 && blockIdx.y == 0) {
+                raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
+            }
         }
+        s_row[threadIdx.x] = row;
     }
     __syncthreads();
-    for (uint32_t it = blockIdx.y * blockDim.x + threadIdx.x; it < p.items; it += gridDim.y * blockDim.x) {
-        const Place w = rope_place(p, it, t, cache_row);
-        if (!w.live) continue;
-        if constexpr (VEC) {
-            float a[8], b[8];
-            if (!w.turns) {
-                raw8_unpack(raw8_load(w.src, p.in_t, w.from + w.item * 8), p.in_t, a);
-                store8(w.dst, p.out_t, w.to + w.item * 8, a);
-            } else if (INTER) {
-                const uint32_t i0 = w.item * 4;
-                raw8_unpack(raw8_load(w.src, p.in_t, w.from + w.item * 8), p.in_t, a);
-                if (i0 < half) {
+}
+
+// Eight values of a compile-time type.
+template <int T> __device__ __forceinline__ Raw8 rope_load(const char *src) {
+    Raw8 r;
+    r.a = r.b = *reinterpret_cast<const uint4 *>(src);
+    if constexpr (T == FM_X_F32) r.b = reinterpret_cast<const uint4 *>(src)[1];
+    return r;
+}
+
+// Heads, strides and rot/2 (interleaved: rot) in whole eights.  A thread keeps its place
+// in the head -- eight values, or eight pairs (i, i + rot/2) -- and up to U of the heads of
+// q, k and (interleaved, where their places are the same) v, whose addresses only move on
+// from token to token of the CTA's batch: per token U loads under way together, then the
+// turns and the stores.  Measured with 8192 tokens of 32 + 8 heads of 128, bf16 (201 MB,
+// 31 us at the measured copy rate): 39 us; U = 2 or 4, 41; an index over all of a token's
+// eights with its divisions, 44 (issue slots 65% busy); the cosines worked out by every
+// thread for itself, 64.  Bound by the loads under way: registers against warps.
+template <bool INTER, int IN, int OUT>
+__global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kernel(const RopeParams p) {
+    constexpr int PAIRS = INTER ? 4 : 8, U = IN == FM_X_F32 || !INTER ? 2 : 3;
+    constexpr int SI = x_size(IN), SO = x_size(OUT);
+    __shared__ float2 s_turns[ROPE_TURNS];
+    __shared__ int64_t s_row[ROPE_BATCH];
+    const uint32_t t0 = blockIdx.x * p.batch, n = p.tokens - t0 < p.batch ? p.tokens - t0 : p.batch;
+    const uint32_t half = p.rot / 2, at_once = blockDim.x / p.head_items; // heads at once
+    const uint32_t item = threadIdx.x % p.head_items, lane_head = threadIdx.x / p.head_items;
+    const bool pair = item * 8 < (INTER ? p.rot : half);
+    const uint32_t ea = item * 8 + (INTER || pair ? 0 : half); // copied values lie behind the pairs
+    const uint32_t step = at_once * gridDim.y, turned = p.heads + p.kv_heads;
+    const uint32_t heads = lane_head >= at_once ? 0 : INTER ? turned + p.kv_heads : turned;
+    const float2 *my_turns = s_turns + (INTER ? item * 4 : ea);
+    rope_tokens(p, t0, n, s_turns, s_row);
+    for (uint32_t h1 = blockIdx.y * at_once + lane_head; h1 < heads; h1 += U * step) {
+        const char *src[U];
+        char *dst[U];
+        int64_t move[U];
+        bool here[U], cached[U], turns[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const uint32_t h = h1 + x * step;
+            here[x] = h < heads;
+            cached[x] = h >= p.heads;
+            turns[x] = pair && h < turned;
+            const bool key = h < turned;
+            if (!cached[x]) {
+                src[x] = static_cast<const char *>(p.q) + (static_cast<int64_t>(t0) * p.qt + h * p.qh + ea) * SI;
+                dst[x] = static_cast<char *>(p.q_out) + (static_cast<int64_t>(t0) * p.ot + h * p.oh + ea) * SO;
+                move[x] = p.qt * SI;
+            } else {
+                const uint32_t c = h - (key ? p.heads : turned);
+                const int64_t from = static_cast<int64_t>(t0) * (key ? p.kt : p.vt) + c * (key ? p.kh : p.vh);
+                src[x] = static_cast<const char *>(key ? p.k : p.v) + (from + ea) * SI;
+                dst[x] = static_cast<char *>(key ? p.kc : p.vc) + (c * p.ch + ea) * SO;
+                move[x] = (key ? p.kt : p.vt) * SI;
+            }
+        }
+#pragma unroll 1
+        for (uint32_t k = 0; k < n; ++k) {
+            const int64_t row = s_row[k];
+            Raw8 a[U], b[INTER ? 1 : U];
+            bool live[U];
+#pragma unroll
+            for (int x = 0; x < U; ++x) {
+                live[x] = here[x] && (!cached[x] || row >= 0);
+                if (live[x]) {
+                    a[x] = rope_load<IN>(src[x]);
+                    if (!INTER && turns[x]) b[x] = rope_load<IN>(src[x] + half * SI);
+                }
+                src[x] += move[x];
+            }
+            float2 cs[PAIRS];
+            if (pair) {
+#pragma unroll
+                for (int j = 0; j < PAIRS; ++j) cs[j] = my_turns[k * half + j];
+            }
+#pragma unroll
+            for (int x = 0; x < U; ++x) {
+                if (!live[x]) continue;
+                char *to = dst[x] + (cached[x] ? row : k * p.ot) * SO;
+                float f[8], g[8];
+                raw8_unpack(a[x], IN, f);
+                if (!turns[x]) {
+                    store8(to, OUT, 0, f);
+                } else if (INTER) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float2 cs = s_turn[i0 + j];
-                        b[2 * j] = a[2 * j] * cs.x - a[2 * j + 1] * cs.y;
-                        b[2 * j + 1] = a[2 * j] * cs.y + a[2 * j + 1] * cs.x;
+                        g[2 * j] = f[2 * j] * cs[j].x - f[2 * j + 1] * cs[j].y;
+                        g[2 * j + 1] = f[2 * j] * cs[j].y + f[2 * j + 1] * cs[j].x;
                     }
-                    store8(w.dst, p.out_t, w.to + w.item * 8, b);
+                    store8(to, OUT, 0, g);
                 } else {
-                    store8(w.dst, p.out_t, w.to + w.item * 8, a);
-                }
-            } else if (w.item * 8 < half) {
-                const uint32_t i0 = w.item * 8;
-                raw8_unpack(raw8_load(w.src, p.in_t, w.from + i0), p.in_t, a);
-                raw8_unpack(raw8_load(w.src, p.in_t, w.from + half + i0), p.in_t, b);
+                    raw8_unpack(b[INTER ? 0 : x], IN, g);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 cs = s_turn[i0 + j];
-                    const float x = a[j] * cs.x - b[j] * cs.y;
-                    b[j] = a[j] * cs.y + b[j] * cs.x;
-                    a[j] = x;
+                    for (int j = 0; j < 8; ++j) {
+                        const float c = f[j] * cs[j % PAIRS].x - g[j] * cs[j % PAIRS].y;
+                        g[j] = f[j] * cs[j % PAIRS].y + g[j] * cs[j % PAIRS].x;
+                        f[j] = c;
+                    }
+                    store8(to, OUT, 0, f);
+                    store8(to + half * SO, OUT, 0, g);
                 }
-                store8(w.dst, p.out_t, w.to + i0, a);
-                store8(w.dst, p.out_t, w.to + half + i0, b);
-            } else {
-                const uint32_t e = w.item * 8 + half; // behind the pairs
-                raw8_unpack(raw8_load(w.src, p.in_t, w.from + e), p.in_t, a);
-                store8(w.dst, p.out_t, w.to + e, a);
-            }
-        } else {
-            if (w.turns && w.item < half) {
-                const uint32_t ea = INTER ? 2 * w.item : w.item, eb = INTER ? ea + 1 : ea + half;
-                const float a = load1(w.src, p.in_t, w.from + ea), b = load1(w.src, p.in_t, w.from + eb);
-                const float2 cs = s_turn[w.item];
-                store1(w.dst, p.out_t, w.to + ea, a * cs.x - b * cs.y);
-                store1(w.dst, p.out_t, w.to + eb, a * cs.y + b * cs.x);
-            } else {
-                const uint32_t e = w.turns ? w.item + half : w.item;
-                store1(w.dst, p.out_t, w.to + e, load1(w.src, p.in_t, w.from + e));
             }
         }
     }
+    if (INTER) return;
+    // values: copied, eight at a time, all tokens of the batch
+    const uint32_t all = p.kv_heads * p.value_items;
+    for (uint32_t i = blockIdx.y * blockDim.x + threadIdx.x; i < all; i += gridDim.y * blockDim.x) {
+        const uint32_t h = i / p.value_items, e = i % p.value_items * 8;
+        const char *src =
+            static_cast<const char *>(p.v) + (static_cast<int64_t>(t0) * p.vt + h * p.vh + e) * SI;
+        char *dst = static_cast<char *>(p.vc) + (h * p.ch + e) * SO;
+#pragma unroll 4
+        for (uint32_t k = 0; k < n; ++k) {
+            const int64_t row = s_row[k];
+            if (row < 0) continue;
+            float f[8];
+            raw8_unpack(rope_load<IN>(src + k * p.vt * SI), IN, f);
+            store8(dst + row * SO, OUT, 0, f);
+        }
+    }
+}
+
+// Any widths, strides and alignments: an item is one pair or one value, consecutive
+// threads take consecutive ones.
+template <bool INTER> __global__ void __launch_bounds__(ROPE_THREADS) rope_append_any_kernel(const RopeParams p) {
+    __shared__ float2 s_turns[ROPE_TURNS];
+    __shared__ int64_t s_row[ROPE_BATCH];
+    const int64_t t = blockIdx.x;
+    rope_tokens(p, blockIdx.x, 1, s_turns, s_row);
+    const int64_t cache_row = s_row[0];
+    const uint32_t half = p.rot / 2, turned = p.heads + p.kv_heads, head_items = p.dim - half;
+    const uint32_t items = turned * head_items + p.kv_heads * p.dim;
+    for (uint32_t it = blockIdx.y * blockDim.x + threadIdx.x; it < items; it += gridDim.y * blockDim.x) {
+        const bool turns = it < turned * head_items;
+        const uint32_t rest = turns ? it : it - turned * head_items, width = turns ? head_items : p.dim;
+        uint32_t h = rest / width;
+        const uint32_t item = rest - h * width;
+        const void *src = p.q;
+        void *dst = p.q_out;
+        int64_t from = t * p.qt + h * p.qh, to = t * p.ot + h * p.oh;
+        if (!turns || h >= p.heads) {
+            if (cache_row < 0) continue;
+            if (turns) h -= p.heads;
+            src = turns ? p.k : p.v;
+            dst = turns ? p.kc : p.vc;
+            from = turns ? t * p.kt + h * p.kh : t * p.vt + h * p.vh;
+            to = cache_row + h * p.ch;
+        }
+        if (turns && item < half) {
+            const uint32_t ea = INTER ? 2 * item : item, eb = INTER ? ea + 1 : ea + half;
+            const float a = load1(src, p.in_t, from + ea), b = load1(src, p.in_t, from + eb);
+            const float2 cs = s_turns[item];
+            store1(dst, p.out_t, to + ea, a * cs.x - b * cs.y);
+            store1(dst, p.out_t, to + eb, a * cs.y + b * cs.x);
+        } else {
+            const uint32_t e = turns ? item + half : item;
+            store1(dst, p.out_t, to + e, load1(src, p.in_t, from + e));
+        }
+    }
+}
+
+template <bool INTER, int IN> void launch_rope_in(const RopeParams &p, dim3 grid, uint32_t threads, cudaStream_t s) {
+    if (p.out_t == FM_X_F32)
+        rope_append_kernel<INTER, IN, FM_X_F32><<<grid, threads, 0, s>>>(p);
+    else if (p.out_t == FM_X_BF16)
+        rope_append_kernel<INTER, IN, FM_X_BF16><<<grid, threads, 0, s>>>(p);
+    else
+        rope_append_kernel<INTER, IN, FM_X_F16><<<grid, threads, 0, s>>>(p);
+}
+
+template <bool INTER> void launch_rope(const RopeParams &p, dim3 grid, uint32_t threads, cudaStream_t s) {
+    if (p.in_t == FM_X_F32)
+        launch_rope_in<INTER, FM_X_F32>(p, grid, threads, s);
+    else if (p.in_t == FM_X_BF16)
+        launch_rope_in<INTER, FM_X_BF16>(p, grid, threads, s);
+    else
+        launch_rope_in<INTER, FM_X_F16>(p, grid, threads, s);
 }
 
 } // namespace
@@ -244,32 +332,40 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
               eights(a->v_head_stride) && eights(a->cache_page_stride) && eights(a->cache_head_stride) &&
               eights(a->cache_row_stride) && aligned16(a->k) && aligned16(a->v) && aligned16(a->k_cache) &&
               aligned16(a->v_cache);
-    const uint32_t unit = vec ? 8 : 1;
-    const uint32_t head_items = (a->head_dim - (a->interleaved && vec ? 0 : half)) / unit;
-    const uint32_t value_items = a->head_dim / unit;
-    const RopeParams p{a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache, a->positions, a->slots, a->inv_freq,
+    RopeParams p{a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache, a->positions, a->slots, a->inv_freq,
                        a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride,
                        a->v_head_stride, a->q_out_token_stride, a->q_out_head_stride, a->cache_page_stride,
                        a->cache_head_stride, a->cache_row_stride, a->in_dtype, a->out_dtype, a->heads, kvh,
                        a->head_dim, a->rot_dim, a->attention_factor, cached ? a->page_size : 1,
-                       cached ? static_cast<uint64_t>(a->n_pages) * a->page_size : 0, head_items, value_items,
-                       (a->heads + kvh) * head_items + kvh * value_items, status};
-    // few tokens: a token's items over several CTAs, until every SM has one
-    const uint32_t rounds = (p.items + ROPE_THREADS - 1) / ROPE_THREADS;
-    uint32_t parts = static_cast<uint32_t>(device_sm_count()) / a->tokens;
+                       cached ? static_cast<uint64_t>(a->n_pages) * a->page_size : 0,
+                       (a->head_dim - (a->interleaved ? 0 : half)) / 8, a->head_dim / 8, a->tokens, 1, status};
+    const uint32_t sms = static_cast<uint32_t>(device_sm_count());
+    // few tokens: a token's heads (or items) over several CTAs, until every SM has one
+    uint32_t threads = ROPE_THREADS, rounds;
+    if (vec) {
+        const uint32_t at_once = ROPE_THREADS / p.head_items, all = a->heads + kvh * (a->interleaved ? 2 : 1);
+        rounds = (all + at_once - 1) / at_once;
+        if (rounds == 1) threads = (all * p.head_items + 31) & ~31u;
+    } else {
+        const uint64_t items = static_cast<uint64_t>(a->heads + kvh) * (a->head_dim - half) + kvh * a->head_dim;
+        rounds = static_cast<uint32_t>((items + ROPE_THREADS - 1) / ROPE_THREADS);
+    }
+    uint32_t parts = sms / a->tokens;
     parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
-    const uint32_t each = (rounds + parts - 1) / parts;
-    uint32_t threads = (p.items + parts * each - 1) / (parts * each);
-    threads = (threads + 31) & ~31u;
-    const dim3 grid(a->tokens, parts);
+    if (vec && a->tokens >= sms * 8) {
+        // many: as many to a CTA as its threads have cosines to work out
+        p.batch = half ? ROPE_THREADS / half : ROPE_BATCH;
+        p.batch = p.batch < 1 ? 1 : p.batch > ROPE_BATCH ? ROPE_BATCH : p.batch;
+    }
+    const dim3 grid((a->tokens + p.batch - 1) / p.batch, parts);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (vec && a->interleaved)
-        rope_append_kernel<true, true><<<grid, threads, 0, s>>>(p);
+        launch_rope<true>(p, grid, threads, s);
     else if (vec)
-        rope_append_kernel<true, false><<<grid, threads, 0, s>>>(p);
+        launch_rope<false>(p, grid, threads, s);
     else if (a->interleaved)
-        rope_append_kernel<false, true><<<grid, threads, 0, s>>>(p);
+        rope_append_any_kernel<true><<<grid, threads, 0, s>>>(p);
     else
-        rope_append_kernel<false, false><<<grid, threads, 0, s>>>(p);
+        rope_append_any_kernel<false><<<grid, threads, 0, s>>>(p);
     return check_launch("rope_append_kernel");
 }

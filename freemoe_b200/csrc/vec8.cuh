@@ -32,7 +32,7 @@ __device__ __forceinline__ Raw8 raw8_load(const void *p, int32_t dtype, uint64_t
 }
 
 __device__ __forceinline__ void raw8_unpack(const Raw8 &r, int32_t dtype, float (&v)[8]) {
-    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w}; // (b: f32 only)
     if (dtype == FM_X_F32) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
