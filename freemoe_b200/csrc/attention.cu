@@ -128,77 +128,44 @@ int check_attention(const fmcuda_paged_attention_args *a) {
     return FM_STATUS_OK;
 }
 
-// A launch that may begin while the kernel before it on the stream ends (the kernel itself
-// waits, griddepcontrol.wait, before it reads what that one wrote).
-template <typename P>
-int launch_after(void (*kernel)(P), dim3 grid, uint32_t threads, cudaStream_t s, const P &p, const char *what) {
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
+// A kernel and its launch.  `early`: it may begin while the kernel before it on the stream
+// still runs (and waits itself, griddepcontrol.wait, where it has to).
+struct Launch {
+    dim3 grid;
+    uint32_t threads, smem;
+    bool early;
+    uint32_t cluster; // CTAs a cluster, 1: none
+};
+template <typename... K, typename... A>
+int launch(const char *what, void (*kernel)(K...), const Launch &l, cudaStream_t s, const A &...args) {
+    if (l.smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(l.smem));
+        if (e != cudaSuccess) return cuda_status(e, what);
+    }
+    cudaLaunchAttribute attrs[2]{};
     cudaLaunchConfig_t config{};
-    config.gridDim = grid;
-    config.blockDim = dim3(threads);
+    config.gridDim = l.grid;
+    config.blockDim = dim3(l.threads);
+    config.dynamicSmemBytes = l.smem;
     config.stream = s;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
+    config.attrs = attrs;
+    if (l.early) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (l.cluster > 1) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs].val.clusterDim.x = l.cluster;
+        attrs[config.numAttrs].val.clusterDim.y = attrs[config.numAttrs].val.clusterDim.z = 1;
+        ++config.numAttrs;
+    }
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
     if (err != cudaSuccess) {
         (void)cudaGetLastError();
         return cuda_status(err, what);
     }
     return FM_STATUS_OK;
-}
-
-template <int DP, bool BF16>
-int launch_cluster(const AttnParams &p, const AttnPlan &n, cudaStream_t s) {
-    static bool ready[64] = {};
-    auto kfn = attn_cluster_kernel<DP, BF16>;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, ARows<DP>::SMEM);
-        if (e != cudaSuccess) return cuda_status(e, "attention shared memory");
-        if (dev >= 0 && dev < 64) ready[dev] = true;
-    }
-    cudaLaunchAttribute size{};
-    size.id = cudaLaunchAttributeClusterDimension;
-    size.val.clusterDim.x = n.cluster;
-    size.val.clusterDim.y = size.val.clusterDim.z = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(p.seqs * p.kv_heads * n.tiles * n.cluster);
-    config.blockDim = dim3(AR_THREADS);
-    config.dynamicSmemBytes = ARows<DP>::SMEM;
-    config.stream = s;
-    config.attrs = &size;
-    config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, kfn, p, n.tiles);
-    if (err != cudaSuccess) {
-        (void)cudaGetLastError();
-        return cuda_status(err, "attn_cluster_kernel");
-    }
-    return FM_STATUS_OK;
-}
-
-template <int DP, bool BF16> int launch_rows(const AttnParams &p, uint32_t rows, cudaStream_t s) {
-    static bool ready[64] = {};
-    auto kfn = attn_rows_kernel<DP, BF16>;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, ARows<DP>::SMEM);
-        if (e != cudaSuccess) return cuda_status(e, "attention shared memory");
-        if (dev >= 0 && dev < 64) ready[dev] = true;
-    }
-    kfn<<<p.workers / AR_WARPS, AR_THREADS, ARows<DP>::SMEM, s>>>(p);
-    int rc = check_launch("attn_rows_kernel");
-    if (rc) return rc;
-    // few units are cut into many fragments each
-    const dim3 grid(p.seqs * p.kv_heads, rows);
-    if (p.seqs * p.kv_heads * 16 <= p.workers)
-        return launch_after(attn_combine_kernel<DP, BF16, 16>, grid, 16 * 32, s, p, "attn_combine_kernel");
-    return launch_after(attn_combine_kernel<DP, BF16, 4>, grid, 4 * 32, s, p, "attn_combine_kernel");
 }
 
 // The cache as boxes of 64 values x box_rows rows of one head of one page, the
@@ -239,49 +206,45 @@ int make_cache_map(CUtensorMap *map, const fmcuda_paged_attention_args &a, const
 }
 
 template <int DP, bool BF16>
-int launch_prompt(const fmcuda_paged_attention_args &a, const AttnPlan &n, const AttnParams &ap, uint8_t *ws,
-                  cudaStream_t s) {
-    using L = APrompt<DP>;
-    static bool ready[64] = {};
-    auto kfn = attn_prompt_kernel<DP, BF16>;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-        if (e != cudaSuccess) return cuda_status(e, "attention shared memory");
-        if (dev >= 0 && dev < 64) ready[dev] = true;
-    }
-    APParams p{};
-    p.a = ap;
-    p.box_rows = a.page_size & (~a.page_size + 1u); // its lowest set bit
-    if (p.box_rows > AP_KEYS) p.box_rows = AP_KEYS;
-    p.heads_first = a.cache_head_stride < a.cache_row_stride;
-    p.wide = a.head_dim % 16 == 0 && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0 &&
-             reinterpret_cast<uintptr_t>(a.out) % 32 == 0;
-    p.deal = n.deal;
-    p.max_pairs = n.pairs;
-    p.part = reinterpret_cast<float *>(ws + n.ppart);
-    p.part_ml = reinterpret_cast<float2 *>(ws + n.ppart_ml);
-    p.tail = reinterpret_cast<int4 *>(ws + n.tail);
-    CUtensorMap map_k, map_v;
-    int rc = make_cache_map(&map_k, a, a.k_cache, p.box_rows, p.heads_first);
-    if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, p.box_rows, p.heads_first);
-    if (rc) return rc;
-    kfn<<<n.ctas, AP_THREADS, L::SMEM, s>>>(map_k, map_v, p);
-    rc = check_launch("attn_prompt_kernel");
-    if (rc || !n.deal) return rc;
-    return launch_after(attn_join_kernel<DP, BF16>, dim3(n.ctas, AJ_SLICES), 256, s, p, "attn_join_kernel");
-}
-
-template <int DP, bool BF16>
 int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, const AttnParams &p, uint8_t *ws,
                      cudaStream_t s) {
     int rc = FM_STATUS_OK;
-    if (n.prompt) rc = launch_prompt<DP, BF16>(a, n, p, ws, s);
-    if (rc || !n.rows) return rc;
-    if (n.cluster) return launch_cluster<DP, BF16>(p, n, s);
-    const uint64_t rows = static_cast<uint64_t>(a.max_q_len) * n.group;
-    return launch_rows<DP, BF16>(p, rows < ROW_LIMIT ? static_cast<uint32_t>(rows) : ROW_LIMIT, s);
+    APParams pp{};
+    if (n.prompt) {
+        pp.a = p;
+        pp.box_rows = a.page_size & (~a.page_size + 1u); // its lowest set bit
+        if (pp.box_rows > AP_KEYS) pp.box_rows = AP_KEYS;
+        pp.heads_first = a.cache_head_stride < a.cache_row_stride;
+        pp.wide = a.head_dim % 16 == 0 && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(a.out) % 32 == 0;
+        pp.deal = n.deal;
+        pp.max_pairs = n.pairs;
+        pp.part = reinterpret_cast<float *>(ws + n.ppart);
+        pp.part_ml = reinterpret_cast<float2 *>(ws + n.ppart_ml);
+        pp.tail = reinterpret_cast<int4 *>(ws + n.tail);
+        CUtensorMap map_k, map_v;
+        rc = make_cache_map(&map_k, a, a.k_cache, pp.box_rows, pp.heads_first);
+        if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, pp.box_rows, pp.heads_first);
+        if (!rc)
+            rc = launch("attn_prompt_kernel", attn_prompt_kernel<DP, BF16>,
+                        {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, false, 1}, s, map_k, map_v, pp);
+    }
+    if (!rc && n.cluster)
+        rc = launch("attn_cluster_kernel", attn_cluster_kernel<DP, BF16>,
+                    {dim3(p.seqs * p.kv_heads * n.tiles * n.cluster), AR_THREADS, ARows<DP>::SMEM, n.prompt, n.cluster},
+                    s, p, n.tiles);
+    else if (!rc && n.rows)
+        rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16>,
+                    {dim3(p.workers / AR_WARPS), AR_THREADS, ARows<DP>::SMEM, n.prompt, 1}, s, p);
+    if (!rc && n.prompt && n.deal)
+        rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, true, 1}, s, pp);
+    if (rc || !n.rows || n.cluster) return rc;
+    const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group;
+    const dim3 grid(p.seqs * p.kv_heads, most < ROW_LIMIT ? static_cast<uint32_t>(most) : ROW_LIMIT);
+    // few units are cut into many fragments each
+    if (static_cast<uint64_t>(p.seqs) * p.kv_heads * 16 <= p.workers)
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 16>, {grid, 16 * 32, 0, true, 1}, s, p);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4>, {grid, 4 * 32, 0, true, 1}, s, p);
 }
 
 } // namespace

@@ -342,6 +342,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     volatile uint32_t *abort_flag = misc + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
+    // what follows on the stream may come to the SMs that have nothing to do here; it waits
+    // for the end of this grid before it reads from it, or ends itself
+    asm volatile("griddepcontrol.launch_dependents;\n");
+
     // ---- this CTA's share -------------------------------------------------------------
     // where blocks are dealt out: the sequences that have pairs and their first ones, and
     // the cost before each pair, in the place of the keys
@@ -470,8 +474,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
-    // the join may come on the SMs that have ended; it waits for all of this grid
-    if (pp.deal) asm volatile("griddepcontrol.launch_dependents;\n");
 
     // Readers of segments: the k-th one, or false at the end.
     auto segment = [&](uint32_t k) -> const APShared * {
@@ -879,6 +881,7 @@ constexpr uint32_t AJ_SLICES = 16;
 template <int DP, bool BF16> __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ APParams pp) {
     constexpr int V = DP / 32;
     const AttnParams &p = pp.a;
+    asm volatile("griddepcontrol.launch_dependents;\n");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int4 tail = pp.tail[blockIdx.x];
     if (tail.x < 0) return;

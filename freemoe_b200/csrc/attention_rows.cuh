@@ -75,6 +75,14 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The kernels here begin beside a prompt kernel that the same call launched before them,
+// on the SMs that it leaves free: they share nothing with it.  But the grid does not end
+// before it, so that what follows on the stream finds both done: its first CTA waits (were
+// all to wait, the CTAs behind them would find no SM until then).
+__device__ __forceinline__ void after_prompt_kernel() {
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+
 // A place in the laid-out work.
 struct ARCursor {
     uint32_t b, tile, step; // tile: key head * row tiles + row tile
@@ -334,7 +342,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     asm volatile("griddepcontrol.launch_dependents;\n");
     const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
     const uint64_t begin = worker * per;
-    if (begin >= total) return;
+    if (begin >= total) {
+        after_prompt_kernel();
+        return;
+    }
     const uint32_t count = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
 
     ARCursor c;
@@ -417,6 +428,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         if (i + 1 < count) ar_advance(p, c);
     }
     cp_async_wait<0>();
+    after_prompt_kernel();
 }
 
 // ---- few units of short sequences: a cluster each ----------------------------------
@@ -460,7 +472,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
     const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
     const ARShape sh = ar_shape(p, s);
-    if (rt >= sh.tiles) return; // the whole cluster
+    if (rt >= sh.tiles) { // the whole cluster
+        after_prompt_kernel();
+        return;
+    }
 
     const uint32_t part = rank * AR_WARPS + warp, parts = ranks * AR_WARPS;
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * part / parts);
@@ -548,6 +563,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
             p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
     cluster_sync(); // nobody leaves while its shared memory is read
+    after_prompt_kernel();
 }
 
 // Joins the fragments of the units that were cut: a CTA of W warps a unit and row.
