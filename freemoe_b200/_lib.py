@@ -6,7 +6,6 @@ shared library is missing, build it with ``python freemoe_b200/build.py``.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from pathlib import Path
 
 import os
@@ -378,26 +377,6 @@ def load() -> C.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
-
-
-_PACK = {C.c_void_p: "P", C.c_int64: "q", C.c_uint64: "Q", C.c_int32: "i", C.c_uint32: "I", C.c_double: "d",
-         C.c_float: "f"}
-
-
-def packer(args: type[C.Structure]) -> struct.Struct:
-    """The argument struct's layout for ``struct.pack``: a call that fills it anew
-    each time pays a fifth of what filling the ctypes structure costs."""
-    s = struct.Struct("@" + "".join(_PACK[t] for _, t in args._fields_) + "0P")
-    assert s.size == C.sizeof(args)
-    return s
-
-
-def packed_entry(name: str, *argtypes):
-    """Another handle of an entry point, taking its first argument as packed bytes."""
-    fn = load()[name]
-    fn.restype = C.c_int
-    fn.argtypes = [C.c_char_p, *argtypes]
-    return fn
 
 
 def check(rc: int) -> None:

@@ -1,4 +1,5 @@
-"""Build recipe for the sm_100a shared library (``libfreemoe_b200.so``).
+"""Build recipe for the sm_100a shared library (``libfreemoe_b200.so``) and the
+entry points for torch tensors beside it (``_torch_calls.so``).
 
 The library is built in-tree with nvcc so that the ``.so`` travels with the
 source tree; nothing is JIT-compiled or installed into site-packages.
@@ -40,8 +41,34 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles ``csrc/torch_calls.cpp``, the entry points for torch tensors, against the
+    installed torch (host code only: it calls the library through the addresses it is given)."""
+    src, target = CSRC / "torch_calls.cpp", PKG / "_torch_calls.so"
+    if not force and not _stale(target, [src, Path(__file__), *INCLUDE.glob("*.h")]):
+        return target
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include", str(INCLUDE)]
+    tmp = target.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_torch_calls",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in include), str(src),
+           f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib}",
+           "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, target)
+    return target
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     """Compiles every ``csrc/*.cu`` for sm_100a into ``libfreemoe_b200.so``."""
+    build_torch_calls(force, verbose)
     deps = sources() + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h")) + [Path(__file__)]
     if not force and not _stale(LIB, deps):
         return LIB

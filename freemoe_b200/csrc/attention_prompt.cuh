@@ -13,12 +13,13 @@
 // keys and values page by page (TMA boxes of as many rows as divide a page);
 // warp 9 issues Q K^T and warp 10 P V; warp 11 copies Q.  P has a place of its
 // own, so that the next S is computed while the softmax still works on this
-// block; heads of 128 then leave room for a single S, which the tiles use in
-// turn: a softmax moves it to registers at once, and the turns keep the tiles
-// half a block apart, one in its softmax while the other has the tensor cores
-// (left to themselves they fall into step).  A softmax thread rescales O in
-// place, and only when the maximum has grown by more than 2^8, since any
-// reference exponent in that range gives the same P / sum.
+// block.  There is one S, which the tiles use in turn: a softmax moves it to
+// registers at once, and the turns keep the tiles apart, one in its exponentials
+// while the other waits (left to themselves they fall into step; heads of 64
+// have room for an S each, but that was 5% slower, and for heads of 128 there is
+// none).  A softmax thread rescales O in place, and only when the maximum has
+// grown by more than 2^8, since any reference exponent in that range gives the
+// same P / sum.
 //
 // A tile's keys end at its last row's position; only blocks that some row sees
 // in part are masked.  In the first and last block V's rows outside the
@@ -49,12 +50,10 @@ template <int DP> struct APrompt {
     static constexpr uint32_t HALF = AP_KEYS * 128;        // 128 rows of 64 values
     static constexpr uint32_t BLOCK = HALVES * HALF;       // a Q tile, a K block, a V block
     static constexpr uint32_t STAGES = DP == 128 ? 5 : 8;
-    // Tensor memory, 512 columns: P (64) and O (DP) of each tile, and S (128): one of each
-    // tile where there is room, else one that the tiles use in turn.
-    static constexpr bool ONE_S = DP == 128;
+    // Tensor memory, 512 columns: O (DP) and P (64) of each tile, and one S (128).
     __host__ __device__ static constexpr uint32_t o_col(uint32_t t) { return t * DP; }
     __host__ __device__ static constexpr uint32_t p_col(uint32_t t) { return 2 * DP + t * 64; }
-    __host__ __device__ static constexpr uint32_t s_col(uint32_t t) { return 2 * DP + 128 + (ONE_S ? 0 : t * 128); }
+    static constexpr uint32_t S_COL = 2 * DP + 128;
     static constexpr uint32_t OFF_KV = 2 * BLOCK;
     static constexpr uint32_t OFF_BAR = OFF_KV + STAGES * BLOCK;
     static constexpr uint32_t OFF_SEG = OFF_BAR + 512;
@@ -146,9 +145,15 @@ __device__ __forceinline__ void store_32b(void *dst, const uint32_t *v) {
                  : "memory");
 }
 
+// Largest of three or two; NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
@@ -332,13 +337,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     extern __shared__ uint8_t ap_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ap_smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
-    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 6, *p_full = bars + 8;
-    uint64_t *o_done = bars + 10, *drain = bars + 12, *edge = bars + 14, *seg_full = bars + 15;
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_done = bars + 8;
+    uint64_t *drain = bars + 10, *s_free = bars + 12, *edge = bars + 13, *seg_full = bars + 14;
     uint64_t *seg_empty = seg_full + AP_SEG_SLOTS, *kv_full = seg_empty + AP_SEG_SLOTS, *kv_empty = kv_full + L::STAGES;
     // TMEM base, abort, pairs, then the CTA's first item: sequence, pair, head, cost before
     uint32_t *misc = reinterpret_cast<uint32_t *>(kv_empty + L::STAGES);
     APShared *segs = reinterpret_cast<APShared *>(smem + L::OFF_SEG);
-    static_assert((15 + 2 * AP_SEG_SLOTS + 2 * L::STAGES) * 8 + 32 <= 512, "barriers outgrow their place");
+    static_assert((14 + 2 * AP_SEG_SLOTS + 2 * L::STAGES) * 8 + 32 <= 512, "barriers outgrow their place");
     volatile uint32_t *abort_flag = misc + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -387,7 +392,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 128);
             mbar_init(&p_full[i], 128);
             mbar_init(&o_done[i], 1);
             mbar_init(&drain[i], 1);
@@ -396,6 +400,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_init(&seg_full[i], 1);
             mbar_init(&seg_empty[i], AP_SEG_READERS);
         }
+        mbar_init(s_free, 128);
         mbar_init(edge, 1);
         for (uint32_t i = 0; i < L::STAGES; ++i) {
             mbar_init(&kv_full[i], 1);
@@ -656,9 +661,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                         if (!ok || j < tb[t] || j >= te[t]) continue;
                         if (scores) {
                             if (j == tb[t]) ok = ap_wait(&q_full[t], q[t]++ & 1u, abort_flag, p.status);
-                            const uint32_t used = L::ONE_S ? s_used : n[t];
-                            if (ok && used)
-                                ok = ap_wait(&s_free[L::ONE_S ? 0 : t], (used - 1) & 1u, abort_flag, p.status);
+                            if (ok && s_used) ok = ap_wait(s_free, (s_used - 1) & 1u, abort_flag, p.status);
                             if (!ok) break;
                             tc_fence_after();
                             if (lane == 0) {
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
                                 for (uint32_t i = 0; i < DP / 16; ++i) {
                                     const uint32_t off = (i >> 2) * L::HALF + (i & 3u) * 32;
-                                    mma_f16_ss(tmem + L::s_col(t), smem_desc_sw128(q_addr + off),
+                                    mma_f16_ss(tmem + L::S_COL, smem_desc_sw128(q_addr + off),
                                                smem_desc_sw128(kv + off), id_s, i != 0);
                                 }
                                 tc_commit(&s_full[t]);
@@ -702,7 +705,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         // ---- softmax: one thread a row ------------------------------------------------
         const uint32_t t = warp >> 2, r = threadIdx.x & 127u;
         const uint32_t lane_addr = ((warp & 3u) * 32u) << 16;
-        const uint32_t s_tmem = tmem + (t ? L::s_col(1) : L::s_col(0)) + lane_addr;
+        const uint32_t s_tmem = tmem + L::S_COL + lane_addr;
         const uint32_t p_tmem = tmem + (t ? L::p_col(1) : L::p_col(0)) + lane_addr;
         const uint32_t o_tmem = tmem + (t ? L::o_col(1) : L::o_col(0)) + lane_addr;
         const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
@@ -729,7 +732,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const uint32_t lse_at = static_cast<uint32_t>(token * p.heads) + qhead;
             release(k);
             float m = -INFINITY; // in log2
-            uint64_t sum2 = 0;   // two f32 sums
+            uint64_t sums[4] = {0, 0, 0, 0}; // two f32 sums each
             for (uint32_t n = 0; n < blocks; ++n, ++count) {
                 ok = ap_wait(&s_full[t], count & 1u, abort_flag, p.status);
                 if (!ok) break;
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) pin(x[c]);
                 tc_fence_before();
-                mbar_arrive(&s_free[L::ONE_S ? 0 : t]);
+                mbar_arrive(s_free);
                 const uint32_t key0 = (tb + n) * AP_KEYS;
                 if (key0 + AP_KEYS > whole_hi || key0 < whole_lo) {
                     // the row sees keys [gone, seen) of the block; most 32s are all or nothing to a warp
@@ -762,20 +765,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
                     for (int i = 1; i < 31; i += 2)
                         top[c] = max3(top[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-                    top[c] = fmaxf(top[c], __uint_as_float(x[c][31]));
+                    top[c] = max2(top[c], __uint_as_float(x[c][31]));
                 }
-                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-                if (__any_sync(0xFFFFFFFFu, high > m + 8.0f)) {
-                    const float to = fmaxf(m, high);
+                const float high = max2(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
+                if (__any_sync(0xFFFFFFFFu, !(high <= m + 8.0f))) {
+                    const float to = max2(m, high);
                     const float f = m == -INFINITY ? 0.0f : exp2_approx(m - to);
                     m = to;
                     if (n) { // the last block's product has written O
                         ok = ap_wait(&o_done[t], (count - 1) & 1u, abort_flag, p.status);
                         if (!ok) break;
                         tc_fence_after();
-                        float a, c2;
-                        unpack_f32x2(sum2, a, c2);
-                        sum2 = pack_f32x2(a * f, c2 * f);
+                        const uint64_t f2 = pack_f32x2(f, f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sums[i] = fma_f32x2(sums[i], f2, 0);
 #pragma unroll
                         for (int c = 0; c < DP / 16; ++c) {
                             uint32_t o[16];
@@ -788,30 +791,27 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : -m;
+                const float base = m == -INFINITY ? 0.0f : m - m - m; // NaN where m is or is infinite
                 const uint64_t base2 = pack_f32x2(base, base);
+                // all of the row's weights before the first store: the special-function unit runs on
+                uint32_t w[2][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float a, c2;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])),
-                                               scale2, base2),
-                                     a, c2);
-                        a = exp2_approx(a);
-                        c2 = exp2_approx(c2);
-                        sum2 = add_f32x2(sum2, pack_f32x2(a, c2));
-                        w[i] = pack_pair<BF16>(a, c2);
-                    }
-                    if (c == 0 && n) { // the last block's product has read P
-                        ok = ap_wait(&o_done[t], (count - 1) & 1u, abort_flag, p.status);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    tmem_st16(p_tmem + c * 16, w);
+                for (int i = 0; i < 64; ++i) {
+                    const uint32_t *e = &x[i >> 4][(i & 15) * 2];
+                    float a, c2;
+                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(e[0]), __uint_as_float(e[1])), scale2, base2), a, c2);
+                    a = exp2_approx(a);
+                    c2 = exp2_approx(c2);
+                    sums[i & 3] = add_f32x2(sums[i & 3], pack_f32x2(a, c2));
+                    w[i >> 5][i & 31] = pack_pair<BF16>(a, c2);
+                }
+                if (n) { // the last block's product has read P
+                    ok = ap_wait(&o_done[t], (count - 1) & 1u, abort_flag, p.status);
+                    tc_fence_after();
                 }
                 if (!ok) break;
+                tmem_st32(p_tmem, w[0]);
+                tmem_st32(p_tmem + 32, w[1]);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (!ok || __ballot_sync(0xFFFFFFFFu, valid) == 0) continue;
             tc_fence_after();
             float a, c2;
-            unpack_f32x2(sum2, a, c2);
+            unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), a, c2);
             const float sum = blocks ? a + c2 : 0.0f;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             uint16_t *out = static_cast<uint16_t *>(p.out) + out_at;

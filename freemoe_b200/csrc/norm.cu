@@ -38,24 +38,33 @@ template <int NT> __device__ __forceinline__ float team_sum(float v, float *s_pa
 }
 
 // A team of NT threads (a warp, or the CTA) takes a row; thread c of the team
-// holds chunks c, c + NT, ... of 8 values.  VEC: a chunk is 8 consecutive
+// holds chunks c, c + NT, ... of 8 values.  VEC 8: a chunk is 8 consecutive
 // values (16-byte accesses).  Otherwise the chunks of a group of 128 values are
-// dealt out value by value over 16 lanes, so that the accesses of the lanes
-// still lie side by side.  Either way 16 neighbouring lanes hold a scale's group.
-template <bool VEC> __device__ __forceinline__ uint32_t value_at(uint32_t c, int j) {
-    return VEC ? c * 8 + j : (c >> 4) * 128 + j * 16 + (c & 15u);
+// dealt out by VEC values (2, or 1) over 16 lanes, so that the accesses of the
+// lanes still lie side by side.  Always 16 neighbouring lanes hold a scale's group.
+template <int VEC> __device__ __forceinline__ uint32_t value_at(uint32_t c, int j) {
+    return VEC == 8 ? c * 8 + j : (c >> 4) * 128 + j / VEC * (16 * VEC) + (c & 15u) * VEC + j % VEC;
 }
 
-template <bool VEC>
+template <int VEC>
 __device__ __forceinline__ void load_chunk(const void *p, int32_t t, int64_t row, uint32_t c, uint32_t d,
                                            float (&v)[8]) {
-    if constexpr (VEC) {
+    if constexpr (VEC == 8) {
         if (c * 8 < d) {
             raw8_unpack(raw8_load(p, t, row + c * 8), t, v);
             return;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else if constexpr (VEC == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t e = value_at<VEC>(c, j);
+            float2 f = make_float2(0.0f, 0.0f);
+            if (e < d) f = load2(p, t, row + e);
+            v[j] = f.x;
+            v[j + 1] = f.y;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -65,11 +74,17 @@ __device__ __forceinline__ void load_chunk(const void *p, int32_t t, int64_t row
     }
 }
 
-template <bool VEC>
+template <int VEC>
 __device__ __forceinline__ void store_chunk(void *p, int32_t t, int64_t row, uint32_t c, uint32_t d,
                                             const float (&v)[8]) {
-    if constexpr (VEC) {
+    if constexpr (VEC == 8) {
         if (c * 8 < d) store8(p, t, row + c * 8, v);
+    } else if constexpr (VEC == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t e = value_at<VEC>(c, j);
+            if (e < d) store2(p, t, row + e, v[j], v[j + 1]);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -80,7 +95,7 @@ __device__ __forceinline__ void store_chunk(void *p, int32_t t, int64_t row, uin
 }
 
 // The 16 lanes of a group call this together; lanes past the row's end hold zeros.
-template <bool VEC>
+template <int VEC>
 __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, uint32_t c, const float (&v)[8]) {
     float top = 0.0f;
 #pragma unroll
@@ -98,7 +113,7 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
     uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
     const uint32_t groups = (p.d + 127) / 128;
     if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;
-    if constexpr (VEC) {
+    if constexpr (VEC == 8) {
         if (c * 8 < p.d) {
             uint32_t w[2];
 #pragma unroll
@@ -119,8 +134,8 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
 // are on their way while this one is summed and written.  The weight waits in shared
 // memory, as f32 in the chunks' order.
 // WIDE: x or the residual is f32, whose eights take two accesses.
-template <bool VEC, bool WIDE, int ITER> struct NormRow {
-    uint4 x[ITER], r[ITER];                       // VEC
+template <int VEC, bool WIDE, int ITER> struct NormRow {
+    uint4 x[ITER], r[ITER];                       // VEC 8
     uint4 x2[WIDE ? ITER : 1], r2[WIDE ? ITER : 1];
     float h[ITER][8];                             // otherwise: already h
 
@@ -128,7 +143,7 @@ template <bool VEC, bool WIDE, int ITER> struct NormRow {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const uint32_t c = c0 + i * step;
-            if constexpr (VEC) {
+            if constexpr (VEC == 8) {
                 x[i] = r[i] = make_uint4(0, 0, 0, 0);
                 if (WIDE) x2[i] = r2[i] = make_uint4(0, 0, 0, 0);
                 if (c * 8 < p.d) {
@@ -149,10 +164,10 @@ template <bool VEC, bool WIDE, int ITER> struct NormRow {
                     }
                 }
             } else {
-                load_chunk<false>(p.x, p.xt, row * p.xs, c, p.d, h[i]);
+                load_chunk<VEC>(p.x, p.xt, row * p.xs, c, p.d, h[i]);
                 if (p.res) {
                     float v[8];
-                    load_chunk<false>(p.res, p.rt, row * p.rs, c, p.d, v);
+                    load_chunk<VEC>(p.res, p.rt, row * p.rs, c, p.d, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[i][j] += v[j];
                 }
@@ -162,7 +177,7 @@ template <bool VEC, bool WIDE, int ITER> struct NormRow {
     __device__ __forceinline__ void get(const NormParams &p, float (&out)[ITER][8]) const {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            if constexpr (VEC) {
+            if constexpr (VEC == 8) {
                 raw8_unpack(Raw8{x[i], x2[WIDE ? i : 0]}, p.xt, out[i]);
                 if (p.res) {
                     float v[8];
@@ -178,7 +193,7 @@ template <bool VEC, bool WIDE, int ITER> struct NormRow {
     }
 };
 
-template <bool VEC, bool WIDE, int NT, int ITER>
+template <int VEC, bool WIDE, int NT, int ITER>
 __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const NormParams p) {
     constexpr uint32_t THREADS = NT < 128 ? 128 : NT, TEAMS = THREADS / NT;
     extern __shared__ float4 s_w[]; // chunk c: s_w[2 c], s_w[2 c + 1]
@@ -228,7 +243,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const
 }
 
 // Rows longer than the registers of a CTA hold: read twice, the second time from L2.
-template <bool VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(const NormParams p) {
+template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(const NormParams p) {
     __shared__ float s_part[2][32];
     const uint32_t chunks = ((p.d + 127) / 128) * 16;
     uint32_t turn = 0;
@@ -271,7 +286,7 @@ template <bool VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ke
     }
 }
 
-template <bool VEC, bool WIDE, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
+template <int VEC, bool WIDE, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
     constexpr uint32_t threads = NT < 128 ? 128 : NT, teams = threads / NT, smem = NT * ITER * 32;
     auto kfn = add_rms_norm_kernel<VEC, WIDE, NT, ITER>;
     const uint32_t want = (p.tokens + teams - 1) / teams;
@@ -287,7 +302,7 @@ template <bool VEC, bool WIDE, int NT, int ITER> void launch_norm(const NormPara
     kfn<<<want < most ? want : most, threads, smem, s>>>(p);
 }
 
-template <bool VEC, bool WIDE> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+template <int VEC, bool WIDE> void dispatch_norm(const NormParams &p, cudaStream_t s) {
     if (p.d <= 256)
         launch_norm<VEC, WIDE, 32, 1>(p, s);
     else if (p.d <= 1024)
@@ -336,15 +351,22 @@ extern "C" int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *a, void *stream) 
     const NormParams p{a->x,        a->residual,        a->weight,   a->y,       a->residual_out,  a->scales,
                        a->x_stride, a->residual_stride, a->y_stride, a->x_dtype, a->residual_dtype, a->weight_dtype,
                        a->y_dtype,  a->tokens,          a->d_model,  a->epsilon};
-    const bool vec = d % 8 == 0 && a->x_stride % 8 == 0 && a->y_stride % 8 == 0 && a->residual_stride % 8 == 0 &&
-                     aligned16(a->x) && aligned16(a->residual) && aligned16(a->weight) && aligned16(a->y) &&
-                     aligned16(a->residual_out);
+    auto fits = [&](int64_t values, uint32_t bytes) {
+        auto at = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; };
+        return d % values == 0 && a->x_stride % values == 0 && a->y_stride % values == 0 &&
+               a->residual_stride % values == 0 && at(a->x) && at(a->residual) && at(a->weight) && at(a->y) &&
+               at(a->residual_out);
+    };
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!vec)
-        dispatch_norm<false, true>(p, s);
-    else if (p.xt == FM_X_F32 || (p.res && p.rt == FM_X_F32))
-        dispatch_norm<true, true>(p, s);
-    else
-        dispatch_norm<true, false>(p, s);
+    if (fits(8, 16)) {
+        if (p.xt == FM_X_F32 || (p.res && p.rt == FM_X_F32))
+            dispatch_norm<8, true>(p, s);
+        else
+            dispatch_norm<8, false>(p, s);
+    } else if (fits(2, 8)) {
+        dispatch_norm<2, true>(p, s);
+    } else {
+        dispatch_norm<1, true>(p, s);
+    }
     return check_launch("add_rms_norm_kernel");
 }

@@ -100,8 +100,9 @@ __global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kerne
     const uint32_t step = at_once * gridDim.y, turned = p.heads + p.kv_heads;
     const uint32_t heads = lane_head >= at_once ? 0 : INTER ? turned + p.kv_heads : turned;
     const float2 *my_turns = s_turns + (INTER ? item * 4 : ea);
-    rope_tokens(p, t0, n, s_turns, s_row);
-    for (uint32_t h1 = blockIdx.y * at_once + lane_head; h1 < heads; h1 += U * step) {
+    bool ready = false;
+    uint32_t h1 = blockIdx.y * at_once + lane_head;
+    do {
         const char *src[U];
         char *dst[U];
         int64_t move[U];
@@ -125,20 +126,24 @@ __global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kerne
                 move[x] = (key ? p.kt : p.vt) * SI;
             }
         }
-#pragma unroll 1
-        for (uint32_t k = 0; k < n; ++k) {
-            const int64_t row = s_row[k];
-            Raw8 a[U], b[INTER ? 1 : U];
-            bool live[U];
+        Raw8 a[U], b[INTER ? 1 : U];
+        auto load = [&] {
 #pragma unroll
             for (int x = 0; x < U; ++x) {
-                live[x] = here[x] && (!cached[x] || row >= 0);
-                if (live[x]) {
+                if (here[x]) {
                     a[x] = rope_load<IN>(src[x]);
                     if (!INTER && turns[x]) b[x] = rope_load<IN>(src[x] + half * SI);
                 }
                 src[x] += move[x];
             }
+        };
+        load();
+        if (!ready) rope_tokens(p, t0, n, s_turns, s_row); // every thread's first round: its barrier
+        ready = true;
+#pragma unroll 1
+        for (uint32_t k = 0; k < n; ++k) {
+            if (k) load();
+            const int64_t row = s_row[k];
             float2 cs[PAIRS];
             if (pair) {
 #pragma unroll
@@ -146,7 +151,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kerne
             }
 #pragma unroll
             for (int x = 0; x < U; ++x) {
-                if (!live[x]) continue;
+                if (!here[x] || (cached[x] && row < 0)) continue;
                 char *to = dst[x] + (cached[x] ? row : k * p.ot) * SO;
                 float f[8], g[8];
                 raw8_unpack(a[x], IN, f);
@@ -172,7 +177,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kerne
                 }
             }
         }
-    }
+        h1 += U * step;
+    } while (h1 < heads);
     if (INTER) return;
     // values: copied, eight at a time, all tokens of the batch
     const uint32_t all = p.kv_heads * p.value_items;

@@ -88,6 +88,21 @@ __device__ __forceinline__ void store1(void *p, int32_t dtype, uint64_t at, floa
         static_cast<__half *>(p)[at] = __float2half_rn(v);
 }
 
+// Two values, where their pairs are aligned.
+__device__ __forceinline__ float2 load2(const void *p, int32_t dtype, uint64_t at) {
+    if (dtype == FM_X_F32) return *reinterpret_cast<const float2 *>(static_cast<const float *>(p) + at);
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p) + at);
+    if (dtype == FM_X_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+
+__device__ __forceinline__ void store2(void *p, int32_t dtype, uint64_t at, float lo, float hi) {
+    if (dtype == FM_X_F32)
+        *reinterpret_cast<float2 *>(static_cast<float *>(p) + at) = make_float2(lo, hi);
+    else
+        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p) + at) = pack2(lo, hi, dtype);
+}
+
 // Two e4m3 codes, `lo` in the low byte; round to nearest even, largest 448, NaN kept.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
