@@ -25,20 +25,21 @@ struct NormParams {
     float eps;
 };
 
-template <int NT> __device__ __forceinline__ float team_sum(float v, float *s_part) {
+// The sum over a team: a warp, or (CTA) all warps of the CTA.
+template <bool CTA> __device__ __forceinline__ float team_sum(float v, float *s_part) {
     v = warp_sum(v);
-    if constexpr (NT > 32) {
+    if constexpr (CTA) {
         const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
         if (lane == 0) s_part[warp] = v;
         __syncthreads();
-        v = lane < NT / 32 ? s_part[lane] : 0.0f;
+        v = lane < blockDim.x / 32 ? s_part[lane] : 0.0f;
         v = warp_sum(v);
     }
     return v;
 }
 
-// A team of NT threads (a warp, or the CTA) takes a row; thread c of the team
-// holds chunks c, c + NT, ... of 8 values.  VEC 8: a chunk is 8 consecutive
+// A team (a warp, or the CTA) of n threads takes a row; its thread c
+// holds chunks c, c + n, ... of 8 values.  VEC 8: a chunk is 8 consecutive
 // values (16-byte accesses).  Otherwise the chunks of a group of 128 values are
 // dealt out by VEC values (2, or 1) over 16 lanes, so that the accesses of the
 // lanes still lie side by side.  Always 16 neighbouring lanes hold a scale's group.
@@ -193,18 +194,18 @@ template <int VEC, bool WIDE, int ITER> struct NormRow {
     }
 };
 
-template <int VEC, bool WIDE, int NT, int ITER>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const NormParams p) {
-    constexpr uint32_t THREADS = NT < 128 ? 128 : NT, TEAMS = THREADS / NT;
+template <int VEC, bool WIDE, bool CTA, int ITER, int MOST>
+__global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) {
+    const uint32_t nt = CTA ? blockDim.x : 32u, teams = CTA ? 1u : blockDim.x / 32;
     extern __shared__ float4 s_w[]; // chunk c: s_w[2 c], s_w[2 c + 1]
     __shared__ float s_part[2][32];
-    const uint32_t c0 = NT < 128 ? threadIdx.x % NT : threadIdx.x;
-    const uint32_t team = blockIdx.x * TEAMS + (NT < 128 ? threadIdx.x / NT : 0);
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * TEAMS;
+    const uint32_t c0 = CTA ? threadIdx.x : threadIdx.x % 32;
+    const uint32_t team = CTA ? blockIdx.x : blockIdx.x * teams + threadIdx.x / 32;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
     uint64_t row = team;
     NormRow<VEC, WIDE, ITER> next;
-    if (row < p.tokens) next.load(p, row, c0, NT);
-    for (uint32_t c = threadIdx.x; c < NT * ITER; c += THREADS) {
+    if (row < p.tokens) next.load(p, row, c0, nt);
+    for (uint32_t c = threadIdx.x; c < nt * ITER; c += blockDim.x) {
         float w[8];
         load_chunk<VEC>(p.w, p.wt, 0, c, p.d, w);
         s_w[2 * c] = make_float4(w[0], w[1], w[2], w[3]);
@@ -214,22 +215,22 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(const
     for (uint32_t turn = 0; row < p.tokens; row += step, turn ^= 1u) {
         float h[ITER][8];
         next.get(p, h);
-        if (row + step < p.tokens) next.load(p, row + step, c0, NT);
+        if (row + step < p.tokens) next.load(p, row + step, c0, nt);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
         // two buffers of partial sums: a thread that is ahead by a row writes the other one
-        sum = team_sum<NT>(sum, s_part[turn]);
+        sum = team_sum<CTA>(sum, s_part[turn]);
         const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
         if (p.res_out) {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) store_chunk<VEC>(p.res_out, p.rt, row * p.rs, c0 + i * NT, p.d, h[i]);
+            for (int i = 0; i < ITER; ++i) store_chunk<VEC>(p.res_out, p.rt, row * p.rs, c0 + i * nt, p.d, h[i]);
         }
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            const uint32_t c = c0 + i * NT;
+            const uint32_t c = c0 + i * nt;
             const float4 wa = s_w[2 * c], wb = s_w[2 * c + 1];
             const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
@@ -262,7 +263,7 @@ template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ker
             for (int j = 0; j < 8; ++j) part = fmaf(h[j], h[j], part);
             sum += part;
         }
-        sum = team_sum<1024>(sum, s_part[turn]);
+        sum = team_sum<true>(sum, s_part[turn]);
         const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
         // whole warps go round together: a scale's 16 lanes exchange inside
         for (uint32_t c0 = threadIdx.x & ~31u; c0 < chunks; c0 += 1024) {
@@ -286,35 +287,41 @@ template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ker
     }
 }
 
-template <int VEC, bool WIDE, int NT, int ITER> void launch_norm(const NormParams &p, cudaStream_t s) {
-    constexpr uint32_t threads = NT < 128 ? 128 : NT, teams = threads / NT, smem = NT * ITER * 32;
-    auto kfn = add_rms_norm_kernel<VEC, WIDE, NT, ITER>;
-    const uint32_t want = (p.tokens + teams - 1) / teams;
-    static int per_sm = 0; // CTAs that an SM holds: the same on every device of this library's architecture
-    if (!per_sm) {
-        cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <int VEC, bool WIDE, bool CTA, int ITER, int MOST>
+void launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
+    auto kfn = add_rms_norm_kernel<VEC, WIDE, CTA, ITER, MOST>;
+    const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
+    const uint32_t smem = (CTA ? threads : 32) * ITER * 32;
+    uint32_t grid = static_cast<uint32_t>(device_sm_count());
+    if (want > grid) { // as many CTAs as the GPU holds; otherwise one a row
+        int per_sm = 0;
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
             (void)cudaGetLastError();
             per_sm = 1;
         }
+        grid *= static_cast<uint32_t>(per_sm);
+    } else if (smem > 48 * 1024) {
+        cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     }
-    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * per_sm;
-    kfn<<<want < most ? want : most, threads, smem, s>>>(p);
+    kfn<<<want < grid ? want : grid, threads, smem, s>>>(p);
 }
 
+// Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
+// there are rows for half the threads of the GPU only (latency counts then).
 template <int VEC, bool WIDE> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+    const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
+    const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
     if (p.d <= 256)
-        launch_norm<VEC, WIDE, 32, 1>(p, s);
+        launch_norm<VEC, WIDE, false, 1, 128>(p, 128, s);
     else if (p.d <= 1024)
-        launch_norm<VEC, WIDE, 32, 4>(p, s);
-    else if (p.d <= 2048)
-        launch_norm<VEC, WIDE, 128, 2>(p, s);
-    else if (p.d <= 4096)
-        launch_norm<VEC, WIDE, 256, 2>(p, s);
-    else if (p.d <= 8192)
-        launch_norm<VEC, WIDE, 512, 2>(p, s);
-    else if (p.d <= 16384)
-        launch_norm<VEC, WIDE, 1024, 2>(p, s);
+        launch_norm<VEC, WIDE, false, 4, 128>(p, 128, s);
+    else if (few && one <= 1024)
+        launch_norm<VEC, WIDE, true, 1, 1024>(p, one, s);
+    else if (two <= 512)
+        launch_norm<VEC, WIDE, true, 2, 512>(p, two, s);
+    else if (two <= 1024)
+        launch_norm<VEC, WIDE, true, 2, 1024>(p, two, s);
     else {
         const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
         add_rms_norm_long_kernel<VEC><<<p.tokens < most ? p.tokens : most, 1024, 0, s>>>(p);

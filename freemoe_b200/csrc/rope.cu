@@ -87,7 +87,7 @@ template <int T> __device__ __forceinline__ Raw8 rope_load(const char *src) {
 // eights with its divisions, 44 (issue slots 65% busy); the cosines worked out by every
 // thread for itself, 64.  Bound by the loads under way: registers against warps.
 template <bool INTER, int IN, int OUT>
-__global__ void __launch_bounds__(ROPE_THREADS, INTER ? 4 : 4) rope_append_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4) rope_append_kernel(const RopeParams p) {
     constexpr int PAIRS = INTER ? 4 : 8, U = IN == FM_X_F32 || !INTER ? 2 : 3;
     constexpr int SI = x_size(IN), SO = x_size(OUT);
     __shared__ float2 s_turns[ROPE_TURNS];
@@ -358,9 +358,12 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
     }
     uint32_t parts = sms / a->tokens;
     parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
-    if (vec && a->tokens >= sms * 8) {
-        // many: as many to a CTA as its threads have cosines to work out
-        p.batch = half ? ROPE_THREADS / half : ROPE_BATCH;
+    if (vec && a->tokens > sms * 4) {
+        // more than the GPU holds at once: several to a CTA, as many as its threads have
+        // cosines to work out
+        const uint32_t most = half ? ROPE_THREADS / half : ROPE_BATCH;
+        p.batch = (a->tokens + sms * 4 - 1) / (sms * 4);
+        p.batch = p.batch > most ? most : p.batch;
         p.batch = p.batch < 1 ? 1 : p.batch > ROPE_BATCH ? ROPE_BATCH : p.batch;
     }
     const dim3 grid((a->tokens + p.batch - 1) / p.batch, parts);
