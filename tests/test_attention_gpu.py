@@ -195,6 +195,73 @@ def test_long_axis_is_split(cuda, lens):
     check(Batch(lens, 8, 1, 128, 64, seed=3), cuda)
 
 
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [
+    ([(2500, 2500)], 8, 2, 128),                                   # items dealt whole, one prompt
+    ([(64, 64 + b % 50) for b in range(100)], 16, 16, 64),         # items dealt whole, many sequences
+    ([(100 + 7 * b, 2000 + 31 * b) for b in range(20)], 8, 8, 64), # blocks dealt out, several items a CTA
+    ([(40, 100), (300, 300), (1, 5000), (33, 9000)], 8, 4, 128),   # small and large items, rows beside them
+])
+def test_ways_of_dealing_out_the_work(cuda, lens, heads, kv_heads, dim):
+    check(Batch(lens, heads, kv_heads, dim, 64, seed=21), cuda)
+
+
+def test_not_a_number_stays_in_its_row(cuda):
+    """A NaN in a query row gives NaN there and nowhere else; an infinite score gives NaN."""
+    for value in (float("nan"), float("inf")):
+        for lens in ([(1, 100), (1, 90)], [(200, 300), (1, 90)]):
+            b = Batch(lens, 4, 2, 64, 16, seed=22)
+            want, _ = b.run()
+            b.q[0, 1, 5] = value
+            got, lse = b.run()
+            assert torch.isnan(got[0, 1]).all() and torch.isnan(lse[0, 1])
+            got[0, 1] = want[0, 1]
+            assert torch.equal(got, want)
+            assert cuda.device_status() == 0
+
+
+def test_not_a_number_among_the_keys(cuda):
+    """A key that every row of its sequence sees: NaN there, the other sequence as before."""
+    for n in (1, 150):
+        b = Batch([(n, 300), (n, 200)], 4, 2, 64, 16, seed=23, causal=False)
+        want, _ = b.run()
+        page, row = divmod(77, 16)
+        b.k_cache[b.table[0, page], 1, row, 3] = float("nan")
+        got, _ = b.run()
+        assert torch.isnan(got[:n, 2:]).all()
+        assert torch.equal(got[:n, :2], want[:n, :2]) and torch.equal(got[n:], want[n:])
+
+
+def test_calls_that_overlap(cuda):
+    """Two streams, a workspace each (the calls allocate their own)."""
+    a, b = Batch([(1, 7000), (150, 900)], 8, 2, 128, 16, seed=24), Batch([(1, 9000), (40, 4000)], 8, 2, 128, 16, seed=25)
+    want = a.run()[0], b.run()[0]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [x.run(stream=s)[0] for x, s in zip((a, b), streams)]
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_the_example_layer(cuda):
+    """A whole layer in one chunk, in chunks and token by token: within what two roundings
+    of the stream to bf16 (2^-8 each, relative) and their way through the experts may differ."""
+    import sys
+
+    from conftest import ROOT
+
+    sys.path.insert(0, str(ROOT / "examples"))
+    import decoder_layer as example
+
+    config, lens = example.Config(window=100), [130, 1, 77]
+    whole = example.run(config, lens, steps=2)
+    for chunk in (1, 40):
+        parts = example.run(config, lens, steps=2, chunk=chunk)
+        for a, b in zip(whole, parts):
+            assert torch.isfinite(a.float()).all()
+            assert float((a.float() - b.float()).norm() / a.float().norm()) < 4 * 2.0 ** -8
+
+
 def test_many_sequences(cuda):
     """More sequences than a CTA has threads."""
     lens = [(1, 1 + (37 * b) % 90) for b in range(700)]
