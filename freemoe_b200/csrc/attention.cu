@@ -73,7 +73,7 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
     if (n.rows && units && units <= sms) {
         // the largest cluster that one wave holds and that has a step for each warp
         const uint64_t steps = keys / AR_KEYS + 1;
-        uint32_t c = 8;
+        uint32_t c = AR_MAX_CLUSTER;
         while (c > 1 && (units * c > sms || steps < c * AR_WARPS)) c /= 2;
         if (steps <= static_cast<uint64_t>(c) * AR_WARPS * CLUSTER_STEPS) n.cluster = c;
     }
@@ -243,8 +243,8 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
     const dim3 grid(p.seqs * p.kv_heads, most < ROW_LIMIT ? static_cast<uint32_t>(most) : ROW_LIMIT);
     // few units are cut into many fragments each
     if (static_cast<uint64_t>(p.seqs) * p.kv_heads * 16 <= p.workers)
-        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 16>, {grid, 16 * 32, 0, true, 1}, s, p);
-    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4>, {grid, 4 * 32, 0, true, 1}, s, p);
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>, {grid, 32 * 32, 0, true, 1}, s, p);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, true, 1}, s, p);
 }
 
 } // namespace

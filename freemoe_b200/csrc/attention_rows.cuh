@@ -24,7 +24,7 @@
 namespace fmb {
 
 constexpr uint32_t AR_WARPS = 8, AR_THREADS = AR_WARPS * 32;
-constexpr uint32_t AR_ROWS = 16, AR_KEYS = 16;
+constexpr uint32_t AR_ROWS = 16, AR_KEYS = 16, AR_MAX_CLUSTER = 8;
 
 template <int DP> struct ARows {
     static constexpr uint32_t ROW_BYTES = DP * 2;
@@ -504,12 +504,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     }
     cp_async_wait<0>();
     __syncwarp();
-    // the warp's O over its ring, 16 rows of DP
+    // the warp's O over its ring, rows of DP
+    const uint32_t all = s.ql * p.group - rt * AR_ROWS, rows = all < AR_ROWS ? all : AR_ROWS;
     float *mine = reinterpret_cast<float *>(ar_smem + warp * (L::STAGES * L::STAGE));
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const float sum = u.sum(r);
         const uint32_t in = lane / 4 + r * 8;
+        if (in >= rows) continue;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
             *reinterpret_cast<float2 *>(mine + in * DP + n * 8 + (lane & 3u) * 2) =
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     __syncthreads();
     // the CTA's O behind warp 0's
     float *joined = reinterpret_cast<float *>(ar_smem) + AR_ROWS * DP;
-    for (uint32_t i = threadIdx.x; i < AR_ROWS * DP; i += AR_THREADS) {
+    for (uint32_t i = threadIdx.x; i < rows * DP; i += AR_THREADS) {
         const uint32_t in = i / DP;
         float top = -INFINITY, acc = 0.0f, sum = 0.0f;
 #pragma unroll
@@ -544,16 +546,29 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     const uint32_t top_at = smem_u32(s_top), sum_at = smem_u32(s_sum), o_at = smem_u32(joined);
     for (uint32_t i = threadIdx.x; i < AR_ROWS / ranks * (DP / 2); i += AR_THREADS) {
         const uint32_t in = i / (DP / 2) * ranks + rank, col = i % (DP / 2) * 2;
+        if (in >= rows || col >= p.dim) continue;
         const uint32_t row = rt * AR_ROWS + in, t = row / p.group, g = row - t * p.group;
-        if (t >= s.ql || col >= p.dim) continue;
+        // all CTAs' values under way together
+        float m[AR_MAX_CLUSTER], l[AR_MAX_CLUSTER], v0[AR_MAX_CLUSTER], v1[AR_MAX_CLUSTER];
+#pragma unroll
+        for (uint32_t k = 0; k < AR_MAX_CLUSTER; ++k) {
+            m[k] = -INFINITY;
+            l[k] = v0[k] = v1[k] = 0.0f;
+            if (k >= ranks) continue;
+            m[k] = cluster_load(top_at + in * 4, k);
+            l[k] = cluster_load(sum_at + in * 4, k);
+            v0[k] = cluster_load(o_at + (in * DP + col) * 4, k);
+            v1[k] = cluster_load(o_at + (in * DP + col) * 4 + 4, k);
+        }
         float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
-        for (uint32_t k = 0; k < ranks; ++k) top = fmaxf(top, cluster_load(top_at + in * 4, k));
-        for (uint32_t k = 0; k < ranks; ++k) {
-            const float m = cluster_load(top_at + in * 4, k);
-            const float f = m == -INFINITY ? 0.0f : exp2_approx(m - top);
-            sum += cluster_load(sum_at + in * 4, k) * f;
-            a0 += cluster_load(o_at + (in * DP + col) * 4, k) * f;
-            a1 += cluster_load(o_at + (in * DP + col) * 4 + 4, k) * f;
+#pragma unroll
+        for (uint32_t k = 0; k < AR_MAX_CLUSTER; ++k) top = fmaxf(top, m[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < AR_MAX_CLUSTER; ++k) {
+            const float f = m[k] == -INFINITY ? 0.0f : exp2_approx(m[k] - top);
+            sum += l[k] * f;
+            a0 += v0[k] * f;
+            a1 += v1[k] * f;
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
@@ -568,8 +583,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
 
 // Joins the fragments of the units that were cut: a CTA of W warps a unit and row.
 // Warp i takes fragments i, i + W, ..., a lane four (two) values of the head, with the
-// loads of four fragments under way together.
-template <int DP, bool BF16, int W> __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p) {
+// loads of F fragments under way together.
+template <int DP, bool BF16, int W, int F>
+__global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p) {
     constexpr int V = DP / 32;
     __shared__ float s_o[W][DP];
     __shared__ float s_m[W], s_l[W];
@@ -589,11 +605,11 @@ template <int DP, bool BF16, int W> __global__ void __launch_bounds__(W * 32) at
     const uint32_t n = static_cast<uint32_t>((first + sh.steps - 1) / per - w0) + 1;
     if (n == 1) return; // written by its one warp
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
-    for (uint32_t f0 = warp; f0 < n; f0 += 4 * W) {
-        float2 ml[4];
-        float v[4][V];
+    for (uint32_t f0 = warp; f0 < n; f0 += F * W) {
+        float2 ml[F];
+        float v[F][V];
 #pragma unroll
-        for (uint32_t x = 0; x < 4; ++x) {
+        for (uint32_t x = 0; x < F; ++x) {
             const uint32_t f = f0 + x * W;
             ml[x] = make_float2(-INFINITY, 0.0f);
             if (f < n) {
@@ -604,7 +620,7 @@ template <int DP, bool BF16, int W> __global__ void __launch_bounds__(W * 32) at
             }
         }
 #pragma unroll
-        for (uint32_t x = 0; x < 4; ++x) {
+        for (uint32_t x = 0; x < F; ++x) {
             if (ml[x].x == -INFINITY) continue;
             const float to = fmaxf(m, ml[x].x);
             const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to), fb = exp2_approx(ml[x].x - to);
