@@ -103,14 +103,17 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
     for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float scale = fmaxf(top, 1e-10f) / 448.0f;
-    const float inv = 1.0f / scale;
-    // v / scale, correctly rounded but for rare cases: the product's error, from one fused
-    // operation, corrects it (a code is a rounding of it: an error in its last bit flips codes)
-    auto code = [&](float x) {
+    // Quotients as a product with the reciprocal and one correction by the product's error,
+    // which a fused operation gives exactly: correctly rounded but for rare cases.  (A code
+    // is a rounding of its quotient: an error in the last bit flips codes.)
+    auto quotient = [](float x, float y, float inv) {
         const float q = x * inv;
-        return fmaf(fmaf(-q, scale, x), inv, q);
+        return fmaf(fmaf(-q, y, x), inv, q);
     };
+    const float scale = quotient(fmaxf(top, 1e-10f), 448.0f, 1.0f / 448.0f);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(scale));
+    auto code = [&](float x) { return quotient(x, scale, inv); };
     uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
     const uint32_t groups = (p.d + 127) / 128;
     if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;
@@ -134,9 +137,11 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
 // ITER chunks a thread, held in registers from the read to the write; the next row's
 // are on their way while this one is summed and written.  The weight waits in shared
 // memory, as f32 in the chunks' order.
-// WIDE: x or the residual is f32, whose eights take two accesses.
-template <int VEC, bool WIDE, int ITER> struct NormRow {
+// IN: FM_X_BF16 or FM_X_F16 where x and the residual have that type; FM_X_F32: types at
+// run time, and room for f32 eights, which take two accesses.
+template <int VEC, int IN, int ITER> struct NormRow {
     uint4 x[ITER], r[ITER];                       // VEC 8
+    static constexpr bool WIDE = IN == FM_X_F32;
     uint4 x2[WIDE ? ITER : 1], r2[WIDE ? ITER : 1];
     float h[ITER][8];                             // otherwise: already h
 
@@ -179,10 +184,10 @@ template <int VEC, bool WIDE, int ITER> struct NormRow {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             if constexpr (VEC == 8) {
-                raw8_unpack(Raw8{x[i], x2[WIDE ? i : 0]}, p.xt, out[i]);
+                raw8_unpack(Raw8{x[i], x2[WIDE ? i : 0]}, WIDE ? p.xt : IN, out[i]);
                 if (p.res) {
                     float v[8];
-                    raw8_unpack(Raw8{r[i], r2[WIDE ? i : 0]}, p.rt, v);
+                    raw8_unpack(Raw8{r[i], r2[WIDE ? i : 0]}, WIDE ? p.rt : IN, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) out[i][j] += v[j];
                 }
@@ -194,7 +199,7 @@ template <int VEC, bool WIDE, int ITER> struct NormRow {
     }
 };
 
-template <int VEC, bool WIDE, bool CTA, int ITER, int MOST>
+template <int VEC, int IN, bool CTA, int ITER, int MOST>
 __global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) {
     const uint32_t nt = CTA ? blockDim.x : 32u, teams = CTA ? 1u : blockDim.x / 32;
     extern __shared__ float4 s_w[]; // chunk c: s_w[2 c], s_w[2 c + 1]
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) 
     const uint32_t team = CTA ? blockIdx.x : blockIdx.x * teams + threadIdx.x / 32;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
     uint64_t row = team;
-    NormRow<VEC, WIDE, ITER> next;
+    NormRow<VEC, IN, ITER> next;
     if (row < p.tokens) next.load(p, row, c0, nt);
     for (uint32_t c = threadIdx.x; c < nt * ITER; c += blockDim.x) {
         float w[8];
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) 
         const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
         if (p.res_out) {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) store_chunk<VEC>(p.res_out, p.rt, row * p.rs, c0 + i * nt, p.d, h[i]);
+            for (int i = 0; i < ITER; ++i) store_chunk<VEC>(p.res_out, IN == FM_X_F32 ? p.rt : IN, row * p.rs, c0 + i * nt, p.d, h[i]);
         }
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -287,9 +292,9 @@ template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ker
     }
 }
 
-template <int VEC, bool WIDE, bool CTA, int ITER, int MOST>
+template <int VEC, int IN, bool CTA, int ITER, int MOST>
 void launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
-    auto kfn = add_rms_norm_kernel<VEC, WIDE, CTA, ITER, MOST>;
+    auto kfn = add_rms_norm_kernel<VEC, IN, CTA, ITER, MOST>;
     const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
     const uint32_t smem = (CTA ? threads : 32) * ITER * 32;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
@@ -309,19 +314,19 @@ void launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
 // there are rows for half the threads of the GPU only (latency counts then).
-template <int VEC, bool WIDE> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+template <int VEC, int IN> void dispatch_norm(const NormParams &p, cudaStream_t s) {
     const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
     const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
     if (p.d <= 256)
-        launch_norm<VEC, WIDE, false, 1, 128>(p, 128, s);
+        launch_norm<VEC, IN, false, 1, 128>(p, 128, s);
     else if (p.d <= 1024)
-        launch_norm<VEC, WIDE, false, 4, 128>(p, 128, s);
+        launch_norm<VEC, IN, false, 4, 128>(p, 128, s);
     else if (few && one <= 1024)
-        launch_norm<VEC, WIDE, true, 1, 1024>(p, one, s);
+        launch_norm<VEC, IN, true, 1, 1024>(p, one, s);
     else if (two <= 512)
-        launch_norm<VEC, WIDE, true, 2, 512>(p, two, s);
+        launch_norm<VEC, IN, true, 2, 512>(p, two, s);
     else if (two <= 1024)
-        launch_norm<VEC, WIDE, true, 2, 1024>(p, two, s);
+        launch_norm<VEC, IN, true, 2, 1024>(p, two, s);
     else {
         const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
         add_rms_norm_long_kernel<VEC><<<p.tokens < most ? p.tokens : most, 1024, 0, s>>>(p);
@@ -366,14 +371,17 @@ extern "C" int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *a, void *stream) 
     };
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (fits(8, 16)) {
-        if (p.xt == FM_X_F32 || (p.res && p.rt == FM_X_F32))
-            dispatch_norm<8, true>(p, s);
+        const bool one_type = !(p.res || p.res_out) || p.xt == p.rt;
+        if (one_type && p.xt == FM_X_BF16)
+            dispatch_norm<8, FM_X_BF16>(p, s);
+        else if (one_type && p.xt == FM_X_F16)
+            dispatch_norm<8, FM_X_F16>(p, s);
         else
-            dispatch_norm<8, false>(p, s);
+            dispatch_norm<8, FM_X_F32>(p, s);
     } else if (fits(2, 8)) {
-        dispatch_norm<2, true>(p, s);
+        dispatch_norm<2, FM_X_F32>(p, s);
     } else {
-        dispatch_norm<1, true>(p, s);
+        dispatch_norm<1, FM_X_F32>(p, s);
     }
     return check_launch("add_rms_norm_kernel");
 }

@@ -66,9 +66,14 @@ __device__ __forceinline__ void store8(void *p, int32_t dtype, uint64_t at, cons
         float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
         q[0] = make_float4(v[0], v[1], v[2], v[3]);
         q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if (dtype == FM_X_BF16) {
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) =
+            make_uint4(pack2(v[0], v[1], FM_X_BF16), pack2(v[2], v[3], FM_X_BF16), pack2(v[4], v[5], FM_X_BF16),
+                       pack2(v[6], v[7], FM_X_BF16));
     } else {
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = make_uint4(
-            pack2(v[0], v[1], dtype), pack2(v[2], v[3], dtype), pack2(v[4], v[5], dtype), pack2(v[6], v[7], dtype));
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) =
+            make_uint4(pack2(v[0], v[1], FM_X_F16), pack2(v[2], v[3], FM_X_F16), pack2(v[4], v[5], FM_X_F16),
+                       pack2(v[6], v[7], FM_X_F16));
     }
 }
 
