@@ -13,6 +13,7 @@
 
 #include "attention_prompt.cuh"
 #include "attention_rows.cuh"
+#include "launch.cuh"
 
 namespace fmb {
 namespace {
@@ -128,46 +129,6 @@ int check_attention(const fmcuda_paged_attention_args *a) {
     return FM_STATUS_OK;
 }
 
-// A kernel and its launch.  `early`: it may begin while the kernel before it on the stream
-// still runs (and waits itself, griddepcontrol.wait, where it has to).
-struct Launch {
-    dim3 grid;
-    uint32_t threads, smem;
-    bool early;
-    uint32_t cluster; // CTAs a cluster, 1: none
-};
-template <typename... K, typename... A>
-int launch(const char *what, void (*kernel)(K...), const Launch &l, cudaStream_t s, const A &...args) {
-    if (l.smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(l.smem));
-        if (e != cudaSuccess) return cuda_status(e, what);
-    }
-    cudaLaunchAttribute attrs[2]{};
-    cudaLaunchConfig_t config{};
-    config.gridDim = l.grid;
-    config.blockDim = dim3(l.threads);
-    config.dynamicSmemBytes = l.smem;
-    config.stream = s;
-    config.attrs = attrs;
-    if (l.early) {
-        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (l.cluster > 1) {
-        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attrs[config.numAttrs].val.clusterDim.x = l.cluster;
-        attrs[config.numAttrs].val.clusterDim.y = attrs[config.numAttrs].val.clusterDim.z = 1;
-        ++config.numAttrs;
-    }
-    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
-    if (err != cudaSuccess) {
-        (void)cudaGetLastError();
-        return cuda_status(err, what);
-    }
-    return FM_STATUS_OK;
-}
-
 // The cache as boxes of 64 values x box_rows rows of one head of one page, the
 // dimensions in the order of their strides (`heads_first`: a page's heads lie
 // inside its rows).
@@ -227,24 +188,23 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
         if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, pp.box_rows, pp.heads_first);
         if (!rc)
             rc = launch("attn_prompt_kernel", attn_prompt_kernel<DP, BF16>,
-                        {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, false, 1}, s, map_k, map_v, pp);
+                        {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, 1}, s, map_k, map_v, pp);
     }
     if (!rc && n.cluster)
         rc = launch("attn_cluster_kernel", attn_cluster_kernel<DP, BF16>,
-                    {dim3(p.seqs * p.kv_heads * n.tiles * n.cluster), AR_THREADS, ARows<DP>::SMEM, n.prompt, n.cluster},
-                    s, p, n.tiles);
+                    {dim3(p.seqs * p.kv_heads * n.tiles * n.cluster), AR_THREADS, ARows<DP>::SMEM, n.cluster}, s, p, n.tiles);
     else if (!rc && n.rows)
         rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16>,
-                    {dim3(p.workers / AR_WARPS), AR_THREADS, ARows<DP>::SMEM, n.prompt, 1}, s, p);
+                    {dim3(p.workers / AR_WARPS), AR_THREADS, ARows<DP>::SMEM, 1}, s, p);
     if (!rc && n.prompt && n.deal)
-        rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, true, 1}, s, pp);
+        rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1}, s, pp);
     if (rc || !n.rows || n.cluster) return rc;
     const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group;
     const dim3 grid(p.seqs * p.kv_heads, most < ROW_LIMIT ? static_cast<uint32_t>(most) : ROW_LIMIT);
     // few units are cut into many fragments each
     if (static_cast<uint64_t>(p.seqs) * p.kv_heads * 16 <= p.workers)
-        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>, {grid, 32 * 32, 0, true, 1}, s, p);
-    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, true, 1}, s, p);
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>, {grid, 32 * 32, 0, 1}, s, p);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, 1}, s, p);
 }
 
 } // namespace
@@ -313,6 +273,7 @@ extern "C" int fmcuda_paged_attention(const fmcuda_paged_attention_args *a, void
     p.workers = n.workers;
     p.least = 4;
     p.row_limit = n.rows ? ROW_LIMIT : 0;
+    p.beside = n.prompt;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = a->dtype == FM_X_BF16;
     if (n.dp == 64)

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "ptx.cuh"
 
 namespace fmb {
@@ -24,6 +25,7 @@ struct AttnParams {
     float *part;      // partial sums
     float2 *part_ml;  // their (largest exponent in log2, sum)
     uint32_t workers, least; // rows kernel: warps, and the least steps a warp takes
+    bool beside;             // a prompt kernel of the same call was launched before the rows kernel
     uint32_t row_limit;      // rows x group up to which a sequence is the rows kernel's
 };
 

@@ -347,9 +347,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     volatile uint32_t *abort_flag = misc + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
-    // what follows on the stream may come to the SMs that have nothing to do here; it waits
-    // for the end of this grid before it reads from it, or ends itself
-    asm volatile("griddepcontrol.launch_dependents;\n");
+    // what follows on the stream may come to the SMs that have nothing to do here
+    after_stream();
+    let_next();
 
     // ---- this CTA's share -------------------------------------------------------------
     // where blocks are dealt out: the sequences that have pairs and their first ones, and
@@ -881,8 +881,8 @@ constexpr uint32_t AJ_SLICES = 16;
 template <int DP, bool BF16> __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ APParams pp) {
     constexpr int V = DP / 32;
     const AttnParams &p = pp.a;
-    asm volatile("griddepcontrol.launch_dependents;\n");
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    after_stream();
+    let_next();
     const int4 tail = pp.tail[blockIdx.x];
     if (tail.x < 0) return;
     const uint32_t lane = threadIdx.x & 31u;

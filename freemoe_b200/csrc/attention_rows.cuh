@@ -75,12 +75,16 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The kernels here begin beside a prompt kernel that the same call launched before them,
-// on the SMs that it leaves free: they share nothing with it.  But the grid does not end
-// before it, so that what follows on the stream finds both done: its first CTA waits (were
-// all to wait, the CTAs behind them would find no SM until then).
-__device__ __forceinline__ void after_prompt_kernel() {
-    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+// The kernels here begin beside a prompt kernel that the same call launched before them
+// (and that waited for the stream), on the SMs that it leaves free: they share nothing with
+// it.  But the grid does not end before it, so that what follows on the stream finds both
+// done: its first CTA waits (were all to wait, the CTAs behind them would find no SM until
+// then).  Without a prompt kernel they wait for the stream like any other.
+__device__ __forceinline__ void before_rows(const AttnParams &p) {
+    if (!p.beside) after_stream();
+}
+__device__ __forceinline__ void after_rows(const AttnParams &p) {
+    if (p.beside && blockIdx.x == 0) after_stream();
 }
 
 // A place in the laid-out work.
@@ -294,6 +298,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     __shared__ uint32_t s_seq[AR_WARPS];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
+    before_rows(p);
+    let_next();
     // ---- this warp's range, and the sequence that it begins in -------------------
     uint64_t total = 0, mine = 0, before = 0;
     const bool few = p.seqs <= AR_THREADS;
@@ -339,11 +345,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         }
     }
     __syncthreads();
-    asm volatile("griddepcontrol.launch_dependents;\n");
     const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
     const uint64_t begin = worker * per;
     if (begin >= total) {
-        after_prompt_kernel();
+        after_rows(p);
         return;
     }
     const uint32_t count = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         if (i + 1 < count) ar_advance(p, c);
     }
     cp_async_wait<0>();
-    after_prompt_kernel();
+    after_rows(p);
 }
 
 // ---- few units of short sequences: a cluster each ----------------------------------
@@ -470,10 +475,12 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
     const uint32_t unit = blockIdx.x / ranks, rt = unit % unit_tiles;
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
+    before_rows(p);
+    let_next();
     const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
     const ARShape sh = ar_shape(p, s);
     if (rt >= sh.tiles) { // the whole cluster
-        after_prompt_kernel();
+        after_rows(p);
         return;
     }
 
@@ -578,7 +585,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
             p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
     cluster_sync(); // nobody leaves while its shared memory is read
-    after_prompt_kernel();
+    after_rows(p);
 }
 
 // Joins the fragments of the units that were cut: a CTA of W warps a unit and row.
@@ -591,11 +598,12 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
     __shared__ float s_m[W], s_l[W];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t b = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
+    after_stream();
+    let_next();
     const AttnSeq s = attn_seq(p, b, false);
     const ARShape sh = ar_shape(p, s);
     const uint32_t row = blockIdx.y;
     if (sh.tiles == 0 || row >= s.ql * p.group) return;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const uint64_t total = p.prefix[p.seqs];
     const uint64_t even = (total + p.workers - 1) / p.workers;
     const uint64_t per = even > p.least ? even : p.least;

@@ -9,6 +9,7 @@
 // h; the weight stays on the SM over the rows of a CTA.
 #include <string>
 
+#include "launch.cuh"
 #include "vec8.cuh"
 
 namespace fmb {
@@ -207,6 +208,8 @@ __global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) 
     const uint32_t c0 = CTA ? threadIdx.x : threadIdx.x % 32;
     const uint32_t team = CTA ? blockIdx.x : blockIdx.x * teams + threadIdx.x / 32;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
+    after_stream();
+    let_next();
     uint64_t row = team;
     NormRow<VEC, IN, ITER> next;
     if (row < p.tokens) next.load(p, row, c0, nt);
@@ -252,6 +255,8 @@ __global__ void __launch_bounds__(MOST) add_rms_norm_kernel(const NormParams p) 
 template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(const NormParams p) {
     __shared__ float s_part[2][32];
     const uint32_t chunks = ((p.d + 127) / 128) * 16;
+    after_stream();
+    let_next();
     uint32_t turn = 0;
     for (uint64_t row = blockIdx.x; row < p.tokens; row += gridDim.x, turn ^= 1u) {
         float sum = 0.0f;
@@ -293,7 +298,7 @@ template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ker
 }
 
 template <int VEC, int IN, bool CTA, int ITER, int MOST>
-void launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
+int launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
     auto kfn = add_rms_norm_kernel<VEC, IN, CTA, ITER, MOST>;
     const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
     const uint32_t smem = (CTA ? threads : 32) * ITER * 32;
@@ -306,31 +311,23 @@ void launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
             per_sm = 1;
         }
         grid *= static_cast<uint32_t>(per_sm);
-    } else if (smem > 48 * 1024) {
-        cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     }
-    kfn<<<want < grid ? want : grid, threads, smem, s>>>(p);
+    return launch("add_rms_norm_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1}, s, p);
 }
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
 // there are rows for half the threads of the GPU only (latency counts then).
-template <int VEC, int IN> void dispatch_norm(const NormParams &p, cudaStream_t s) {
+template <int VEC, int IN> int dispatch_norm(const NormParams &p, cudaStream_t s) {
     const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
     const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
-    if (p.d <= 256)
-        launch_norm<VEC, IN, false, 1, 128>(p, 128, s);
-    else if (p.d <= 1024)
-        launch_norm<VEC, IN, false, 4, 128>(p, 128, s);
-    else if (few && one <= 1024)
-        launch_norm<VEC, IN, true, 1, 1024>(p, one, s);
-    else if (two <= 512)
-        launch_norm<VEC, IN, true, 2, 512>(p, two, s);
-    else if (two <= 1024)
-        launch_norm<VEC, IN, true, 2, 1024>(p, two, s);
-    else {
-        const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
-        add_rms_norm_long_kernel<VEC><<<p.tokens < most ? p.tokens : most, 1024, 0, s>>>(p);
-    }
+    if (p.d <= 256) return launch_norm<VEC, IN, false, 1, 128>(p, 128, s);
+    if (p.d <= 1024) return launch_norm<VEC, IN, false, 4, 128>(p, 128, s);
+    if (few && one <= 1024) return launch_norm<VEC, IN, true, 1, 1024>(p, one, s);
+    if (two <= 512) return launch_norm<VEC, IN, true, 2, 512>(p, two, s);
+    if (two <= 1024) return launch_norm<VEC, IN, true, 2, 1024>(p, two, s);
+    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
+    return launch("add_rms_norm_long_kernel", add_rms_norm_long_kernel<VEC>,
+                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1}, s, p);
 }
 
 } // namespace
@@ -372,16 +369,9 @@ extern "C" int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *a, void *stream) 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (fits(8, 16)) {
         const bool one_type = !(p.res || p.res_out) || p.xt == p.rt;
-        if (one_type && p.xt == FM_X_BF16)
-            dispatch_norm<8, FM_X_BF16>(p, s);
-        else if (one_type && p.xt == FM_X_F16)
-            dispatch_norm<8, FM_X_F16>(p, s);
-        else
-            dispatch_norm<8, FM_X_F32>(p, s);
-    } else if (fits(2, 8)) {
-        dispatch_norm<2, FM_X_F32>(p, s);
-    } else {
-        dispatch_norm<1, FM_X_F32>(p, s);
+        if (one_type && p.xt == FM_X_BF16) return dispatch_norm<8, FM_X_BF16>(p, s);
+        if (one_type && p.xt == FM_X_F16) return dispatch_norm<8, FM_X_F16>(p, s);
+        return dispatch_norm<8, FM_X_F32>(p, s);
     }
-    return check_launch("add_rms_norm_kernel");
+    return fits(2, 8) ? dispatch_norm<2, FM_X_F32>(p, s) : dispatch_norm<1, FM_X_F32>(p, s);
 }

@@ -16,6 +16,7 @@
 #include <cmath>
 #include <string>
 
+#include "launch.cuh"
 #include "vec8.cuh"
 
 namespace fmb {
@@ -100,6 +101,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4
     const uint32_t step = at_once * gridDim.y, turned = p.heads + p.kv_heads;
     const uint32_t heads = lane_head >= at_once ? 0 : INTER ? turned + p.kv_heads : turned;
     const float2 *my_turns = s_turns + (INTER ? item * 4 : ea);
+    after_stream();
+    let_next();
     bool ready = false;
     uint32_t h1 = blockIdx.y * at_once + lane_head;
     do {
@@ -204,6 +207,8 @@ template <bool INTER> __global__ void __launch_bounds__(ROPE_THREADS) rope_appen
     __shared__ float2 s_turns[ROPE_TURNS];
     __shared__ int64_t s_row[ROPE_BATCH];
     const int64_t t = blockIdx.x;
+    after_stream();
+    let_next();
     rope_tokens(p, blockIdx.x, 1, s_turns, s_row);
     const int64_t cache_row = s_row[0];
     const uint32_t half = p.rot / 2, turned = p.heads + p.kv_heads, head_items = p.dim - half;
@@ -237,22 +242,18 @@ template <bool INTER> __global__ void __launch_bounds__(ROPE_THREADS) rope_appen
     }
 }
 
-template <bool INTER, int IN> void launch_rope_in(const RopeParams &p, dim3 grid, uint32_t threads, cudaStream_t s) {
-    if (p.out_t == FM_X_F32)
-        rope_append_kernel<INTER, IN, FM_X_F32><<<grid, threads, 0, s>>>(p);
-    else if (p.out_t == FM_X_BF16)
-        rope_append_kernel<INTER, IN, FM_X_BF16><<<grid, threads, 0, s>>>(p);
-    else
-        rope_append_kernel<INTER, IN, FM_X_F16><<<grid, threads, 0, s>>>(p);
+template <bool INTER, int IN> int launch_rope_in(const RopeParams &p, const Launch &l, cudaStream_t s) {
+    auto kfn = p.out_t == FM_X_F32    ? rope_append_kernel<INTER, IN, FM_X_F32>
+               : p.out_t == FM_X_BF16 ? rope_append_kernel<INTER, IN, FM_X_BF16>
+                                      : rope_append_kernel<INTER, IN, FM_X_F16>;
+    return launch("rope_append_kernel", kfn, l, s, p);
 }
 
-template <bool INTER> void launch_rope(const RopeParams &p, dim3 grid, uint32_t threads, cudaStream_t s) {
-    if (p.in_t == FM_X_F32)
-        launch_rope_in<INTER, FM_X_F32>(p, grid, threads, s);
-    else if (p.in_t == FM_X_BF16)
-        launch_rope_in<INTER, FM_X_BF16>(p, grid, threads, s);
-    else
-        launch_rope_in<INTER, FM_X_F16>(p, grid, threads, s);
+template <bool INTER> int launch_rope(const RopeParams &p, bool vec, const Launch &l, cudaStream_t s) {
+    if (!vec) return launch("rope_append_any_kernel", rope_append_any_kernel<INTER>, l, s, p);
+    if (p.in_t == FM_X_F32) return launch_rope_in<INTER, FM_X_F32>(p, l, s);
+    if (p.in_t == FM_X_BF16) return launch_rope_in<INTER, FM_X_BF16>(p, l, s);
+    return launch_rope_in<INTER, FM_X_F16>(p, l, s);
 }
 
 } // namespace
@@ -366,15 +367,7 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
         p.batch = p.batch > most ? most : p.batch;
         p.batch = p.batch < 1 ? 1 : p.batch > ROPE_BATCH ? ROPE_BATCH : p.batch;
     }
-    const dim3 grid((a->tokens + p.batch - 1) / p.batch, parts);
+    const Launch l{dim3((a->tokens + p.batch - 1) / p.batch, parts), threads, 0, 1};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (vec && a->interleaved)
-        launch_rope<true>(p, grid, threads, s);
-    else if (vec)
-        launch_rope<false>(p, grid, threads, s);
-    else if (a->interleaved)
-        rope_append_any_kernel<true><<<grid, threads, 0, s>>>(p);
-    else
-        rope_append_any_kernel<false><<<grid, threads, 0, s>>>(p);
-    return check_launch("rope_append_kernel");
+    return a->interleaved ? launch_rope<true>(p, vec, l, s) : launch_rope<false>(p, vec, l, s);
 }
