@@ -79,33 +79,48 @@ template <int T> __device__ __forceinline__ Raw8 rope_load(const char *src) {
     return r;
 }
 
+__device__ __forceinline__ uint4 rope_shuffle(uint4 v, uint32_t lane) {
+    return make_uint4(__shfl_sync(0xFFFFFFFFu, v.x, lane), __shfl_sync(0xFFFFFFFFu, v.y, lane),
+                      __shfl_sync(0xFFFFFFFFu, v.z, lane), __shfl_sync(0xFFFFFFFFu, v.w, lane));
+}
+
 // Heads, strides and rot/2 (interleaved: rot) in whole eights.  A thread keeps its place
-// in the head -- eight values, or eight pairs (i, i + rot/2) -- and up to U of the heads of
-// q, k and (interleaved, where their places are the same) v, whose addresses only move on
-// from token to token of the CTA's batch: per token U loads under way together, then the
-// turns and the stores.  Measured with 8192 tokens of 32 + 8 heads of 128, bf16 (201 MB,
-// 31 us at the measured copy rate): 39 us; U = 2 or 4, 41; an index over all of a token's
-// eights with its divisions, 44 (issue slots 65% busy); the cosines worked out by every
-// thread for itself, 64.  Bound by the loads under way: registers against warps.
-template <bool INTER, int IN, int OUT>
-__global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4) rope_append_kernel(const RopeParams p) {
-    constexpr int PAIRS = INTER ? 4 : 8, U = IN == FM_X_F32 || !INTER ? 2 : 3;
+// in the head -- eight values; PAIRED: eight pairs (i, i + rot/2) -- and up to U of the
+// heads of q, k and (not PAIRED, where their places are the same) v, whose addresses only
+// move on from token to token of the CTA's batch: per token U loads under way together,
+// then the turns and the stores.  HALVES: the partners at i +- rot/2 come from the lane
+// that loaded them, where a head's eights divide a warp; PAIRED is for heads that do not.
+// Measured with 8192 tokens of 32 + 8 heads of 128, bf16 (201 MB, 31 us at the measured
+// copy rate): 37 us; U = 2 or 4, 39; an index over all of a token's eights with its
+// divisions, 44 (issue slots 65% busy); the cosines worked out by every thread for
+// itself, 64.  Bound by the loads under way: registers against warps.
+enum { ROPE_INTER, ROPE_HALVES, ROPE_PAIRED };
+
+template <int LAYOUT, int IN, int OUT>
+__global__ void __launch_bounds__(ROPE_THREADS, LAYOUT == ROPE_PAIRED && IN == FM_X_F32 ? 2 : 4)
+    rope_append_kernel(const RopeParams p) {
+    constexpr bool INTER = LAYOUT == ROPE_INTER, PAIRED = LAYOUT == ROPE_PAIRED;
+    constexpr int PAIRS = INTER ? 4 : 8, U = IN == FM_X_F32 || PAIRED ? 2 : 3;
     constexpr int SI = x_size(IN), SO = x_size(OUT);
     __shared__ float2 s_turns[ROPE_TURNS];
     __shared__ int64_t s_row[ROPE_BATCH];
     const uint32_t t0 = blockIdx.x * p.batch, n = p.tokens - t0 < p.batch ? p.tokens - t0 : p.batch;
     const uint32_t half = p.rot / 2, at_once = blockDim.x / p.head_items; // heads at once
     const uint32_t item = threadIdx.x % p.head_items, lane_head = threadIdx.x / p.head_items;
-    const bool pair = item * 8 < (INTER ? p.rot : half);
-    const uint32_t ea = item * 8 + (INTER || pair ? 0 : half); // copied values lie behind the pairs
+    const bool pair = item * 8 < (PAIRED ? half : p.rot);
+    const uint32_t ea = item * 8 + (!PAIRED || pair ? 0 : half); // copied values lie behind the pairs
     const uint32_t step = at_once * gridDim.y, turned = p.heads + p.kv_heads;
-    const uint32_t heads = lane_head >= at_once ? 0 : INTER ? turned + p.kv_heads : turned;
-    const float2 *my_turns = s_turns + (INTER ? item * 4 : ea);
+    const uint32_t heads = lane_head >= at_once ? 0 : PAIRED ? turned : turned + p.kv_heads;
+    // HALVES: the lane with the partners, and whether they are the first of their pairs
+    const bool second = item * 8 >= half;
+    const uint32_t partner = (threadIdx.x & 31u) + (pair ? second ? 0u - half / 8 : half / 8 : 0u);
+    const float2 *my_turns = s_turns + (INTER ? item * 4 : LAYOUT == ROPE_HALVES && second ? ea - half : ea);
     after_stream();
     let_next();
     bool ready = false;
     uint32_t h1 = blockIdx.y * at_once + lane_head;
-    do {
+    // whole warps go round together: lanes exchange inside
+    while (__any_sync(0xFFFFFFFFu, h1 < heads || !ready)) {
         const char *src[U];
         char *dst[U];
         int64_t move[U];
@@ -129,13 +144,13 @@ __global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4
                 move[x] = (key ? p.kt : p.vt) * SI;
             }
         }
-        Raw8 a[U], b[INTER ? 1 : U];
+        Raw8 a[U], b[PAIRED ? U : 1];
         auto load = [&] {
 #pragma unroll
             for (int x = 0; x < U; ++x) {
                 if (here[x]) {
                     a[x] = rope_load<IN>(src[x]);
-                    if (!INTER && turns[x]) b[x] = rope_load<IN>(src[x] + half * SI);
+                    if (PAIRED && turns[x]) b[x] = rope_load<IN>(src[x] + half * SI);
                 }
                 src[x] += move[x];
             }
@@ -154,9 +169,14 @@ __global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4
             }
 #pragma unroll
             for (int x = 0; x < U; ++x) {
+                float f[8], g[8];
+                Raw8 other;
+                if constexpr (LAYOUT == ROPE_HALVES) {
+                    other.a = rope_shuffle(a[x].a, partner);
+                    other.b = IN == FM_X_F32 ? rope_shuffle(a[x].b, partner) : other.a;
+                }
                 if (!here[x] || (cached[x] && row < 0)) continue;
                 char *to = dst[x] + (cached[x] ? row : k * p.ot) * SO;
-                float f[8], g[8];
                 raw8_unpack(a[x], IN, f);
                 if (!turns[x]) {
                     store8(to, OUT, 0, f);
@@ -167,8 +187,16 @@ __global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4
                         g[2 * j + 1] = f[2 * j] * cs[j].y + f[2 * j + 1] * cs[j].x;
                     }
                     store8(to, OUT, 0, g);
+                } else if (LAYOUT == ROPE_HALVES) {
+                    raw8_unpack(other, IN, g);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float sn = second ? cs[j % PAIRS].y : -cs[j % PAIRS].y;
+                        f[j] = f[j] * cs[j % PAIRS].x + g[j] * sn;
+                    }
+                    store8(to, OUT, 0, f);
                 } else {
-                    raw8_unpack(b[INTER ? 0 : x], IN, g);
+                    raw8_unpack(b[PAIRED ? x : 0], IN, g);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float c = f[j] * cs[j % PAIRS].x - g[j] * cs[j % PAIRS].y;
@@ -181,8 +209,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, !INTER && IN == FM_X_F32 ? 2 : 4
             }
         }
         h1 += U * step;
-    } while (h1 < heads);
-    if (INTER) return;
+    }
+    if (!PAIRED) return;
     // values: copied, eight at a time, all tokens of the batch
     const uint32_t all = p.kv_heads * p.value_items;
     for (uint32_t i = blockIdx.y * blockDim.x + threadIdx.x; i < all; i += gridDim.y * blockDim.x) {
@@ -242,18 +270,17 @@ template <bool INTER> __global__ void __launch_bounds__(ROPE_THREADS) rope_appen
     }
 }
 
-template <bool INTER, int IN> int launch_rope_in(const RopeParams &p, const Launch &l, cudaStream_t s) {
-    auto kfn = p.out_t == FM_X_F32    ? rope_append_kernel<INTER, IN, FM_X_F32>
-               : p.out_t == FM_X_BF16 ? rope_append_kernel<INTER, IN, FM_X_BF16>
-                                      : rope_append_kernel<INTER, IN, FM_X_F16>;
+template <int LAYOUT, int IN> int launch_rope_in(const RopeParams &p, const Launch &l, cudaStream_t s) {
+    auto kfn = p.out_t == FM_X_F32    ? rope_append_kernel<LAYOUT, IN, FM_X_F32>
+               : p.out_t == FM_X_BF16 ? rope_append_kernel<LAYOUT, IN, FM_X_BF16>
+                                      : rope_append_kernel<LAYOUT, IN, FM_X_F16>;
     return launch("rope_append_kernel", kfn, l, s, p);
 }
 
-template <bool INTER> int launch_rope(const RopeParams &p, bool vec, const Launch &l, cudaStream_t s) {
-    if (!vec) return launch("rope_append_any_kernel", rope_append_any_kernel<INTER>, l, s, p);
-    if (p.in_t == FM_X_F32) return launch_rope_in<INTER, FM_X_F32>(p, l, s);
-    if (p.in_t == FM_X_BF16) return launch_rope_in<INTER, FM_X_BF16>(p, l, s);
-    return launch_rope_in<INTER, FM_X_F16>(p, l, s);
+template <int LAYOUT> int launch_rope(const RopeParams &p, const Launch &l, cudaStream_t s) {
+    if (p.in_t == FM_X_F32) return launch_rope_in<LAYOUT, FM_X_F32>(p, l, s);
+    if (p.in_t == FM_X_BF16) return launch_rope_in<LAYOUT, FM_X_BF16>(p, l, s);
+    return launch_rope_in<LAYOUT, FM_X_F16>(p, l, s);
 }
 
 } // namespace
@@ -345,12 +372,15 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
                        a->cache_head_stride, a->cache_row_stride, a->in_dtype, a->out_dtype, a->heads, kvh,
                        a->head_dim, a->rot_dim, a->attention_factor, cached ? a->page_size : 1,
                        cached ? static_cast<uint64_t>(a->n_pages) * a->page_size : 0,
-                       (a->head_dim - (a->interleaved ? 0 : half)) / 8, a->head_dim / 8, a->tokens, 1, status};
+                       a->head_dim / 8, a->head_dim / 8, a->tokens, 1, status};
+    // a head's eights divide a warp: partners are in the same one
+    const bool paired = vec && !a->interleaved && half && 256 % a->head_dim;
+    if (paired) p.head_items -= half / 8;
     const uint32_t sms = static_cast<uint32_t>(device_sm_count());
     // few tokens: a token's heads (or items) over several CTAs, until every SM has one
     uint32_t threads = ROPE_THREADS, rounds;
     if (vec) {
-        const uint32_t at_once = ROPE_THREADS / p.head_items, all = a->heads + kvh * (a->interleaved ? 2 : 1);
+        const uint32_t at_once = ROPE_THREADS / p.head_items, all = a->heads + kvh * (paired ? 1 : 2);
         rounds = (all + at_once - 1) / at_once;
         if (rounds == 1) threads = (all * p.head_items + 31) & ~31u;
     } else {
@@ -369,5 +399,8 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
     }
     const Launch l{dim3((a->tokens + p.batch - 1) / p.batch, parts), threads, 0, 1};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return a->interleaved ? launch_rope<true>(p, vec, l, s) : launch_rope<false>(p, vec, l, s);
+    if (!vec && a->interleaved) return launch("rope_append_any_kernel", rope_append_any_kernel<true>, l, s, p);
+    if (!vec) return launch("rope_append_any_kernel", rope_append_any_kernel<false>, l, s, p);
+    if (a->interleaved) return launch_rope<ROPE_INTER>(p, l, s);
+    return paired ? launch_rope<ROPE_PAIRED>(p, l, s) : launch_rope<ROPE_HALVES>(p, l, s);
 }
