@@ -24,8 +24,13 @@ inline uint64_t a256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
 // kernel that joins the fragments cost less than the SMs that the clusters leave idle.
 constexpr uint32_t CLUSTER_STEPS = 16;
 
-// Rows (tokens x group) up to which a sequence is the rows kernel's.
-constexpr uint32_t ROW_LIMIT = 32;
+// Rows (tokens x group) up to which a sequence is the rows kernel's: one tile of 16, or
+// two, which read the cache twice (the second time from L2), where all of the batch's keys
+// and values are few (by their bound, max_kv_len each).  Measured, 32 rows a sequence and
+// key head, 8 key heads of 128, ragged lengths up to 4096 keys: 16 sequences 54 us there
+// against 60 on the prompt kernel, 64 sequences 181 against 136.
+constexpr uint32_t MOST_ROWS = 2 * AR_ROWS;
+constexpr uint64_t TWICE_BYTES = 256u << 20;
 
 // The prompt kernel's work is dealt out by blocks where whole items would leave
 // CTAs idle: with fewer than DEAL_ITEMS items a CTA, or one a CTA where one
@@ -35,6 +40,7 @@ constexpr uint32_t DEAL_ITEMS = 6, WHOLE_BLOCKS = 10;
 
 struct AttnPlan {
     uint32_t dp, workers, group;
+    uint32_t row_limit;
     bool rows, prompt;       // which kernels have work
     uint32_t cluster;        // CTAs a unit of the cluster form of the rows kernel; 0: the other form
     uint32_t tiles;          // row tiles of a unit's sequence and head, at most
@@ -56,11 +62,13 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
     const uint32_t sms = static_cast<uint32_t>(device_sm_count());
     n.workers = sms * AR_WARPS;
     const uint64_t all = static_cast<uint64_t>(a.tokens) * n.group;
-    n.prompt = static_cast<uint64_t>(a.max_q_len) * n.group > ROW_LIMIT;
+    const uint64_t bytes = keys_seen(a, MOST_ROWS) * a.seqs * a.kv_heads * a.head_dim * 4;
+    n.row_limit = bytes <= TWICE_BYTES ? MOST_ROWS : AR_ROWS;
+    n.prompt = static_cast<uint64_t>(a.max_q_len) * n.group > n.row_limit;
     // a sequence has at least tokens - (seqs - 1) * max_q_len rows, where that bound can be
     // true; without the rows kernel the other one takes sequences of any length
     const uint64_t others = static_cast<uint64_t>(a.seqs - 1) * a.max_q_len;
-    n.rows = all <= others * n.group + ROW_LIMIT || a.tokens > others + a.max_q_len;
+    n.rows = all <= others * n.group + n.row_limit || a.tokens > others + a.max_q_len;
     uint64_t o = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t at = o;
@@ -68,12 +76,12 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         return at;
     };
     const uint64_t most_rows = static_cast<uint64_t>(a.max_q_len) * n.group;
-    n.tiles = static_cast<uint32_t>((most_rows < ROW_LIMIT ? most_rows + AR_ROWS - 1 : ROW_LIMIT) / AR_ROWS);
-    const uint64_t keys = keys_seen(a, ROW_LIMIT);
+    n.tiles = static_cast<uint32_t>((most_rows < n.row_limit ? most_rows + AR_ROWS - 1 : n.row_limit) / AR_ROWS);
+    const uint64_t keys = keys_seen(a, MOST_ROWS);
     const uint64_t units = static_cast<uint64_t>(a.seqs) * a.kv_heads * n.tiles;
     if (n.rows && units && units <= sms) {
         // the largest cluster that one wave holds and that has a step for each warp
-        const uint64_t steps = keys / AR_KEYS + 1;
+        const uint64_t steps = keys / ar_keys(static_cast<int>(n.dp)) + 1;
         uint32_t c = AR_MAX_CLUSTER;
         while (c > 1 && (units * c > sms || steps < c * AR_WARPS)) c /= 2;
         if (steps <= static_cast<uint64_t>(c) * AR_WARPS * CLUSTER_STEPS) n.cluster = c;
@@ -84,7 +92,7 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         n.part_ml = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * 8);
     }
     if (n.prompt) {
-        const uint64_t big = all / ((n.rows ? ROW_LIMIT : 0) + 1);
+        const uint64_t big = all / ((n.rows ? n.row_limit : 0) + 1);
         n.pairs = static_cast<uint32_t>(all / AP_PAIR + (big < a.seqs ? big : a.seqs));
         const uint64_t items = static_cast<uint64_t>(n.pairs) * a.kv_heads;
         const bool prompt = a.seqs == 1 && a.causal && !a.window && a.max_q_len == a.max_kv_len;
@@ -200,7 +208,7 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
         rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1}, s, pp);
     if (rc || !n.rows || n.cluster) return rc;
     const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group;
-    const dim3 grid(p.seqs * p.kv_heads, most < ROW_LIMIT ? static_cast<uint32_t>(most) : ROW_LIMIT);
+    const dim3 grid(p.seqs * p.kv_heads, most < n.row_limit ? static_cast<uint32_t>(most) : n.row_limit);
     // few units are cut into many fragments each
     if (static_cast<uint64_t>(p.seqs) * p.kv_heads * 16 <= p.workers)
         return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>, {grid, 32 * 32, 0, 1}, s, p);
@@ -272,7 +280,7 @@ extern "C" int fmcuda_paged_attention(const fmcuda_paged_attention_args *a, void
     p.part_ml = reinterpret_cast<float2 *>(ws + n.part_ml);
     p.workers = n.workers;
     p.least = 4;
-    p.row_limit = n.rows ? ROW_LIMIT : 0;
+    p.row_limit = n.rows ? n.row_limit : 0;
     p.beside = n.prompt;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = a->dtype == FM_X_BF16;

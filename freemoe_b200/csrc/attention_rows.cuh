@@ -2,7 +2,9 @@
 // paged cache: one read of the keys and values, limited by HBM.
 //
 // The rows of a key head -- tokens x the query heads that share it -- make
-// 16-row tiles, the M of mma.sync.m16n8k16; a step is 16 keys: S = Q K^T (keys
+// 16-row tiles, the M of mma.sync.m16n8k16; a step is 16 keys (32 of heads up to 64:
+// with 16, a step's fixed work and not HBM set the pace, 125 us against 172 for twice
+// the bytes): S = Q K^T (keys
 // are the N), the running maximum and sum of the softmax, O += P V (keys are
 // the K, P's accumulator fragments are its A fragments).  The contraction is
 // far below what mma.sync does; the point is the stream of keys, so each warp
@@ -24,11 +26,13 @@
 namespace fmb {
 
 constexpr uint32_t AR_WARPS = 8, AR_THREADS = AR_WARPS * 32;
-constexpr uint32_t AR_ROWS = 16, AR_KEYS = 16, AR_MAX_CLUSTER = 8;
+constexpr uint32_t AR_ROWS = 16, AR_MAX_CLUSTER = 8;
+__host__ __device__ constexpr uint32_t ar_keys(int dp) { return dp == 64 ? 32 : 16; } // keys a step
 
 template <int DP> struct ARows {
     static constexpr uint32_t ROW_BYTES = DP * 2;
-    static constexpr uint32_t HALF = AR_KEYS * ROW_BYTES; // K or V of a step
+    static constexpr uint32_t KEYS = ar_keys(DP);
+    static constexpr uint32_t HALF = KEYS * ROW_BYTES; // K or V of a step
     static constexpr uint32_t STAGE = 2 * HALF;
     static constexpr uint32_t STAGES = 24576 / STAGE; // 24 KB a warp
     static constexpr uint32_t SMEM = AR_WARPS * STAGES * STAGE;
@@ -38,12 +42,13 @@ template <int DP> struct ARows {
 struct ARShape {
     uint32_t tiles, step0, steps;
 };
-__device__ __forceinline__ ARShape ar_shape(const AttnParams &p, const AttnSeq &s) {
+template <int DP> __device__ __forceinline__ ARShape ar_shape(const AttnParams &p, const AttnSeq &s) {
+    constexpr uint32_t KEYS = ar_keys(DP);
     ARShape r;
     const uint64_t rows = static_cast<uint64_t>(s.ql) * p.group;
     r.tiles = rows <= p.row_limit ? static_cast<uint32_t>((rows + AR_ROWS - 1) / AR_ROWS) : 0;
-    r.step0 = s.lo / AR_KEYS;
-    const uint32_t last = (s.kl + AR_KEYS - 1) / AR_KEYS;
+    r.step0 = s.lo / KEYS;
+    const uint32_t last = (s.kl + KEYS - 1) / KEYS;
     r.steps = last > r.step0 ? last - r.step0 : 1; // a unit without keys still writes its zeros
     return r;
 }
@@ -94,32 +99,32 @@ struct ARCursor {
     ARShape sh;
 };
 
-__device__ __forceinline__ void ar_enter(const AttnParams &p, ARCursor &c) {
+template <int DP> __device__ __forceinline__ void ar_enter(const AttnParams &p, ARCursor &c) {
     // the next sequence that has tiles; the caller stops at the range's end before there is none
     while (c.b < p.seqs) {
         c.s = attn_seq(p, c.b, false);
-        c.sh = ar_shape(p, c.s);
+        c.sh = ar_shape<DP>(p, c.s);
         if (c.sh.tiles) return;
         ++c.b;
     }
 }
 
-__device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
+template <int DP> __device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
     if (++c.step < c.sh.steps) return;
     c.step = 0;
     if (++c.tile < c.sh.tiles * p.kv_heads) return;
     c.tile = 0;
     ++c.b;
-    ar_enter(p, c);
+    ar_enter<DP>(p, c);
 }
 
-// Queues the copies of a step's 16 keys and values; what is not to be read becomes zeros.
+// Queues the copies of a step's keys and values; what is not to be read becomes zeros.
 template <int DP>
 __device__ __forceinline__ void ar_fetch(const AttnParams &p, uint32_t stage, int64_t offset, uint32_t lane) {
     constexpr uint32_t CH = DP / 8, PER = 32 / CH; // 16-byte pieces a row, rows a round
     const uint32_t piece = lane % CH;
 #pragma unroll
-    for (uint32_t i = 0; i < AR_KEYS / PER; ++i) {
+    for (uint32_t i = 0; i < ARows<DP>::KEYS / PER; ++i) {
         const uint32_t row = i * PER + lane / CH;
         const int64_t at = __shfl_sync(0xFFFFFFFFu, offset, row);
         const bool live = at >= 0 && piece * 8 < p.dim;
@@ -200,23 +205,27 @@ template <int DP, bool BF16> struct ARState {
             for (int x = 0; x < 4; ++x) o[n][x] = 0.0f;
     }
 
-    // The 16 keys and values of stage `st`, the first of them key `key`.
+    // The keys and values of stage `st`, the first of them key `key_first`.
     __device__ __forceinline__ void step(const AttnParams &p, uint32_t st, uint32_t key_first, uint32_t lane) {
         using L = ARows<DP>;
-        // S = Q K^T: two 8-key tiles
-        float sc[2][4] = {};
+        constexpr int N = L::KEYS / 8; // 8-key tiles
+        // S = Q K^T
+        float sc[N][4] = {};
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-            uint32_t b[4];
-            const uint32_t row = ((lane >> 4) << 3) + (lane & 7u), piece = k * 2 + ((lane >> 3) & 1u);
-            ldsm4(st + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
-            mma_16816<BF16>(sc[0], qf[k], b[0], b[1]);
-            mma_16816<BF16>(sc[1], qf[k], b[2], b[3]);
+#pragma unroll
+            for (int n = 0; n < N; n += 2) {
+                uint32_t b[4];
+                const uint32_t row = n * 8 + ((lane >> 4) << 3) + (lane & 7u), piece = k * 2 + ((lane >> 3) & 1u);
+                ldsm4(st + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+                mma_16816<BF16>(sc[n], qf[k], b[0], b[1]);
+                mma_16816<BF16>(sc[n + 1], qf[k], b[2], b[3]);
+            }
         }
         const uint32_t key0 = key_first + (lane & 3u) * 2;
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int r = x >> 1;
@@ -246,26 +255,28 @@ template <int DP, bool BF16> struct ARState {
                 for (int x = 0; x < 4; ++x) o[n][x] *= f2[x >> 1];
         }
         const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-        uint32_t pf[4];
+        uint32_t pf[N / 2][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < N; ++n) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 sc[n][x] = exp2_approx(sc[n][x] - base[x >> 1]);
                 l[x >> 1] += sc[n][x];
             }
-            pf[2 * n] = pack_pair<BF16>(sc[n][0], sc[n][1]);
-            pf[2 * n + 1] = pack_pair<BF16>(sc[n][2], sc[n][3]);
+            pf[n / 2][2 * (n & 1)] = pack_pair<BF16>(sc[n][0], sc[n][1]);
+            pf[n / 2][2 * (n & 1) + 1] = pack_pair<BF16>(sc[n][2], sc[n][3]);
         }
         // O += P V
 #pragma unroll
-        for (int n = 0; n < DP / 16; ++n) {
-            uint32_t b[4];
-            const uint32_t row = (((lane >> 3) & 1u) << 3) + (lane & 7u), piece = n * 2 + (lane >> 4);
-            ldsm4_t(st + L::HALF + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
-            mma_16816<BF16>(o[2 * n], pf, b[0], b[1]);
-            mma_16816<BF16>(o[2 * n + 1], pf, b[2], b[3]);
-        }
+        for (int k = 0; k < N / 2; ++k)
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) {
+                uint32_t b[4];
+                const uint32_t row = k * 16 + (((lane >> 3) & 1u) << 3) + (lane & 7u), piece = n * 2 + (lane >> 4);
+                ldsm4_t(st + L::HALF + row * L::ROW_BYTES + ((piece ^ (row & 7u)) << 4), b);
+                mma_16816<BF16>(o[2 * n], pf[k], b[0], b[1]);
+                mma_16816<BF16>(o[2 * n + 1], pf[k], b[2], b[3]);
+            }
     }
 
     // The rows' sums, in every lane of a row's four.
@@ -276,10 +287,11 @@ template <int DP, bool BF16> struct ARState {
     }
 };
 
-// A cache row's place: the offset of the key of lane & 15 among 16 from `key_first` on.
-__device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq &s, uint32_t b, uint32_t head,
+// A cache row's place: the offset of the lane's key (lane modulo the keys of a step) from
+// `key_first` on, or -1: not to be read.
+template <int DP> __device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq &s, uint32_t b, uint32_t head,
                                              uint32_t key_first, uint32_t lane) {
-    const uint32_t key = key_first + (lane & 15u);
+    const uint32_t key = key_first + (lane & (ar_keys(DP) - 1));
     if (key < s.lo || key >= s.kl) return -1;
     const uint32_t page = key / p.page_size;
     const int32_t id = __ldg(p.table + b * p.tb + page);
@@ -308,7 +320,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         mine = 0;
         if (b < p.seqs) {
             const AttnSeq s = attn_seq(p, b, blockIdx.x == 0);
-            const ARShape sh = ar_shape(p, s);
+            const ARShape sh = ar_shape<DP>(p, s);
             mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
         }
         uint64_t sum;
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
             mine = 0;
             if (b < p.seqs) {
                 const AttnSeq s = attn_seq(p, b, false);
-                const ARShape sh = ar_shape(p, s);
+                const ARShape sh = ar_shape<DP>(p, s);
                 mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
             }
             uint64_t sum;
@@ -356,7 +368,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     ARCursor c;
     c.b = s_seq[warp];
     c.s = attn_seq(p, c.b, false);
-    c.sh = ar_shape(p, c.s);
+    c.sh = ar_shape<DP>(p, c.s);
     const uint64_t inside = begin - s_first[warp];
     c.tile = static_cast<uint32_t>(inside / c.sh.steps);
     c.step = static_cast<uint32_t>(inside - static_cast<uint64_t>(c.tile) * c.sh.steps);
@@ -365,13 +377,13 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
     uint32_t fetched = 0;
-    auto place = [&] { return ar_key_at(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * AR_KEYS, lane); };
+    auto place = [&] { return ar_key_at<DP>(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * L::KEYS, lane); };
     int64_t next = place(); // one step ahead of the copies: hides the table's latency
     auto fetch = [&] {
         if (fetched < count) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
             if (++fetched < count) {
-                ar_advance(p, f);
+                ar_advance<DP>(p, f);
                 next = place();
             }
         }
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         }
         cp_async_wait<L::STAGES - 2>();
         __syncwarp();
-        u.step(p, ring + (i % L::STAGES) * L::STAGE, (c.sh.step0 + c.step) * AR_KEYS, lane);
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, (c.sh.step0 + c.step) * L::KEYS, lane);
         __syncwarp(); // every lane has read the stage that the next copies fill
         fetch();
 
@@ -430,7 +442,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
                 }
             }
         }
-        if (i + 1 < count) ar_advance(p, c);
+        if (i + 1 < count) ar_advance<DP>(p, c);
     }
     cp_async_wait<0>();
     after_rows(p);
@@ -478,7 +490,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     before_rows(p);
     let_next();
     const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
-    const ARShape sh = ar_shape(p, s);
+    const ARShape sh = ar_shape<DP>(p, s);
     if (rt >= sh.tiles) { // the whole cluster
         after_rows(p);
         return;
@@ -487,14 +499,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     const uint32_t part = rank * AR_WARPS + warp, parts = ranks * AR_WARPS;
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * part / parts);
     const uint32_t count = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * (part + 1) / parts) - begin;
-    const uint32_t key_first = (sh.step0 + begin) * AR_KEYS;
+    const uint32_t key_first = (sh.step0 + begin) * L::KEYS;
     const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
     uint32_t fetched = 0;
-    int64_t next = count ? ar_key_at(p, s, b, head, key_first, lane) : -1;
+    int64_t next = count ? ar_key_at<DP>(p, s, b, head, key_first, lane) : -1;
     auto fetch = [&] {
         if (fetched < count) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
-            if (++fetched < count) next = ar_key_at(p, s, b, head, key_first + fetched * AR_KEYS, lane);
+            if (++fetched < count) next = ar_key_at<DP>(p, s, b, head, key_first + fetched * L::KEYS, lane);
         }
         cp_async_commit();
     };
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     for (uint32_t i = 0; i < count; ++i) {
         cp_async_wait<L::STAGES - 2>();
         __syncwarp();
-        u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * AR_KEYS, lane);
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * L::KEYS, lane);
         __syncwarp();
         fetch();
     }
@@ -601,7 +613,7 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
     after_stream();
     let_next();
     const AttnSeq s = attn_seq(p, b, false);
-    const ARShape sh = ar_shape(p, s);
+    const ARShape sh = ar_shape<DP>(p, s);
     const uint32_t row = blockIdx.y;
     if (sh.tiles == 0 || row >= s.ql * p.group) return;
     const uint64_t total = p.prefix[p.seqs];

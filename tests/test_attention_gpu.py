@@ -245,7 +245,9 @@ def test_calls_that_overlap(cuda):
 
 def test_the_example_layer(cuda):
     """A whole layer in one chunk, in chunks and token by token: within what two roundings
-    of the stream to bf16 (2^-8 each, relative) and their way through the experts may differ."""
+    of the stream to bf16 (2^-8 each, relative) and their way through the experts may differ,
+    over the rows that took the same experts (a row whose second and third expert are within
+    rounding of each other may take either, and is then another row); those are nearly all."""
     import sys
 
     from conftest import ROOT
@@ -254,12 +256,15 @@ def test_the_example_layer(cuda):
     import decoder_layer as example
 
     config, lens = example.Config(window=100), [130, 1, 77]
-    whole = example.run(config, lens, steps=2)
+    whole, took = example.run(config, lens, steps=2)
     for chunk in (1, 40):
-        parts = example.run(config, lens, steps=2, chunk=chunk)
-        for a, b in zip(whole, parts):
+        parts, took2 = example.run(config, lens, steps=2, chunk=chunk)
+        for a, b, i, j in zip(whole, parts, took, took2):
             assert torch.isfinite(a.float()).all()
-            assert float((a.float() - b.float()).norm() / a.float().norm()) < 4 * 2.0 ** -8
+            same = (i == j).all(1)
+            assert int((~same).sum()) <= 0.05 * same.numel()
+            a, b = a.float()[same], b.float()[same]
+            assert float((a - b).norm() / a.norm()) < 4 * 2.0 ** -8
 
 
 def test_many_sequences(cuda):
