@@ -24,6 +24,11 @@ inline uint64_t a256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
 // kernel that joins the fragments cost less than the SMs that the clusters leave idle.
 constexpr uint32_t CLUSTER_STEPS = 16;
 
+// Keys up to which a unit is one warp's.  Measured against ranges cut evenly, heads of 128:
+// 160 units of 128 keys 9.8 against 13 us, of up to 256 keys 15.8 against 13 to 16, of up to
+// 400 keys 22 against 14; 1024 units of up to 256 keys 20 against 26.
+constexpr uint32_t UNIT_KEYS = 256;
+
 // Rows (tokens x group) up to which a sequence is the rows kernel's: one tile of 16, or
 // two, which read the cache twice (the second time from L2), where all of the batch's keys
 // and values are few (by their bound, max_kv_len each).  Measured, 32 rows a sequence and
@@ -43,10 +48,11 @@ struct AttnPlan {
     uint32_t row_limit;
     bool rows, prompt;       // which kernels have work
     uint32_t cluster;        // CTAs a unit of the cluster form of the rows kernel; 0: the other form
+    bool units;              // a warp a unit
     uint32_t tiles;          // row tiles of a unit's sequence and head, at most
     bool deal;               // prompt kernel: blocks are dealt out, not items
     uint32_t pairs, ctas;    // its pairs of tiles (a bound), and its grid
-    uint64_t prefix, part, part_ml, ppart, ppart_ml, tail, total; // workspace offsets
+    uint64_t prefix, part, part_ml, tail_rows, ppart, ppart_ml, tail, total; // workspace offsets
 };
 
 // Keys that `rows` packed rows of a sequence see together, at most.
@@ -86,10 +92,12 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
         while (c > 1 && (units * c > sms || steps < c * AR_WARPS)) c /= 2;
         if (steps <= static_cast<uint64_t>(c) * AR_WARPS * CLUSTER_STEPS) n.cluster = c;
     }
-    if (n.rows && !n.cluster) {
+    n.units = n.rows && !n.cluster && keys <= UNIT_KEYS;
+    if (n.rows && !n.cluster && !n.units) {
         n.prefix = take((static_cast<uint64_t>(a.seqs) + 1) * 8);
         n.part = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * n.dp * 4);
         n.part_ml = take(static_cast<uint64_t>(n.workers) * 2 * AR_ROWS * 8);
+        n.tail_rows = take(static_cast<uint64_t>(n.workers) * 16);
     }
     if (n.prompt) {
         const uint64_t big = all / ((n.rows ? n.row_limit : 0) + 1);
@@ -201,18 +209,29 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
     if (!rc && n.cluster)
         rc = launch("attn_cluster_kernel", attn_cluster_kernel<DP, BF16>,
                     {dim3(p.seqs * p.kv_heads * n.tiles * n.cluster), AR_THREADS, ARows<DP>::SMEM, n.cluster}, s, p, n.tiles);
-    else if (!rc && n.rows)
+    else if (!rc && n.units) {
+        // a warp a CTA until there is one on every SM
+        const uint64_t units = static_cast<uint64_t>(p.seqs) * p.kv_heads * n.tiles, sms = device_sm_count();
+        const uint32_t warps = units < sms * AR_WARPS ? static_cast<uint32_t>((units + sms - 1) / sms) : AR_WARPS;
+        rc = launch("attn_unit_kernel", attn_unit_kernel<DP, BF16>,
+                    {dim3(static_cast<uint32_t>((units + warps - 1) / warps)), warps * 32,
+                     ARows<DP>::SMEM / AR_WARPS * warps, 1},
+                    s, p, n.tiles);
+    } else if (!rc && n.rows)
         rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16>,
                     {dim3(p.workers / AR_WARPS), AR_THREADS, ARows<DP>::SMEM, 1}, s, p);
     if (!rc && n.prompt && n.deal)
         rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1}, s, pp);
-    if (rc || !n.rows || n.cluster) return rc;
-    const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group;
-    const dim3 grid(p.seqs * p.kv_heads, most < n.row_limit ? static_cast<uint32_t>(most) : n.row_limit);
-    // few units are cut into many fragments each
-    if (static_cast<uint64_t>(p.seqs) * p.kv_heads * 16 <= p.workers)
-        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>, {grid, 32 * 32, 0, 1}, s, p);
-    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, 1}, s, p);
+    if (rc || !n.rows || n.cluster || n.units) return rc;
+    const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group, units = static_cast<uint64_t>(p.seqs) * p.kv_heads;
+    const uint32_t rows = most < n.row_limit ? static_cast<uint32_t>(most) : n.row_limit;
+    // few units are cut into many fragments each; of many units, few are cut
+    if (units * 16 <= p.workers)
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>,
+                      {dim3(static_cast<uint32_t>(units), rows), 32 * 32, 0, 1}, s, p, false);
+    const bool by_worker = units * n.tiles > p.workers;
+    const dim3 grid = by_worker ? dim3(p.workers, rows < AR_ROWS ? rows : AR_ROWS) : dim3(static_cast<uint32_t>(units), rows);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, 1}, s, p, by_worker);
 }
 
 } // namespace
@@ -278,6 +297,7 @@ extern "C" int fmcuda_paged_attention(const fmcuda_paged_attention_args *a, void
     p.prefix = reinterpret_cast<uint64_t *>(ws + n.prefix);
     p.part = reinterpret_cast<float *>(ws + n.part);
     p.part_ml = reinterpret_cast<float2 *>(ws + n.part_ml);
+    p.tail_rows = reinterpret_cast<int4 *>(ws + n.tail_rows);
     p.workers = n.workers;
     p.least = 4;
     p.row_limit = n.rows ? n.row_limit : 0;

@@ -13,11 +13,17 @@
 //
 // Work split: all (sequence, key head, row tile) units laid end to end, in
 // steps of 16 keys, are cut into equal ranges, one a warp; whatever the lengths,
-// every warp reads the same number of bytes.  A unit inside one range is written
+// every warp has the same work.  A unit counts for AR_UNIT_COST steps more than it has (its
+// queries, its result): without that, 512 sequences of 2 to 1200 keys took 259 us, not 207,
+// because some warps had dozens of units of a few keys.  A unit inside one range is written
 // out at once; the fragments of a cut unit leave (O, max, sum) in f32 and
 // attn_combine_kernel joins them, in order, so that the result does not depend
 // on timing.  A warp has at most two fragments: of the unit that began before
 // its range, and of the unit that goes on after it.
+//
+// Measured, 8 key heads of 128: 64 sequences of up to 8192 keys (1.09 GB) 172 us, 98% of
+// the rate of a copy; one sequence of 131071 keys and 4 key heads (268 MB) 57 us, of which
+// the join of 1184 fragments takes 8.
 #pragma once
 
 #include "attention.cuh"
@@ -27,6 +33,7 @@ namespace fmb {
 
 constexpr uint32_t AR_WARPS = 8, AR_THREADS = AR_WARPS * 32;
 constexpr uint32_t AR_ROWS = 16, AR_MAX_CLUSTER = 8;
+constexpr uint32_t AR_UNIT_COST = 2;
 __host__ __device__ constexpr uint32_t ar_keys(int dp) { return dp == 64 ? 32 : 16; } // keys a step
 
 template <int DP> struct ARows {
@@ -51,6 +58,10 @@ template <int DP> __device__ __forceinline__ ARShape ar_shape(const AttnParams &
     const uint32_t last = (s.kl + KEYS - 1) / KEYS;
     r.steps = last > r.step0 ? last - r.step0 : 1; // a unit without keys still writes its zeros
     return r;
+}
+// The sequence's place in the laid-out work; its units are `steps` + AR_UNIT_COST long, the cost first.
+__device__ __forceinline__ uint64_t ar_length(const AttnParams &p, const ARShape &sh) {
+    return static_cast<uint64_t>(sh.tiles) * p.kv_heads * (sh.steps + AR_UNIT_COST);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -95,6 +106,7 @@ __device__ __forceinline__ void after_rows(const AttnParams &p) {
 // A place in the laid-out work.
 struct ARCursor {
     uint32_t b, tile, step; // tile: key head * row tiles + row tile
+    uint32_t at;            // from the range's begin
     AttnSeq s;
     ARShape sh;
 };
@@ -110,8 +122,10 @@ template <int DP> __device__ __forceinline__ void ar_enter(const AttnParams &p, 
 }
 
 template <int DP> __device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
+    ++c.at;
     if (++c.step < c.sh.steps) return;
     c.step = 0;
+    c.at += AR_UNIT_COST;
     if (++c.tile < c.sh.tiles * p.kv_heads) return;
     c.tile = 0;
     ++c.b;
@@ -302,6 +316,24 @@ template <int DP> __device__ __forceinline__ int64_t ar_key_at(const AttnParams 
     return id * p.cp + static_cast<int64_t>(key - page * p.page_size) * p.cr + head * p.ch;
 }
 
+// The result of row r of the lane's two, row `row` of the sequence and key head.
+template <int DP, bool BF16>
+__device__ __forceinline__ void ar_store_row(const AttnParams &p, const AttnSeq &s, uint32_t head, uint32_t row,
+                                             const ARState<DP, BF16> &u, int r, float sum, uint32_t lane) {
+    const uint32_t t = row / p.group, g = row - t * p.group;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
+    uint16_t *dst = static_cast<uint16_t *>(p.out) + token * p.ot + h * p.oh;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+        const uint32_t col = n * 8 + (lane & 3u) * 2;
+        if (col < p.dim)
+            *reinterpret_cast<uint32_t *>(dst + col) = pack_pair<BF16>(u.o[n][2 * r] * inv, u.o[n][2 * r + 1] * inv);
+    }
+    if (p.lse && (lane & 3u) == 0)
+        p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : u.m[r] * 0.6931471805599453f + logf(sum);
+}
+
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnParams p) {
     using L = ARows<DP>;
@@ -321,7 +353,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         if (b < p.seqs) {
             const AttnSeq s = attn_seq(p, b, blockIdx.x == 0);
             const ARShape sh = ar_shape<DP>(p, s);
-            mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
+            mine = ar_length(p, sh);
         }
         uint64_t sum;
         before = ar_block_scan(mine, s_part, &sum);
@@ -339,7 +371,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
             if (b < p.seqs) {
                 const AttnSeq s = attn_seq(p, b, false);
                 const ARShape sh = ar_shape<DP>(p, s);
-                mine = static_cast<uint64_t>(sh.tiles) * p.kv_heads * sh.steps;
+                mine = ar_length(p, sh);
             }
             uint64_t sum;
             before = running + ar_block_scan(mine, s_part, &sum);
@@ -359,33 +391,37 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     __syncthreads();
     const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
     const uint64_t begin = worker * per;
+    int4 tail = make_int4(-1, 0, 0, 0); // the unit that begins here and goes on after the range
     if (begin >= total) {
+        if (lane == 0) p.tail_rows[worker] = tail;
         after_rows(p);
         return;
     }
-    const uint32_t count = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
+    const uint32_t end = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
 
     ARCursor c;
     c.b = s_seq[warp];
     c.s = attn_seq(p, c.b, false);
     c.sh = ar_shape<DP>(p, c.s);
     const uint64_t inside = begin - s_first[warp];
-    c.tile = static_cast<uint32_t>(inside / c.sh.steps);
-    c.step = static_cast<uint32_t>(inside - static_cast<uint64_t>(c.tile) * c.sh.steps);
+    const uint32_t unit = c.sh.steps + AR_UNIT_COST;
+    c.tile = static_cast<uint32_t>(inside / unit);
+    const uint32_t in_unit = static_cast<uint32_t>(inside - static_cast<uint64_t>(c.tile) * unit);
+    c.step = in_unit > AR_UNIT_COST ? in_unit - AR_UNIT_COST : 0;
+    c.at = in_unit < AR_UNIT_COST ? AR_UNIT_COST - in_unit : 0;
 
     // ---- the stream of keys -------------------------------------------------------
     const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
     uint32_t fetched = 0;
     auto place = [&] { return ar_key_at<DP>(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * L::KEYS, lane); };
-    int64_t next = place(); // one step ahead of the copies: hides the table's latency
+    int64_t next = c.at < end ? place() : -1; // one step ahead of the copies: hides the table's latency
     auto fetch = [&] {
-        if (fetched < count) {
+        if (f.at < end) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
-            if (++fetched < count) {
-                ar_advance<DP>(p, f);
-                next = place();
-            }
+            ++fetched;
+            ar_advance<DP>(p, f);
+            if (f.at < end) next = place();
         }
         cp_async_commit();
     };
@@ -395,7 +431,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     ARState<DP, BF16> u;
     bool fresh = true;
     uint32_t first_step = 0;
-    for (uint32_t i = 0; i < count; ++i) {
+    for (uint32_t i = 0; c.at < end; ++i) {
         const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
         if (fresh) {
             fresh = false;
@@ -408,30 +444,22 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         __syncwarp(); // every lane has read the stage that the next copies fill
         fetch();
 
-        if (c.step + 1 == c.sh.steps || i + 1 == count) {
+        const bool done = c.step + 1 == c.sh.steps;
+        if (done || c.at + 1 == end) {
             fresh = true;
-            const bool whole = first_step == 0 && c.step + 1 == c.sh.steps;
+            const bool whole = first_step == 0 && done;
+            if (first_step == 0 && !done) {
+                const uint64_t last = static_cast<uint64_t>(c.at) + (c.sh.steps - 1 - c.step);
+                tail = make_int4(static_cast<int>(c.b), static_cast<int>(c.tile), static_cast<int>(last / per) + 1, 0);
+            }
             const uint64_t slot = worker * 2 + (first_step == 0 ? 1 : 0);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const float sum = u.sum(r);
                 const uint32_t in = lane / 4 + r * 8, row = rt * AR_ROWS + in;
-                const uint32_t t = row / p.group, g = row - t * p.group;
-                if (t >= c.s.ql) continue;
+                if (row >= c.s.ql * p.group) continue;
                 if (whole) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(c.s.q0) + t;
-                    uint16_t *dst = static_cast<uint16_t *>(p.out) + token * p.ot + h * p.oh;
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        const uint32_t col = n * 8 + (lane & 3u) * 2;
-                        if (col < p.dim)
-                            *reinterpret_cast<uint32_t *>(dst + col) =
-                                pack_pair<BF16>(u.o[n][2 * r] * inv, u.o[n][2 * r + 1] * inv);
-                    }
-                    if (p.lse && (lane & 3u) == 0)
-                        p.lse[token * p.heads + h] =
-                            sum == 0.0f ? -INFINITY : u.m[r] * 0.6931471805599453f + logf(sum);
+                    ar_store_row<DP, BF16>(p, c.s, head, row, u, r, sum, lane);
                 } else {
                     float *dst = p.part + (slot * AR_ROWS + in) * DP;
 #pragma unroll
@@ -442,8 +470,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
                 }
             }
         }
-        if (i + 1 < count) ar_advance<DP>(p, c);
+        ar_advance<DP>(p, c);
     }
+    if (lane == 0) p.tail_rows[worker] = tail;
     cp_async_wait<0>();
     after_rows(p);
 }
@@ -600,30 +629,101 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     after_rows(p);
 }
 
-// Joins the fragments of the units that were cut: a CTA of W warps a unit and row.
-// Warp i takes fragments i, i + W, ..., a lane four (two) values of the head, with the
-// loads of F fragments under way together.
+// ---- many units of very short sequences: a warp each ------------------------------
+//
+// Where a unit has few steps, reading is soon done and what is around it counts: the
+// warps of a CTA take a unit each, from its first key to its last, and write its rows.
+// No sums over the sequences to find the work, no fragments, one launch.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnParams p, uint32_t unit_tiles) {
+    using L = ARows<DP>;
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t unit = warp * gridDim.x + blockIdx.x, rt = unit % unit_tiles;
+    const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
+    before_rows(p);
+    let_next();
+    if (b < p.seqs) {
+        const AttnSeq s = attn_seq(p, b, lane == 0 && rt == 0 && head == 0);
+        const ARShape sh = ar_shape<DP>(p, s);
+        if (rt < sh.tiles) {
+            const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE), key_first = sh.step0 * L::KEYS;
+            uint32_t fetched = 0;
+            int64_t next = ar_key_at<DP>(p, s, b, head, key_first, lane);
+            auto fetch = [&] {
+                if (fetched < sh.steps) {
+                    ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
+                    if (++fetched < sh.steps) next = ar_key_at<DP>(p, s, b, head, key_first + fetched * L::KEYS, lane);
+                }
+                cp_async_commit();
+            };
+#pragma unroll
+            for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
+            ARState<DP, BF16> u;
+            u.begin(p, s, head, rt, lane);
+            for (uint32_t i = 0; i < sh.steps; ++i) {
+                cp_async_wait<L::STAGES - 2>();
+                __syncwarp();
+                u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * L::KEYS, lane);
+                __syncwarp();
+                fetch();
+            }
+            cp_async_wait<0>();
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float sum = u.sum(r);
+                const uint32_t row = rt * AR_ROWS + lane / 4 + r * 8;
+                if (row < s.ql * p.group) ar_store_row<DP, BF16>(p, s, head, row, u, r, sum, lane);
+            }
+        }
+    }
+    after_rows(p);
+}
+
+// Joins the fragments of the units that were cut.  A CTA of W warps takes a row of a
+// unit: of unit blockIdx.x, or, where there are more units than warps in the rows kernel,
+// of the unit that was cut at the end of warp blockIdx.x's range.  Warp i takes fragments
+// i, i + W, ..., a lane four (two) values of the head, with the loads of F fragments under
+// way together.
 template <int DP, bool BF16, int W, int F>
-__global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p, bool by_worker) {
     constexpr int V = DP / 32;
     __shared__ float s_o[W][DP];
     __shared__ float s_m[W], s_l[W];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t b = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
     after_stream();
     let_next();
-    const AttnSeq s = attn_seq(p, b, false);
-    const ARShape sh = ar_shape<DP>(p, s);
-    const uint32_t row = blockIdx.y;
-    if (sh.tiles == 0 || row >= s.ql * p.group) return;
-    const uint64_t total = p.prefix[p.seqs];
-    const uint64_t even = (total + p.workers - 1) / p.workers;
-    const uint64_t per = even > p.least ? even : p.least;
+    AttnSeq s;
+    uint32_t head, row, n;
+    uint64_t w0;
+    if (by_worker) {
+        const int4 tail = p.tail_rows[blockIdx.x];
+        if (tail.x < 0) return;
+        s = attn_seq(p, static_cast<uint32_t>(tail.x), false);
+        const ARShape sh = ar_shape<DP>(p, s);
+        const uint32_t tile = static_cast<uint32_t>(tail.y);
+        head = tile / sh.tiles;
+        row = (tile - head * sh.tiles) * AR_ROWS + blockIdx.y;
+        n = static_cast<uint32_t>(tail.z);
+        w0 = blockIdx.x;
+        if (row >= s.ql * p.group) return;
+    } else {
+        const uint32_t b = blockIdx.x / p.kv_heads;
+        head = blockIdx.x % p.kv_heads;
+        row = blockIdx.y;
+        s = attn_seq(p, b, false);
+        const ARShape sh = ar_shape<DP>(p, s);
+        if (sh.tiles == 0 || row >= s.ql * p.group) return;
+        const uint64_t total = p.prefix[p.seqs];
+        const uint64_t even = (total + p.workers - 1) / p.workers;
+        const uint64_t per = even > p.least ? even : p.least;
+        const uint64_t first = p.prefix[b] + AR_UNIT_COST +
+                               static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * (sh.steps + AR_UNIT_COST);
+        w0 = first / per;
+        n = static_cast<uint32_t>((first + sh.steps - 1) / per - w0) + 1;
+        if (n == 1) return; // written by its one warp
+    }
     const uint32_t t = row / p.group, g = row % p.group, in = row % AR_ROWS;
-    const uint64_t first = p.prefix[b] + static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * sh.steps;
-    const uint64_t w0 = first / per;
-    const uint32_t n = static_cast<uint32_t>((first + sh.steps - 1) / per - w0) + 1;
-    if (n == 1) return; // written by its one warp
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
     for (uint32_t f0 = warp; f0 < n; f0 += F * W) {
         float2 ml[F];

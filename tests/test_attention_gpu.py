@@ -273,6 +273,20 @@ def test_many_sequences(cuda):
     check(Batch(lens, 4, 2, 64, 16, seed=9), cuda)
 
 
+@pytest.mark.parametrize("lens,heads,kv_heads,dim,window", [
+    ([(1, 1 + (37 * b) % 600) for b in range(700)], 4, 2, 128, 0),                  # more units than warps, cut, past 256 sequences
+    ([(b % 4, 2 + b % 9 if b % 50 else 1500) for b in range(300)], 16, 4, 64, 0),   # many tiny units around long ones
+    ([(1 + b % 8, 8 + b * 13 % 600) for b in range(90)], 64, 16, 96, 0),            # two row tiles, more units than warps
+    ([(1, 1 + (37 * b) % 256) for b in range(200)], 8, 2, 128, 0),                  # a warp a unit
+    ([(b % 5, 4 + b * 7 % 250) for b in range(60)], 16, 4, 80, 0),                  # the same, two row tiles, some without rows
+    ([(1, b % 3) for b in range(170)], 8, 1, 64, 0),                                # units without keys
+    ([(2, 9000 - 40 * b) for b in range(100)], 8, 4, 64, 100),                      # short by their window
+    ([(1, 1 + b % 200) for b in range(150)] + [(70, 256)], 8, 2, 128, 0),           # beside a chunk
+])
+def test_many_units(cuda, lens, heads, kv_heads, dim, window):
+    check(Batch(lens, heads, kv_heads, dim, 32, window=window, seed=33), cuda)
+
+
 def test_sharp_and_growing_scores(cuda):
     """Scores of some hundred, the largest one last: the running maximum moves at every step."""
     b = Batch([(1, 600), (140, 600)], 4, 2, 64, 16, torch.float16, seed=5, q_scale=4.0)
