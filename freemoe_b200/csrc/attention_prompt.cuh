@@ -31,7 +31,9 @@
 // back.  Where there are few, all their blocks laid end to end are cut into equal
 // ranges, one a CTA; the cut items' fragments (O, m, sum) are added up in order
 // by attn_join_kernel.  A CTA has at most two: of the item that began before its
-// range and of the one that goes on after it.
+// range and of the one that goes on after it.  Where there are fewer items than CTAs,
+// each is cut into pieces of its own, so that no CTA begins a second item (8 chunks of 128
+// behind 2000 keys: 69 -> 51 us); not with the rows kernel beside, which wants SMs.
 #pragma once
 
 #include "attention.cuh"
@@ -41,8 +43,11 @@ namespace fmb {
 
 constexpr uint32_t AP_THREADS = 384, AP_TILE = 128, AP_PAIR = 256, AP_KEYS = 128;
 // Where blocks are dealt out: what an item costs beside its blocks (its Q, its
-// result), in blocks, and the least that a CTA takes.
+// result), in blocks, and the least that a CTA takes.  Where each CTA has a piece of
+// one item: its least blocks, and the blocks that cutting the longest item has to
+// save, for the fragments and their join.
 constexpr uint32_t AP_ITEM_COST = 5, AP_LEAST_COST = 6 + AP_ITEM_COST;
+constexpr uint32_t AP_LEAST_PIECE = 4, AP_LEAST_SAVED = 4;
 constexpr uint32_t AP_MAX_PAIRS = 1024; // pairs of tiles whose blocks can be dealt out
 
 template <int DP> struct APrompt {
@@ -237,6 +242,7 @@ struct APWalk {
     uint32_t b, pair, head, off; // dealt blocks: the next item, and the cost of it that is not this CTA's
     uint64_t left;               // cost left; or items in all
     uint32_t round;              // dealt items
+    uint32_t piece;              // blocks of a piece where each CTA has one piece of one item; else 0
 };
 struct APSeg {
     AttnSeq s;
@@ -304,12 +310,14 @@ __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g)
         g.starts = g.whole = true;
         if (pp.deal) {
             // the item's cost lies before its blocks: a range that ends in it has none of them
-            const uint32_t cost = span.y - span.x + AP_ITEM_COST;
+            const uint32_t len = span.y - span.x, before = w.piece ? 0 : AP_ITEM_COST;
+            const uint32_t cost = w.piece ? (len + w.piece - 1) / w.piece * w.piece : len + before;
             const uint32_t take = cost - w.off > w.left ? static_cast<uint32_t>(w.left) : cost - w.off;
             const uint32_t end = w.off + take;
-            g.jb += w.off > AP_ITEM_COST ? w.off - AP_ITEM_COST : 0;
-            g.je = span.x + (end > AP_ITEM_COST ? end - AP_ITEM_COST : 0);
-            g.starts = w.off <= AP_ITEM_COST;
+            const uint32_t last = end > before ? end - before : 0;
+            g.jb += w.off > before ? w.off - before : 0;
+            g.je = span.x + (last < len ? last : len);
+            g.starts = w.off <= before;
             g.whole = g.starts && end == cost;
             w.left -= take;
             w.off = 0;
@@ -426,13 +434,43 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const AttnSeq s = attn_seq(p, seq_of[lo], false);
             const uint32_t row0 = (i - first_of[lo]) * AP_PAIR;
             const uint2 span = ap_span(ap_tile(p, s, row0), ap_tile(p, s, row0 + AP_TILE));
-            cost_before[i + 1] = span.y - span.x + AP_ITEM_COST;
+            cost_before[i + 1] = span.y - span.x;
         }
         __syncthreads();
         if (warp == 0) {
+            uint32_t piece = 0;
+            const uint32_t budget = gridDim.x / p.kv_heads; // pieces that the CTAs take of one head's items
+            if (pairs && pairs <= budget && !p.row_limit) {
+                // the shortest pieces of which there are no more than CTAs
+                uint32_t all = 0, longest = 0;
+                for (uint32_t i = lane; i < pairs; i += 32) {
+                    const uint32_t len = static_cast<uint32_t>(cost_before[i + 1]);
+                    all += len;
+                    longest = len > longest ? len : longest;
+                }
+                all = __reduce_add_sync(0xFFFFFFFFu, all);
+                longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+                uint32_t lo = (all + budget - 1) / budget, hi = longest;
+                while (lo < hi) {
+                    const uint32_t mid = (lo + hi) / 2;
+                    uint32_t n = 0;
+                    for (uint32_t i = lane; i < pairs; i += 32)
+                        n += (static_cast<uint32_t>(cost_before[i + 1]) + mid - 1) / mid;
+                    if (__reduce_add_sync(0xFFFFFFFFu, n) <= budget)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+                piece = lo < AP_LEAST_PIECE ? AP_LEAST_PIECE : lo;
+                if (piece + AP_LEAST_SAVED > longest) piece = longest;
+                // many CTAs idle: even ranges are shorter, with what a second item in them costs
+                if (piece > all * p.kv_heads / gridDim.x + AP_LEAST_SAVED) piece = 0;
+            }
+            if (lane == 0) misc[0] = piece;
             uint64_t before = 0;
             for (uint32_t i0 = 0; i0 < pairs; i0 += 32) {
                 uint64_t inc = i0 + lane < pairs ? cost_before[i0 + lane + 1] : 0;
+                if (inc) inc = piece ? (static_cast<uint32_t>(inc) + piece - 1) / piece * piece : inc + AP_ITEM_COST;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint64_t t = __shfl_up_sync(0xFFFFFFFFu, inc, o);
@@ -445,7 +483,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         __syncthreads();
         const uint64_t total = cost_before[pairs] * p.kv_heads, even = (total + gridDim.x - 1) / gridDim.x;
-        per = even > AP_LEAST_COST ? even : AP_LEAST_COST;
+        walk.piece = misc[0];
+        per = walk.piece ? walk.piece : even > AP_LEAST_COST ? even : AP_LEAST_COST;
         const uint64_t begin = blockIdx.x * per;
         if (threadIdx.x == 0) pp.tail[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (begin >= total) return;

@@ -205,6 +205,17 @@ def test_ways_of_dealing_out_the_work(cuda, lens, heads, kv_heads, dim):
     check(Batch(lens, heads, kv_heads, dim, 64, seed=21), cuda)
 
 
+@pytest.mark.parametrize("lens,heads,kv_heads,dim,window", [
+    ([(100, 2000)], 32, 8, 128, 0),                                 # sixteen items, pieces of a few blocks
+    ([(64, 9000), (0, 50), (700, 1500), (33, 33)], 16, 2, 64, 0),   # long and short items, some not cut, one empty
+    ([(300, 9000), (64, 64)], 8, 2, 128, 3000),                     # the pieces begin at the window
+    ([(40, 1700 + 300 * b) for b in range(30)], 16, 4, 96, 0),      # pieces close to whole items: even ranges
+    ([(260, 20), (300, 5000)], 8, 1, 80, 0),                        # rows without keys in an item that is not cut
+])
+def test_pieces_of_items(cuda, lens, heads, kv_heads, dim, window):
+    check(Batch(lens, heads, kv_heads, dim, 32, window=window, seed=41), cuda)
+
+
 def test_not_a_number_stays_in_its_row(cuda):
     """A NaN in a query row gives NaN there and nowhere else; an infinite score gives NaN."""
     for value in (float("nan"), float("inf")):
