@@ -33,7 +33,7 @@
 // by attn_join_kernel.  A CTA has at most two: of the item that began before its
 // range and of the one that goes on after it.  Where there are fewer items than CTAs,
 // each is cut into pieces of its own, so that no CTA begins a second item (8 chunks of 128
-// behind 2000 keys: 69 -> 51 us); not with the rows kernel beside, which wants SMs.
+// behind 2000 keys: 69 -> 51 us; of 200 behind 3000 beside 3 decoding sequences 43 -> 36).
 #pragma once
 
 #include "attention.cuh"
@@ -439,8 +439,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         __syncthreads();
         if (warp == 0) {
             uint32_t piece = 0;
-            const uint32_t budget = gridDim.x / p.kv_heads; // pieces that the CTAs take of one head's items
-            if (pairs && pairs <= budget && !p.row_limit) {
+            // pieces that the CTAs take of one head's items; the rows kernel's keep half of the SMs
+            const uint32_t budget = gridDim.x / (p.row_limit ? 2u : 1u) / p.kv_heads;
+            if (pairs && pairs <= budget) {
                 // the shortest pieces of which there are no more than CTAs
                 uint32_t all = 0, longest = 0;
                 for (uint32_t i = lane; i < pairs; i += 32) {
