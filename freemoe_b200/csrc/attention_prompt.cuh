@@ -34,6 +34,11 @@
 // range and of the one that goes on after it.  Where there are fewer items than CTAs,
 // each is cut into pieces of its own, so that no CTA begins a second item (8 chunks of 128
 // behind 2000 keys: 69 -> 51 us; of 200 behind 3000 beside 3 decoding sequences 43 -> 36).
+//
+// Measured: a prompt of 8192, 32/8 heads of 128, bf16: 545 us, 1.0 PFLOP/s of the 1.66 of a
+// library product, with the tensor pipe 54% busy and the exponentials 54% at 1.64 GHz (the
+// power cap): a block's two tiles take 3200 cycles where either alone would take 2048.
+// Chunks behind contexts, heads of 64: 158 us, bound by the exponentials (58%).
 #pragma once
 
 #include "attention.cuh"
