@@ -226,12 +226,15 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
     const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group, units = static_cast<uint64_t>(p.seqs) * p.kv_heads;
     const uint32_t rows = most < n.row_limit ? static_cast<uint32_t>(most) : n.row_limit;
     // few units are cut into many fragments each; of many units, few are cut
-    if (units * 16 <= p.workers)
-        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5>,
-                      {dim3(static_cast<uint32_t>(units), rows), 32 * 32, 0, 1}, s, p, false);
+    if (units * 16 <= p.workers) {
+        const dim3 whole(static_cast<uint32_t>(units), rows), parts(static_cast<uint32_t>(units), rows * 2);
+        if (units * rows * 2 <= static_cast<uint64_t>(device_sm_count())) // one such CTA an SM
+            return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5, 2>, {parts, 32 * 32, 0, 1}, s, p, false);
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 32, 5, 1>, {whole, 32 * 32, 0, 1}, s, p, false);
+    }
     const bool by_worker = units * n.tiles > p.workers;
     const dim3 grid = by_worker ? dim3(p.workers, rows < AR_ROWS ? rows : AR_ROWS) : dim3(static_cast<uint32_t>(units), rows);
-    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2>, {grid, 4 * 32, 0, 1}, s, p, by_worker);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, 4, 2, 1>, {grid, 4 * 32, 0, 1}, s, p, by_worker);
 }
 
 } // namespace

@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         total += sum;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.seqs] = total;
-    const uint64_t even = (total + p.workers - 1) / p.workers;
+    const uint64_t even = quotient(total + p.workers - 1, p.workers);
     const uint64_t per = even > p.least ? even : p.least;
     uint64_t running = 0;
     for (uint32_t b0 = 0; b0 < p.seqs; b0 += AR_THREADS) {
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     c.sh = ar_shape<DP>(p, c.s);
     const uint64_t inside = begin - s_first[warp];
     const uint32_t unit = c.sh.steps + AR_UNIT_COST;
-    c.tile = static_cast<uint32_t>(inside / unit);
+    c.tile = static_cast<uint32_t>(quotient(inside, unit));
     const uint32_t in_unit = static_cast<uint32_t>(inside - static_cast<uint64_t>(c.tile) * unit);
     c.step = in_unit > AR_UNIT_COST ? in_unit - AR_UNIT_COST : 0;
     c.at = in_unit < AR_UNIT_COST ? AR_UNIT_COST - in_unit : 0;
@@ -413,9 +413,13 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     // ---- the stream of keys -------------------------------------------------------
     const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
+    ARState<DP, BF16> u;
+    uint32_t first_step = c.step;
+    bool fresh = false;
     uint32_t fetched = 0;
     auto place = [&] { return ar_key_at<DP>(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * L::KEYS, lane); };
     int64_t next = c.at < end ? place() : -1; // one step ahead of the copies: hides the table's latency
+    if (c.at < end) u.begin(p, c.s, c.tile / c.sh.tiles, c.tile % c.sh.tiles, lane); // its loads before the keys'
     auto fetch = [&] {
         if (f.at < end) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
@@ -428,9 +432,6 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
 #pragma unroll
     for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
 
-    ARState<DP, BF16> u;
-    bool fresh = true;
-    uint32_t first_step = 0;
     for (uint32_t i = 0; c.at < end; ++i) {
         const uint32_t head = c.tile / c.sh.tiles, rt = c.tile - head * c.sh.tiles;
         if (fresh) {
@@ -450,7 +451,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
             const bool whole = first_step == 0 && done;
             if (first_step == 0 && !done) {
                 const uint64_t last = static_cast<uint64_t>(c.at) + (c.sh.steps - 1 - c.step);
-                tail = make_int4(static_cast<int>(c.b), static_cast<int>(c.tile), static_cast<int>(last / per) + 1, 0);
+                tail = make_int4(static_cast<int>(c.b), static_cast<int>(c.tile),
+                                 static_cast<int>(quotient(last, per)) + 1, 0);
             }
             const uint64_t slot = worker * 2 + (first_step == 0 ? 1 : 0);
 #pragma unroll
@@ -648,8 +650,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnPara
         const ARShape sh = ar_shape<DP>(p, s);
         if (rt < sh.tiles) {
             const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE), key_first = sh.step0 * L::KEYS;
+            ARState<DP, BF16> u;
             uint32_t fetched = 0;
             int64_t next = ar_key_at<DP>(p, s, b, head, key_first, lane);
+            u.begin(p, s, head, rt, lane); // its loads before the keys'
             auto fetch = [&] {
                 if (fetched < sh.steps) {
                     ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
@@ -659,8 +663,6 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnPara
             };
 #pragma unroll
             for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
-            ARState<DP, BF16> u;
-            u.begin(p, s, head, rt, lane);
             for (uint32_t i = 0; i < sh.steps; ++i) {
                 cp_async_wait<L::STAGES - 2>();
                 __syncwarp();
@@ -680,19 +682,21 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnPara
     after_rows(p);
 }
 
-// Joins the fragments of the units that were cut.  A CTA of W warps takes a row of a
-// unit: of unit blockIdx.x, or, where there are more units than warps in the rows kernel,
-// of the unit that was cut at the end of warp blockIdx.x's range.  Warp i takes fragments
-// i, i + W, ..., a lane four (two) values of the head, with the loads of F fragments under
+// Joins the fragments of the units that were cut.  A CTA of W warps takes a row (one of C
+// parts of it, so that few rows keep more SMs busy) of a unit: of unit blockIdx.x, or, where
+// there are more units than warps in the rows kernel, of the unit that was cut at the end of
+// warp blockIdx.x's range.  Warp i takes fragments
+// i, i + W, ..., a lane DP / 32 / C values of the head, with the loads of F fragments under
 // way together.
-template <int DP, bool BF16, int W, int F>
+template <int DP, bool BF16, int W, int F, int C>
 __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p, bool by_worker) {
-    constexpr int V = DP / 32;
-    __shared__ float s_o[W][DP];
+    constexpr int V = DP / 32 / C;
+    __shared__ float s_o[W][DP / C];
     __shared__ float s_m[W], s_l[W];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     after_stream();
     let_next();
+    const uint32_t y = blockIdx.y / C, col0 = blockIdx.y % C * (DP / C);
     AttnSeq s;
     uint32_t head, row, n;
     uint64_t w0;
@@ -703,24 +707,27 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
         const ARShape sh = ar_shape<DP>(p, s);
         const uint32_t tile = static_cast<uint32_t>(tail.y);
         head = tile / sh.tiles;
-        row = (tile - head * sh.tiles) * AR_ROWS + blockIdx.y;
+        row = (tile - head * sh.tiles) * AR_ROWS + y;
         n = static_cast<uint32_t>(tail.z);
         w0 = blockIdx.x;
         if (row >= s.ql * p.group) return;
     } else {
         const uint32_t b = blockIdx.x / p.kv_heads;
         head = blockIdx.x % p.kv_heads;
-        row = blockIdx.y;
+        row = y;
+        // with the lengths where all CTAs have a row; where many have none, they go without it
+        uint64_t total = 0, before = 0;
+        if (W == 32) total = p.prefix[p.seqs], before = p.prefix[b];
         s = attn_seq(p, b, false);
         const ARShape sh = ar_shape<DP>(p, s);
         if (sh.tiles == 0 || row >= s.ql * p.group) return;
-        const uint64_t total = p.prefix[p.seqs];
-        const uint64_t even = (total + p.workers - 1) / p.workers;
+        if (W != 32) total = p.prefix[p.seqs], before = p.prefix[b];
+        const uint64_t even = quotient(total + p.workers - 1, p.workers);
         const uint64_t per = even > p.least ? even : p.least;
-        const uint64_t first = p.prefix[b] + AR_UNIT_COST +
+        const uint64_t first = before + AR_UNIT_COST +
                                static_cast<uint64_t>(head * sh.tiles + row / AR_ROWS) * (sh.steps + AR_UNIT_COST);
-        w0 = first / per;
-        n = static_cast<uint32_t>((first + sh.steps - 1) / per - w0) + 1;
+        w0 = quotient(first, per);
+        n = static_cast<uint32_t>(quotient(first + sh.steps - 1, per) - w0) + 1;
         if (n == 1) return; // written by its one warp
     }
     const uint32_t t = row / p.group, g = row % p.group, in = row % AR_ROWS;
@@ -736,7 +743,7 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
                 const uint64_t slot = ((w0 + f) * 2 + (f == 0 ? 1 : 0)) * AR_ROWS + in;
                 ml[x] = p.part_ml[slot];
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[x][i] = p.part[slot * DP + lane * V + i];
+                for (int i = 0; i < V; ++i) v[x][i] = p.part[slot * DP + col0 + lane * V + i];
             }
         }
 #pragma unroll
@@ -757,8 +764,8 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
         s_l[warp] = l;
     }
     __syncthreads();
-    const uint32_t col = threadIdx.x * 2;
-    if (col >= p.dim) return;
+    const uint32_t in_part = threadIdx.x * 2, col = col0 + in_part;
+    if (in_part >= DP / C || col >= p.dim) return;
     float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) top = fmaxf(top, s_m[w]);
@@ -766,8 +773,8 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
     for (uint32_t w = 0; w < W; ++w) {
         const float f = s_m[w] == -INFINITY ? 0.0f : exp2_approx(s_m[w] - top);
         sum += s_l[w] * f;
-        a0 += s_o[w][col] * f;
-        a1 += s_o[w][col + 1] * f;
+        a0 += s_o[w][in_part] * f;
+        a1 += s_o[w][in_part + 1] * f;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
