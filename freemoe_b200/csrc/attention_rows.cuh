@@ -748,9 +748,12 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
         }
 #pragma unroll
         for (uint32_t x = 0; x < F; ++x) {
-            if (ml[x].x == -INFINITY) continue;
+            if (f0 + x * W >= n) break;
+            // a fragment without a largest exponent weighs nothing, but is added: if its scores
+            // were NaN so are its sums, and times zero they stay that
             const float to = fmaxf(m, ml[x].x);
-            const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to), fb = exp2_approx(ml[x].x - to);
+            const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - to);
+            const float fb = ml[x].x == -INFINITY ? 0.0f : exp2_approx(ml[x].x - to);
             m = to;
             l = l * fa + ml[x].y * fb;
 #pragma unroll
