@@ -113,16 +113,21 @@ __device__ __forceinline__ void store_e4m3(const NormParams &p, uint64_t row, ui
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     // Quotients as a product with the reciprocal and one correction by the product's error,
-    // which a fused operation gives exactly: correctly rounded but for rare cases.  (A code
-    // is a rounding of its quotient: an error in the last bit flips codes.)
+    // which a fused operation gives exactly (Markstein, IBM J. Res. Dev. 34, 1990): correctly
+    // rounded but for rare cases.  (A code is a rounding of its quotient: an error in the last
+    // bit flips codes.)
     auto quotient = [](float x, float y, float inv) {
         const float q = x * inv;
         return fmaf(fmaf(-q, y, x), inv, q);
     };
-    const float scale = quotient(fmaxf(top, 1e-10f), 448.0f, 1.0f / 448.0f);
+    // An infinite scale has no correction (it would be infinity times zero): inv is 0 then, a
+    // finite value by it 0 and an infinite one NaN, and with 0 for the divisor they stay so.
+    const bool finite = top < INFINITY;
+    const float scale = finite ? quotient(fmaxf(top, 1e-10f), 448.0f, 1.0f / 448.0f) : INFINITY;
+    const float divisor = finite ? scale : 0.0f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(scale));
-    auto code = [&](float x) { return quotient(x, scale, inv); };
+    auto code = [&](float x) { return quotient(x, divisor, inv); };
     uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
     const uint32_t groups = (p.d + 127) / 128;
     if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;

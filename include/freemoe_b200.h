@@ -605,7 +605,8 @@ int fmcuda_record_load(fmcuda_record_loader *loader, const fmcuda_extent *extent
  * reads h before any rounding.  y_dtype FM_X_E4M3 writes 8-bit codes and one f32
  * scale for each 128 consecutive values of a row (the last group may be shorter):
  *   scale = max(largest |y| of the group, 1e-10) / 448,  y ~ code * scale;
- * a NaN is coded as NaN and does not count for the largest.
+ * a NaN is coded as NaN and does not count for the largest.  Where the largest is infinite
+ * the scale is, finite values are coded 0 and infinite ones NaN.
  * y may be x and residual_out may be residual where type and stride are the same. */
 typedef struct fmcuda_rms_norm_args {
     const void *x;              /* [tokens][d_model] */

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from test_attention_gpu import Batch
+from test_norm_rope_gpu import tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,31 @@ def test_not_a_number_of_many_keys_outlives_the_join(cuda, lens, heads, kv_heads
     assert torch.isnan(got[:rows, :group]).all() and torch.isnan(lse[:rows, :group]).all()
     got[:rows, :group], lse[:rows, :group] = want[:rows, :group], want_lse[:rows, :group]
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+# widths of 16-byte accesses, of pairs and of single values, in a warp, in a CTA and read twice
+@pytest.mark.parametrize("d", [512, 514, 513, 4096, 4098, 4097, 20000, 20002, 20001])
+def test_infinite_results_to_8_bits(cuda, d):
+    """The scale of a group with an infinity is infinite: finite values are 0 there, infinite
+    ones infinity by infinity; the other groups are as they were."""
+    from freemoe_b200 import attention
+
+    x, w = tensor(5, d, seed=d), tensor(d, seed=1) + 2
+    want, want_scales, _ = attention.add_rms_norm_fp8(x, w)
+    at = 200
+    w[at] = INF
+    x[3, at] = 0  # 0 * infinity: NaN, which does not count for the largest
+    want3, want3_scales, _ = attention.add_rms_norm_fp8(x, torch.where(w == INF, 0, w))
+    codes, scales, _ = attention.add_rms_norm_fp8(x, w)
+    codes, want, want3 = codes.float(), want.float(), want3.float()
+    want[3], want_scales[3] = want3[3], want3_scales[3]
+    rows = torch.tensor([0, 1, 2, 4], device="cuda")
+    assert (scales[rows, 1] == INF).all()
+    group = codes[rows, 128:256].clone()
+    assert torch.isnan(group[:, at - 128]).all()
+    group[:, at - 128] = 0
+    assert (group == 0).all()
+    assert torch.isnan(codes[3, at])
+    codes[3, at] = 0
+    codes[rows, 128:256], scales[rows, 1] = want[rows, 128:256], want_scales[rows, 1]
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
