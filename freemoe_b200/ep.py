@@ -60,10 +60,9 @@ class DeviceOps:
     def __init__(self, *, experts_total: int, top_k: int, d_model: int, ffn: int, gate_type: int,
                  up_type: int, down_type: int, local_slots, up_offset: int, down_offset: int):
         from . import hotpath
-        from ._lib import X_BF16, X_F32, check, load
+        from ._lib import check, load
 
         self.h, self.lib, self.check = hotpath, load(), check
-        self.X_BF16, self.X_F32 = X_BF16, X_F32
         self.E, self.k, self.d, self.ffn = experts_total, top_k, d_model, ffn
         self.types = (gate_type, up_type, down_type)
         self.up_offset, self.down_offset = up_offset, down_offset
@@ -100,7 +99,7 @@ class DeviceOps:
         send_x = torch.empty(max(P, 1), d, dtype=torch.float16, device=dev)
         send_e = torch.empty(max(P, 1), dtype=torch.int32, device=dev)
         scratch = self._buf("dispatch", self.lib.fmcuda_ep_dispatch_scratch_bytes(T, k, world), dev)
-        xdt = self.X_BF16 if x.dtype == torch.bfloat16 else self.X_F32
+        xdt = self.h.x_type(x)
         self.check(self.lib.fmcuda_ep_dispatch(
             C.c_void_p(ids.data_ptr()), T, k, per_rank, world, C.c_void_p(x.data_ptr()), xdt, d,
             C.c_void_p(counts32.data_ptr()), C.c_void_p(offsets.data_ptr()), C.c_void_p(send_pairs.data_ptr()),
@@ -136,7 +135,7 @@ class DeviceOps:
         meta_e = torch.empty(max(n, 1), k, dtype=torch.int32, device=dev)
         meta_w = torch.empty(max(n, 1), k, dtype=torch.float32, device=dev)
         scratch = self._buf("dispatch_rows", self.lib.fmcuda_ep_dispatch_rows_scratch_bytes(T, world), dev)
-        xdt = self.X_BF16 if x.dtype == torch.bfloat16 else self.X_F32
+        xdt = self.h.x_type(x)
         P = C.c_void_p
         self.check(self.lib.fmcuda_ep_dispatch_rows(
             P(ids.data_ptr()), P(w.data_ptr()), T, k, self.E // world, world, P(x.data_ptr()), xdt, d,
@@ -206,7 +205,7 @@ class DeviceOps:
         dev, world = ids.device, self.world
         row_of = torch.empty(max(T * world, 1), dtype=torch.int32, device=dev)
         scratch = self._buf("p2p_dispatch", self.lib.fmcuda_ep_p2p_dispatch_scratch_bytes(T, world), dev)
-        xdt = self.X_BF16 if x.dtype == torch.bfloat16 else self.X_F32
+        xdt = self.h.x_type(x)
         P = C.c_void_p
         self.check(self.lib.fmcuda_ep_p2p_dispatch(
             P(ids.data_ptr()), P(w.data_ptr()), T, k, self.E // world, world, self.rank, P(x.data_ptr()), xdt, self.d,

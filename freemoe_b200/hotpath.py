@@ -23,6 +23,14 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+def x_type(x: torch.Tensor) -> int:
+    """The C code of activations that products, experts and exchanges read: float32 or bfloat16.
+    (The attention side writes float16 and 8-bit rows too; nothing reads those as activations.)"""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise FmError(26, f"activations must be float32 or bfloat16, not {x.dtype}")
+    return X_BF16 if x.dtype == torch.bfloat16 else X_F32
+
+
 def row_bytes(type_id: int, in_dim: int) -> int:
     bs, bb = GEOMETRY[type_id]
     if in_dim % bs:
@@ -60,9 +68,7 @@ def gemv_quant(type_id: int, w: torch.Tensor, x: torch.Tensor, out_dim: int, in_
     ``x`` is [tokens, in_dim] (or [in_dim]) in float32 or bfloat16; returns
     float32 [tokens, out_dim]."""
     x2 = x.reshape(-1, in_dim).contiguous()
-    dt = X_BF16 if x2.dtype == torch.bfloat16 else X_F32
-    if x2.dtype not in (torch.bfloat16, torch.float32):
-        raise FmError(26, "activations must be float32 or bfloat16")
+    dt = x_type(x2)
     y = torch.empty(x2.shape[0], out_dim, dtype=torch.float32, device=x2.device)
     check(load().fmcuda_gemv(type_id, _ptr(w), _ptr(x2), dt, _ptr(y), x2.shape[0], out_dim, in_dim,
                              _stream(stream)))
@@ -158,7 +164,7 @@ def moe_args(x, logits, slot_table, *, experts, top_k, d_model, ffn, gate_type, 
     handles (or None).  The caller keeps every referenced tensor alive."""
     a = MoeArgs()
     a.x = x.data_ptr()
-    a.x_dtype = X_BF16 if x.dtype == torch.bfloat16 else X_F32
+    a.x_dtype = x_type(x)
     a.logits = logits.data_ptr()
     a.tokens = x.shape[0]
     a.experts = experts

@@ -1,0 +1,47 @@
+"""What the attention side hands on and takes at its edges, without a GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from freemoe_b200 import TYPE_Q8_0, hotpath
+from freemoe_b200._lib import X_BF16, X_F32, FmError
+
+ARG = 26
+UNREAD = [torch.float16, torch.float8_e4m3fn, torch.float64]  # rows that no product, expert or exchange reads
+
+
+def refused(code, call):
+    with pytest.raises(FmError) as e:
+        call()
+    assert e.value.code == code
+
+
+@pytest.mark.parametrize("dtype", UNREAD)
+def test_experts_refuse_rows_that_they_do_not_read(dtype):
+    x, logits = torch.zeros(3, 64).to(dtype), torch.zeros(3, 2)
+    slots = [torch.zeros(3 * 64 * 68, dtype=torch.uint8) for _ in range(2)]
+    table, y = hotpath.slot_table(slots, "cpu"), torch.zeros(3, 64)
+
+    def args(rows):
+        return hotpath.moe_args(rows, logits, table, experts=2, top_k=1, d_model=64, ffn=64, gate_type=TYPE_Q8_0,
+                                up_type=TYPE_Q8_0, down_type=TYPE_Q8_0, up_offset=0, down_offset=0, y=y)
+
+    assert args(x.float()).x_dtype == X_F32 and args(x.bfloat16()).x_dtype == X_BF16
+    refused(ARG, lambda: args(x))
+    for block in (hotpath.moe_block, hotpath.moe_prefill):
+        refused(ARG, lambda: block(x, logits, slots, top_k=1, ffn=64, gate_type=TYPE_Q8_0))
+    refused(ARG, lambda: hotpath.gemv_quant(TYPE_Q8_0, slots[0], x, 64, 64))
+
+
+@pytest.mark.parametrize("dtype", UNREAD)
+def test_exchanges_refuse_rows_that_they_do_not_read(dtype):
+    from freemoe_b200.ep import DeviceOps
+
+    ops = DeviceOps(experts_total=4, top_k=2, d_model=64, ffn=64, gate_type=TYPE_Q8_0, up_type=TYPE_Q8_0,
+                    down_type=TYPE_Q8_0, local_slots=[], up_offset=0, down_offset=0)
+    ops.world, ops.rank, ops.capacity, ops.timeout_ms = 2, 0, 16, 0
+    x, ids, w = torch.zeros(3, 64).to(dtype), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2)
+    refused(ARG, lambda: ops.dispatch(ids, x, 2))
+    refused(ARG, lambda: ops.dispatch_rows(ids, w, x, 2))
+    refused(ARG, lambda: ops.p2p_dispatch(ids, w, x, 1))
