@@ -1,9 +1,9 @@
 // attention.cu -- attention of new tokens over a paged cache: argument checks,
 // workspace and launches.  Sequences with few rows go to the kernel that is
 // limited by reading the cache (attention_rows.cuh), the others to the one on
-// the tensor cores (attention_prompt.cuh); each kernel finds its sequences
-// from the lengths on the device, and a kernel that the bounds rule out is not
-// launched.
+// the tensor cores (attention_prompt.cuh); each finds its sequences from the
+// lengths on the device, what the bounds rule out is not launched, and where
+// both have work they are parts of one grid.
 #include <cudaTypedefs.h>
 
 #include <cmath>
@@ -12,7 +12,6 @@
 #include <utility>
 
 #include "attention_prompt.cuh"
-#include "attention_rows.cuh"
 #include "launch.cuh"
 
 namespace fmb {
@@ -88,7 +87,9 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a) {
     if (n.rows && units && units <= sms) {
         // the largest cluster that one wave holds and that has a step for each warp
         const uint64_t steps = keys / ar_keys(static_cast<int>(n.dp)) + 1;
-        uint32_t c = AR_MAX_CLUSTER;
+        // (a grid that takes chunks too has none: ranges and their join, a chunk of 150 behind 1500
+        // keys beside 3 sequences 43 us, against 38 for clusters of 4 in a launch beside the chunk's)
+        uint32_t c = n.prompt ? 1 : AR_MAX_CLUSTER;
         while (c > 1 && (units * c > sms || steps < c * AR_WARPS)) c /= 2;
         if (steps <= static_cast<uint64_t>(c) * AR_WARPS * CLUSTER_STEPS) n.cluster = c;
     }
@@ -186,6 +187,13 @@ template <int DP, bool BF16>
 int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, const AttnParams &p, uint8_t *ws,
                      cudaStream_t s) {
     int rc = FM_STATUS_OK;
+    // sequences of few rows: a cluster a unit; a warp a unit, one a CTA until there is one on every
+    // SM; or ranges
+    const uint64_t row_units = static_cast<uint64_t>(p.seqs) * p.kv_heads * n.tiles, sms = device_sm_count();
+    const uint32_t unit_warps = row_units < sms * AR_WARPS ? static_cast<uint32_t>((row_units + sms - 1) / sms) : AR_WARPS;
+    const uint32_t rows_ctas = n.cluster ? static_cast<uint32_t>(row_units) * n.cluster
+                               : n.units ? static_cast<uint32_t>((row_units + unit_warps - 1) / unit_warps)
+                                         : p.workers / AR_WARPS;
     APParams pp{};
     if (n.prompt) {
         pp.a = p;
@@ -199,27 +207,29 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
         pp.part = reinterpret_cast<float *>(ws + n.ppart);
         pp.part_ml = reinterpret_cast<float2 *>(ws + n.ppart_ml);
         pp.tail = reinterpret_cast<int4 *>(ws + n.tail);
+        pp.ctas = n.ctas;
+        pp.rows_form = n.cluster ? AR_CLUSTER : n.units ? AR_UNIT : AR_RANGES;
+        pp.rows_tiles = n.tiles;
+        pp.rows_warps = unit_warps;
         CUtensorMap map_k, map_v;
         rc = make_cache_map(&map_k, a, a.k_cache, pp.box_rows, pp.heads_first);
         if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, pp.box_rows, pp.heads_first);
-        if (!rc)
+        if (!rc && n.rows)
+            rc = launch("attn_beside_kernel", attn_beside_kernel<DP, BF16>,
+                        {dim3(n.ctas + rows_ctas), AP_THREADS, AP_BESIDE_SMEM<DP>, 1}, s, map_k, map_v, pp);
+        else if (!rc)
             rc = launch("attn_prompt_kernel", attn_prompt_kernel<DP, BF16>,
                         {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, 1}, s, map_k, map_v, pp);
-    }
-    if (!rc && n.cluster)
+    } else if (n.cluster) {
         rc = launch("attn_cluster_kernel", attn_cluster_kernel<DP, BF16>,
-                    {dim3(p.seqs * p.kv_heads * n.tiles * n.cluster), AR_THREADS, ARows<DP>::SMEM, n.cluster}, s, p, n.tiles);
-    else if (!rc && n.units) {
-        // a warp a CTA until there is one on every SM
-        const uint64_t units = static_cast<uint64_t>(p.seqs) * p.kv_heads * n.tiles, sms = device_sm_count();
-        const uint32_t warps = units < sms * AR_WARPS ? static_cast<uint32_t>((units + sms - 1) / sms) : AR_WARPS;
+                    {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, n.cluster}, s, p, n.tiles);
+    } else if (n.units) {
         rc = launch("attn_unit_kernel", attn_unit_kernel<DP, BF16>,
-                    {dim3(static_cast<uint32_t>((units + warps - 1) / warps)), warps * 32,
-                     ARows<DP>::SMEM / AR_WARPS * warps, 1},
-                    s, p, n.tiles);
-    } else if (!rc && n.rows)
-        rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16>,
-                    {dim3(p.workers / AR_WARPS), AR_THREADS, ARows<DP>::SMEM, 1}, s, p);
+                    {dim3(rows_ctas), unit_warps * 32, ARows<DP>::RINGS / AR_WARPS * unit_warps, 1}, s, p, n.tiles);
+    } else {
+        rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16>, {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, 1}, s,
+                    p);
+    }
     if (!rc && n.prompt && n.deal)
         rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1}, s, pp);
     if (rc || !n.rows || n.cluster || n.units) return rc;
@@ -304,7 +314,6 @@ extern "C" int fmcuda_paged_attention(const fmcuda_paged_attention_args *a, void
     p.workers = n.workers;
     p.least = 4;
     p.row_limit = n.rows ? n.row_limit : 0;
-    p.beside = n.prompt;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = a->dtype == FM_X_BF16;
     if (n.dp == 64)

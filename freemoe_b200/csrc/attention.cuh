@@ -26,7 +26,6 @@ struct AttnParams {
     float2 *part_ml;  // their (largest exponent in log2, sum)
     int4 *tail_rows;         // [workers]: the unit that begins in a warp's range and is cut: sequence (or -1), tile, fragments
     uint32_t workers, least; // rows kernel: warps, and the least work of a warp, in steps
-    bool beside;             // a prompt kernel of the same call was launched before the rows kernel
     uint32_t row_limit;      // rows x group up to which a sequence is the rows kernel's
 };
 

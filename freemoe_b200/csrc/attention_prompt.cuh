@@ -41,8 +41,7 @@
 // Chunks behind contexts, heads of 64: 158 us, bound by the exponentials (58%).
 #pragma once
 
-#include "attention.cuh"
-#include "tcgen05.cuh"
+#include "attention_rows.cuh"
 
 namespace fmb {
 
@@ -77,6 +76,9 @@ struct APParams {
     bool wide;         // rows of out lie and end on 32 bytes
     bool deal;         // blocks are dealt out, not items
     uint32_t max_pairs;
+    uint32_t ctas;     // CTAs of the prompt kernel; the others of attn_beside_kernel take few-row sequences
+    ARForm rows_form;  // and how: a CTA a unit, a warp a unit, or even ranges
+    uint32_t rows_tiles, rows_warps; // row tiles a unit's sequence and head; warps that a unit each takes
     float *part;       // [CTA][began before, goes on][256][DP]
     float2 *part_ml;
     int4 *tail;        // [CTA] the item that goes on after it: sequence (or -1), pair, head, fragments
@@ -274,8 +276,8 @@ __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g)
     const AttnParams &p = pp.a;
     const uint32_t lane = threadIdx.x & 31u;
     if (!pp.deal) {
-        const uint64_t rank = static_cast<uint64_t>(w.round) * gridDim.x +
-                              (w.round & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const uint64_t rank = static_cast<uint64_t>(w.round) * pp.ctas +
+                              (w.round & 1u ? pp.ctas - 1 - blockIdx.x : blockIdx.x);
         if (rank >= w.left) return false;
         ++w.round;
         const uint64_t item = w.left - 1 - rank; // the longest tiles of a sequence are its last
@@ -342,12 +344,10 @@ __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g)
 // ---- the kernel ---------------------------------------------------------------------
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(AP_THREADS, 1)
-    attn_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                       const __grid_constant__ APParams pp) {
+__device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtensorMap &map_v, const APParams &pp,
+                                          uint8_t *ap_smem_raw) {
     using L = APrompt<DP>;
     const AttnParams &p = pp.a;
-    extern __shared__ uint8_t ap_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ap_smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_done = bars + 8;
@@ -359,10 +359,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     static_assert((14 + 2 * AP_SEG_SLOTS + 2 * L::STAGES) * 8 + 32 <= 512, "barriers outgrow their place");
     volatile uint32_t *abort_flag = misc + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-
-    // what follows on the stream may come to the SMs that have nothing to do here
-    after_stream();
-    let_next();
 
     // ---- this CTA's share -------------------------------------------------------------
     // where blocks are dealt out: the sequences that have pairs and their first ones, and
@@ -445,7 +441,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (warp == 0) {
             uint32_t piece = 0;
             // pieces that the CTAs take of one head's items; the rows kernel's keep half of the SMs
-            const uint32_t budget = gridDim.x / (p.row_limit ? 2u : 1u) / p.kv_heads;
+            const uint32_t budget = pp.ctas / (p.row_limit ? 2u : 1u) / p.kv_heads;
             if (pairs && pairs <= budget) {
                 // the shortest pieces of which there are no more than CTAs
                 uint32_t all = 0, longest = 0;
@@ -470,7 +466,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 piece = lo < AP_LEAST_PIECE ? AP_LEAST_PIECE : lo;
                 if (piece + AP_LEAST_SAVED > longest) piece = longest;
                 // many CTAs idle: even ranges are shorter, with what a second item in them costs
-                if (piece > all * p.kv_heads / gridDim.x + AP_LEAST_SAVED) piece = 0;
+                if (piece > all * p.kv_heads / pp.ctas + AP_LEAST_SAVED) piece = 0;
             }
             if (lane == 0) misc[0] = piece;
             uint64_t before = 0;
@@ -488,7 +484,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (lane == 0) cost_before[0] = 0;
         }
         __syncthreads();
-        const uint64_t total = cost_before[pairs] * p.kv_heads, even = (total + gridDim.x - 1) / gridDim.x;
+        const uint64_t total = cost_before[pairs] * p.kv_heads, even = (total + pp.ctas - 1) / pp.ctas;
         walk.piece = misc[0];
         per = walk.piece ? walk.piece : even > AP_LEAST_COST ? even : AP_LEAST_COST;
         const uint64_t begin = blockIdx.x * per;
@@ -917,6 +913,52 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == 11) tmem_dealloc(tmem, 512);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AP_THREADS, 1)
+    attn_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ APParams pp) {
+    extern __shared__ __align__(1024) uint8_t ap_smem_raw[];
+    // what follows on the stream may come to the SMs that have nothing to do here
+    after_stream();
+    let_next();
+    ap_chunks<DP, BF16>(map_k, map_v, pp, ap_smem_raw);
+}
+
+template <int DP> constexpr uint32_t AP_BESIDE_SMEM = ARows<DP>::SMEM > APrompt<DP>::SMEM ? ARows<DP>::SMEM : APrompt<DP>::SMEM;
+
+// Chunks, and beside them the sequences of few rows on the SMs that the chunks leave free: one
+// grid, whose CTAs all wait for what came before it on the stream.  (As a launch of its own that
+// began beside the chunks' the second part could not wait without running after the first.)  The
+// first CTAs are the prompt kernel's; of the threads of the others two warpgroups work, with the
+// third one's registers.  Measured, heads of 128, 8 key heads: a chunk of up to 512 behind 4000
+// keys beside 31 decoding sequences 103 us, against 119 with one kernel after the other; of 510
+// beside 7 with a window of 1000 keys (16 key heads) 44 against 65.
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AP_THREADS, 1)
+    attn_beside_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ APParams pp) {
+    extern __shared__ __align__(1024) uint8_t ap_smem_raw[];
+    static_assert(AR_THREADS == 256, "two warpgroups");
+    after_stream();
+    let_next();
+    if (blockIdx.x < pp.ctas) {
+        ap_chunks<DP, BF16>(map_k, map_v, pp, ap_smem_raw);
+        return;
+    }
+    if (threadIdx.x >= AR_THREADS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+    const uint32_t cta = blockIdx.x - pp.ctas, ctas = gridDim.x - pp.ctas;
+    if (pp.rows_form == AR_CLUSTER)
+        ar_cluster<DP, BF16>(pp.a, ap_smem_raw, cta, pp.rows_tiles);
+    else if (pp.rows_form == AR_RANGES)
+        ar_ranges<DP, BF16>(pp.a, ap_smem_raw, cta, ctas);
+    else if (threadIdx.x < pp.rows_warps * 32)
+        ar_unit<DP, BF16>(pp.a, ap_smem_raw, cta, ctas, pp.rows_tiles);
 }
 
 // Adds up the fragments of the items that were cut: blockIdx.x the CTA in which

@@ -34,6 +34,7 @@ namespace fmb {
 constexpr uint32_t AR_WARPS = 8, AR_THREADS = AR_WARPS * 32;
 constexpr uint32_t AR_ROWS = 16, AR_MAX_CLUSTER = 8;
 constexpr uint32_t AR_UNIT_COST = 2;
+enum ARForm : uint32_t { AR_RANGES, AR_CLUSTER, AR_UNIT }; // see ar_ranges, ar_cluster, ar_unit
 __host__ __device__ constexpr uint32_t ar_keys(int dp) { return dp == 64 ? 32 : 16; } // keys a step
 
 template <int DP> struct ARows {
@@ -42,7 +43,8 @@ template <int DP> struct ARows {
     static constexpr uint32_t HALF = KEYS * ROW_BYTES; // K or V of a step
     static constexpr uint32_t STAGE = 2 * HALF;
     static constexpr uint32_t STAGES = 24576 / STAGE; // 24 KB a warp
-    static constexpr uint32_t SMEM = AR_WARPS * STAGES * STAGE;
+    static constexpr uint32_t RINGS = AR_WARPS * STAGES * STAGE;
+    static constexpr uint32_t SMEM = RINGS + 2048; // and what the warps tell each other
 };
 
 // Row tiles and steps a unit of sequence s in the rows kernel (no tiles: not its work).
@@ -91,17 +93,9 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The kernels here begin beside a prompt kernel that the same call launched before them
-// (and that waited for the stream), on the SMs that it leaves free: they share nothing with
-// it.  But the grid does not end before it, so that what follows on the stream finds both
-// done: its first CTA waits (were all to wait, the CTAs behind them would find no SM until
-// then).  Without a prompt kernel they wait for the stream like any other.
-__device__ __forceinline__ void before_rows(const AttnParams &p) {
-    if (!p.beside) after_stream();
-}
-__device__ __forceinline__ void after_rows(const AttnParams &p) {
-    if (p.beside && blockIdx.x == 0) after_stream();
-}
+// The three forms below are device functions of CTA `cta` of `ctas` with 256 threads and shared
+// memory at `smem`: kernels of their own, or a part of the grid of attn_beside_kernel, whose
+// other CTAs take the chunks.
 
 // A place in the laid-out work.
 struct ARCursor {
@@ -335,15 +329,12 @@ __device__ __forceinline__ void ar_store_row(const AttnParams &p, const AttnSeq 
 }
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnParams p) {
+__device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t ctas) {
     using L = ARows<DP>;
-    extern __shared__ __align__(1024) uint8_t ar_smem[];
-    __shared__ uint64_t s_part[AR_WARPS], s_first[AR_WARPS];
-    __shared__ uint32_t s_seq[AR_WARPS];
+    uint64_t *s_part = reinterpret_cast<uint64_t *>(smem + L::RINGS), *s_first = s_part + AR_WARPS;
+    uint32_t *s_seq = reinterpret_cast<uint32_t *>(s_first + AR_WARPS);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
-    before_rows(p);
-    let_next();
     // ---- this warp's range, and the sequence that it begins in -------------------
     uint64_t total = 0, mine = 0, before = 0;
     const bool few = p.seqs <= AR_THREADS;
@@ -351,16 +342,16 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         const uint32_t b = b0 + threadIdx.x;
         mine = 0;
         if (b < p.seqs) {
-            const AttnSeq s = attn_seq(p, b, blockIdx.x == 0);
+            const AttnSeq s = attn_seq(p, b, cta == 0);
             const ARShape sh = ar_shape<DP>(p, s);
             mine = ar_length(p, sh);
         }
         uint64_t sum;
         before = ar_block_scan(mine, s_part, &sum);
-        if (blockIdx.x == 0 && b < p.seqs) p.prefix[b] = total + before;
+        if (cta == 0 && b < p.seqs) p.prefix[b] = total + before;
         total += sum;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.seqs] = total;
+    if (cta == 0 && threadIdx.x == 0) p.prefix[p.seqs] = total;
     const uint64_t even = quotient(total + p.workers - 1, p.workers);
     const uint64_t per = even > p.least ? even : p.least;
     uint64_t running = 0;
@@ -380,7 +371,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         if (mine) {
 #pragma unroll
             for (uint32_t w = 0; w < AR_WARPS; ++w) {
-                const uint64_t at = (static_cast<uint64_t>(w) * gridDim.x + blockIdx.x) * per;
+                const uint64_t at = (static_cast<uint64_t>(w) * ctas + cta) * per;
                 if (at >= before && at < before + mine) {
                     s_seq[w] = b;
                     s_first[w] = before;
@@ -389,12 +380,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
         }
     }
     __syncthreads();
-    const uint64_t worker = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
+    const uint64_t worker = static_cast<uint64_t>(warp) * ctas + cta;
     const uint64_t begin = worker * per;
     int4 tail = make_int4(-1, 0, 0, 0); // the unit that begins here and goes on after the range
     if (begin >= total) {
         if (lane == 0) p.tail_rows[worker] = tail;
-        after_rows(p);
         return;
     }
     const uint32_t end = static_cast<uint32_t>((total - begin < per) ? total - begin : per);
@@ -411,7 +401,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     c.at = in_unit < AR_UNIT_COST ? AR_UNIT_COST - in_unit : 0;
 
     // ---- the stream of keys -------------------------------------------------------
-    const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
+    const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
     ARState<DP, BF16> u;
     uint32_t first_step = c.step;
@@ -476,7 +466,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
     }
     if (lane == 0) p.tail_rows[worker] = tail;
     cp_async_wait<0>();
-    after_rows(p);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnParams p) {
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    after_stream();
+    let_next();
+    ar_ranges<DP, BF16>(p, ar_smem, blockIdx.x, gridDim.x);
 }
 
 // ---- few units of short sequences: a cluster each ----------------------------------
@@ -509,29 +506,24 @@ __device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
 }
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnParams p, uint32_t unit_tiles) {
+__device__ __forceinline__ void ar_cluster(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t unit_tiles) {
     using L = ARows<DP>;
-    extern __shared__ __align__(1024) uint8_t ar_smem[];
-    __shared__ float s_m[AR_WARPS][AR_ROWS], s_l[AR_WARPS][AR_ROWS]; // of the warps
-    __shared__ float s_top[AR_ROWS], s_sum[AR_ROWS];                 // of the CTA
+    float(*s_m)[AR_ROWS] = reinterpret_cast<float(*)[AR_ROWS]>(smem + L::RINGS), (*s_l)[AR_ROWS] = s_m + AR_WARPS; // of the warps
+    float *s_top = s_l[AR_WARPS], *s_sum = s_top + AR_ROWS;                                                      // of the CTA
+    static_assert((2 * AR_WARPS + 2) * AR_ROWS * 4 <= L::SMEM - L::RINGS, "the sums outgrow their place");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
-    const uint32_t unit = blockIdx.x / ranks, rt = unit % unit_tiles;
+    const uint32_t unit = cta / ranks, rt = unit % unit_tiles;
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
-    before_rows(p);
-    let_next();
     const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
     const ARShape sh = ar_shape<DP>(p, s);
-    if (rt >= sh.tiles) { // the whole cluster
-        after_rows(p);
-        return;
-    }
+    if (rt >= sh.tiles) return; // the whole cluster
 
     const uint32_t part = rank * AR_WARPS + warp, parts = ranks * AR_WARPS;
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * part / parts);
     const uint32_t count = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * (part + 1) / parts) - begin;
     const uint32_t key_first = (sh.step0 + begin) * L::KEYS;
-    const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE);
+    const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE);
     uint32_t fetched = 0;
     int64_t next = count ? ar_key_at<DP>(p, s, b, head, key_first, lane) : -1;
     auto fetch = [&] {
@@ -556,7 +548,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     __syncwarp();
     // the warp's O over its ring, rows of DP
     const uint32_t all = s.ql * p.group - rt * AR_ROWS, rows = all < AR_ROWS ? all : AR_ROWS;
-    float *mine = reinterpret_cast<float *>(ar_smem + warp * (L::STAGES * L::STAGE));
+    float *mine = reinterpret_cast<float *>(smem + warp * (L::STAGES * L::STAGE));
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const float sum = u.sum(r);
@@ -573,7 +565,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
     }
     __syncthreads();
     // the CTA's O behind warp 0's
-    float *joined = reinterpret_cast<float *>(ar_smem) + AR_ROWS * DP;
+    float *joined = reinterpret_cast<float *>(smem) + AR_ROWS * DP;
     for (uint32_t i = threadIdx.x; i < rows * DP; i += AR_THREADS) {
         const uint32_t in = i / DP;
         float top = -INFINITY, acc = 0.0f, sum = 0.0f;
@@ -583,7 +575,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
         for (uint32_t w = 0; w < AR_WARPS; ++w) {
             const float f = s_m[w][in] == -INFINITY ? 0.0f : exp2_approx(s_m[w][in] - top);
             sum += s_l[w][in] * f;
-            acc += reinterpret_cast<const float *>(ar_smem + w * (L::STAGES * L::STAGE))[i] * f;
+            acc += reinterpret_cast<const float *>(smem + w * (L::STAGES * L::STAGE))[i] * f;
         }
         joined[i] = acc;
         if (i % DP == 0) {
@@ -628,7 +620,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
             p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
     cluster_sync(); // nobody leaves while its shared memory is read
-    after_rows(p);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnParams p, uint32_t unit_tiles) {
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    after_stream();
+    let_next();
+    ar_cluster<DP, BF16>(p, ar_smem, blockIdx.x, unit_tiles);
 }
 
 // ---- many units of very short sequences: a warp each ------------------------------
@@ -637,19 +636,16 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
 // warps of a CTA take a unit each, from its first key to its last, and write its rows.
 // No sums over the sequences to find the work, no fragments, one launch.
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnParams p, uint32_t unit_tiles) {
+__device__ __forceinline__ void ar_unit(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t ctas, uint32_t unit_tiles) {
     using L = ARows<DP>;
-    extern __shared__ __align__(1024) uint8_t ar_smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t unit = warp * gridDim.x + blockIdx.x, rt = unit % unit_tiles;
+    const uint32_t unit = warp * ctas + cta, rt = unit % unit_tiles;
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
-    before_rows(p);
-    let_next();
     if (b < p.seqs) {
         const AttnSeq s = attn_seq(p, b, lane == 0 && rt == 0 && head == 0);
         const ARShape sh = ar_shape<DP>(p, s);
         if (rt < sh.tiles) {
-            const uint32_t ring = smem_u32(ar_smem) + warp * (L::STAGES * L::STAGE), key_first = sh.step0 * L::KEYS;
+            const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE), key_first = sh.step0 * L::KEYS;
             ARState<DP, BF16> u;
             uint32_t fetched = 0;
             int64_t next = ar_key_at<DP>(p, s, b, head, key_first, lane);
@@ -679,7 +675,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnPara
             }
         }
     }
-    after_rows(p);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnParams p, uint32_t unit_tiles) {
+    extern __shared__ __align__(1024) uint8_t ar_smem[];
+    after_stream();
+    let_next();
+    ar_unit<DP, BF16>(p, ar_smem, blockIdx.x, gridDim.x, unit_tiles);
 }
 
 // Joins the fragments of the units that were cut.  A CTA of W warps takes a row (one of C

@@ -74,3 +74,30 @@ def test_infinite_results_to_8_bits(cuda, d):
     codes[3, at] = 0
     codes[rows, 128:256], scales[rows, 1] = want[rows, 128:256], want_scales[rows, 1]
     assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+
+
+# the sequences beside the chunk in even ranges, a CTA each, a warp each
+@pytest.mark.parametrize("lens", [[(1, 7000), (150, 900), (1, 300), (1, 9000)], [(1, 700), (150, 900), (1, 300)],
+                                  [(1, 100 + b) for b in range(150)] + [(70, 256)]])
+def test_calls_see_what_was_written_just_before(cuda, lens):
+    """Queries, keys, lengths and pages come from kernels right before the call, in both parts of its
+    grid: other ones each time, and the results those of calls that nothing runs beside."""
+    a, b = (Batch(lens, 8, 2, 128, 16, seed=61 + i) for i in range(2))
+    names = ("q", "k_cache", "v_cache", "table")
+    versions = [[getattr(x, n).clone() for n in names] + [x.kv_len - i] for i, x in enumerate((a, b))]
+    want = []
+    for version in versions:
+        for n, t in zip((*names, "kv_len"), version):
+            getattr(a, n).copy_(t)
+        torch.cuda.synchronize()
+        want.append(a.run())
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0][0], want[1][0])
+    got = []
+    for i in range(20):
+        for n, t in zip((*names, "kv_len"), versions[i % 2]):
+            getattr(a, n).copy_(t)
+        got.append(a.run())
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+    assert cuda.device_status() == 0
