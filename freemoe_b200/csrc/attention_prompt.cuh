@@ -568,11 +568,13 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     o.whole = g.whole;
                     mbar_arrive(&seg_full[k % AP_SEG_SLOTS]);
                     if (more && pp.deal && g.starts && g.je < g.j1) {
-                        // the rest of the item goes to the next CTAs, `per` blocks each
-                        const uint64_t rest = g.j1 - g.je;
-                        pp.tail[blockIdx.x] =
-                            make_int4(static_cast<int>(g.b), static_cast<int>(g.pair), static_cast<int>(g.head),
-                                      1 + static_cast<int>((rest + per - 1) / per));
+                        // the rest of the item goes to the next CTAs, `per` blocks each (to fewer
+                        // than that takes where sequences overlap in q, which has been reported)
+                        const uint64_t rest = g.j1 - g.je, most = pp.ctas - blockIdx.x;
+                        const uint64_t parts = 1 + (rest + per - 1) / per;
+                        pp.tail[blockIdx.x] = make_int4(static_cast<int>(g.b), static_cast<int>(g.pair),
+                                                        static_cast<int>(g.head),
+                                                        static_cast<int>(parts < most ? parts : most));
                     }
                 }
                 if (!more) break;

@@ -698,8 +698,9 @@ int fmcuda_rope_append(const fmcuda_rope_append_args *args, void *stream);
  * max_q_len and max_kv_len bound the sequences' rows and keys (they set the
  * launch; the lengths themselves stay on the device).  A length past its bound,
  * rows past `tokens`, or a page of a visible key outside [0, n_pages) sets the
- * device status to INVALID_ARGUMENT; the rows concerned are then undefined and
- * no memory outside the arguments is touched.
+ * device status to INVALID_ARGUMENT; the rows concerned are then undefined (all
+ * rows, where q_start is not ascending) and no memory outside the arguments is
+ * touched.  With max_q_len 0 the call returns at once and looks at no length.
  *
  * head_dim: multiple of 8, at most 128; page_size: multiple of 8; heads a
  * multiple of kv_heads; strides multiples of 8 and pointers 16-byte aligned. */

@@ -4,6 +4,8 @@ Tolerances are those of tests/test_attention_gpu.py and tests/test_norm_rope_gpu
 the same row in another call is compared bit by bit."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -100,4 +102,37 @@ def test_calls_see_what_was_written_just_before(cuda, lens):
         got.append(a.run())
     for i, (out, lse) in enumerate(got):
         assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+    assert cuda.device_status() == 0
+
+
+# blocks dealt out in even ranges (the range that ends the first sequence goes on in one that was left
+# out, and is longer than the CTAs behind it take) and in pieces, and items dealt whole
+@pytest.mark.parametrize("rows,kvs", [(3000, [3000, 9, 60000, 9, 3000, 9, 3000, 9, 3000]), (300, [9000] * 9), (300, [600] * 9)])
+def test_sequences_that_overlap_are_reported(cuda, rows, kvs):
+    """q_start that goes back: more tiles than there are rows for.  Nothing is written but the rows and
+    the workspace, and the next call is right."""
+    from freemoe_b200._lib import PagedAttentionArgs, check, load
+
+    good = Batch([(rows, kvs[0]), (1, 40)], 8, 2, 128, 64, seed=71)
+    want, _ = good.run()
+    b = Batch([(rows if i == 0 else 0, kv) for i, kv in enumerate(kvs)], 8, 2, 128, 64, seed=72)
+    b.q_start.copy_(torch.tensor([0, rows] * 2 + [0, 64] * 3, dtype=torch.int32))
+    args = PagedAttentionArgs(
+        q=b.q.data_ptr(), k_cache=b.k_cache.data_ptr(), v_cache=b.v_cache.data_ptr(), out=b.q.data_ptr(),
+        page_table=b.table.data_ptr(), q_start=b.q_start.data_ptr(), kv_len=b.kv_len.data_ptr(), q_token_stride=1024,
+        q_head_stride=128, out_token_stride=1024, out_head_stride=128, cache_page_stride=b.k_cache.stride(0),
+        cache_head_stride=b.k_cache.stride(1), cache_row_stride=128, page_table_stride=b.table.stride(0), dtype=1, seqs=9,
+        tokens=rows, heads=8, kv_heads=2, head_dim=128, n_pages=b.k_cache.shape[0], page_size=64, max_q_len=rows,
+        max_kv_len=max(kvs), causal=1, scale=b.scale)
+    size = C.c_uint64()
+    check(load().fmcuda_paged_attention_workspace_bytes(C.byref(args), C.byref(size)))
+    guard = 1 << 20
+    workspace = torch.full((size.value + guard,), 90, dtype=torch.uint8, device="cuda")
+    out = torch.full((rows * 8 * 128 + guard,), 1.5, dtype=b.dtype, device="cuda")
+    args.out = out.data_ptr()
+    check(load().fmcuda_paged_attention(C.byref(args), workspace.data_ptr(), size.value,
+                                        torch.cuda.current_stream().cuda_stream))
+    assert cuda.device_status() == 26
+    assert (workspace[size.value:] == 90).all() and (out[rows * 8 * 128:] == 1.5).all()
+    assert torch.equal(good.run()[0], want)
     assert cuda.device_status() == 0
