@@ -346,11 +346,11 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
     if (!is_float_x(a->in_dtype) || !is_float_x(a->out_dtype))
         return set_error(FM_STATUS_INVALID_ARGUMENT, "rotary types must be float32, bfloat16 or float16");
     const bool cached = a->k || a->v || a->k_cache || a->v_cache;
-    if (cached && (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slots))
-        return set_error(FM_STATUS_INVALID_ARGUMENT, "k, v, their caches and slots come together");
     if (cached && (a->kv_heads == 0 || a->page_size == 0))
         return set_error(FM_STATUS_SHAPE_MISMATCH, "a cache has at least one head and one row a page");
-    if (a->tokens == 0) return FM_STATUS_OK;
+    if (a->tokens == 0) return FM_STATUS_OK; // its k, v and slots may be null beside caches that are not
+    if (cached && (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slots))
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "k, v, their caches and slots come together");
     if (!a->q || !a->q_out || !a->positions || (a->rot_dim && !a->inv_freq))
         return set_error(FM_STATUS_INVALID_ARGUMENT, "null rotary buffer");
     if (!aligned_to_value(a->q, a->in_dtype) || !aligned_to_value(a->k, a->in_dtype) ||

@@ -1,13 +1,16 @@
 """What the attention side hands on and takes at its edges, without a GPU."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
-from freemoe_b200 import TYPE_Q8_0, hotpath
+from freemoe_b200 import TYPE_Q8_0, hotpath, load
 from freemoe_b200._lib import X_BF16, X_F32, FmError
+from test_attention_cpu import rope_args
 
-ARG = 26
+OK, SHAPE, ARG = 0, 8, 26
 UNREAD = [torch.float16, torch.float8_e4m3fn, torch.float64]  # rows that no product, expert or exchange reads
 
 
@@ -45,3 +48,15 @@ def test_exchanges_refuse_rows_that_they_do_not_read(dtype):
     refused(ARG, lambda: ops.dispatch(ids, x, 2))
     refused(ARG, lambda: ops.dispatch_rows(ids, w, x, 2))
     refused(ARG, lambda: ops.p2p_dispatch(ids, w, x, 1))
+
+
+def test_a_rotation_of_no_tokens_takes_null_rows():
+    """The rows and slots of an empty batch have no address; its caches have."""
+    lib = load()
+
+    def code(**change):
+        return lib.fmcuda_rope_append(C.byref(rope_args(tokens=0, q=None, k=None, v=None, q_out=None, positions=None,
+                                                        slots=None, **change)), None)
+
+    assert code() == OK and code(k_cache=None, v_cache=None) == OK
+    assert code(in_dtype=3) == ARG and code(page_size=0) == SHAPE and code(rot_dim=63) == SHAPE

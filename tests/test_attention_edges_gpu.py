@@ -136,3 +136,17 @@ def test_sequences_that_overlap_are_reported(cuda, rows, kvs):
     assert (workspace[size.value:] == 90).all() and (out[rows * 8 * 128:] == 1.5).all()
     assert torch.equal(good.run()[0], want)
     assert cuda.device_status() == 0
+
+
+def test_a_rotation_of_no_tokens(cuda):
+    from freemoe_b200 import attention
+
+    q, k = tensor(3, 4, 64, dtype=torch.bfloat16), tensor(3, 2, 64, dtype=torch.bfloat16, seed=1)
+    kc, vc = (torch.full((2, 2, 8, 64), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    inv_freq, _ = attention.rope_frequencies(64)
+    at = torch.arange(3, device="cuda")
+    for n in (slice(0, 0), slice(3, 3)):
+        got = attention.rope_append(q[n], k[n], k[n], at.int()[n], inv_freq, kc, vc, at[n])
+        assert got.shape == (0, 4, 64) and got.dtype == kc.dtype
+        assert attention.rope_append(q[n], None, None, at.int()[n], inv_freq, None, None, None).shape == (0, 4, 64)
+    assert (kc == 7).all() and (vc == 7).all() and cuda.device_status() == 0
