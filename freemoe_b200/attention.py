@@ -14,14 +14,13 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
-from pathlib import Path
 
 import torch
 
 from ._lib import (ROPE_BANDS, ROPE_BASE, ROPE_LINEAR, ROPE_PLAIN, ROPE_RAMP, FmError, RopeScaling, check, load)
+from .build import torch_calls_path
 
 FP8_GROUP = 128
-CALLS_PATH = Path(__file__).resolve().parent / "_torch_calls.so"
 _ROPE_KINDS = {"plain": ROPE_PLAIN, "linear": ROPE_LINEAR, "base": ROPE_BASE, "ramp": ROPE_RAMP, "bands": ROPE_BANDS}
 INVALID_ARGUMENT, SHAPE_MISMATCH = 26, 8
 
@@ -31,9 +30,10 @@ class _Calls:
     their first use; a missing build is an error, there is no fallback."""
 
     def __getattr__(self, name: str):
-        if not CALLS_PATH.exists():
-            raise FmError(24, f"{CALLS_PATH} is missing: build it with `python freemoe_b200/build.py`")
-        spec = importlib.util.spec_from_file_location("_torch_calls", CALLS_PATH)
+        path = torch_calls_path()
+        if not path.exists():
+            raise FmError(24, f"{path} is missing: build it with `python freemoe_b200/build.py`")
+        spec = importlib.util.spec_from_file_location("_torch_calls", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         lib = load()

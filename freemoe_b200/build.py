@@ -1,5 +1,6 @@
-"""Build recipe for the sm_100a shared library (``libfreemoe_b200.so``) and the
-entry points for torch tensors beside it (``_torch_calls.so``).
+"""Build recipe for the sm_100a shared library (``libfreemoe_b200.so``), which
+needs nvcc alone, and the entry points for torch tensors beside it
+(``_torch_calls.<python>.torch-<version>.so``), where torch is installed.
 
 The library is built in-tree with nvcc so that the ``.so`` travels with the
 source tree; nothing is JIT-compiled or installed into site-packages.
@@ -9,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -41,10 +43,23 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
+def torch_calls_path() -> Path:
+    """The build of the entry points for this Python and this torch: another's is never loaded."""
+    import torch
+
+    return PKG / f"_torch_calls.{sys.implementation.cache_tag}.torch-{torch.__version__}.so"
+
+
+def build_torch_calls(force: bool = False, verbose: bool = False) -> Path | None:
     """Compiles ``csrc/torch_calls.cpp``, the entry points for torch tensors, against the
-    installed torch (host code only: it calls the library through the addresses it is given)."""
-    src, target = CSRC / "torch_calls.cpp", PKG / "_torch_calls.so"
+    installed torch (host code only: it calls the library through the addresses it is given).
+    Without a torch there are none, and nothing here needs them."""
+    try:
+        target = torch_calls_path()
+    except ImportError:
+        print("torch is not installed: the library is built without entry points for its tensors", file=sys.stderr)
+        return None
+    src = CSRC / "torch_calls.cpp"
     if not force and not _stale(target, [src, Path(__file__), *INCLUDE.glob("*.h")]):
         return target
     import sysconfig
@@ -67,8 +82,17 @@ def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
+    """The library, and meanwhile the entry points for torch tensors; what fails in these is
+    raised when the library is there."""
+    with ThreadPoolExecutor(1) as pool:
+        calls = pool.submit(build_torch_calls, force, verbose)
+        lib = build_library(force, verbose, ptxas_verbose)
+        calls.result()
+    return lib
+
+
+def build_library(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     """Compiles every ``csrc/*.cu`` for sm_100a into ``libfreemoe_b200.so``."""
-    build_torch_calls(force, verbose)
     deps = sources() + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h")) + [Path(__file__)]
     if not force and not _stale(LIB, deps):
         return LIB

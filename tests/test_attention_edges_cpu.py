@@ -60,3 +60,28 @@ def test_a_rotation_of_no_tokens_takes_null_rows():
 
     assert code() == OK and code(k_cache=None, v_cache=None) == OK
     assert code(in_dtype=3) == ARG and code(page_size=0) == SHAPE and code(rot_dim=63) == SHAPE
+
+
+def test_the_library_needs_no_torch(tmp_path, monkeypatch, capsys):
+    """Without torch the entry points for its tensors are left out, and the library is built."""
+    import sys
+
+    from freemoe_b200 import build
+
+    monkeypatch.setattr(build, "PKG", tmp_path)  # no entry points there yet
+    monkeypatch.setitem(sys.modules, "torch", None)  # importing it fails
+    assert build.build() == build.LIB and build.LIB.exists()
+    assert "torch is not installed" in capsys.readouterr().err
+    assert not list(tmp_path.glob("*.so"))
+
+
+def test_entry_points_are_those_of_this_torch(monkeypatch):
+    from freemoe_b200 import attention, build
+
+    mine = build.torch_calls_path()
+    assert mine.exists() and mine.name.startswith("_torch_calls.")
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert build.torch_calls_path() != mine
+    with pytest.raises(FmError) as e:
+        attention._Calls().add_rms_norm
+    assert e.value.code == 24 and "0.0.1" in str(e.value)
