@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from test_attention_gpu import Batch
-from test_norm_rope_gpu import tensor
+from test_norm_rope_gpu import BF16, F16, F32, e4m3_step, hold_norm, norm_exact, rope_case, tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +150,66 @@ def test_a_rotation_of_no_tokens(cuda):
         assert got.shape == (0, 4, 64) and got.dtype == kc.dtype
         assert attention.rope_append(q[n], None, None, at.int()[n], inv_freq, None, None, None).shape == (0, 4, 64)
     assert (kc == 7).all() and (vc == 7).all() and cuda.device_status() == 0
+
+
+def hold_codes(codes, scales, x, w, res):
+    """As in tests/test_norm_rope_gpu.py: a code is the value nearest to y / scale or, at a boundary, its neighbour."""
+    rows, d = x.shape
+    _, want, root = norm_exact(x, w, res, 1e-5)
+    groups = -(-d // 128)
+    pad = torch.zeros(rows, groups * 128, dtype=torch.float64, device="cuda")
+    pad[:, :d] = want
+    top = pad.view(rows, groups, 128).abs().amax(-1).clamp(min=1e-10) / 448
+    assert ((scales.double() - top).abs() <= 60 * 2.0 ** -24 * top).all()
+    scale = scales.double().repeat_interleave(128, 1)[:, :d]
+    c = codes.float().double()
+    slack = 2.0 ** -22 * (x.double().abs() + res.double().abs()) * w.double().abs() / root
+    step = torch.maximum(e4m3_step(c), e4m3_step(want / scale))
+    assert ((c * scale - want).abs() <= 0.5 * (1 + 1e-4) * step * scale + slack).all()
+
+
+# rows for teams of a warp (up to 1024 values) and of a CTA, in eights, pairs and single values,
+# and more of them than the GPU holds at once: every team takes several
+@pytest.mark.parametrize("tokens,d", [(20011, 200), (20011, 202), (20011, 201), (12007, 1024), (12007, 1022), (12007, 1021),
+                                      (5003, 2048), (5003, 2050), (5003, 2049), (2999, 4096), (2999, 4094), (2999, 4095),
+                                      (1201, 16384), (1201, 16382), (1201, 16381), (601, 20000), (601, 20001)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_norm_of_more_rows_than_teams(cuda, tokens, d, dtype):
+    from freemoe_b200 import attention
+    from freemoe_b200._lib import RmsNormArgs, check, load
+
+    x, w, res = tensor(tokens, d, dtype=dtype, seed=d), tensor(d, seed=1) + 1, tensor(tokens, d, dtype=dtype, seed=2)
+    y, h = attention.add_rms_norm(x, w, residual=res)
+    hold_norm(y, x, w, res, 1e-5, dtype)
+    assert torch.equal(h, (x.float() + res.float()).to(dtype))
+    y32, _ = attention.add_rms_norm(x, w, out_dtype=F32)
+    hold_norm(y32, x, w, None, 1e-5, F32)
+    del y32
+    codes, scales, h8 = attention.add_rms_norm_fp8(x, w, residual=res)
+    assert torch.equal(h8, h)
+    hold_codes(codes, scales, x, w, res)
+    kind = {F32: 0, BF16: 1, F16: 2}[dtype]  # y on x and residual_out on residual
+    a = RmsNormArgs(x.data_ptr(), res.data_ptr(), w.data_ptr(), x.data_ptr(), res.data_ptr(), None, d, d, d, kind, kind, 0,
+                    kind, tokens, d, 1e-5)
+    check(load().fmcuda_add_rms_norm(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(x, y) and torch.equal(res, h)
+
+
+# more tokens than four an SM: several to a CTA, fewer to the last one
+@pytest.mark.parametrize("tokens", [1001, 2371, 5000])
+@pytest.mark.parametrize("dim,rot,interleaved", [(128, 128, True), (80, 42, True), (128, 128, False), (64, 32, False),
+                                                 (96, 96, False), (80, 32, False), (80, 42, False), (128, 0, False)])
+@pytest.mark.parametrize("in_dtype,out_dtype", [(F32, BF16), (BF16, BF16), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_rotation_of_batches_of_tokens(cuda, tokens, dim, rot, interleaved, in_dtype, out_dtype, layout):
+    if rot == 0:
+        q, k = tensor(tokens, 3, dim, dtype=in_dtype), tensor(tokens, 1, dim, dtype=in_dtype, seed=1)
+        kc, vc = (torch.zeros(tokens, 1, 8, dim, dtype=out_dtype, device="cuda") for _ in range(2))
+        at = torch.arange(tokens, device="cuda")
+        from freemoe_b200 import attention
+
+        got = attention.rope_append(q, k, k, at.int(), torch.empty(0, device="cuda"), kc, vc, at * 8 + 3)
+        assert torch.equal(got, q.to(out_dtype)) and torch.equal(kc[:, :, 3], k.to(out_dtype)) and torch.equal(kc, vc)
+    else:
+        rope_case(tokens, 5, 2, dim, rot, in_dtype, out_dtype, 48, interleaved, layout=layout, seed=tokens)
+    assert cuda.device_status() == 0
