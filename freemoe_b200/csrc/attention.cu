@@ -271,6 +271,10 @@ extern "C" int fmcuda_paged_attention(const fmcuda_paged_attention_args *a, void
     for (const void *x : aligned)
         if (reinterpret_cast<uintptr_t>(x) % 16)
             return set_error(FM_STATUS_INVALID_ARGUMENT, "attention buffers must be 16-byte aligned");
+    const void *words[] = {a->page_table, a->q_start, a->kv_len, a->lse};
+    for (const void *x : words)
+        if (reinterpret_cast<uintptr_t>(x) % 4)
+            return set_error(FM_STATUS_INVALID_ARGUMENT, "lengths, pages and lse must be aligned to their values");
     const AttnPlan n = attn_plan(*a);
     if ((n.total && !workspace) || workspace_bytes < n.total || reinterpret_cast<uintptr_t>(workspace) % 256)
         return set_error(FM_STATUS_INVALID_ARGUMENT, "attention workspace is too small or not 256-byte aligned");

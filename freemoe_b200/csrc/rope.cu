@@ -357,6 +357,9 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
         !aligned_to_value(a->v, a->in_dtype) || !aligned_to_value(a->q_out, a->out_dtype) ||
         !aligned_to_value(a->k_cache, a->out_dtype) || !aligned_to_value(a->v_cache, a->out_dtype))
         return set_error(FM_STATUS_INVALID_ARGUMENT, "rotary buffer is not aligned to its values");
+    if (reinterpret_cast<uintptr_t>(a->positions) % 4 || (cached && reinterpret_cast<uintptr_t>(a->slots) % 8) ||
+        reinterpret_cast<uintptr_t>(a->inv_freq) % 4)
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "positions, slots or frequencies are not aligned to their values");
     if (a->tokens > 0x7FFFFFFFu) return set_error(FM_STATUS_SHAPE_MISMATCH, "too many tokens in a call");
     int *status = device_status_word();
     const uint32_t half = a->rot_dim / 2, kvh = cached ? a->kv_heads : 0;

@@ -8,7 +8,7 @@ import torch
 
 from freemoe_b200 import TYPE_Q8_0, hotpath, load
 from freemoe_b200._lib import X_BF16, X_F32, FmError
-from test_attention_cpu import rope_args
+from test_attention_cpu import P, attention_args, rope_args
 
 OK, SHAPE, ARG = 0, 8, 26
 UNREAD = [torch.float16, torch.float8_e4m3fn, torch.float64]  # rows that no product, expert or exchange reads
@@ -85,3 +85,19 @@ def test_entry_points_are_those_of_this_torch(monkeypatch):
     with pytest.raises(FmError) as e:
         attention._Calls().add_rms_norm
     assert e.value.code == 24 and "0.0.1" in str(e.value)
+
+
+@pytest.mark.parametrize("name,off", [("positions", 2), ("slots", 4), ("inv_freq", 1)])
+def test_rotation_refuses_arrays_that_are_not_aligned(name, off):
+    lib, args = load(), rope_args()
+    setattr(args, name, P + off)
+    assert lib.fmcuda_rope_append(C.byref(args), None) == ARG
+    assert b"aligned" in lib.fmcuda_last_error()
+
+
+@pytest.mark.parametrize("name,off", [("lse", 2), ("page_table", 1), ("q_start", 2), ("kv_len", 3)])
+def test_attention_refuses_arrays_that_are_not_aligned(name, off):
+    lib, args = load(), attention_args()
+    setattr(args, name, P + off)
+    assert lib.fmcuda_paged_attention(C.byref(args), None, 0, None) == ARG
+    assert b"aligned to their values" in lib.fmcuda_last_error()
