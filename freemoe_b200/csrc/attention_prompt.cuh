@@ -15,11 +15,19 @@
 // own, so that the next S is computed while the softmax still works on this
 // block.  There is one S, which the tiles use in turn: a softmax moves it to
 // registers at once, and the turns keep the tiles apart, one in its exponentials
-// while the other waits (left to themselves they fall into step; heads of 64
-// have room for an S each, but that was 5% slower, and for heads of 128 there is
-// none).  A softmax thread rescales O in place, and only when the maximum has
+// while the other waits (left to themselves they fall into step).  Heads of 64
+// have room for an S each, but that was 5% slower.  With heads of 128 there is
+// none beside a P with columns of its own; with P over S's columns two S fit, as
+// in an early form of this kernel, which took 617 us where P's own columns then
+// took 492 (a prompt of 8192; not tried again with the later steps around it).
+// A softmax thread rescales O in place, and only when the maximum has
 // grown by more than 2^8, since any reference exponent in that range gives the
 // same P / sum.
+//
+// P is rounded to the cache's 16-bit type because the matrix instructions take
+// both operands in one type; the sums take it unrounded.  For bf16 the result is then
+// within 0.0021 to 0.0023 of the 64-bit form (relative, as a norm), of which its own
+// rounding is 0.0017.
 //
 // A tile's keys end at its last row's position; only blocks that some row sees
 // in part are masked.  In the first and last block V's rows outside the
@@ -33,12 +41,13 @@
 // by attn_join_kernel.  A CTA has at most two: of the item that began before its
 // range and of the one that goes on after it.  Where there are fewer items than CTAs,
 // each is cut into pieces of its own, so that no CTA begins a second item (8 chunks of 128
-// behind 2000 keys: 69 -> 51 us; of 200 behind 3000 beside 3 decoding sequences 43 -> 36).
+// behind 2000 keys: 69 -> 51 us).
 //
-// Measured: a prompt of 8192, 32/8 heads of 128, bf16: 545 us, 1.0 PFLOP/s of the 1.66 of a
-// library product, with the tensor pipe 54% busy and the exponentials 54% at 1.64 GHz (the
-// power cap): a block's two tiles take 3200 cycles where either alone would take 2048.
-// Chunks behind contexts, heads of 64: 158 us, bound by the exponentials (58%).
+// Measured: a prompt of 8192, 32/8 heads of 128, bf16: 505 to 550 us by machine and heat, 1.0
+// to 1.1 PFLOP/s of the 1.66 of a library product, with the tensor pipe 54% busy and the
+// exponentials 54% at 1.64 GHz (the power cap): a block's two tiles take 3200 cycles where
+// either alone would take 2048.  Chunks behind contexts, heads of 64: 160 us; the exponentials
+// alone are 80 of them, the special-function unit is 58% busy.
 #pragma once
 
 #include "attention_rows.cuh"
@@ -171,7 +180,8 @@ __device__ __forceinline__ float max2(float a, float b) {
 
 // Bounded wait of a whole warp that also gives up once another role has; the
 // same answer in every lane.  (All lanes poll: with one, and the others waiting
-// for it, a prompt of 8192 tokens takes 730 us instead of 460.)
+// for it, a prompt of 8192 tokens took 730 us where it then took 460, single calls on a
+// cool GPU.)
 __device__ __forceinline__ bool ap_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag, int *status) {
     bool done = mbar_try_wait(bar, parity);
     if (!done) {
@@ -440,7 +450,9 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
         __syncthreads();
         if (warp == 0) {
             uint32_t piece = 0;
-            // pieces that the CTAs take of one head's items; the rows kernel's keep half of the SMs
+            // pieces that the CTAs take of one head's items; sequences of few rows beside them keep
+            // half of the SMs (chunks of 64 rows, 16 heads on one key head, behind 16000 keys beside 7
+            // sequences 59 us, 65 without; of 300 behind 2000 beside one 44 and 40)
             const uint32_t budget = pp.ctas / (p.row_limit ? 2u : 1u) / p.kv_heads;
             if (pairs && pairs <= budget) {
                 // the shortest pieces of which there are no more than CTAs

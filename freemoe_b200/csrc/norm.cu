@@ -8,11 +8,12 @@
 // pairwise).  The operator is one read of x and residual and one write of y and
 // h; the weight stays on the SM over the rows of a CTA.
 //
-// Measured, 8192 rows of 4096, bf16 with the residual, to 8 bits (236 MB): 40 us, 91% of
-// the rate of a copy; f32 throughout (537 MB) 97 us, 86%.  What it took: the next row's
+// Measured, 8192 rows of 4096, bf16 with the residual, to 8 bits (236 MB): 40 to 44 us by
+// machine, 84 to 91% of the rate of a copy; to bf16 (268 MB) 49 us, 85%; f32 throughout
+// (537 MB) 96 us, 87%.  What it took: the next row's
 // loads under way while a row is summed (61 -> 42), types fixed at compile time and
 // quotients without a division (49 -> 40 with the issue slots 70% busy before).  Widths
-// that are not whole eights: 4094 51 us, 4095 80 (bound by accesses of two bytes).
+// that are not whole eights: 4094 50 us, 4095 80 (bound by accesses of two bytes).
 // One row: 2.4 us, latency.
 #include <string>
 #include <type_traits>

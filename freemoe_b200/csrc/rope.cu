@@ -90,10 +90,12 @@ __device__ __forceinline__ uint4 rope_shuffle(uint4 v, uint32_t lane) {
 // move on from token to token of the CTA's batch: per token U loads under way together,
 // then the turns and the stores.  HALVES: the partners at i +- rot/2 come from the lane
 // that loaded them, where a head's eights divide a warp; PAIRED is for heads that do not.
-// Measured with 8192 tokens of 32 + 8 heads of 128, bf16 (201 MB, 31 us at the measured
-// copy rate): 37 us; U = 2 or 4, 39; an index over all of a token's eights with its
+// Measured with 8192 tokens of 32 + 8 heads of 128, bf16, interleaved (201 MB, 31 us at the
+// measured copy rate): 37 us; U = 2 or 4, 39; an index over all of a token's eights with its
 // divisions, 44 (issue slots 65% busy); the cosines worked out by every thread for
-// itself, 64.  Bound by the loads under way: registers against warps.
+// itself, 64.  Bound by the loads under way: registers against warps.  HALVES: 42 us, from
+// f32 to bf16 (302 MB) 65 against 47; it reads twice the cosines for an eight and shuffles,
+// and what bounds it has not been profiled.
 enum { ROPE_INTER, ROPE_HALVES, ROPE_PAIRED };
 
 template <int LAYOUT, int IN, int OUT>
