@@ -179,6 +179,35 @@ class RmsNormArgs(C.Structure):
     ]
 
 
+class NormAddNormArgs(C.Structure):
+    """fmcuda_norm_add_norm_args."""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("post_weight", C.c_void_p),
+        ("gate", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("pre_weight", C.c_void_p),
+        ("y", C.c_void_p),
+        ("residual_out", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("residual_stride", C.c_int64),
+        ("y_stride", C.c_int64),
+        ("gate_stride", C.c_int64),
+        ("gate_per_token", C.c_int32),
+        ("x_dtype", C.c_int32),
+        ("residual_dtype", C.c_int32),
+        ("weight_dtype", C.c_int32),
+        ("gate_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("tokens", C.c_uint32),
+        ("d_model", C.c_uint32),
+        ("scale", C.c_float),
+        ("residual_scale", C.c_float),
+        ("epsilon", C.c_float),
+    ]
+
+
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP, ROPE_BANDS = range(5)
 
 
@@ -352,9 +381,12 @@ SIGNATURES = [
     ("fmcuda_record_load", C.c_int, [_P, C.POINTER(Extent), _U32, _P, _U64, C.c_int, _U64, _P, _U64, _P, _U32,
                                      C.POINTER(RecordLoadStats)]),
     ("fmcuda_add_rms_norm", C.c_int, [C.POINTER(RmsNormArgs), _P]),
+    ("fmcuda_norm_add_norm", C.c_int, [C.POINTER(NormAddNormArgs), _P]),
     ("fmcuda_rope_frequencies", C.c_int, [_U32, _D, C.POINTER(RopeScaling), C.POINTER(C.c_float),
                                           C.POINTER(C.c_float)]),
     ("fmcuda_rope_append", C.c_int, [C.POINTER(RopeAppendArgs), _P]),
+    ("fmcuda_rope_append_axes", C.c_int, [C.POINTER(RopeAppendArgs), _P, _U32, C.c_int64, _P]),
+    ("fmcuda_rope_axes", C.c_int, [C.POINTER(C.c_uint32), _U32, _I32, _U32, C.POINTER(C.c_uint8)]),
     ("fmcuda_paged_attention_workspace_bytes", C.c_int, [C.POINTER(PagedAttentionArgs), C.POINTER(C.c_uint64)]),
     ("fmcuda_paged_attention", C.c_int, [C.POINTER(PagedAttentionArgs), _P, _U64, _P]),
     ("fmcuda_synth_weights", C.c_int, [_U32, _P, _U64, _U32, _U64, _F, _P]),

@@ -1,5 +1,5 @@
 """The attention side of a decoder layer over the C ABI: RMS norm with the
-residual's addition, rotary positions with the write into a paged K/V cache,
+residual's addition, norms around a gated block, rotary positions with the write into a paged K/V cache,
 and attention of new tokens over that cache.
 
 Like :mod:`freemoe_b200.hotpath` these are thin calls through
@@ -25,6 +25,12 @@ _ROPE_KINDS = {"plain": ROPE_PLAIN, "linear": ROPE_LINEAR, "base": ROPE_BASE, "r
 INVALID_ARGUMENT, SHAPE_MISMATCH = 26, 8
 
 
+_ENTRIES = ("fmcuda_last_error", "fmcuda_add_rms_norm", "fmcuda_norm_add_norm", "fmcuda_rope_append",
+            "fmcuda_rope_append_axes", "fmcuda_paged_attention_workspace_bytes", "fmcuda_paged_attention")
+_TORCH_CALLS = ("add_rms_norm", "add_rms_norm_fp8", "norm_add_norm", "norm_add_norm_fp8", "rope_append",
+                "paged_attention")
+
+
 class _Calls:
     """The entry points for torch tensors, loaded and given the library's addresses at
     their first use; a missing build is an error, there is no fallback."""
@@ -37,10 +43,8 @@ class _Calls:
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         lib = load()
-        module.bind(FmError, *(C.cast(getattr(lib, f), C.c_void_p).value for f in (
-            "fmcuda_last_error", "fmcuda_add_rms_norm", "fmcuda_rope_append", "fmcuda_paged_attention_workspace_bytes",
-            "fmcuda_paged_attention")))
-        for f in ("add_rms_norm", "add_rms_norm_fp8", "rope_append", "paged_attention"):
+        module.bind(FmError, {f: C.cast(getattr(lib, f), C.c_void_p).value for f in _ENTRIES})
+        for f in _TORCH_CALLS:
             setattr(self, f, getattr(module, f))
         return getattr(self, name)
 
@@ -72,6 +76,49 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.T
     return _calls.add_rms_norm_fp8(x, weight, residual, epsilon)
 
 
+def norm_add_norm(x: torch.Tensor, post_weight: torch.Tensor | None, residual: torch.Tensor,
+                  pre_weight: torch.Tensor | None, *, gate: torch.Tensor | None = None, scale: float = 1.0,
+                  residual_scale: float = 1.0, epsilon: float = 1e-5, out_dtype: torch.dtype | None = None, stream=None):
+    """The norms around a block: ``h = residual_scale * residual + scale * gate * norm(x; post_weight)``,
+    ``y = norm(h; pre_weight)`` (``fmcuda_norm_add_norm``).
+
+    ``x`` [tokens, d_model] is the block's output; ``gate`` is [d_model], [tokens, d_model]
+    or [tokens, 1].  Without ``post_weight`` x is added as it is, without ``pre_weight``
+    there is no y (None).  Returns ``(y, h)``, ``h`` in the residual's type."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _calls.norm_add_norm(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon,
+                                        out_dtype)
+    return _calls.norm_add_norm(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon, out_dtype)
+
+
+def norm_add_norm_fp8(x: torch.Tensor, post_weight: torch.Tensor | None, residual: torch.Tensor,
+                      pre_weight: torch.Tensor, *, gate: torch.Tensor | None = None, scale: float = 1.0,
+                      residual_scale: float = 1.0, epsilon: float = 1e-5, stream=None):
+    """The norms around a block with y in 8 bits: ``(codes, scales, h)`` as in
+    :func:`add_rms_norm_fp8`."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _calls.norm_add_norm_fp8(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon)
+    return _calls.norm_add_norm_fp8(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon)
+
+
+def rope_axes(sections, order: str = "blocks", device="cuda") -> torch.Tensor:
+    """The axis of each rotated pair for positions of several axes: uint8 [sum(sections)]
+    (``fmcuda_rope_axes``).  Axis a has ``sections[a]`` pairs, in "blocks" one after the
+    other or dealt out in "turn"."""
+    if order not in ("blocks", "turn"):
+        raise FmError(INVALID_ARGUMENT, f"unknown order of rotary axes {order!r}")
+    sections = [int(n) for n in sections]
+    pairs = sum(sections)
+    if any(n < 0 for n in sections) or pairs > 512:
+        raise FmError(SHAPE_MISMATCH, "rotary width must be even, 2 to 1024")
+    host = (C.c_uint8 * max(1, pairs))()
+    check(load().fmcuda_rope_axes((C.c_uint32 * max(1, len(sections)))(*sections), len(sections), int(order == "turn"),
+                                  2 * pairs, host))
+    return torch.tensor(list(host), dtype=torch.uint8).to(device)
+
+
 def rope_frequencies(rot_dim: int, base: float = 10000.0, *, kind: str = "plain", factor: float = 1.0,
                      trained_context: float = 0.0, fast: float = 0.0, slow: float = 0.0, device="cuda"):
     """Rotary frequencies, scaled for contexts longer than the trained one:
@@ -92,20 +139,22 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, *, kind: str = "plain"
 def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.Tensor,
                 inv_freq: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torch.Tensor | None,
                 slots: torch.Tensor | None, *, interleaved: bool = False, attention_factor: float = 1.0,
-                out_dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
+                out_dtype: torch.dtype | None = None, axes: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Rotates ``q`` [tokens, heads, head_dim] and ``k`` [tokens, kv_heads,
     head_dim] by their positions, writes ``k`` and ``v`` into the caches' pages at
     ``slots`` (int64: page * page_size + row; negative: nowhere) and returns the
     rotated q in the caches' type (``out_dtype`` without caches)
     (``fmcuda_rope_append``).
 
-    ``positions`` int32 [tokens]; ``inv_freq`` f32, one per rotated pair."""
+    ``positions`` int32 [tokens]; ``inv_freq`` f32, one per rotated pair.  With ``axes``
+    (:func:`rope_axes`: uint8, the axis of each pair) positions are int32 [axes, tokens],
+    time, height and width say (``fmcuda_rope_append_axes``)."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return _calls.rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved,
-                                      attention_factor, out_dtype)
+                                      attention_factor, out_dtype, axes)
     return _calls.rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved, attention_factor,
-                              out_dtype)
+                              out_dtype, axes)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

@@ -23,6 +23,7 @@ namespace fmb {
 namespace {
 
 constexpr uint32_t ROPE_THREADS = 256;
+constexpr uint32_t ROPE_MAX_AXES = 8;
 constexpr uint32_t ROPE_MAX_DIM = 1024, ROPE_TURNS = ROPE_MAX_DIM / 2, ROPE_BATCH = 8;
 
 struct RopeParams {
@@ -40,6 +41,9 @@ struct RopeParams {
     uint32_t head_items, value_items; // eights (or pairs of eights) of a rotated head, of a value head
     uint32_t tokens, batch;                  // tokens a CTA takes together
     int *status;
+    const uint8_t *axis; // each pair's axis; null: one axis
+    uint32_t axes;
+    int64_t axis_stride; // positions from axis to axis
 };
 
 // The cosines of the CTA's tokens, and their rows of the cache (-1: a slot below zero or,
@@ -49,7 +53,15 @@ __device__ __forceinline__ void rope_tokens(const RopeParams &p, uint32_t t0, ui
     const uint32_t half = p.rot / 2;
     for (uint32_t i = threadIdx.x; i < n * half; i += blockDim.x) {
         const uint32_t k = i / half;
-        const double turns = static_cast<double>(p.positions[t0 + k]) *
+        const int32_t *positions = p.positions + t0 + k;
+        if (p.axis) {
+            const uint32_t axis = p.axis[i - k * half];
+            if (axis < p.axes)
+                positions += axis * p.axis_stride;
+            else
+                raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
+        }
+        const double turns = static_cast<double>(*positions) *
                              static_cast<double>(p.inv_freq[i - k * half]) * 0.15915494309189533577; // 1 / (2 pi)
         float sn, cs;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
@@ -339,7 +351,29 @@ extern "C" int fmcuda_rope_frequencies(uint32_t rot_dim, double base, const fmcu
     return FM_STATUS_OK;
 }
 
-extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream) {
+extern "C" int fmcuda_rope_axes(const uint32_t *sections, uint32_t axes, int32_t in_turn, uint32_t rot_dim,
+                                uint8_t *axis_of_pair) {
+    if (!sections || !axis_of_pair) return set_error(FM_STATUS_INVALID_ARGUMENT, "null rotary sections");
+    if (axes == 0 || axes > ROPE_MAX_AXES) return set_error(FM_STATUS_SHAPE_MISMATCH, "rotary axes must be 1 to 8");
+    if (rot_dim == 0 || rot_dim % 2 || rot_dim > ROPE_MAX_DIM)
+        return set_error(FM_STATUS_SHAPE_MISMATCH, "rotary width must be even, 2 to 1024");
+    uint32_t left[ROPE_MAX_AXES];
+    uint64_t all = 0;
+    for (uint32_t a = 0; a < axes; ++a) all += left[a] = sections[a];
+    if (all != rot_dim / 2) return set_error(FM_STATUS_SHAPE_MISMATCH, "rotary sections must add up to the pairs");
+    uint32_t a = 0;
+    for (uint32_t i = 0; i < rot_dim / 2; ++i) {
+        while (left[a] == 0) a = a + 1 == axes ? 0 : a + 1;
+        --left[a];
+        axis_of_pair[i] = static_cast<uint8_t>(a);
+        if (in_turn) a = a + 1 == axes ? 0 : a + 1;
+    }
+    return FM_STATUS_OK;
+}
+
+namespace {
+
+int rope_append(const fmcuda_rope_append_args *a, const uint8_t *axis, uint32_t axes, int64_t axis_stride, void *stream) {
     if (!a) return set_error(FM_STATUS_INVALID_ARGUMENT, "null rotary arguments");
     if (a->heads == 0 || a->head_dim == 0 || a->head_dim > ROPE_MAX_DIM || a->heads > 65535 || a->kv_heads > 65535)
         return set_error(FM_STATUS_SHAPE_MISMATCH, "heads must be 1 to 65535 and head_dim 1 to 1024");
@@ -380,7 +414,7 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
                        a->cache_head_stride, a->cache_row_stride, a->in_dtype, a->out_dtype, a->heads, kvh,
                        a->head_dim, a->rot_dim, a->attention_factor, cached ? a->page_size : 1,
                        cached ? static_cast<uint64_t>(a->n_pages) * a->page_size : 0,
-                       a->head_dim / 8, a->head_dim / 8, a->tokens, 1, status};
+                       a->head_dim / 8, a->head_dim / 8, a->tokens, 1, status, axis, axes, axis_stride};
     // a head's eights divide a warp: partners are in the same one
     const bool paired = vec && !a->interleaved && half && 256 % a->head_dim;
     if (paired) p.head_items -= half / 8;
@@ -411,4 +445,20 @@ extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream
     if (!vec) return launch("rope_append_any_kernel", rope_append_any_kernel<false>, l, s, p);
     if (a->interleaved) return launch_rope<ROPE_INTER>(p, l, s);
     return paired ? launch_rope<ROPE_PAIRED>(p, l, s) : launch_rope<ROPE_HALVES>(p, l, s);
+}
+
+} // namespace
+
+extern "C" int fmcuda_rope_append(const fmcuda_rope_append_args *a, void *stream) {
+    return rope_append(a, nullptr, 1, 0, stream);
+}
+
+extern "C" int fmcuda_rope_append_axes(const fmcuda_rope_append_args *a, const uint8_t *axis_of_pair, uint32_t axes,
+                                       int64_t position_stride, void *stream) {
+    if (axes == 0 || axes > ROPE_MAX_AXES) return set_error(FM_STATUS_SHAPE_MISMATCH, "rotary axes must be 1 to 8");
+    if (a && a->tokens && a->rot_dim && !axis_of_pair)
+        return set_error(FM_STATUS_INVALID_ARGUMENT, "null rotary axes");
+    if (a && axes > 1 && position_stride < static_cast<int64_t>(a->tokens))
+        return set_error(FM_STATUS_SHAPE_MISMATCH, "an axis has fewer positions than there are tokens");
+    return rope_append(a, a && a->rot_dim ? axis_of_pair : nullptr, axes, position_stride, stream);
 }

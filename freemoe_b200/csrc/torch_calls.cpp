@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <map>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -25,7 +26,9 @@ namespace {
 struct Entries {
     decltype(&fmcuda_last_error) last_error;
     decltype(&fmcuda_add_rms_norm) norm;
+    decltype(&fmcuda_norm_add_norm) norm_pair;
     decltype(&fmcuda_rope_append) rope;
+    decltype(&fmcuda_rope_append_axes) rope_axes;
     decltype(&fmcuda_paged_attention_workspace_bytes) attention_bytes;
     decltype(&fmcuda_paged_attention) attention;
 } entries{};
@@ -132,19 +135,99 @@ std::tuple<Tensor, Tensor, MaybeTensor> add_rms_norm_fp8(const Tensor &x, const 
     return {codes, scales, residual ? MaybeTensor(h) : std::nullopt};
 }
 
+Tensor run_norm_pair(const Tensor &x, const MaybeTensor &post_weight, const Tensor &residual,
+                     const MaybeTensor &pre_weight, const MaybeTensor &gate, double scale, double residual_scale,
+                     double epsilon, const MaybeTensor &y, float *scales, const Here &here) {
+    here(residual), here(post_weight), here(pre_weight), here(gate);
+    const int64_t tokens = x.size(0), d = x.size(1);
+    auto weight = [&](const MaybeTensor &w) { return !w || (w->dim() == 1 && w->size(0) == d && dense(*w)); };
+    need(residual.sizes() == x.sizes() && weight(post_weight) && weight(pre_weight),
+         "norm takes [tokens, d_model], weights of d_model and a residual like x");
+    need(!post_weight || !pre_weight || post_weight->scalar_type() == pre_weight->scalar_type(),
+         "the two weights have one type", FM_STATUS_INVALID_ARGUMENT);
+    need(dense(x) && dense(residual), "norm inputs must be contiguous in their rows");
+    // like the residual in memory too: the C entry takes one stride for both
+    const Tensor h = at::empty_strided(residual.sizes(), residual.strides(), residual.options());
+    fmcuda_norm_add_norm_args a{};
+    if (gate) {
+        const int64_t rows = gate->dim() == 2 ? gate->size(0) : 1;
+        const int64_t values = gate->dim() == 1 || gate->dim() == 2 ? gate->size(-1) : -1;
+        need((values == d || (values == 1 && gate->dim() == 2)) && (rows == tokens || rows == 1),
+             "the gate is [d_model], [tokens, d_model] or [tokens, 1]");
+        need(values == 1 || dense(*gate), "the gate must be contiguous in its rows");
+        a.gate = gate->data_ptr();
+        a.gate_stride = rows == 1 ? 0 : gate->stride(0);
+        a.gate_per_token = values == 1;
+        a.gate_dtype = dtype_of(*gate);
+    }
+    a.x = x.data_ptr();
+    a.post_weight = at_of(post_weight);
+    a.residual = residual.data_ptr();
+    a.pre_weight = at_of(pre_weight);
+    a.y = at_of(y);
+    a.residual_out = h.data_ptr();
+    a.scales = scales;
+    a.x_stride = x.stride(0);
+    a.residual_stride = residual.stride(0);
+    a.y_stride = d;
+    a.x_dtype = dtype_of(x);
+    a.residual_dtype = dtype_of(residual);
+    a.weight_dtype = post_weight ? dtype_of(*post_weight) : pre_weight ? dtype_of(*pre_weight) : FM_X_F32;
+    a.y_dtype = !y ? FM_X_F32 : scales ? FM_X_E4M3 : dtype_of(*y);
+    a.tokens = static_cast<uint32_t>(tokens);
+    a.d_model = static_cast<uint32_t>(d);
+    a.scale = static_cast<float>(scale);
+    a.residual_scale = static_cast<float>(residual_scale);
+    a.epsilon = static_cast<float>(epsilon);
+    check(entries.norm_pair(&a, here.stream()));
+    return h;
+}
+
+std::tuple<MaybeTensor, Tensor> norm_add_norm(const Tensor &x, const MaybeTensor &post_weight, const Tensor &residual,
+                                              const MaybeTensor &pre_weight, const MaybeTensor &gate, double scale,
+                                              double residual_scale, double epsilon,
+                                              std::optional<at::ScalarType> out_dtype) {
+    need_rows(x);
+    const Here here(x);
+    MaybeTensor y;
+    if (pre_weight) y = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+    const Tensor h =
+        run_norm_pair(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon, y, nullptr, here);
+    return {y, h};
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_add_norm_fp8(const Tensor &x, const MaybeTensor &post_weight,
+                                                     const Tensor &residual, const Tensor &pre_weight,
+                                                     const MaybeTensor &gate, double scale, double residual_scale,
+                                                     double epsilon) {
+    need_rows(x);
+    const Here here(x);
+    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    const Tensor scales = at::empty({x.size(0), (x.size(1) + 127) / 128}, x.options().dtype(at::kFloat));
+    const Tensor h = run_norm_pair(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon, codes,
+                                   static_cast<float *>(scales.data_ptr()), here);
+    return {codes, scales, h};
+}
+
 Tensor rope_append(const Tensor &q, const MaybeTensor &k, const MaybeTensor &v, const Tensor &positions,
                    const Tensor &inv_freq, const MaybeTensor &k_cache, const MaybeTensor &v_cache,
                    const MaybeTensor &slots, bool interleaved, double attention_factor,
-                   std::optional<at::ScalarType> out_dtype) {
+                   std::optional<at::ScalarType> out_dtype, const MaybeTensor &axes) {
     need(q.dim() == 3, "q is [tokens, heads, head_dim]");
     const Here here(q);
-    here(k), here(v), here(positions), here(inv_freq), here(k_cache), here(v_cache), here(slots);
+    here(k), here(v), here(positions), here(inv_freq), here(k_cache), here(v_cache), here(slots), here(axes);
     const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2);
     need(tokens <= INT32_MAX && heads <= INT32_MAX && dim <= INT32_MAX, "too many tokens in a call");
-    need(positions.dim() == 1 && positions.size(0) == tokens && positions.scalar_type() == at::kInt &&
-             positions.is_contiguous() && inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat &&
+    // positions are [tokens], beside axes [axes, tokens]
+    const int64_t n_axes = axes && positions.dim() == 2 ? positions.size(0) : 1;
+    need(positions.dim() == (axes ? 2 : 1) && positions.size(-1) == tokens && positions.scalar_type() == at::kInt &&
+             dense(positions) && (n_axes <= 1 || positions.stride(0) >= tokens) && n_axes <= INT32_MAX &&
+             inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat &&
              inv_freq.is_contiguous() && inv_freq.size(0) <= INT32_MAX / 2,
-         "positions are int32 [tokens], inv_freq is float32 [rot_dim / 2]");
+         "positions are int32 [tokens] (with axes, [axes, tokens]), inv_freq is float32 [rot_dim / 2]");
+    need(!axes || (axes->dim() == 1 && axes->scalar_type() == at::kByte && axes->is_contiguous() &&
+                   axes->size(0) == inv_freq.size(0)),
+         "axes are uint8 [rot_dim / 2]");
     need(dense(q), "q, k, v and caches must be contiguous in their heads");
     fmcuda_rope_append_args a{};
     at::ScalarType kind = out_dtype.value_or(q.scalar_type());
@@ -198,7 +281,11 @@ Tensor rope_append(const Tensor &q, const MaybeTensor &k, const MaybeTensor &v, 
     a.rot_dim = static_cast<uint32_t>(2 * inv_freq.size(0));
     a.interleaved = interleaved;
     a.attention_factor = static_cast<float>(attention_factor);
-    check(entries.rope(&a, here.stream()));
+    if (axes)
+        check(entries.rope_axes(&a, static_cast<const uint8_t *>(axes->data_ptr()), static_cast<uint32_t>(n_axes),
+                                positions.stride(0), here.stream()));
+    else
+        check(entries.rope(&a, here.stream()));
     return out;
 }
 
@@ -277,14 +364,19 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     return {out, return_lse ? MaybeTensor(lse) : std::nullopt};
 }
 
-void bind(py::object error, uint64_t last_error, uint64_t norm, uint64_t rope, uint64_t attention_bytes,
-          uint64_t attention) {
+// The package's error class and the library's entries by name.
+void bind(py::object error, const std::map<std::string, uint64_t> &at) {
     error_class = error.release().ptr(); // kept for the life of the process
-    entries.last_error = reinterpret_cast<decltype(entries.last_error)>(last_error);
-    entries.norm = reinterpret_cast<decltype(entries.norm)>(norm);
-    entries.rope = reinterpret_cast<decltype(entries.rope)>(rope);
-    entries.attention_bytes = reinterpret_cast<decltype(entries.attention_bytes)>(attention_bytes);
-    entries.attention = reinterpret_cast<decltype(entries.attention)>(attention);
+    auto take = [&](auto &entry, const char *name) {
+        entry = reinterpret_cast<std::remove_reference_t<decltype(entry)>>(at.at(name));
+    };
+    take(entries.last_error, "fmcuda_last_error");
+    take(entries.norm, "fmcuda_add_rms_norm");
+    take(entries.norm_pair, "fmcuda_norm_add_norm");
+    take(entries.rope, "fmcuda_rope_append");
+    take(entries.rope_axes, "fmcuda_rope_append_axes");
+    take(entries.attention_bytes, "fmcuda_paged_attention_workspace_bytes");
+    take(entries.attention, "fmcuda_paged_attention");
 }
 
 } // namespace
@@ -293,6 +385,8 @@ PYBIND11_MODULE(_torch_calls, m) {
     m.def("bind", &bind);
     m.def("add_rms_norm", &add_rms_norm);
     m.def("add_rms_norm_fp8", &add_rms_norm_fp8);
+    m.def("norm_add_norm", &norm_add_norm);
+    m.def("norm_add_norm_fp8", &norm_add_norm_fp8);
     m.def("rope_append", &rope_append);
     m.def("paged_attention", &paged_attention);
 }

@@ -628,6 +628,39 @@ typedef struct fmcuda_rms_norm_args {
 } fmcuda_rms_norm_args;
 int fmcuda_add_rms_norm(const fmcuda_rms_norm_args *args, void *stream);
 
+/* The norms around a block, with its gated and scaled addition to the residual stream:
+ *   n = x * post_weight / sqrt(mean(x^2) + epsilon)       (without post_weight: n = x)
+ *   h = residual_scale * residual + scale * gate * n      (without gate: 1)
+ *   y = h * pre_weight / sqrt(mean(h^2) + epsilon)        (without pre_weight: h alone)
+ * x is the output of an attention or expert block, y the input of the next one.  Sums,
+ * n and h are held in f32 and each result is rounded once to its type; y and its 8-bit
+ * form are as in fmcuda_add_rms_norm, and so are the rules on buffers that may coincide. */
+typedef struct fmcuda_norm_add_norm_args {
+    const void *x;              /* [tokens][d_model] */
+    const void *post_weight;    /* optional [d_model] */
+    const void *gate;           /* optional: [d_model] (gate_stride 0), [tokens][d_model] or, per token, [tokens] */
+    const void *residual;       /* [tokens][d_model] */
+    const void *pre_weight;     /* optional [d_model] */
+    void *y;                    /* [tokens][d_model], with pre_weight */
+    void *residual_out;         /* h, in residual_dtype; optional with pre_weight */
+    float *scales;              /* [tokens][ceil(d_model / 128)] with FM_X_E4M3, else unused */
+    int64_t x_stride;           /* from row to row, at least d_model */
+    int64_t residual_stride;    /* of residual and of residual_out */
+    int64_t y_stride;
+    int64_t gate_stride;        /* 0: one row (or one value) for all tokens */
+    int32_t gate_per_token;     /* a row of the gate is one value */
+    int32_t x_dtype;            /* FM_X_F32, FM_X_BF16, FM_X_F16 */
+    int32_t residual_dtype;     /* the same three */
+    int32_t weight_dtype;       /* the same three, of both weights */
+    int32_t gate_dtype;         /* the same three */
+    int32_t y_dtype;            /* the same three, or FM_X_E4M3 */
+    uint32_t tokens;
+    uint32_t d_model;           /* 1 .. 2^24 */
+    float scale, residual_scale; /* finite */
+    float epsilon;              /* >= 0 */
+} fmcuda_norm_add_norm_args;
+int fmcuda_norm_add_norm(const fmcuda_norm_add_norm_args *args, void *stream);
+
 /* Rotary frequencies f_i = base^(-2i / rot_dim), i < rot_dim / 2, and their
  * scalings for contexts longer than the trained one (host arithmetic in double,
  * rounded once).  *attention_factor is what cos and sin are multiplied by. */
@@ -675,6 +708,18 @@ typedef struct fmcuda_rope_append_args {
     uint32_t n_pages, page_size;
 } fmcuda_rope_append_args;
 int fmcuda_rope_append(const fmcuda_rope_append_args *args, void *stream);
+
+/* The same with positions of several axes (time, height and width of images and
+ * video): args->positions is [axes][position_stride], and pair i turns by
+ * positions[axis_of_pair[i]][t] * inv_freq[i].  Tokens of text stand at one
+ * position on all axes.  axis_of_pair: device [rot_dim / 2]; a value of `axes` or
+ * more sets the device status to INVALID_ARGUMENT and turns by the first axis. */
+int fmcuda_rope_append_axes(const fmcuda_rope_append_args *args, const uint8_t *axis_of_pair, uint32_t axes,
+                            int64_t position_stride, void *stream);
+/* Such axes on the host: axis a has sections[a] pairs (rot_dim / 2 in all), one
+ * axis's pairs after the other's or, in_turn, dealt out in turn, an axis that has its
+ * number left out.  1 to 8 axes. */
+int fmcuda_rope_axes(const uint32_t *sections, uint32_t axes, int32_t in_turn, uint32_t rot_dim, uint8_t *axis_of_pair);
 
 /* Attention of new tokens over a paged cache: for row t of sequence b and query
  * head j, over the keys i that the row sees,
