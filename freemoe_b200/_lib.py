@@ -294,6 +294,24 @@ class PagedAttentionArgs(C.Structure):
     ]
 
 
+class TokenLogprobsArgs(C.Structure):
+    """fmcuda_token_logprobs_args."""
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("token", C.c_void_p),
+        ("logprobs", C.c_void_p),
+        ("entropy", C.c_void_p),
+        ("top_logprobs", C.c_void_p),
+        ("top_ids", C.c_void_p),
+        ("row_stride", C.c_int64),
+        ("scale", C.c_double),
+        ("dtype", C.c_int32),
+        ("tokens", C.c_uint32),
+        ("vocab", C.c_uint32),
+        ("top", C.c_uint32),
+    ]
+
+
 READER_BUFFERED, READER_DIRECT = 1, 3  # fm::ReaderMode ordinals
 
 MOE_STAGES = ("router", "grouping", "x_planes", "gate_up", "act_planes", "down", "combine")
@@ -389,6 +407,7 @@ SIGNATURES = [
     ("fmcuda_rope_axes", C.c_int, [C.POINTER(C.c_uint32), _U32, _I32, _U32, C.POINTER(C.c_uint8)]),
     ("fmcuda_paged_attention_workspace_bytes", C.c_int, [C.POINTER(PagedAttentionArgs), C.POINTER(C.c_uint64)]),
     ("fmcuda_paged_attention", C.c_int, [C.POINTER(PagedAttentionArgs), _P, _U64, _P]),
+    ("fmcuda_token_logprobs", C.c_int, [C.POINTER(TokenLogprobsArgs), _P]),
     ("fmcuda_synth_weights", C.c_int, [_U32, _P, _U64, _U32, _U64, _F, _P]),
 ]
 

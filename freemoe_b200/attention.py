@@ -26,9 +26,10 @@ INVALID_ARGUMENT, SHAPE_MISMATCH = 26, 8
 
 
 _ENTRIES = ("fmcuda_last_error", "fmcuda_add_rms_norm", "fmcuda_norm_add_norm", "fmcuda_rope_append",
-            "fmcuda_rope_append_axes", "fmcuda_paged_attention_workspace_bytes", "fmcuda_paged_attention")
+            "fmcuda_rope_append_axes", "fmcuda_paged_attention_workspace_bytes", "fmcuda_paged_attention",
+            "fmcuda_token_logprobs")
 _TORCH_CALLS = ("add_rms_norm", "add_rms_norm_fp8", "norm_add_norm", "norm_add_norm_fp8", "rope_append",
-                "paged_attention")
+                "paged_attention", "token_logprobs")
 
 
 class _Calls:

@@ -68,12 +68,6 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
     return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <bool BF16> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     uint32_t r;
     if constexpr (BF16)

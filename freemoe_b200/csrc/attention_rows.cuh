@@ -485,28 +485,6 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
 // warps are joined in its shared memory and the CTAs through each other's: one
 // launch, no fragments in global memory.  blockIdx.x / cluster size: (sequence,
 // key head, row tile), `unit_tiles` row tiles a sequence and head.
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-// A value of CTA `rank`'s shared memory, at the address that `addr` has in this one's.
-__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-
 template <int DP, bool BF16>
 __device__ __forceinline__ void ar_cluster(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t unit_tiles) {
     using L = ARows<DP>;

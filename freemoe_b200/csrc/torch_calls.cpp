@@ -1,4 +1,5 @@
-// torch_calls.cpp -- the attention side's entry points for torch tensors.
+// torch_calls.cpp -- entry points for torch tensors: the attention side's, and the
+// probabilities of tokens.
 //
 // A decoding step makes these calls for every layer, with two or three
 // microseconds of GPU work in each; through ctypes the call itself took ten.
@@ -31,6 +32,7 @@ struct Entries {
     decltype(&fmcuda_rope_append_axes) rope_axes;
     decltype(&fmcuda_paged_attention_workspace_bytes) attention_bytes;
     decltype(&fmcuda_paged_attention) attention;
+    decltype(&fmcuda_token_logprobs) logprobs;
 } entries{};
 PyObject *error_class = nullptr; // FmError(code, message)
 
@@ -364,6 +366,37 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     return {out, return_lse ? MaybeTensor(lse) : std::nullopt};
 }
 
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &tokens, int64_t top,
+                                                          double scale) {
+    need(logits.dim() == 2 && logits.size(0) <= INT32_MAX && logits.size(1) <= INT32_MAX, "logits are [tokens, vocab]");
+    const Here here(logits);
+    here(tokens);
+    const int64_t rows = logits.size(0);
+    need(tokens.dim() == 1 && tokens.size(0) == rows && tokens.scalar_type() == at::kInt && tokens.is_contiguous(),
+         "tokens are int32 [tokens]");
+    need(dense(logits), "logits must be contiguous in their rows");
+    need(top >= 0 && top <= logits.size(1), "top must not be negative or above the vocabulary",
+         FM_STATUS_INVALID_ARGUMENT);
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const Tensor chosen = at::empty({rows}, f32), entropy = at::empty({rows}, f32), best = at::empty({rows, top}, f32);
+    const Tensor ids = at::empty({rows, top}, logits.options().dtype(at::kInt));
+    fmcuda_token_logprobs_args a{};
+    a.logits = logits.data_ptr();
+    a.token = static_cast<const int32_t *>(tokens.data_ptr());
+    a.logprobs = static_cast<float *>(chosen.data_ptr());
+    a.entropy = static_cast<float *>(entropy.data_ptr());
+    a.top_logprobs = static_cast<float *>(best.data_ptr());
+    a.top_ids = static_cast<int32_t *>(ids.data_ptr());
+    a.row_stride = logits.stride(0);
+    a.scale = scale;
+    a.dtype = dtype_of(logits);
+    a.tokens = static_cast<uint32_t>(rows);
+    a.vocab = static_cast<uint32_t>(logits.size(1));
+    a.top = static_cast<uint32_t>(top);
+    check(entries.logprobs(&a, here.stream()));
+    return {chosen, entropy, best, ids};
+}
+
 // The package's error class and the library's entries by name.
 void bind(py::object error, const std::map<std::string, uint64_t> &at) {
     error_class = error.release().ptr(); // kept for the life of the process
@@ -377,6 +410,7 @@ void bind(py::object error, const std::map<std::string, uint64_t> &at) {
     take(entries.rope_axes, "fmcuda_rope_append_axes");
     take(entries.attention_bytes, "fmcuda_paged_attention_workspace_bytes");
     take(entries.attention, "fmcuda_paged_attention");
+    take(entries.logprobs, "fmcuda_token_logprobs");
 }
 
 } // namespace
@@ -389,4 +423,5 @@ PYBIND11_MODULE(_torch_calls, m) {
     m.def("norm_add_norm_fp8", &norm_add_norm_fp8);
     m.def("rope_append", &rope_append);
     m.def("paged_attention", &paged_attention);
+    m.def("token_logprobs", &token_logprobs);
 }

@@ -12,6 +12,7 @@ import torch
 
 from ._lib import (GEOMETRY, ORDER_ANY, TYPE_F32, X_BF16, X_F32, DeviceInfo, FmError, MoeArgs, RouterConfig, SharedExpert,
                    check, load)
+from .attention import _calls
 
 
 def _stream(stream=None) -> int:
@@ -121,6 +122,20 @@ def route_ex(logits: torch.Tensor, top_k: int, config: RouterConfig, want_probs:
     check(load().fmcuda_route_ex(_ptr(logits.contiguous()), T, E, top_k, C.byref(config), _ptr(ids), _ptr(w),
                                  _ptr(probs) if probs is not None else None, _stream(stream)))
     return (ids, w, probs) if want_probs else (ids, w)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, scale: float = 1.0, stream=None):
+    """Log probabilities of given tokens under ``softmax(scale * logits)``, the entropy, and the
+    ``top`` most probable tokens, in one read of the logits (``fmcuda_token_logprobs``).
+
+    ``logits`` [tokens, vocab] float32, bfloat16 or float16, ``tokens`` int32 [tokens] (negative:
+    none, its log probability is 0).  Returns ``(logprobs [tokens], entropy [tokens],
+    top_logprobs [tokens, top], top_ids [tokens, top])``, float32 and int32, the tops in the
+    order of a stable descending sort."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _calls.token_logprobs(logits, tokens, top, scale)
+    return _calls.token_logprobs(logits, tokens, top, scale)
 
 
 def group_by_expert(ids: torch.Tensor, experts: int, stream=None):

@@ -773,6 +773,35 @@ int fmcuda_paged_attention_workspace_bytes(const fmcuda_paged_attention_args *ar
 int fmcuda_paged_attention(const fmcuda_paged_attention_args *args, void *workspace, uint64_t workspace_bytes,
                            void *stream);
 
+/* ==================== probabilities of tokens ==================== *
+ * What follows the output head (fmcuda_gemv over its rows): the sampler's softmax
+ * (src/engine.cpp) without the sampling.  With z = scale * logits[t] and
+ * L = log sum_i exp(z_i), in one read of the logits:
+ *   logprobs[t] = z[token[t]] - L                 log probability of a given token
+ *   entropy[t]  = -sum_i p_i log p_i              of the distribution, p = exp(z - L)
+ *   top_ids, top_logprobs [t][top]                its most probable tokens, the first ones of a
+ *                                                 stable descending sort (ties to the lower id)
+ * Sums are f32, joined in 64 bits at the end.  A logit of -inf (a token ruled out) has
+ * probability 0; where all are -inf the log probabilities are -inf, the entropy 0 and the
+ * ids the first ones.  A row with NaN or +inf has NaN for probabilities and entropy, and ids
+ * in which NaN counts as -inf.  A negative token is none: its log probability is 0.  One past
+ * the vocabulary gives NaN and sets the device status to INVALID_ARGUMENT. */
+typedef struct fmcuda_token_logprobs_args {
+    const void *logits;         /* [tokens][vocab] */
+    const int32_t *token;       /* device [tokens] */
+    float *logprobs;            /* [tokens] */
+    float *entropy;             /* [tokens] */
+    float *top_logprobs;        /* [tokens][top]; unused without top */
+    int32_t *top_ids;           /* [tokens][top] */
+    int64_t row_stride;         /* from row to row, in elements, at least vocab */
+    double scale;               /* 1 / temperature: 1e-30 to 1e30 */
+    int32_t dtype;              /* FM_X_F32, FM_X_BF16, FM_X_F16 */
+    uint32_t tokens;
+    uint32_t vocab;             /* 1 .. 2^30 */
+    uint32_t top;               /* 0 .. 32, at most vocab */
+} fmcuda_token_logprobs_args;
+int fmcuda_token_logprobs(const fmcuda_token_logprobs_args *args, void *stream);
+
 /* ====================== synthetic weights (bench/test) ====================== */
 
 /* Fills `dst` with `rows` rows of `cols` values of `type_id` (Q8_0 / Q4_K /

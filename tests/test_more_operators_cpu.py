@@ -9,14 +9,15 @@ import pytest
 import torch
 
 from conftest import ROOT
-from freemoe_b200 import attention, load
-from freemoe_b200._lib import FmError, NormAddNormArgs
+from freemoe_b200 import attention, hotpath, load
+from freemoe_b200._lib import FmError, NormAddNormArgs, TokenLogprobsArgs
 from test_attention_cpu import P, rope_args
 
 OK, SHAPE, ARG = 0, 8, 26
 
 
-@pytest.mark.parametrize("name,struct", [("fmcuda_norm_add_norm_args", NormAddNormArgs)])
+@pytest.mark.parametrize("name,struct", [("fmcuda_norm_add_norm_args", NormAddNormArgs),
+                                         ("fmcuda_token_logprobs_args", TokenLogprobsArgs)])
 def test_struct_layouts_match_the_header(tmp_path, name, struct):
     fields = [f for f, _ in struct._fields_]
     prints = "".join(f'printf("%zu ", offsetof({name}, {f}));' for f in fields)
@@ -102,8 +103,30 @@ def test_axes_of_the_c_entry():
     assert lib.fmcuda_rope_axes(None, 2, 0, 8, out) == ARG and lib.fmcuda_rope_axes(sections, 2, 0, 8, None) == ARG
 
 
+# ---------------------------------------------------------------------- probabilities of tokens
+
+
+@pytest.mark.parametrize("code,change", [
+    (ARG, {"logits": None}), (ARG, {"token": None}), (ARG, {"logprobs": None}), (ARG, {"entropy": None}),
+    (ARG, {"top_logprobs": None}), (ARG, {"top_ids": None}), (ARG, {"dtype": 3}), (ARG, {"dtype": -1}),
+    (SHAPE, {"vocab": 0}), (SHAPE, {"vocab": (1 << 30) + 1}), (ARG, {"top": 33}), (ARG, {"vocab": 4, "top": 5}),
+    (SHAPE, {"row_stride": 99}), (SHAPE, {"tokens": 1 << 31}), (ARG, {"scale": 0.0}), (ARG, {"scale": float("inf")}),
+    (ARG, {"scale": float("nan")}), (ARG, {"logits": P + 1}), (ARG, {"token": P + 2}), (ARG, {"top_ids": P + 1}),
+    (OK, {"tokens": 0}), (OK, {"tokens": 0, "logits": None}),
+])
+def test_logprobs_refuse(code, change):
+    a = TokenLogprobsArgs(logits=P, token=P, logprobs=P, entropy=P, top_logprobs=P, top_ids=P, row_stride=100, scale=1.0,
+                          dtype=1, tokens=3, vocab=100, top=5)
+    for k, v in change.items():
+        setattr(a, k, v)
+    lib = load()
+    assert lib.fmcuda_token_logprobs(C.byref(a), None) == code
+    assert lib.fmcuda_token_logprobs(None, None) == ARG
+
+
 def test_torch_calls_refuse_host_tensors():
     for call in (lambda: attention.norm_add_norm(torch.zeros(2, 8), torch.ones(8), torch.zeros(2, 8), torch.ones(8)),
+                 lambda: hotpath.token_logprobs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)),
                  lambda: attention.norm_add_norm_fp8(torch.zeros(2, 8), None, torch.zeros(2, 8), torch.ones(8)),
                  lambda: attention.rope_append(torch.zeros(2, 1, 8), None, None, torch.zeros(1, 2, dtype=torch.int32),
                                                torch.ones(4), None, None, None,
