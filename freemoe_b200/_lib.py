@@ -407,6 +407,9 @@ SIGNATURES = [
     ("fmcuda_rope_axes", C.c_int, [C.POINTER(C.c_uint32), _U32, _I32, _U32, C.POINTER(C.c_uint8)]),
     ("fmcuda_paged_attention_workspace_bytes", C.c_int, [C.POINTER(PagedAttentionArgs), C.POINTER(C.c_uint64)]),
     ("fmcuda_paged_attention", C.c_int, [C.POINTER(PagedAttentionArgs), _P, _U64, _P]),
+    ("fmcuda_paged_attention_sinks_workspace_bytes", C.c_int, [C.POINTER(PagedAttentionArgs), _U32,
+                                                               C.POINTER(C.c_uint64)]),
+    ("fmcuda_paged_attention_sinks", C.c_int, [C.POINTER(PagedAttentionArgs), _U32, _P, _U64, _P]),
     ("fmcuda_token_logprobs", C.c_int, [C.POINTER(TokenLogprobsArgs), _P]),
     ("fmcuda_synth_weights", C.c_int, [_U32, _P, _U64, _U32, _U64, _F, _P]),
 ]

@@ -26,7 +26,7 @@ INVALID_ARGUMENT, SHAPE_MISMATCH = 26, 8
 
 
 _ENTRIES = ("fmcuda_last_error", "fmcuda_add_rms_norm", "fmcuda_norm_add_norm", "fmcuda_rope_append",
-            "fmcuda_rope_append_axes", "fmcuda_paged_attention_workspace_bytes", "fmcuda_paged_attention",
+            "fmcuda_rope_append_axes", "fmcuda_paged_attention_sinks_workspace_bytes", "fmcuda_paged_attention_sinks",
             "fmcuda_token_logprobs")
 _TORCH_CALLS = ("add_rms_norm", "add_rms_norm_fp8", "norm_add_norm", "norm_add_norm_fp8", "rope_append",
                 "paged_attention", "token_logprobs")
@@ -160,22 +160,24 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     q_start: torch.Tensor, kv_len: torch.Tensor, *, max_q_len: int, max_kv_len: int,
-                    scale: float | None = None, causal: bool = True, window: int = 0, return_lse: bool = False,
-                    workspace: torch.Tensor | None = None, stream=None):
+                    scale: float | None = None, causal: bool = True, window: int = 0, sinks: int = 0,
+                    return_lse: bool = False, workspace: torch.Tensor | None = None, stream=None):
     """Attention of the new tokens ``q`` [tokens, heads, head_dim] over the
     pages of their sequences (``fmcuda_paged_attention``).
 
     Sequence b has the rows ``q_start[b]:q_start[b + 1]`` and ``kv_len[b]`` keys
     (its new tokens' own among them), key i on page ``page_table[b, i //
     page_size]``; all three are int32 on the device.  ``max_q_len`` and
-    ``max_kv_len`` bound the lengths.  ``workspace``: device bytes to use instead
+    ``max_kv_len`` bound the lengths.  With ``window`` a row sees its last ``window`` keys, and
+    the first ``sinks`` of its sequence stay visible (``fmcuda_paged_attention_sinks``): pages
+    between them and the call's windows may be freed.  ``workspace``: device bytes to use instead
     of allocating (256-byte aligned, not shared with a call that overlaps).
     Returns the output, and with ``return_lse`` the f32 [tokens, heads] log-sum-exp."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, max_q_len=max_q_len,
                                    max_kv_len=max_kv_len, scale=scale, causal=causal, window=window,
-                                   return_lse=return_lse, workspace=workspace)
+                                   sinks=sinks, return_lse=return_lse, workspace=workspace)
     out, lse = _calls.paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, max_q_len, max_kv_len, scale,
-                                      causal, window, return_lse, workspace)
+                                      causal, window, sinks, return_lse, workspace)
     return (out, lse) if return_lse else out

@@ -18,6 +18,7 @@ struct AttnParams {
     uint32_t n_pages, page_size;
     uint32_t max_q, max_kv;
     uint32_t window; // 0: none
+    uint32_t sinks;  // first keys that stay visible behind the window
     int32_t causal;
     float scale, scale_log2; // scale, and scale * log2(e)
     int *status;

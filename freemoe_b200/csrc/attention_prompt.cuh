@@ -34,6 +34,10 @@
 // sequence are zeroed after the copy: their weights are zero, but what lies
 // there may be NaN.
 //
+// SINKS: the first p.sinks keys stay visible behind the window.  A pair's blocks are then
+// counted without the gap between those of the first keys and those of its windows (`skip`
+// blocks from block `first` on), and a tile takes the ones before fe and those of [tb, te).
+//
 // A persistent CTA an SM.  Where there are many (pair of tiles, key head) items,
 // they go to the CTAs whole, the longest first, in rounds that run there and
 // back.  Where there are few, all their blocks laid end to end are cut into equal
@@ -246,12 +250,24 @@ __device__ __forceinline__ APRow ap_row(const AttnParams &p, const AttnSeq &s, u
     return {static_cast<uint64_t>(s.q0) + tok, static_cast<uint64_t>(head) * p.group + (row - tok * p.group), tok < s.ql};
 }
 
-// The blocks of a pair; one without keys has a block that no tile takes.
-__device__ __forceinline__ uint2 ap_span(const APTile &t0, const APTile &t1) {
+// The blocks of a pair; one without keys has a block that no tile takes.  With SINKS they are
+// counted from 0: blocks from `first` on lie `skip` blocks further.
+struct APSpan {
+    uint32_t x, y, first, skip;
+};
+template <bool SINKS> __device__ __forceinline__ APSpan ap_span(const AttnParams &p, const APTile &t0, const APTile &t1) {
     const bool e0 = t0.j1 > t0.j0, e1 = t1.j1 > t1.j0;
     const uint32_t j0 = e0 ? t0.j0 : e1 ? t1.j0 : 0;
     const uint32_t j1 = e1 ? (e0 && t0.j1 > t1.j1 ? t0.j1 : t1.j1) : e0 ? t0.j1 : 0;
-    return make_uint2(j0, j1 > j0 ? j1 : j0 + 1);
+    APSpan s{j0, j1 > j0 ? j1 : j0 + 1, 0, 0};
+    if constexpr (SINKS) {
+        const uint32_t first = (p.sinks + AP_KEYS - 1) / AP_KEYS;
+        s.first = first < j0 ? first : j0;
+        s.skip = j0 - s.first;
+        s.x = 0;
+        s.y -= s.skip;
+    }
+    return s;
 }
 
 // A CTA's way through its work, walked by each role for itself.
@@ -265,6 +281,7 @@ struct APSeg {
     AttnSeq s;
     APTile t0, t1;
     uint32_t b, pair, head, jb, je, j1; // blocks [jb, je); the item's end
+    uint32_t first, skip;
     bool starts, whole;
 };
 
@@ -278,11 +295,12 @@ struct APShared {
     uint32_t row0;                       // first row of the pair
     uint32_t q0, ql, kl, head;
     uint32_t starts, whole;
+    uint32_t fe[2], skip; // SINKS: blocks [jb, fe) too (fe 0: none); those of [tb, te) lie `skip` further
 };
 static_assert(sizeof(APShared) * AP_SEG_SLOTS <= 512, "segments outgrow their place");
 
 // Called by whole warps; false at the end.
-__device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g) {
+template <bool SINKS> __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g) {
     const AttnParams &p = pp.a;
     const uint32_t lane = threadIdx.x & 31u;
     if (!pp.deal) {
@@ -321,7 +339,9 @@ __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g)
         g.s = attn_seq(p, g.b, false);
         g.t0 = ap_tile(p, g.s, g.pair * AP_PAIR);
         g.t1 = ap_tile(p, g.s, g.pair * AP_PAIR + AP_TILE);
-        const uint2 span = ap_span(g.t0, g.t1);
+        const APSpan span = ap_span<SINKS>(p, g.t0, g.t1);
+        g.first = span.first;
+        g.skip = span.skip;
         g.jb = span.x;
         g.je = g.j1 = span.y;
         g.starts = g.whole = true;
@@ -353,7 +373,7 @@ __device__ __forceinline__ bool ap_next(const APParams &pp, APWalk &w, APSeg &g)
 
 // ---- the kernel ---------------------------------------------------------------------
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtensorMap &map_v, const APParams &pp,
                                           uint8_t *ap_smem_raw) {
     using L = APrompt<DP>;
@@ -444,7 +464,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
             }
             const AttnSeq s = attn_seq(p, seq_of[lo], false);
             const uint32_t row0 = (i - first_of[lo]) * AP_PAIR;
-            const uint2 span = ap_span(ap_tile(p, s, row0), ap_tile(p, s, row0 + AP_TILE));
+            const APSpan span = ap_span<SINKS>(p, ap_tile(p, s, row0), ap_tile(p, s, row0 + AP_TILE));
             cost_before[i + 1] = span.y - span.x;
         }
         __syncthreads();
@@ -553,7 +573,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
             bool going = true, more = true;
             APSeg g;
             for (uint32_t k = 0; going && more; ++k) {
-                more = ap_next(pp, walk, g);
+                more = ap_next<SINKS>(pp, walk, g);
                 going = ap_wait(&seg_empty[k % AP_SEG_SLOTS], ((k / AP_SEG_SLOTS) & 1u) ^ 1u, abort_flag, p.status);
                 if (!going) break;
                 const AttnSeq &s = g.s;
@@ -564,7 +584,16 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
 #pragma unroll
                     for (uint32_t t = 0; t < 2; ++t) {
                         const APTile &tile = t ? g.t1 : g.t0;
-                        const uint32_t tb = tile.j0 > g.jb ? tile.j0 : g.jb, te = tile.j1 < g.je ? tile.j1 : g.je;
+                        const uint32_t j0 = tile.j0 - (SINKS && tile.j1 > tile.j0 ? g.skip : 0);
+                        const uint32_t j1 = tile.j1 - (SINKS && tile.j1 > tile.j0 ? g.skip : 0);
+                        const uint32_t tb = j0 > g.jb ? j0 : g.jb, te = j1 < g.je ? j1 : g.je;
+                        if constexpr (SINKS) {
+                            // the tile's blocks of the first keys end where its window's begin
+                            uint32_t fe = (p.sinks + AP_KEYS - 1) / AP_KEYS;
+                            if (fe > j0) fe = j0;
+                            if (fe > g.je) fe = g.je;
+                            o.fe[t] = tile.j1 > tile.j0 && fe > g.jb ? fe : 0;
+                        }
                         o.tb[t] = tb;
                         o.te[t] = te > tb ? te : tb;
                         o.whole_lo[t] = tile.whole_lo;
@@ -578,6 +607,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     o.head = g.head;
                     o.starts = g.starts;
                     o.whole = g.whole;
+                    if (SINKS) o.skip = g.skip;
                     mbar_arrive(&seg_full[k % AP_SEG_SLOTS]);
                     if (more && pp.deal && g.starts && g.je < g.j1) {
                         // the rest of the item goes to the next CTAs, `per` blocks each (to fewer
@@ -591,8 +621,8 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                 }
                 if (!more) break;
                 for (uint32_t j = g.jb; j < g.je && going; ++j) {
-                    const uint32_t key = j * AP_KEYS + lane * R;
-                    const bool live = lane < n_boxes && key < s.kl && key + R > s.lo;
+                    const uint32_t key0 = (SINKS && j >= g.first ? j + g.skip : j) * AP_KEYS, key = key0 + lane * R;
+                    const bool live = lane < n_boxes && key < s.kl && (key + R > s.lo || (SINKS && key < p.sinks));
                     int32_t page = 0, row = 0;
                     if (live) {
                         const uint32_t at = key / p.page_size;
@@ -604,7 +634,8 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                         }
                     }
                     const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, live)) * R * 128 * L::HALVES;
-                    const bool at_edge = j * AP_KEYS < s.lo || (j + 1) * AP_KEYS > s.kl;
+                    const bool at_edge = (key0 < s.lo && !(SINKS && (key0 + AP_KEYS <= p.sinks || s.lo <= p.sinks))) ||
+                                         key0 + AP_KEYS > s.kl;
 #pragma unroll
                     for (uint32_t kind = 0; kind < 2; ++kind, ++it) {
                         const uint32_t st = it % L::STAGES;
@@ -630,8 +661,8 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                             }
                             ++edges;
                             for (uint32_t r = lane; r < AP_KEYS; r += 32) {
-                                const uint32_t k = j * AP_KEYS + r;
-                                if (k >= s.lo && k < s.kl) continue;
+                                const uint32_t k = key0 + r;
+                                if ((k >= s.lo || (SINKS && k < p.sinks)) && k < s.kl) continue;
 #pragma unroll
                                 for (uint32_t x = 0; x < L::HALVES * 8; ++x)
                                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(
@@ -660,7 +691,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                 bool ok = true;
 #pragma unroll
                 for (uint32_t t = 0; t < 2; ++t) {
-                    if (g->te[t] == g->tb[t] || !ok) continue;
+                    if ((g->te[t] == g->tb[t] && !(SINKS && g->fe[t])) || !ok) continue;
                     ok = ap_wait(&q_empty[t], (n[t] & 1u) ^ 1u, abort_flag, p.status);
                     if (!ok) break;
                     ++n[t];
@@ -706,6 +737,16 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
             const APShared *g;
             for (uint32_t k = 0; ok && (g = segment(k)) != nullptr; ++k) {
                 const uint32_t jb = g->jb, je = g->je, tb[2] = {g->tb[0], g->tb[1]}, te[2] = {g->te[0], g->te[1]};
+                // a tile's first and last block, and with SINKS the end of its first keys' blocks
+                uint32_t fe[2] = {0, 0}, from[2] = {tb[0], tb[1]}, last[2] = {te[0], te[1]};
+                if constexpr (SINKS) {
+#pragma unroll
+                    for (uint32_t t = 0; t < 2; ++t) {
+                        fe[t] = g->fe[t];
+                        if (fe[t]) from[t] = jb;
+                        if (fe[t] && te[t] == tb[t]) last[t] = fe[t];
+                    }
+                }
                 release(k);
                 for (uint32_t j = jb; j < je && ok; ++j, it += 2) {
                     const uint32_t st = it % L::STAGES;
@@ -713,9 +754,9 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     ok = ap_wait(&kv_full[st], (it / L::STAGES) & 1u, abort_flag, p.status);
 #pragma unroll
                     for (uint32_t t = 0; t < 2; ++t) {
-                        if (!ok || j < tb[t] || j >= te[t]) continue;
+                        if (!ok || ((j < tb[t] || j >= te[t]) && !(SINKS && j < fe[t]))) continue;
                         if (scores) {
-                            if (j == tb[t]) ok = ap_wait(&q_full[t], q[t]++ & 1u, abort_flag, p.status);
+                            if (j == from[t]) ok = ap_wait(&q_full[t], q[t]++ & 1u, abort_flag, p.status);
                             if (ok && s_used) ok = ap_wait(s_free, (s_used - 1) & 1u, abort_flag, p.status);
                             if (!ok) break;
                             tc_fence_after();
@@ -728,7 +769,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                                                smem_desc_sw128(kv + off), id_s, i != 0);
                                 }
                                 tc_commit(&s_full[t]);
-                                if (j + 1 == te[t]) tc_commit(&q_empty[t]);
+                                if (j + 1 == last[t]) tc_commit(&q_empty[t]);
                             }
                             ++s_used;
                         } else {
@@ -739,7 +780,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
 #pragma unroll
                                 for (uint32_t i = 0; i < AP_KEYS / 16; ++i)
                                     mma_f16_ts(tmem + L::o_col(t), tmem + L::p_col(t) + i * 8,
-                                               ap_desc_v(kv + i * 2048, L::HALF), id_o, i != 0 || j != tb[t]);
+                                               ap_desc_v(kv + i * 2048, L::HALF), id_o, i != 0 || j != from[t]);
                                 tc_commit(&o_done[t]);
                             }
                         }
@@ -770,16 +811,19 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
         for (uint32_t k = 0; ok && (g = segment(k)) != nullptr; ++k) {
             // of the segment, only what the loop and the result need is kept: registers
             const bool valid = r < g->rows[t], whole = g->whole;
-            const uint32_t tb = g->tb[t], blocks = g->te[t] - tb;
+            // SINKS: the first `few` blocks are those from jb on, the others from tb on
+            const uint32_t few = SINKS && g->fe[t] ? g->fe[t] - g->jb : 0, jb = g->jb;
+            const uint32_t tb = g->tb[t] + (SINKS ? g->skip - few : 0), blocks = g->te[t] - g->tb[t] + few;
             const uint32_t whole_lo = g->whole_lo[t], whole_hi = g->whole_hi[t];
             const uint32_t slot = (blockIdx.x * 2 + (g->starts ? 1 : 0)) * AP_PAIR + t * AP_TILE + r;
             const uint32_t row = g->row0 + t * AP_TILE + r, tok = row / p.group;
-            uint32_t key_lo = 0, key_hi = g->kl;
+            uint32_t key_lo = 0, key_hi = g->kl, first_hi = 0;
             if (valid) {
                 const int64_t pos = static_cast<int64_t>(g->kl) - g->ql + tok;
                 const int64_t hi = p.causal ? pos + 1 : g->kl, lo = p.window ? pos - p.window + 1 : 0;
                 key_hi = hi > 0 ? static_cast<uint32_t>(hi) : 0;
                 key_lo = lo > 0 ? static_cast<uint32_t>(lo) : 0;
+                if (SINKS) first_hi = p.sinks < key_hi ? p.sinks : key_hi;
             }
             const uint64_t token = static_cast<uint64_t>(g->q0) + tok;
             const uint32_t qhead = g->head * p.group + (row - tok * p.group);
@@ -800,17 +844,18 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                 for (int c = 0; c < 4; ++c) pin(x[c]);
                 tc_fence_before();
                 mbar_arrive(s_free);
-                const uint32_t key0 = (tb + n) * AP_KEYS;
-                if (key0 + AP_KEYS > whole_hi || key0 < whole_lo) {
+                const uint32_t key0 = ((SINKS && n < few ? jb : tb) + n) * AP_KEYS;
+                if (key0 + AP_KEYS > whole_hi || (key0 < whole_lo && !(SINKS && key0 + AP_KEYS <= p.sinks))) {
                     // the row sees keys [gone, seen) of the block; most 32s are all or nothing to a warp
                     const uint32_t seen = key_hi > key0 ? key_hi - key0 : 0;
                     const uint32_t gone = key_lo > key0 ? key_lo - key0 : 0;
+                    const uint32_t kept = SINKS && first_hi > key0 ? first_hi - key0 : 0; // and [0, kept)
 #pragma unroll
                     for (uint32_t c = 0; c < 4; ++c) {
                         if (!__any_sync(0xFFFFFFFFu, seen < c * 32 + 32 || gone > c * 32)) continue;
 #pragma unroll
                         for (uint32_t i = 0; i < 32; ++i)
-                            if (c * 32 + i - gone >= seen - gone) x[c][i] = 0xFF800000u; // -inf
+                            if (c * 32 + i - gone >= seen - gone && !(SINKS && c * 32 + i < kept)) x[c][i] = 0xFF800000u; // -inf
                     }
                 }
                 float top[4];
@@ -929,7 +974,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
     if (warp == 11) tmem_dealloc(tmem, 512);
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ APParams pp) {
@@ -937,7 +982,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     // what follows on the stream may come to the SMs that have nothing to do here
     after_stream();
     let_next();
-    ap_chunks<DP, BF16>(map_k, map_v, pp, ap_smem_raw);
+    ap_chunks<DP, BF16, SINKS>(map_k, map_v, pp, ap_smem_raw);
 }
 
 template <int DP> constexpr uint32_t AP_BESIDE_SMEM = ARows<DP>::SMEM > APrompt<DP>::SMEM ? ARows<DP>::SMEM : APrompt<DP>::SMEM;
@@ -949,7 +994,7 @@ template <int DP> constexpr uint32_t AP_BESIDE_SMEM = ARows<DP>::SMEM > APrompt<
 // third one's registers.  Measured, heads of 128, 8 key heads: a chunk of up to 512 behind 4000
 // keys beside 31 decoding sequences 103 us, against 119 with one kernel after the other; of 510
 // beside 7 with a window of 1000 keys (16 key heads) 44 against 65.
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     attn_beside_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ APParams pp) {
@@ -958,7 +1003,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     after_stream();
     let_next();
     if (blockIdx.x < pp.ctas) {
-        ap_chunks<DP, BF16>(map_k, map_v, pp, ap_smem_raw);
+        ap_chunks<DP, BF16, SINKS>(map_k, map_v, pp, ap_smem_raw);
         return;
     }
     if (threadIdx.x >= AR_THREADS) {
@@ -968,11 +1013,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
     const uint32_t cta = blockIdx.x - pp.ctas, ctas = gridDim.x - pp.ctas;
     if (pp.rows_form == AR_CLUSTER)
-        ar_cluster<DP, BF16>(pp.a, ap_smem_raw, cta, pp.rows_tiles);
+        ar_cluster<DP, BF16, SINKS>(pp.a, ap_smem_raw, cta, pp.rows_tiles);
     else if (pp.rows_form == AR_RANGES)
-        ar_ranges<DP, BF16>(pp.a, ap_smem_raw, cta, ctas);
+        ar_ranges<DP, BF16, SINKS>(pp.a, ap_smem_raw, cta, ctas);
     else if (threadIdx.x < pp.rows_warps * 32)
-        ar_unit<DP, BF16>(pp.a, ap_smem_raw, cta, ctas, pp.rows_tiles);
+        ar_unit<DP, BF16, SINKS>(pp.a, ap_smem_raw, cta, ctas, pp.rows_tiles);
 }
 
 // Adds up the fragments of the items that were cut: blockIdx.x the CTA in which

@@ -23,6 +23,9 @@
 // on timing.  A warp has at most two fragments: of the unit that began before
 // its range, and of the unit that goes on after it.
 //
+// SINKS: the first p.sinks keys stay visible behind the window.  A unit's steps are then those of
+// these keys and, after a gap that is neither read nor counted, those of the window.
+//
 // Measured, 8 key heads of 128: 64 sequences of up to 8192 keys (1.09 GB) 170 to 181 us by
 // machine, 94 to 99% of the rate of a copy; one sequence of 131071 keys and 4 key heads
 // (268 MB) 55 us, of which the join of 1184 fragments takes 8.
@@ -52,16 +55,30 @@ template <int DP> struct ARows {
 // Row tiles and steps a unit of sequence s in the rows kernel (no tiles: not its work).
 struct ARShape {
     uint32_t tiles, step0, steps;
+    uint32_t first; // steps of the first keys, before step0
 };
-template <int DP> __device__ __forceinline__ ARShape ar_shape(const AttnParams &p, const AttnSeq &s) {
+template <int DP, bool SINKS> __device__ __forceinline__ ARShape ar_shape(const AttnParams &p, const AttnSeq &s) {
     constexpr uint32_t KEYS = ar_keys(DP);
     ARShape r;
     const uint64_t rows = static_cast<uint64_t>(s.ql) * p.group;
     r.tiles = rows <= p.row_limit ? static_cast<uint32_t>((rows + AR_ROWS - 1) / AR_ROWS) : 0;
     r.step0 = s.lo / KEYS;
+    r.first = 0;
+    if constexpr (SINKS) {
+        const uint32_t first = (p.sinks + KEYS - 1) / KEYS;
+        if (first < r.step0)
+            r.first = first;
+        else
+            r.step0 = 0; // no gap
+    }
     const uint32_t last = (s.kl + KEYS - 1) / KEYS;
-    r.steps = last > r.step0 ? last - r.step0 : 1; // a unit without keys still writes its zeros
+    r.steps = last > r.step0 ? r.first + last - r.step0 : 1; // a unit without keys still writes its zeros
     return r;
+}
+// The first key of a unit's step.
+template <int DP, bool SINKS> __device__ __forceinline__ uint32_t ar_step_key(const ARShape &sh, uint32_t step) {
+    if (SINKS && step < sh.first) return step * ar_keys(DP);
+    return (sh.step0 + step - (SINKS ? sh.first : 0)) * ar_keys(DP);
 }
 // The sequence's place in the laid-out work; its units are `steps` + AR_UNIT_COST long, the cost first.
 __device__ __forceinline__ uint64_t ar_length(const AttnParams &p, const ARShape &sh) {
@@ -107,17 +124,17 @@ struct ARCursor {
     ARShape sh;
 };
 
-template <int DP> __device__ __forceinline__ void ar_enter(const AttnParams &p, ARCursor &c) {
+template <int DP, bool SINKS> __device__ __forceinline__ void ar_enter(const AttnParams &p, ARCursor &c) {
     // the next sequence that has tiles; the caller stops at the range's end before there is none
     while (c.b < p.seqs) {
         c.s = attn_seq(p, c.b, false);
-        c.sh = ar_shape<DP>(p, c.s);
+        c.sh = ar_shape<DP, SINKS>(p, c.s);
         if (c.sh.tiles) return;
         ++c.b;
     }
 }
 
-template <int DP> __device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
+template <int DP, bool SINKS> __device__ __forceinline__ void ar_advance(const AttnParams &p, ARCursor &c) {
     ++c.at;
     if (++c.step < c.sh.steps) return;
     c.step = 0;
@@ -125,7 +142,7 @@ template <int DP> __device__ __forceinline__ void ar_advance(const AttnParams &p
     if (++c.tile < c.sh.tiles * p.kv_heads) return;
     c.tile = 0;
     ++c.b;
-    ar_enter<DP>(p, c);
+    ar_enter<DP, SINKS>(p, c);
 }
 
 // Queues the copies of a step's keys and values; what is not to be read becomes zeros.
@@ -174,11 +191,12 @@ __device__ __forceinline__ uint64_t ar_block_scan(uint64_t v, uint64_t *s_part, 
 
 // A warp's 16 rows of a unit: Q fragments, O, and of rows lane / 4 and lane / 4 + 8 the
 // reference exponent (in log2), the lane's part of the sum, and the keys that the row sees.
-template <int DP, bool BF16> struct ARState {
+template <int DP, bool BF16, bool SINKS> struct ARState {
     uint32_t qf[DP / 16][4];
     float o[DP / 8][4];
     float m[2], l[2];
     uint32_t key_lo[2], key_hi[2];
+    uint32_t first_hi[2]; // SINKS: and the first keys that it sees
 
     __device__ __forceinline__ void begin(const AttnParams &p, const AttnSeq &s, uint32_t head, uint32_t rt,
                                           uint32_t lane) {
@@ -189,7 +207,7 @@ template <int DP, bool BF16> struct ARState {
             const uint32_t t = row / p.group, g = row - t * p.group;
             m[r] = -INFINITY;
             l[r] = 0.0f;
-            key_lo[r] = key_hi[r] = 0;
+            key_lo[r] = key_hi[r] = first_hi[r] = 0;
             rows[r] = nullptr;
             if (t < s.ql) {
                 const int64_t pos = static_cast<int64_t>(s.kl) - s.ql + t;
@@ -197,6 +215,7 @@ template <int DP, bool BF16> struct ARState {
                 const int64_t lo = p.window ? pos - p.window + 1 : 0;
                 key_hi[r] = hi > 0 ? static_cast<uint32_t>(hi) : 0;
                 key_lo[r] = lo > 0 ? static_cast<uint32_t>(lo) : 0;
+                first_hi[r] = p.sinks < key_hi[r] ? p.sinks : key_hi[r];
                 rows[r] = static_cast<const uint16_t *>(p.q) + (static_cast<uint64_t>(s.q0) + t) * p.qt +
                           static_cast<int64_t>(head * p.group + g) * p.qh;
             }
@@ -240,7 +259,8 @@ template <int DP, bool BF16> struct ARState {
             for (int x = 0; x < 4; ++x) {
                 const int r = x >> 1;
                 const uint32_t key = key0 + n * 8 + (x & 1);
-                sc[n][x] = key >= key_lo[r] && key < key_hi[r] ? sc[n][x] * p.scale_log2 : -INFINITY;
+                const bool seen = (key >= key_lo[r] && key < key_hi[r]) || (SINKS && key < first_hi[r]);
+                sc[n][x] = seen ? sc[n][x] * p.scale_log2 : -INFINITY;
                 top[r] = fmaxf(top[r], sc[n][x]);
             }
 #pragma unroll
@@ -299,10 +319,11 @@ template <int DP, bool BF16> struct ARState {
 
 // A cache row's place: the offset of the lane's key (lane modulo the keys of a step) from
 // `key_first` on, or -1: not to be read.
-template <int DP> __device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq &s, uint32_t b, uint32_t head,
+template <int DP, bool SINKS>
+__device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq &s, uint32_t b, uint32_t head,
                                              uint32_t key_first, uint32_t lane) {
     const uint32_t key = key_first + (lane & (ar_keys(DP) - 1));
-    if (key < s.lo || key >= s.kl) return -1;
+    if ((key < s.lo && !(SINKS && key < p.sinks)) || key >= s.kl) return -1;
     const uint32_t page = key / p.page_size;
     const int32_t id = __ldg(p.table + b * p.tb + page);
     if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
@@ -313,9 +334,9 @@ template <int DP> __device__ __forceinline__ int64_t ar_key_at(const AttnParams 
 }
 
 // The result of row r of the lane's two, row `row` of the sequence and key head.
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __device__ __forceinline__ void ar_store_row(const AttnParams &p, const AttnSeq &s, uint32_t head, uint32_t row,
-                                             const ARState<DP, BF16> &u, int r, float sum, uint32_t lane) {
+                                             const ARState<DP, BF16, SINKS> &u, int r, float sum, uint32_t lane) {
     const uint32_t t = row / p.group, g = row - t * p.group;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint64_t h = head * p.group + g, token = static_cast<uint64_t>(s.q0) + t;
@@ -330,7 +351,7 @@ __device__ __forceinline__ void ar_store_row(const AttnParams &p, const AttnSeq 
         p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : u.m[r] * 0.6931471805599453f + logf(sum);
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t ctas) {
     using L = ARows<DP>;
     uint64_t *s_part = reinterpret_cast<uint64_t *>(smem + L::RINGS), *s_first = s_part + AR_WARPS;
@@ -345,7 +366,7 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
         mine = 0;
         if (b < p.seqs) {
             const AttnSeq s = attn_seq(p, b, cta == 0);
-            const ARShape sh = ar_shape<DP>(p, s);
+            const ARShape sh = ar_shape<DP, SINKS>(p, s);
             mine = ar_length(p, sh);
         }
         uint64_t sum;
@@ -363,7 +384,7 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
             mine = 0;
             if (b < p.seqs) {
                 const AttnSeq s = attn_seq(p, b, false);
-                const ARShape sh = ar_shape<DP>(p, s);
+                const ARShape sh = ar_shape<DP, SINKS>(p, s);
                 mine = ar_length(p, sh);
             }
             uint64_t sum;
@@ -394,7 +415,7 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
     ARCursor c;
     c.b = s_seq[warp];
     c.s = attn_seq(p, c.b, false);
-    c.sh = ar_shape<DP>(p, c.s);
+    c.sh = ar_shape<DP, SINKS>(p, c.s);
     const uint64_t inside = begin - s_first[warp];
     const uint32_t unit = c.sh.steps + AR_UNIT_COST;
     c.tile = static_cast<uint32_t>(quotient(inside, unit));
@@ -405,18 +426,20 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
     // ---- the stream of keys -------------------------------------------------------
     const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE);
     ARCursor f = c;
-    ARState<DP, BF16> u;
+    ARState<DP, BF16, SINKS> u;
     uint32_t first_step = c.step;
     bool fresh = false;
     uint32_t fetched = 0;
-    auto place = [&] { return ar_key_at<DP>(p, f.s, f.b, f.tile / f.sh.tiles, (f.sh.step0 + f.step) * L::KEYS, lane); };
+    auto place = [&] {
+        return ar_key_at<DP, SINKS>(p, f.s, f.b, f.tile / f.sh.tiles, ar_step_key<DP, SINKS>(f.sh, f.step), lane);
+    };
     int64_t next = c.at < end ? place() : -1; // one step ahead of the copies: hides the table's latency
     if (c.at < end) u.begin(p, c.s, c.tile / c.sh.tiles, c.tile % c.sh.tiles, lane); // its loads before the keys'
     auto fetch = [&] {
         if (f.at < end) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
             ++fetched;
-            ar_advance<DP>(p, f);
+            ar_advance<DP, SINKS>(p, f);
             if (f.at < end) next = place();
         }
         cp_async_commit();
@@ -433,7 +456,7 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
         }
         cp_async_wait<L::STAGES - 2>();
         __syncwarp();
-        u.step(p, ring + (i % L::STAGES) * L::STAGE, (c.sh.step0 + c.step) * L::KEYS, lane);
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, ar_step_key<DP, SINKS>(c.sh, c.step), lane);
         __syncwarp(); // every lane has read the stage that the next copies fill
         fetch();
 
@@ -453,7 +476,7 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
                 const uint32_t in = lane / 4 + r * 8, row = rt * AR_ROWS + in;
                 if (row >= c.s.ql * p.group) continue;
                 if (whole) {
-                    ar_store_row<DP, BF16>(p, c.s, head, row, u, r, sum, lane);
+                    ar_store_row<DP, BF16, SINKS>(p, c.s, head, row, u, r, sum, lane);
                 } else {
                     float *dst = p.part + (slot * AR_ROWS + in) * DP;
 #pragma unroll
@@ -464,18 +487,18 @@ __device__ __forceinline__ void ar_ranges(const AttnParams &p, uint8_t *smem, ui
                 }
             }
         }
-        ar_advance<DP>(p, c);
+        ar_advance<DP, SINKS>(p, c);
     }
     if (lane == 0) p.tail_rows[worker] = tail;
     cp_async_wait<0>();
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnParams p) {
     extern __shared__ __align__(1024) uint8_t ar_smem[];
     after_stream();
     let_next();
-    ar_ranges<DP, BF16>(p, ar_smem, blockIdx.x, gridDim.x);
+    ar_ranges<DP, BF16, SINKS>(p, ar_smem, blockIdx.x, gridDim.x);
 }
 
 // ---- few units of short sequences: a cluster each ----------------------------------
@@ -485,7 +508,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnPara
 // warps are joined in its shared memory and the CTAs through each other's: one
 // launch, no fragments in global memory.  blockIdx.x / cluster size: (sequence,
 // key head, row tile), `unit_tiles` row tiles a sequence and head.
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __device__ __forceinline__ void ar_cluster(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t unit_tiles) {
     using L = ARows<DP>;
     float(*s_m)[AR_ROWS] = reinterpret_cast<float(*)[AR_ROWS]>(smem + L::RINGS), (*s_l)[AR_ROWS] = s_m + AR_WARPS; // of the warps
@@ -496,31 +519,31 @@ __device__ __forceinline__ void ar_cluster(const AttnParams &p, uint8_t *smem, u
     const uint32_t unit = cta / ranks, rt = unit % unit_tiles;
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
     const AttnSeq s = attn_seq(p, b, threadIdx.x == 0 && rank == 0 && rt == 0 && head == 0);
-    const ARShape sh = ar_shape<DP>(p, s);
+    const ARShape sh = ar_shape<DP, SINKS>(p, s);
     if (rt >= sh.tiles) return; // the whole cluster
 
     const uint32_t part = rank * AR_WARPS + warp, parts = ranks * AR_WARPS;
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * part / parts);
     const uint32_t count = static_cast<uint32_t>(static_cast<uint64_t>(sh.steps) * (part + 1) / parts) - begin;
-    const uint32_t key_first = (sh.step0 + begin) * L::KEYS;
+    auto key_first = [&](uint32_t i) { return ar_step_key<DP, SINKS>(sh, begin + i); };
     const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE);
     uint32_t fetched = 0;
-    int64_t next = count ? ar_key_at<DP>(p, s, b, head, key_first, lane) : -1;
+    int64_t next = count ? ar_key_at<DP, SINKS>(p, s, b, head, key_first(0), lane) : -1;
     auto fetch = [&] {
         if (fetched < count) {
             ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
-            if (++fetched < count) next = ar_key_at<DP>(p, s, b, head, key_first + fetched * L::KEYS, lane);
+            if (++fetched < count) next = ar_key_at<DP, SINKS>(p, s, b, head, key_first(fetched), lane);
         }
         cp_async_commit();
     };
 #pragma unroll
     for (uint32_t i = 0; i + 1 < L::STAGES; ++i) fetch();
-    ARState<DP, BF16> u;
+    ARState<DP, BF16, SINKS> u;
     u.begin(p, s, head, rt, lane);
     for (uint32_t i = 0; i < count; ++i) {
         cp_async_wait<L::STAGES - 2>();
         __syncwarp();
-        u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * L::KEYS, lane);
+        u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first(i), lane);
         __syncwarp();
         fetch();
     }
@@ -602,12 +625,12 @@ __device__ __forceinline__ void ar_cluster(const AttnParams &p, uint8_t *smem, u
     cluster_sync(); // nobody leaves while its shared memory is read
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnParams p, uint32_t unit_tiles) {
     extern __shared__ __align__(1024) uint8_t ar_smem[];
     after_stream();
     let_next();
-    ar_cluster<DP, BF16>(p, ar_smem, blockIdx.x, unit_tiles);
+    ar_cluster<DP, BF16, SINKS>(p, ar_smem, blockIdx.x, unit_tiles);
 }
 
 // ---- many units of very short sequences: a warp each ------------------------------
@@ -615,7 +638,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_cluster_kernel(const AttnP
 // Where a unit has few steps, reading is soon done and what is around it counts: the
 // warps of a CTA take a unit each, from its first key to its last, and write its rows.
 // No sums over the sequences to find the work, no fragments, one launch.
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __device__ __forceinline__ void ar_unit(const AttnParams &p, uint8_t *smem, uint32_t cta, uint32_t ctas, uint32_t unit_tiles) {
     using L = ARows<DP>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -623,17 +646,18 @@ __device__ __forceinline__ void ar_unit(const AttnParams &p, uint8_t *smem, uint
     const uint32_t head = unit / unit_tiles % p.kv_heads, b = unit / unit_tiles / p.kv_heads;
     if (b < p.seqs) {
         const AttnSeq s = attn_seq(p, b, lane == 0 && rt == 0 && head == 0);
-        const ARShape sh = ar_shape<DP>(p, s);
+        const ARShape sh = ar_shape<DP, SINKS>(p, s);
         if (rt < sh.tiles) {
-            const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE), key_first = sh.step0 * L::KEYS;
-            ARState<DP, BF16> u;
+            const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE);
+            auto key_first = [&](uint32_t i) { return ar_step_key<DP, SINKS>(sh, i); };
+            ARState<DP, BF16, SINKS> u;
             uint32_t fetched = 0;
-            int64_t next = ar_key_at<DP>(p, s, b, head, key_first, lane);
+            int64_t next = ar_key_at<DP, SINKS>(p, s, b, head, key_first(0), lane);
             u.begin(p, s, head, rt, lane); // its loads before the keys'
             auto fetch = [&] {
                 if (fetched < sh.steps) {
                     ar_fetch<DP>(p, ring + (fetched % L::STAGES) * L::STAGE, next, lane);
-                    if (++fetched < sh.steps) next = ar_key_at<DP>(p, s, b, head, key_first + fetched * L::KEYS, lane);
+                    if (++fetched < sh.steps) next = ar_key_at<DP, SINKS>(p, s, b, head, key_first(fetched), lane);
                 }
                 cp_async_commit();
             };
@@ -642,7 +666,7 @@ __device__ __forceinline__ void ar_unit(const AttnParams &p, uint8_t *smem, uint
             for (uint32_t i = 0; i < sh.steps; ++i) {
                 cp_async_wait<L::STAGES - 2>();
                 __syncwarp();
-                u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first + i * L::KEYS, lane);
+                u.step(p, ring + (i % L::STAGES) * L::STAGE, key_first(i), lane);
                 __syncwarp();
                 fetch();
             }
@@ -651,18 +675,18 @@ __device__ __forceinline__ void ar_unit(const AttnParams &p, uint8_t *smem, uint
             for (int r = 0; r < 2; ++r) {
                 const float sum = u.sum(r);
                 const uint32_t row = rt * AR_ROWS + lane / 4 + r * 8;
-                if (row < s.ql * p.group) ar_store_row<DP, BF16>(p, s, head, row, u, r, sum, lane);
+                if (row < s.ql * p.group) ar_store_row<DP, BF16, SINKS>(p, s, head, row, u, r, sum, lane);
             }
         }
     }
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SINKS>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnParams p, uint32_t unit_tiles) {
     extern __shared__ __align__(1024) uint8_t ar_smem[];
     after_stream();
     let_next();
-    ar_unit<DP, BF16>(p, ar_smem, blockIdx.x, gridDim.x, unit_tiles);
+    ar_unit<DP, BF16, SINKS>(p, ar_smem, blockIdx.x, gridDim.x, unit_tiles);
 }
 
 // Joins the fragments of the units that were cut.  A CTA of W warps takes a row (one of C
@@ -671,7 +695,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_unit_kernel(const AttnPara
 // warp blockIdx.x's range.  Warp i takes fragments
 // i, i + W, ..., a lane DP / 32 / C values of the head, with the loads of F fragments under
 // way together.
-template <int DP, bool BF16, int W, int F, int C>
+template <int DP, bool BF16, bool SINKS, int W, int F, int C>
 __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p, bool by_worker) {
     constexpr int V = DP / 32 / C;
     __shared__ float s_o[W][DP / C];
@@ -687,7 +711,7 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
         const int4 tail = p.tail_rows[blockIdx.x];
         if (tail.x < 0) return;
         s = attn_seq(p, static_cast<uint32_t>(tail.x), false);
-        const ARShape sh = ar_shape<DP>(p, s);
+        const ARShape sh = ar_shape<DP, SINKS>(p, s);
         const uint32_t tile = static_cast<uint32_t>(tail.y);
         head = tile / sh.tiles;
         row = (tile - head * sh.tiles) * AR_ROWS + y;
@@ -702,7 +726,7 @@ __global__ void __launch_bounds__(W * 32) attn_combine_kernel(const AttnParams p
         uint64_t total = 0, before = 0;
         if (W == 32) total = p.prefix[p.seqs], before = p.prefix[b];
         s = attn_seq(p, b, false);
-        const ARShape sh = ar_shape<DP>(p, s);
+        const ARShape sh = ar_shape<DP, SINKS>(p, s);
         if (sh.tiles == 0 || row >= s.ql * p.group) return;
         if (W != 32) total = p.prefix[p.seqs], before = p.prefix[b];
         const uint64_t even = quotient(total + p.workers - 1, p.workers);

@@ -30,8 +30,8 @@ struct Entries {
     decltype(&fmcuda_norm_add_norm) norm_pair;
     decltype(&fmcuda_rope_append) rope;
     decltype(&fmcuda_rope_append_axes) rope_axes;
-    decltype(&fmcuda_paged_attention_workspace_bytes) attention_bytes;
-    decltype(&fmcuda_paged_attention) attention;
+    decltype(&fmcuda_paged_attention_sinks_workspace_bytes) attention_bytes;
+    decltype(&fmcuda_paged_attention_sinks) attention;
     decltype(&fmcuda_token_logprobs) logprobs;
 } entries{};
 PyObject *error_class = nullptr; // FmError(code, message)
@@ -294,7 +294,7 @@ Tensor rope_append(const Tensor &q, const MaybeTensor &k, const MaybeTensor &v, 
 std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache,
                                                 const Tensor &page_table, const Tensor &q_start, const Tensor &kv_len,
                                                 int64_t max_q_len, int64_t max_kv_len, std::optional<double> scale,
-                                                bool causal, int64_t window, bool return_lse,
+                                                bool causal, int64_t window, int64_t sinks, bool return_lse,
                                                 const MaybeTensor &workspace) {
     need(q.dim() == 3 && k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
              v_cache.strides() == k_cache.strides() && k_cache.size(3) == q.size(2) && q.size(2) > 0,
@@ -309,8 +309,8 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     need(page_table.scalar_type() == at::kInt && q_start.scalar_type() == at::kInt &&
              kv_len.scalar_type() == at::kInt && q_start.is_contiguous() && kv_len.is_contiguous(),
          "page_table, q_start and kv_len are int32", FM_STATUS_INVALID_ARGUMENT);
-    need(max_q_len >= 0 && max_kv_len >= 0 && window >= 0, "lengths must not be negative", FM_STATUS_INVALID_ARGUMENT);
-    need(max_kv_len <= INT32_MAX && window <= UINT32_MAX && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
+    need(max_q_len >= 0 && max_kv_len >= 0 && window >= 0 && sinks >= 0, "lengths must not be negative", FM_STATUS_INVALID_ARGUMENT);
+    need(max_kv_len <= INT32_MAX && window <= UINT32_MAX && sinks <= UINT32_MAX && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
              seqs < INT32_MAX && k_cache.size(0) <= INT32_MAX && k_cache.size(1) <= INT32_MAX &&
              k_cache.size(2) <= INT32_MAX && q.size(2) <= INT32_MAX,
          "attention lengths out of range");
@@ -352,17 +352,18 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     a.causal = causal;
     a.window = static_cast<uint32_t>(window);
     a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
+    const uint32_t kept = static_cast<uint32_t>(sinks);
     Tensor own;
     void *at = at_of(workspace);
     uint64_t bytes = workspace ? workspace->nbytes() : 0;
     if (!workspace) {
-        check(entries.attention_bytes(&a, &bytes));
+        check(entries.attention_bytes(&a, kept, &bytes));
         if (bytes) {
             own = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
             at = own.data_ptr();
         }
     }
-    check(entries.attention(&a, at, bytes, here.stream()));
+    check(entries.attention(&a, kept, at, bytes, here.stream()));
     return {out, return_lse ? MaybeTensor(lse) : std::nullopt};
 }
 
@@ -408,8 +409,8 @@ void bind(py::object error, const std::map<std::string, uint64_t> &at) {
     take(entries.norm_pair, "fmcuda_norm_add_norm");
     take(entries.rope, "fmcuda_rope_append");
     take(entries.rope_axes, "fmcuda_rope_append_axes");
-    take(entries.attention_bytes, "fmcuda_paged_attention_workspace_bytes");
-    take(entries.attention, "fmcuda_paged_attention");
+    take(entries.attention_bytes, "fmcuda_paged_attention_sinks_workspace_bytes");
+    take(entries.attention, "fmcuda_paged_attention_sinks");
     take(entries.logprobs, "fmcuda_token_logprobs");
 }
 

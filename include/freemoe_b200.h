@@ -773,6 +773,16 @@ int fmcuda_paged_attention_workspace_bytes(const fmcuda_paged_attention_args *ar
 int fmcuda_paged_attention(const fmcuda_paged_attention_args *args, void *workspace, uint64_t workspace_bytes,
                            void *stream);
 
+/* The same with the first keys of a sequence visible behind the window: a row at position p
+ * sees the keys i <= p with i > p - window or i < sinks.  So a stream of any length needs the
+ * pages of its first keys and of its window alone: those between (before the window of the
+ * call's first row) may be freed, their table entries are not followed.  sinks needs a window;
+ * with 0 it is fmcuda_paged_attention. */
+int fmcuda_paged_attention_sinks_workspace_bytes(const fmcuda_paged_attention_args *args, uint32_t sinks,
+                                                 uint64_t *bytes);
+int fmcuda_paged_attention_sinks(const fmcuda_paged_attention_args *args, uint32_t sinks, void *workspace,
+                                 uint64_t workspace_bytes, void *stream);
+
 /* ==================== probabilities of tokens ==================== *
  * What follows the output head (fmcuda_gemv over its rows): the sampler's softmax
  * (src/engine.cpp) without the sampling.  With z = scale * logits[t] and

@@ -11,7 +11,7 @@ import torch
 from conftest import ROOT
 from freemoe_b200 import attention, hotpath, load
 from freemoe_b200._lib import FmError, NormAddNormArgs, TokenLogprobsArgs
-from test_attention_cpu import P, rope_args
+from test_attention_cpu import P, attention_args, rope_args
 
 OK, SHAPE, ARG = 0, 8, 26
 
@@ -101,6 +101,39 @@ def test_axes_of_the_c_entry():
     assert lib.fmcuda_rope_axes(sections, 2, 0, 10, out) == SHAPE  # not the pairs' number
     assert lib.fmcuda_rope_axes((C.c_uint32 * 2)(0xFFFFFFFF, 5), 2, 0, 8, out) == SHAPE
     assert lib.fmcuda_rope_axes(None, 2, 0, 8, out) == ARG and lib.fmcuda_rope_axes(sections, 2, 0, 8, None) == ARG
+
+
+# -------------------------------------------------------------------- first keys behind a window
+
+
+@pytest.mark.parametrize("code,sinks,change", [
+    (ARG, 4, {}), (ARG, 4, {"causal": 0}), (ARG, 4, {"window": 9, "causal": 0}), (SHAPE, 4, {"window": 9, "head_dim": 100}),
+    (SHAPE, 4, {"window": 9, "max_kv_len": 1025}), (ARG, 4, {"window": 9, "kv_len": None}), (ARG, 4, {"window": 9, "lse": P + 2}),
+    (ARG, 1 << 20, {"window": 9, "max_kv_len": 1 << 20, "page_table_stride": 1 << 16}),  # no workspace, and fragments to keep
+    (OK, 4, {"window": 9, "seqs": 0}), (OK, 0xFFFFFFFF, {"window": 9, "tokens": 0, "max_q_len": 0}),
+])
+def test_attention_with_first_keys_refuses(code, sinks, change):
+    assert load().fmcuda_paged_attention_sinks(C.byref(attention_args(**change)), sinks, None, 0, None) == code
+
+
+def test_workspace_with_first_keys():
+    lib = load()
+
+    def bytes_of(sinks, **change):
+        v = C.c_uint64()
+        assert lib.fmcuda_paged_attention_sinks_workspace_bytes(C.byref(attention_args(**change)), sinks, C.byref(v)) == OK
+        return v.value
+
+    plain = C.c_uint64()
+    assert lib.fmcuda_paged_attention_workspace_bytes(C.byref(attention_args(window=50)), C.byref(plain)) == OK
+    assert bytes_of(0, window=50) == plain.value
+    long = dict(tokens=1, seqs=1, max_q_len=1, max_kv_len=10000000, page_table_stride=1 << 20)
+    assert bytes_of(4, window=100, **long) == 0  # few keys are seen: one launch, no fragments
+    assert 0 < bytes_of(0xFFFFFFFF, window=100, **long) < 32 << 20
+    v = C.c_uint64()
+    assert lib.fmcuda_paged_attention_sinks_workspace_bytes(C.byref(attention_args()), 1, C.byref(v)) == ARG
+    assert lib.fmcuda_paged_attention_sinks_workspace_bytes(None, 1, C.byref(v)) == ARG
+    assert lib.fmcuda_paged_attention_sinks_workspace_bytes(C.byref(attention_args()), 0, None) == ARG
 
 
 # ---------------------------------------------------------------------- probabilities of tokens
