@@ -3,17 +3,26 @@
 //
 //   z = scale * logits,  L = log sum_i e^(z_i),  log p_i = z_i - L,  H = -sum_i p_i log p_i
 //
-// One read of the logits, whatever is asked of them.  Each thread streams chunks of 16
-// bytes with a reference value x0 and, over d = x - x0 in units of log2 (t = d scale log2 e),
-// the sums of 2^t and of t 2^t, which give L and H; the reference moves only when a value
-// exceeds it by 2^8, since any reference in that range gives the same sums.  A difference of
-// inputs loses nothing that a product scale * x would lose at large x.
+// One read of the logits, whatever is asked of them.  Each thread streams chunks of 32
+// bytes with a reference x0 and, over t = (x - x0) scale log2 e, the sums of 2^t and of
+// t 2^t, which give L and H; the reference moves only when a value exceeds it by 2^8, since
+// any in that range gives the same sums.  A difference of inputs loses nothing that a
+// product scale x would lose at large x, and is 0 at x0 itself: a sure token has log
+// probability 0.  16-bit logits arrive at ten values a clock and SM, with a dozen issue slots
+// for each, so that what is not arithmetic is done for two values or for a chunk at a time;
+// -inf (tokens ruled out) is raised to a value whose 2^t is 0, and not looked at again.
+// Where no such value is (references or scales at the ends of their range) a chunk goes the
+// long way, value by value.
 //
-// The k most probable values need no second pass either.  A thread keeps the place of its
-// largest value.  By (value, lower place) these places are distinct, and whatever belongs to
-// the k first of a row lies in one of the k threads whose places come first: every value
-// elsewhere is preceded by those k.  So only these threads' chunks, k of hundreds, are read
-// again (from L2), and of them what does not come behind the last of the k places is sorted.
+// The k most probable values need no second pass either.  A thread keeps its best chunk, by
+// its largest value and then by the lower place, and the largest value of its other chunks.
+// The threads make 32 or 64 groups; the k-th of the groups' best chunks is a bound that k
+// chunks reach, so that nothing that comes behind it belongs to the k first of the row.  A
+// thread whose best chunk reaches it reads that chunk again (from L2); the few of which
+// another one does as well have all of their chunks read again, by the whole CTA.  What
+// these hold up to the bound, little more than k values, is sorted.  (With all chunks of
+// every such thread read again, 4096 rows of 128256 in bf16 took 272 us for 32 of them, where
+// they take 179 for none.)
 //
 // A CTA takes a row; where rows are few a cluster does, whose CTAs are joined through
 // shared memory.
@@ -28,7 +37,7 @@
 namespace fmb {
 namespace {
 
-constexpr uint32_t LP_MAX_TOP = 32, LP_LIST = 1024, LP_MAX_CLUSTER = 8;
+constexpr uint32_t LP_MAX_TOP = 32, LP_GROUPS = 64, LP_LIST = 1024, LP_MAX_CLUSTER = 8, LP_THREADS = 512;
 constexpr float LP_LEAST = -200.0f; // 2^t is 0 from here down; a finite t keeps t 2^t a number
 
 struct LogProbParams {
@@ -38,7 +47,11 @@ struct LogProbParams {
     const int32_t *tokens;
     float *logprobs, *entropy, *top_logprobs;
     int32_t *top_ids;
-    float to_log2; // scale * log2(e)
+    float c;        // scale * log2(e)
+    float raised;   // what values below it are raised to, in the logits' type
+    float step;     // values that exceed a reference by it move it: 8 / c
+    float nothing;  // a reference over which a chunk of raised values adds nothing
+    float ordinary; // a reference from here to -raised goes the short way
     double scale;
     int *status;
 };
@@ -63,78 +76,124 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-template <int T> constexpr int LP_VEC = 16 / static_cast<int>(x_size(T));
+template <int T> constexpr int LP_VEC = 32 / static_cast<int>(x_size(T)); // values a chunk
 
-template <int T> __device__ __forceinline__ void unpack16(uint4 w, float (&v)[LP_VEC<T>]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Chunk {
+    uint32_t w[8];
+};
+__device__ __forceinline__ Chunk load_chunk32(const void *at) {
+    Chunk r;
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                   "=r"(r.w[7])
+                 : "l"(at));
+    return r;
+}
+
+// Values of a 4-byte word; `V` of them.
+template <int T> __device__ __forceinline__ float2 two_of(uint32_t u) {
+    if constexpr (T == FM_X_BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+}
+template <int T> __device__ __forceinline__ void unpack(const Chunk &x, float (&v)[LP_VEC<T>]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         if constexpr (T == FM_X_F32) {
-            v[i] = __uint_as_float(u[i]);
-        } else if constexpr (T == FM_X_BF16) {
-            v[2 * i] = __uint_as_float(u[i] << 16);
-            v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            v[i] = __uint_as_float(x.w[i]);
         } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+            const float2 f = two_of<T>(x.w[i]);
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
         }
     }
 }
 
-// A row as a ragged head, whole chunks at 16-byte addresses, and a ragged tail.  Chunk i is
-// thread i modulo the row's threads's; the head is thread 0's, and the tail is chunk `whole`.
+// The larger of two values of f32, or of two pairs of 16-bit ones; NaN left out, or kept.
+template <int T, bool NAN_KEPT = false> __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (T == FM_X_F32) {
+        if constexpr (NAN_KEPT)
+            asm("max.NaN.f32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+        else
+            asm("max.f32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    } else if constexpr (T == FM_X_BF16) {
+        if constexpr (NAN_KEPT)
+            asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+        else
+            asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    } else {
+        if constexpr (NAN_KEPT)
+            asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+        else
+            asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    }
+    return r;
+}
+
+// A chunk's largest value, NaN left out.
+template <int T> __device__ __forceinline__ float largest(const Chunk &x) {
+    const uint32_t a = larger<T>(larger<T>(x.w[0], x.w[1]), larger<T>(x.w[2], x.w[3]));
+    const uint32_t b = larger<T>(larger<T>(x.w[4], x.w[5]), larger<T>(x.w[6], x.w[7]));
+    const uint32_t top = larger<T>(a, b);
+    if constexpr (T == FM_X_F32) return __uint_as_float(top);
+    const float2 f = two_of<T>(top);
+    return fmaxf(f.x, f.y);
+}
+
+// A row as a ragged head, whole chunks at 32-byte addresses, and a ragged tail: chunks 0, 1 ..
+// whole and whole + 1, either end of which may be empty.  Chunk i is thread i modulo the row's
+// threads's.
 template <int T> struct Row {
     const char *at;
-    uint32_t vocab, head, whole;
+    uint32_t vocab, head, whole, tail;
     __device__ __forceinline__ Row(const LogProbParams &p, uint64_t row) {
         constexpr uint32_t S = x_size(T), V = LP_VEC<T>;
         at = static_cast<const char *>(p.logits) + static_cast<int64_t>(row) * p.stride * S;
         vocab = p.vocab;
-        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at) & 15u) / S;
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at) & 31u) / S;
         head = off ? V - off : 0;
         if (head > vocab) head = vocab;
         whole = (vocab - head) / V;
+        tail = vocab - head - whole * V;
     }
-    __device__ __forceinline__ uint32_t first_of(uint32_t chunk) const { return head + chunk * LP_VEC<T>; }
-    __device__ __forceinline__ uint4 load(uint32_t chunk) const {
-        return __ldg(reinterpret_cast<const uint4 *>(at + static_cast<uint64_t>(first_of(chunk)) * x_size(T)));
+    __device__ __forceinline__ uint32_t first_of(uint32_t chunk) const {
+        return chunk ? head + (chunk - 1) * LP_VEC<T> : 0;
     }
-    // values [first, first + n), n < V; the others -inf
-    __device__ __forceinline__ void ragged(uint32_t first, uint32_t n, float (&v)[LP_VEC<T>]) const {
+    __device__ __forceinline__ uint32_t size_of(uint32_t chunk) const {
+        return chunk == 0 ? head : chunk <= whole ? LP_VEC<T> : chunk == whole + 1 ? tail : 0;
+    }
+    // whole chunk i, from 0
+    __device__ __forceinline__ const char *whole_at(uint32_t i) const {
+        return at + static_cast<uint64_t>(head) * x_size(T) + static_cast<uint64_t>(i) * 32;
+    }
+    // A chunk at an end, or behind the last; what it lacks is -inf.
+    __device__ __noinline__ Chunk end(uint32_t chunk) const {
+        const uint32_t first = first_of(chunk), n = size_of(chunk);
+        constexpr uint32_t NONE = T == FM_X_F32 ? 0xFF800000u : T == FM_X_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
+        Chunk x;
+        if (n == 0) {
 #pragma unroll
-        for (int j = 0; j < LP_VEC<T>; ++j) v[j] = static_cast<uint32_t>(j) < n ? load1(at, T, first + j) : -INFINITY;
+            for (int i = 0; i < 8; ++i) x.w[i] = NONE;
+            return x;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.w[i] = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < LP_VEC<T>; ++j) {
+            if constexpr (T == FM_X_F32) {
+                x.w[j] = j < n ? reinterpret_cast<const uint32_t *>(at)[first + j] : NONE;
+            } else {
+                x.w[j / 2] |= (j < n ? reinterpret_cast<const uint16_t *>(at)[first + j] : NONE & 0xFFFFu) << (j % 2 * 16);
+            }
+        }
+        return x;
     }
 };
 
-// A thread's sums, and its first place by (value, lower place).
-struct Running {
+// Sums over the reference `ref`: a value of the row; -FLT_MAX where there are none.
+struct Sums {
     float ref = -FLT_MAX, sum = 0.0f, tsum = 0.0f;
-    float best = -INFINITY;
-    uint32_t place = 0xFFFFFFFFu; // the first value's of the chunk that holds it; none yet
-
-    template <int V> __device__ __forceinline__ void add(const float (&v)[V], uint32_t first, float c, float step) {
-        float high = v[0];
-#pragma unroll
-        for (int j = 1; j < V; ++j) high = fmaxf(high, v[j]);
-        if (high > best || place == 0xFFFFFFFFu) {
-            best = fmaxf(high, -INFINITY);
-            place = first;
-        }
-        if (high > ref + step) {
-            const float dt = fmaxf((ref - high) * c, LP_LEAST), f = exp2_approx(dt);
-            tsum = f * fmaf(dt, sum, tsum);
-            sum *= f;
-            ref = high;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float t = max_nan((v[j] - ref) * c, LP_LEAST), e = exp2_approx(t);
-            sum += e;
-            tsum = fmaf(e, t, tsum);
-        }
-    }
-    // the sums for another reference that is not below this one
+    // the same for another reference that is not below
     __device__ __forceinline__ void move(float to, float c) {
         const float dt = max_nan((ref - to) * c, LP_LEAST), f = exp2_approx(dt);
         tsum = f * fmaf(dt, sum, tsum);
@@ -143,33 +202,118 @@ struct Running {
     }
 };
 
+// A chunk's sums the long way.
+template <int T> __device__ __noinline__ float2 long_way(Chunk x, float ref, float c) {
+    float v[LP_VEC<T>];
+    unpack<T>(x, v);
+    float2 r = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < LP_VEC<T>; ++j) {
+        const float t = max_nan((v[j] - ref) * c, LP_LEAST), e = exp2_approx(t);
+        r.x += e;
+        r.y = fmaf(e, t, r.y);
+    }
+    return r;
+}
+
+// The same while a row goes by, and the thread's best chunk.  Two sums each, for the operations
+// that take two values.
+template <int T> struct Stream {
+    float ref, limit; // a value above the limit moves the reference
+    float best, second; // the best chunk's largest value, and the other chunks'
+    uint32_t chunk;     // 0xFFFFFFFF: none
+    uint64_t sum, tsum;
+    float base; // the reference, or where a chunk of the short way is all -inf a value that is high enough
+    uint32_t raised;
+
+    // `first`: the thread's first chunk, if there is one
+    __device__ __forceinline__ Stream(const LogProbParams &p, uint32_t first)
+        : ref(-FLT_MAX), limit(-INFINITY), best(-INFINITY), second(-INFINITY), chunk(first), sum(0), tsum(0), base(p.nothing) {
+        if constexpr (T == FM_X_F32)
+            raised = __float_as_uint(p.raised);
+        else
+            raised = pack2(p.raised, p.raised, T);
+    }
+
+    // Whole warps come here together, each lane with a chunk of its own.
+    __device__ __forceinline__ void add(const LogProbParams &p, Chunk &x, uint32_t at) {
+        const float high = largest<T>(x);
+        if (high > best) chunk = at;
+        second = fmaxf(second, fminf(best, high));
+        best = fmaxf(best, high);
+        if (__any_sync(0xFFFFFFFFu, high > limit)) move(p, x, high);
+        const uint64_t c2 = pack_f32x2(p.c, p.c), to = pack_f32x2(-base, -base);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.w[i] = larger<T, true>(x.w[i], raised);
+        float v[LP_VEC<T>];
+        unpack<T>(x, v);
+#pragma unroll
+        for (int j = 0; j < LP_VEC<T>; j += 2) {
+            const uint64_t t = mul_f32x2(add_f32x2(pack_f32x2(v[j], v[j + 1]), to), c2);
+            float a, b;
+            unpack_f32x2(t, a, b);
+            const uint64_t e = pack_f32x2(exp2_approx(a), exp2_approx(b));
+            sum = add_f32x2(sum, e);
+            tsum = fma_f32x2(e, t, tsum);
+        }
+    }
+
+    // Moves the lanes' references up to their chunks' largest values; a chunk whose reference
+    // does not go the short way is added here, and leaves nothing to add.
+    __device__ __forceinline__ void move(const LogProbParams &p, Chunk &x, float high) {
+        const bool over = high > limit;
+        const float to = over && high > ref ? high : ref;
+        const float dt = ref == to ? 0.0f : max_nan((ref - to) * p.c, LP_LEAST), f = exp2_approx(dt);
+        const uint64_t f2 = pack_f32x2(f, f);
+        tsum = mul_f32x2(f2, fma_f32x2(pack_f32x2(dt, dt), sum, tsum));
+        sum = mul_f32x2(f2, sum);
+        ref = to;
+        const bool ordinary = ref >= p.ordinary && ref <= -p.raised;
+        base = ordinary ? ref : p.nothing;
+        limit = ordinary ? ref + p.step : -INFINITY;
+        if (over && !ordinary) {
+            const float2 more = long_way<T>(x, ref, p.c);
+            sum = add_f32x2(sum, pack_f32x2(more.x, 0.0f));
+            tsum = add_f32x2(tsum, pack_f32x2(more.y, 0.0f));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.w[i] = raised;
+        }
+    }
+
+    __device__ __forceinline__ Sums sums() const {
+        Sums r;
+        float a, b;
+        unpack_f32x2(sum, a, b);
+        r.sum = a + b;
+        unpack_f32x2(tsum, a, b);
+        r.tsum = a + b;
+        r.ref = ref;
+        return r;
+    }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t key) {
     const uint32_t hi = static_cast<uint32_t>(key >> 32), top = __reduce_max_sync(0xFFFFFFFFu, hi);
     const uint32_t lo = __reduce_max_sync(0xFFFFFFFFu, hi == top ? static_cast<uint32_t>(key) : 0u);
     return static_cast<uint64_t>(top) << 32 | lo;
 }
 
-// The warp's keys, largest in lane 0.
-__device__ __forceinline__ uint64_t warp_sort(uint64_t key, uint32_t lane) {
-#pragma unroll
-    for (uint32_t size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (uint32_t dist = size / 2; dist > 0; dist >>= 1) {
-            const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, key, dist);
-            const bool larger = ((lane & dist) == 0) == ((lane & size) == 0 || size == 32);
-            if ((other > key) == larger) key = other;
-        }
-    return key;
-}
-
 struct LPShared {
-    uint64_t sorted[32][32]; // the warps' threads by their places
+    uint64_t groups[LP_GROUPS]; // their best chunks
+    uint64_t bound;
     uint64_t list[LP_LIST];
-    uint64_t first[LP_MAX_TOP]; // the row's (the CTA's part's) first values
-    uint64_t chosen[LP_MAX_TOP];
-    float ref[32], sum[32], tsum[32];
+    uint64_t first[LP_MAX_TOP]; // the first values of the row, or of the CTA's part of it
+    float ref[LP_THREADS / 32], sum[LP_THREADS / 32], tsum[LP_THREADS / 32];
     float all[3]; // ref, sum, tsum of the CTA
-    uint32_t n;
+    uint32_t n, singles, columns;
+    uint32_t single[LP_THREADS];  // chunks that are read again
+    uint16_t column[LP_THREADS];  // threads whose chunks are all read again
 };
 
 // The k first of n keys to `first`, by counting for each how many come before it.
@@ -177,59 +321,60 @@ __device__ __forceinline__ void rank_keys(const uint64_t *keys, uint32_t n, uint
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const uint64_t key = keys[i];
         uint32_t before = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < n; ++j) before += keys[j] > key;
         if (before < k) first[before] = key;
     }
 }
 
-// The k first values of the CTA's part of a row (chunks cta_first.. modulo all), to s.first.
+// The k first values of the CTA's part of a row, to s.first; `mine` is the key of the thread's
+// best chunk, and groups of `lanes` threads have put theirs to s.groups.
 template <int T>
-__device__ __forceinline__ void select_top(const Row<T> &row, const Running &mine, uint32_t k, uint32_t rank,
-                                           uint32_t threads, LPShared &s) {
+__device__ __forceinline__ void select_top(const Row<T> &row, const Stream<T> &stream, uint64_t mine, uint64_t group,
+                                           uint32_t lanes, uint32_t k, uint32_t rank, uint32_t threads, LPShared &s) {
     constexpr uint32_t V = LP_VEC<T>;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
-    uint64_t key = mine.place == 0xFFFFFFFFu ? 0 : key_of(code_of(mine.best), mine.place);
-    s.sorted[warp][lane] = warp_sort(key, lane);
-    if (threadIdx.x == 0) s.n = 0;
+    // the group that k - 1 others come before: its threads share the count
+    const uint32_t groups = blockDim.x / lanes, part = groups / lanes, from = threadIdx.x % lanes * part;
+    uint32_t before = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < part; ++j) before += s.groups[from + j] > group;
+    for (uint32_t o = 1; o < lanes; o <<= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+    if (before == k - 1 && group) s.bound = group; // else fewer groups than k have a chunk, and it stays 0
     __syncthreads();
-    if (warp == 0) {
-        // lane w goes down warp w's list
-        uint32_t next = 0;
-        uint64_t head = lane < warps ? s.sorted[lane][0] : 0;
-        for (uint32_t r = 0; r < k; ++r) {
-            const uint64_t top = warp_max_key(head);
-            if (lane == 0) s.chosen[r] = top;
-            if (head == top) head = ++next < 32 && lane < warps ? s.sorted[lane][next] : 0;
-        }
+    const uint64_t bound = s.bound;
+    const float bound_value = bound ? value_of(static_cast<uint32_t>(bound >> 32)) : -INFINITY;
+    const uint32_t bound_chunk = bound ? place_of(bound) : 0xFFFFFFFFu;
+    if (mine && mine >= bound) {
+        if (stream.second < bound_value)
+            s.single[atomicAdd(&s.singles, 1u)] = stream.chunk;
+        else
+            s.column[atomicAdd(&s.columns, 1u)] = static_cast<uint16_t>(threadIdx.x);
     }
     __syncthreads();
-    // what does not come behind the last of them (0: fewer threads than k have a place)
-    const uint64_t bound = s.chosen[k - 1];
-    const uint32_t bound_code = static_cast<uint32_t>(bound >> 32), bound_place = bound ? place_of(bound) : 0xFFFFFFFFu;
-    const uint32_t tail = row.vocab - row.first_of(row.whole);
-    const uint32_t rounds = (row.whole + threads - 1) / threads, per = rounds + 2;
+    const uint32_t per = (row.whole + 2 + threads - 1) / threads, singles = s.singles, all = singles + s.columns * per;
+    // every value that does not come behind the bound, NaN too
     auto visit = [&](auto &&take) {
-        for (uint32_t w = threadIdx.x; w < k * per; w += blockDim.x) {
-            const uint64_t from = s.chosen[w / per];
-            if (!from) continue;
-            const uint32_t place = place_of(from), owner = place < row.head ? 0 : (place - row.head) / V % threads;
-            const uint32_t i = w % per;
-            float v[V];
-            uint32_t first = 0, n = 0;
-            if (i < rounds) {
-                const uint32_t chunk = owner + i * threads;
-                if (chunk >= row.whole) continue;
-                first = row.first_of(chunk), n = V;
-                unpack16<T>(row.load(chunk), v);
+        for (uint32_t w = threadIdx.x; w < all; w += blockDim.x) {
+            uint32_t chunk;
+            if (w < singles) {
+                chunk = s.single[w];
             } else {
-                if (i == rounds && owner == 0) n = row.head;
-                if (i > rounds && owner == row.whole % threads) first = row.first_of(row.whole), n = tail;
-                row.ragged(first, n, v);
+                const uint32_t c = (w - singles) / per;
+                chunk = rank * blockDim.x + s.column[c] + (w - singles - c * per) * threads;
             }
+            const uint32_t n = row.size_of(chunk), first = row.first_of(chunk);
+            float v[V];
+            unpack<T>(chunk - 1 < row.whole ? load_chunk32(row.whole_at(chunk - 1)) : row.end(chunk), v);
+            const bool ties = chunk <= bound_chunk;
+            uint32_t in = 0;
 #pragma unroll
-            for (uint32_t j = 0; j < V; ++j) {
-                const uint32_t code = code_of(v[j]);
-                if (j < n && (code > bound_code || (code == bound_code && first <= bound_place))) take(key_of(code, first + j));
+            for (uint32_t j = 0; j < V; ++j)
+                if (!(ties ? v[j] < bound_value : v[j] <= bound_value)) in |= 1u << j;
+            in &= (1u << n) - 1u;
+            while (in) {
+                const uint32_t j = __ffs(in) - 1;
+                in &= in - 1;
+                take(key_of(code_of(load1(row.at, T, first + j)), first + j));
             }
         }
     };
@@ -237,13 +382,14 @@ __device__ __forceinline__ void select_top(const Row<T> &row, const Running &min
         const uint32_t at = atomicAdd(&s.n, 1u);
         if (at < LP_LIST) s.list[at] = key;
     });
-    if (threadIdx.x < k) s.first[threadIdx.x] = 0;
     __syncthreads();
     if (s.n <= LP_LIST) {
         rank_keys(s.list, s.n, k, s.first);
     } else {
-        // more than the list holds (values that grow or fall along the row in steps of a thread's): one at a time
+        // more than the list holds (rows of which a few threads have all the large values): one at a time
+        const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
         uint64_t last = ~0ull;
+#pragma unroll 1
         for (uint32_t r = 0; r < k; ++r) {
             uint64_t best = 0;
             visit([&](uint64_t key) {
@@ -254,152 +400,154 @@ __device__ __forceinline__ void select_top(const Row<T> &row, const Running &min
             if (lane == 0) s.list[warp] = best;
             __syncthreads();
             last = 0;
-            for (uint32_t w = 0; w < warps; ++w) last = s.list[w] > last ? s.list[w] : last;
+            for (uint32_t w = 0; w < blockDim.x / 32; ++w) last = s.list[w] > last ? s.list[w] : last;
             if (threadIdx.x == 0) s.first[r] = last;
         }
     }
     __syncthreads();
 }
 
-template <int T>
-__global__ void __launch_bounds__(1024) logprobs_kernel(const LogProbParams p, uint32_t ranks) {
-    constexpr int V = LP_VEC<T>, U = T == FM_X_F32 ? 4 : 4;
+// The logarithm of a sum, as that of its exponent and of a value near 1: f32 for the latter
+// is exact to 2^-26.
+__device__ __forceinline__ double log_of(float sum) {
+    const int k = static_cast<int>(__float_as_uint(sum) - 0x3F400000u) >> 23; // sum / 2^k in [3/4, 3/2)
+    const float near = __uint_as_float(__float_as_uint(sum) - (static_cast<uint32_t>(k) << 23));
+    return (sum > 0.0f && sum < INFINITY) ? 0.69314718055994531 * k + static_cast<double>(logf(near))
+                                          : static_cast<double>(logf(sum));
+}
+
+// FEW: rows that do not fill the GPU, whose threads have four chunks on their way.  Where they
+// do, 64 warps an SM are worth more than that (4096 rows of 128256 in bf16: 192 us with a chunk
+// a thread on its way and 32 registers, 200 with 40, 203 to 211 with two and 64).
+template <int T, bool FEW>
+__global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const LogProbParams p, uint32_t ranks) {
     __shared__ LPShared s;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
     const uint32_t rank = blockIdx.x % ranks, threads = blockDim.x * ranks;
     const uint64_t r = blockIdx.x / ranks;
+    if (threadIdx.x == 0) {
+        s.bound = 0;
+        s.n = s.singles = s.columns = 0;
+    }
+    if (threadIdx.x < LP_MAX_TOP) s.first[threadIdx.x] = 0;
     after_stream();
     let_next();
     const Row<T> row(p, r);
     const uint32_t me = rank * blockDim.x + threadIdx.x;
-    const float c = p.to_log2, step = 8.0f / c;
-    float chosen = 0.0f;
+    float given = 0.0f;
     int32_t token = -1;
     if (me == 0) {
         token = p.tokens[r];
-        if (token >= 0 && static_cast<uint32_t>(token) < row.vocab) chosen = load1(row.at, T, static_cast<uint32_t>(token));
+        if (token >= 0 && static_cast<uint32_t>(token) < row.vocab) given = load1(row.at, T, static_cast<uint32_t>(token));
     }
-    Running mine;
-    float v[V];
-    if (me == 0 && row.head) {
-        row.ragged(0, row.head, v);
-        mine.add(v, 0, c, step);
-    }
-    uint32_t i = me;
-    for (; i + (U - 1) * threads < row.whole; i += U * threads) {
-        uint4 w[U];
+    // chunk 0 may be empty, and so may the last
+    const uint32_t first = me || row.head ? me : threads, last = row.whole + (row.tail ? 1 : 0);
+    Stream<T> stream(p, first <= last ? first : 0xFFFFFFFFu);
+    // the warp's lanes have 32 chunks in a row
+    const uint32_t total = row.whole + 2;
+    uint32_t chunk = me - lane;
+    const char *from = row.at + static_cast<int64_t>(row.head * x_size(T)) + (static_cast<int64_t>(me) - 1) * 32;
+    auto load = [&](uint32_t first) {
+        Chunk x;
+        if (first + lane - 1 < row.whole)
+            x = load_chunk32(from);
+        else
+            x = row.end(first + lane);
+        from += threads * 32ull;
+        return x;
+    };
+    constexpr int U = FEW ? 4 : 1;
+    for (; chunk < total; chunk += U * threads) {
+        Chunk x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = row.load(i + u * threads);
+        for (int u = 0; u < U; ++u) x[u] = load(chunk + u * threads);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            unpack16<T>(w[u], v);
-            mine.add(v, row.first_of(i + u * threads), c, step);
-        }
-    }
-    for (; i < row.whole; i += threads) {
-        unpack16<T>(row.load(i), v);
-        mine.add(v, row.first_of(i), c, step);
-    }
-    const uint32_t tail = row.vocab - row.first_of(row.whole);
-    if (tail && me == row.whole % threads) {
-        row.ragged(row.first_of(row.whole), tail, v);
-        mine.add(v, row.first_of(row.whole), c, step);
+        for (int u = 0; u < U; ++u) stream.add(p, x[u], chunk + u * threads + lane);
     }
 
-    // the CTA's sums
-    float top = mine.ref;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    Running all = mine;
-    all.move(top, c);
+    Sums all = stream.sums();
+    // threads a group, and the group's best chunk
+    const uint32_t lanes = blockDim.x > LP_GROUPS ? blockDim.x / LP_GROUPS : 1;
+    uint64_t mine = 0, group = 0;
+    if (p.top) {
+        group = mine = stream.chunk == 0xFFFFFFFFu ? 0 : key_of(code_of(stream.best), stream.chunk);
+        for (uint32_t o = 1; o < lanes; o <<= 1) {
+            const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, group, o);
+            group = other > group ? other : group;
+        }
+        if (threadIdx.x % lanes == 0) s.groups[threadIdx.x / lanes] = group;
+    }
+    all.move(warp_max(all.ref), p.c);
     all.sum = warp_sum(all.sum);
     all.tsum = warp_sum(all.tsum);
     if (lane == 0) {
-        s.ref[warp] = top;
+        s.ref[warp] = all.ref;
         s.sum[warp] = all.sum;
         s.tsum[warp] = all.tsum;
     }
     __syncthreads();
+    if (p.top) select_top<T>(row, stream, mine, group, lanes, p.top, rank, threads, s);
+    if (ranks == 1 && warp) return;
     if (warp == 0) {
-        all.ref = lane < warps ? s.ref[lane] : -FLT_MAX;
-        all.sum = lane < warps ? s.sum[lane] : 0.0f;
-        all.tsum = lane < warps ? s.tsum[lane] : 0.0f;
-        top = all.ref;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        all.move(top, c);
+        const bool in = lane < warps;
+        all.ref = in ? s.ref[lane] : -FLT_MAX;
+        all.sum = in ? s.sum[lane] : 0.0f;
+        all.tsum = in ? s.tsum[lane] : 0.0f;
+        all.move(warp_max(all.ref), p.c);
         all.sum = warp_sum(all.sum);
         all.tsum = warp_sum(all.tsum);
-        if (lane == 0) {
-            s.all[0] = top;
+        if (ranks > 1 && lane == 0) {
+            s.all[0] = all.ref;
             s.all[1] = all.sum;
             s.all[2] = all.tsum;
         }
     }
-    if (p.top) select_top<T>(row, mine, p.top, rank, threads, s);
-    else __syncthreads();
-
     if (ranks > 1) {
         cluster_sync();
         if (rank == 0) {
-            float ref[LP_MAX_CLUSTER], sum[LP_MAX_CLUSTER], tsum[LP_MAX_CLUSTER];
-            top = -FLT_MAX;
-#pragma unroll
-            for (uint32_t q = 0; q < LP_MAX_CLUSTER; ++q) {
-                ref[q] = -FLT_MAX;
-                sum[q] = tsum[q] = 0.0f;
-                if (q >= ranks) continue;
-                ref[q] = cluster_load(smem_u32(&s.all[0]), q);
-                sum[q] = cluster_load(smem_u32(&s.all[1]), q);
-                tsum[q] = cluster_load(smem_u32(&s.all[2]), q);
-            }
             for (uint32_t w = threadIdx.x; w < ranks * p.top; w += blockDim.x)
                 s.list[w] = cluster_load64(smem_u32(&s.first[w % p.top]), w / p.top);
-#pragma unroll
-            for (uint32_t q = 0; q < LP_MAX_CLUSTER; ++q) top = fmaxf(top, ref[q]);
-            all.sum = all.tsum = 0.0f;
-#pragma unroll
-            for (uint32_t q = 0; q < LP_MAX_CLUSTER; ++q) {
-                Running part;
-                part.ref = ref[q];
-                part.sum = sum[q];
-                part.tsum = tsum[q];
-                part.move(top, c);
-                all.sum += part.sum;
-                all.tsum += part.tsum;
+            if (warp == 0) {
+                const bool in = lane < ranks;
+                all.ref = in ? cluster_load(smem_u32(&s.all[0]), lane) : -FLT_MAX;
+                all.sum = in ? cluster_load(smem_u32(&s.all[1]), lane) : 0.0f;
+                all.tsum = in ? cluster_load(smem_u32(&s.all[2]), lane) : 0.0f;
+                all.move(warp_max(all.ref), p.c);
+                all.sum = warp_sum(all.sum);
+                all.tsum = warp_sum(all.tsum);
             }
         }
         cluster_sync(); // nobody leaves, and nothing of rank 0's is overwritten, while it is read
         if (rank != 0) return;
-        if (threadIdx.x == 0) {
-            s.all[0] = top;
-            s.all[1] = all.sum;
-            s.all[2] = all.tsum;
-        }
         rank_keys(s.list, ranks * p.top, p.top, s.first);
         __syncthreads();
+        if (warp) return;
     }
     // sum 0: a row of nothing but -inf
-    const float ref = s.all[0], sum = s.all[1];
-    const double log_sum = log(static_cast<double>(sum));
+    const double log_sum = log_of(all.sum);
     auto log_p = [&](float x) {
-        return sum == 0.0f ? -INFINITY : static_cast<float>(p.scale * (static_cast<double>(x) - ref) - log_sum);
+        return all.sum == 0.0f ? -INFINITY : static_cast<float>(p.scale * (static_cast<double>(x) - all.ref) - log_sum);
     };
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         if (token >= 0 && static_cast<uint32_t>(token) >= row.vocab) {
             raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
             p.logprobs[r] = NAN;
         } else {
-            p.logprobs[r] = token < 0 ? 0.0f : log_p(chosen);
+            p.logprobs[r] = token < 0 ? 0.0f : log_p(given);
         }
-        const float h = sum == 0.0f ? 0.0f : static_cast<float>(log_sum - 0.69314718055994531 * s.all[2] / sum);
+        const float h =
+            all.sum == 0.0f ? 0.0f : static_cast<float>(log_sum - 0.69314718055994531 * all.tsum / all.sum);
         p.entropy[r] = h < 0.0f ? 0.0f : h;
     }
-    if (threadIdx.x < p.top) {
-        const uint64_t key = s.first[threadIdx.x], at = r * p.top + threadIdx.x;
+    if (lane < p.top) {
+        const uint64_t key = s.first[lane], at = r * p.top + lane;
         p.top_logprobs[at] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
         p.top_ids[at] = static_cast<int32_t>(place_of(key));
     }
+}
+
+template <int T> int launch_logprobs(const LogProbParams &p, const Launch &l, bool few, cudaStream_t s) {
+    return launch("logprobs_kernel", few ? logprobs_kernel<T, true> : logprobs_kernel<T, false>, l, s, p, l.cluster);
 }
 
 } // namespace
@@ -425,19 +573,37 @@ extern "C" int fmcuda_token_logprobs(const fmcuda_token_logprobs_args *a, void *
         !aligned_to_value(a->logprobs, FM_X_F32) || !aligned_to_value(a->entropy, FM_X_F32) ||
         (a->top && (!aligned_to_value(a->top_logprobs, FM_X_F32) || !aligned_to_value(a->top_ids, FM_X_F32))))
         return set_error(FM_STATUS_INVALID_ARGUMENT, "log probability buffer is not aligned to its values");
-    const LogProbParams p{a->logits,       a->row_stride,   a->vocab,
-                          a->top,          a->token,        a->logprobs,
-                          a->entropy,      a->top_logprobs, a->top_ids,
-                          static_cast<float>(a->scale * 1.4426950408889634), a->scale, device_status_word()};
-    // threads with a few chunks each; rows that leave SMs idle go to clusters
-    const uint64_t chunks = static_cast<uint64_t>(a->vocab) * x_size(a->dtype) / 16;
+    LogProbParams p{};
+    p.logits = a->logits;
+    p.stride = a->row_stride;
+    p.vocab = a->vocab;
+    p.top = a->top;
+    p.tokens = a->token;
+    p.logprobs = a->logprobs;
+    p.entropy = a->entropy;
+    p.top_logprobs = a->top_logprobs;
+    p.top_ids = a->top_ids;
+    p.c = static_cast<float>(a->scale * 1.4426950408889634);
+    // 2^t of a raised value is 0 for every reference from `ordinary` on (f16 with small scales
+    // has none), and no difference of the short way overflows
+    p.raised = a->dtype == FM_X_F16 ? -65504.0f : -std::exp2(std::fmin(std::floor(120.0f - std::log2(p.c)), 100.0f));
+    p.ordinary = p.raised * p.c <= 4.0f * LP_LEAST ? p.raised / 2.0f : p.raised - 2.0f * LP_LEAST / p.c;
+    p.nothing = -2.0f * LP_LEAST / p.c;
+    p.step = 8.0f / p.c;
+    p.scale = a->scale;
+    p.status = device_status_word();
+    // rows that leave SMs idle go to clusters, and to more threads
+    const uint64_t chunks = static_cast<uint64_t>(a->vocab) * x_size(a->dtype) / 32;
     const uint64_t sms = static_cast<uint64_t>(device_sm_count());
     uint32_t ranks = 1, threads = 32;
-    while (ranks < LP_MAX_CLUSTER && a->tokens * ranks * 2 <= sms && chunks >= ranks * 2048ull) ranks *= 2;
-    while (threads < 512 && chunks > static_cast<uint64_t>(threads) * ranks * 8) threads *= 2;
+    while (ranks < LP_MAX_CLUSTER && a->tokens * ranks * 2 <= sms && chunks >= ranks * 1024ull) ranks *= 2;
+    auto few = [&](uint32_t n) { return static_cast<uint64_t>(a->tokens) * ranks * n <= sms * 1024; };
+    while ((threads < 256 && chunks > static_cast<uint64_t>(threads) * ranks * 4) ||
+           (threads < LP_THREADS && chunks > static_cast<uint64_t>(threads) * ranks && few(2 * threads)))
+        threads *= 2;
     const Launch l{dim3(a->tokens * ranks), threads, 0, ranks};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->dtype == FM_X_F32) return launch("logprobs_kernel", logprobs_kernel<FM_X_F32>, l, s, p, ranks);
-    if (a->dtype == FM_X_BF16) return launch("logprobs_kernel", logprobs_kernel<FM_X_BF16>, l, s, p, ranks);
-    return launch("logprobs_kernel", logprobs_kernel<FM_X_F16>, l, s, p, ranks);
+    if (a->dtype == FM_X_F32) return launch_logprobs<FM_X_F32>(p, l, few(threads), s);
+    if (a->dtype == FM_X_BF16) return launch_logprobs<FM_X_BF16>(p, l, few(threads), s);
+    return launch_logprobs<FM_X_F16>(p, l, few(threads), s);
 }
