@@ -52,7 +52,7 @@ __device__ __forceinline__ void pair_h(const PairParams &p, uint64_t row, uint32
     for (int j = 0; j < 8; ++j) h[j] = fmaf(v[j], p.res_scale, h[j]);
 }
 
-// A CTA a row, read three times (the second and third time from L2).
+// Rows longer than the registers of a CTA hold: read three times, the second and third from L2.
 template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel(const PairParams p) {
     __shared__ float s_part[2][32];
     const uint32_t chunks = ((p.d + 127) / 128) * 16, n = blockDim.x;
@@ -107,11 +107,227 @@ template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel
     }
 }
 
-template <int VEC> int dispatch_pair(const PairParams &p, cudaStream_t s) {
-    const uint32_t chunks = (p.d + 127) / 128 * 16, threads = chunks >= 1024 ? 1024 : (chunks + 31) / 32 * 32;
-    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 8;
+// A chunk as it was loaded: nothing waits for the loads before get().  VEC 8: of a type that is
+// known, in accesses of 16 bytes.  Otherwise of a type at run time (T is PAIR_ANY), in accesses of
+// two values or one, in the first words of their places.
+constexpr int PAIR_ANY = -1;
+template <int VEC, int T> struct PairChunk {
+    uint32_t w[T == PAIR_ANY || T == FM_X_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const void *p, int32_t t, int64_t row, uint32_t c, uint32_t d) {
+        if constexpr (VEC == 8) {
+            constexpr int N = x_size(T) / 2;
+            const uint4 *at = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + (row + c * 8) * x_size(T));
+            uint4 q[N] = {};
+            if (c * 8 < d) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) q[i] = at[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                w[4 * i] = q[i].x;
+                w[4 * i + 1] = q[i].y;
+                w[4 * i + 2] = q[i].z;
+                w[4 * i + 3] = q[i].w;
+            }
+        } else {
+            const char *base = static_cast<const char *>(p) + row * x_size(t);
+#pragma unroll
+            for (int j = 0; j < 8; j += VEC) {
+                const uint32_t e = value_at<VEC>(c, j);
+                w[j] = 0;
+                if (VEC == 2) w[j + 1] = 0;
+                if (e >= d) continue;
+                const char *at = base + static_cast<uint64_t>(e) * x_size(t);
+                if (VEC == 2 && t == FM_X_F32) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                    w[j] = v.x;
+                    w[j + 1] = v.y;
+                } else if (VEC == 2 || t == FM_X_F32) {
+                    w[j] = *reinterpret_cast<const uint32_t *>(at);
+                } else {
+                    w[j] = *reinterpret_cast<const uint16_t *>(at);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void get(int32_t t, float (&v)[8]) const {
+        if constexpr (VEC == 8) {
+            constexpr int B = T == FM_X_F32 ? 4 : 0; // (raw8_unpack looks at the second four with f32 only)
+            raw8_unpack(Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[B], w[B + 1], w[B + 2], w[B + 3])}, T, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j += VEC) {
+                if constexpr (VEC == 2) {
+                    const float2 f = load2(&w[j], t, 0);
+                    v[j] = f.x;
+                    v[j + 1] = f.y;
+                } else {
+                    v[j] = load1(&w[j], t, 0);
+                }
+            }
+        }
+    }
+};
+
+// A team (see norm_rows.cuh) a row, whose values stay in registers between the two norms;
+// the next row is on its way meanwhile.  The weights wait in shared memory as f32, the first
+// one with the scale and a gate by channels in it.
+template <int VEC, int XT, int RT, bool CTA, int ITER, int MOST>
+__global__ void __launch_bounds__(MOST) norm_pair_kernel(const PairParams p) {
+    const uint32_t nt = CTA ? blockDim.x : 32u, teams = CTA ? 1u : blockDim.x / 32;
+    extern __shared__ float4 s_w[]; // chunk c: w1 in s_w[2 c], s_w[2 c + 1], w2 behind all of w1
+    __shared__ float s_part[2][32];
+    const uint32_t c0 = CTA ? threadIdx.x : threadIdx.x % 32, all = nt * ITER;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
+    after_stream();
+    let_next();
+    uint64_t row = CTA ? blockIdx.x : blockIdx.x * teams + threadIdx.x / 32;
+    PairChunk<VEC, XT> x[ITER];
+    PairChunk<VEC, RT> r[ITER];
+    auto load = [&](uint64_t at) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            x[i].load(p.x, p.xt, at * p.xs, c0 + i * nt, p.d);
+            r[i].load(p.res, p.rt, at * p.rs, c0 + i * nt, p.d);
+        }
+    };
+    if (row < p.tokens) load(row);
+    for (uint32_t c = threadIdx.x; c < all; c += blockDim.x) {
+        float w[8], g[8];
+        if (p.w1)
+            load_chunk<VEC>(p.w1, p.wt, 0, c, p.d, w);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = 1.0f;
+        if (p.gate_kind == GATE_CHANNEL) load_chunk<VEC>(p.gate, p.gt, 0, c, p.d, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] *= p.gate_kind == GATE_CHANNEL ? g[j] * p.scale : p.scale;
+        s_w[2 * c] = make_float4(w[0], w[1], w[2], w[3]);
+        s_w[2 * c + 1] = make_float4(w[4], w[5], w[6], w[7]);
+        if (!p.y) continue;
+        load_chunk<VEC>(p.w2, p.wt, 0, c, p.d, w);
+        s_w[2 * (all + c)] = make_float4(w[0], w[1], w[2], w[3]);
+        s_w[2 * (all + c) + 1] = make_float4(w[4], w[5], w[6], w[7]);
+    }
+    __syncthreads();
+    uint32_t turn = 0; // of the two buffers of partial sums: a thread that is ahead by a sum writes the other
+    for (; row < p.tokens; row += step) {
+        float h[ITER][8];
+        PairChunk<VEC, RT> mine[ITER];
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            x[i].get(p.xt, h[i]);
+            mine[i] = r[i];
+        }
+        if (row + step < p.tokens) load(row + step);
+        float by = 1.0f;
+        if (p.w1) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+            sum = team_sum<CTA>(sum, s_part[turn]);
+            turn ^= 1u;
+            by = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+        }
+        if (p.gate_kind == GATE_TOKEN) by *= load1(p.gate, p.gt, row * p.gs);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const uint32_t c = c0 + i * nt;
+            const float4 wa = s_w[2 * c], wb = s_w[2 * c + 1];
+            const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * by * w[j];
+            if (p.gate_kind == GATE_FULL) {
+                load_chunk<VEC>(p.gate, p.gt, row * p.gs, c, p.d, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= v[j];
+            }
+            mine[i].get(p.rt, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[i][j] = fmaf(v[j], p.res_scale, h[i][j]);
+                sum = fmaf(h[i][j], h[i][j], sum);
+            }
+        }
+        if (p.res_out) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+                store_chunk<VEC>(p.res_out, RT == PAIR_ANY ? p.rt : RT, row * p.rs, c0 + i * nt, p.d, h[i]);
+        }
+        if (!p.y) continue;
+        sum = team_sum<CTA>(sum, s_part[turn]);
+        turn ^= 1u;
+        const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const uint32_t c = c0 + i * nt;
+            const float4 wa = s_w[2 * (all + c)], wb = s_w[2 * (all + c) + 1];
+            const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * root * w[j];
+            if (p.yt == FM_X_E4M3)
+                store_e4m3<VEC>(p, row, c, h[i]);
+            else if (p.yt == FM_X_F32)
+                store_chunk<VEC>(p.y, FM_X_F32, row * p.ys, c, p.d, h[i]);
+            else if (p.yt == FM_X_BF16)
+                store_chunk<VEC>(p.y, FM_X_BF16, row * p.ys, c, p.d, h[i]);
+            else
+                store_chunk<VEC>(p.y, FM_X_F16, row * p.ys, c, p.d, h[i]);
+        }
+    }
+}
+
+template <int VEC, int XT, int RT, bool CTA, int ITER, int MOST>
+int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
+    auto kfn = norm_pair_kernel<VEC, XT, RT, CTA, ITER, MOST>;
+    const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
+    const uint32_t smem = (CTA ? threads : 32) * ITER * 64;
+    uint32_t grid = static_cast<uint32_t>(device_sm_count());
+    if (want > grid) { // as many CTAs as the GPU holds; otherwise one a row
+        int per_sm = 0;
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
+            (void)cudaGetLastError();
+            per_sm = 1;
+        }
+        grid *= static_cast<uint32_t>(per_sm);
+    }
+    return launch("norm_pair_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1}, s, p);
+}
+
+// Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
+// there are rows for half the threads of the GPU only (latency counts then).
+template <int VEC, int XT, int RT> int dispatch_width(const PairParams &p, cudaStream_t s) {
+    const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
+    const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
+    if (p.d <= 256) return launch_pair<VEC, XT, RT, false, 1, 128>(p, 128, s);
+    if (p.d <= 1024) return launch_pair<VEC, XT, RT, false, 4, 128>(p, 128, s);
+    if (few && one <= 1024) return launch_pair<VEC, XT, RT, true, 1, 1024>(p, one, s);
+    if (two <= 512) return launch_pair<VEC, XT, RT, true, 2, 512>(p, two, s);
+    if (two <= 1024) return launch_pair<VEC, XT, RT, true, 2, 1024>(p, two, s);
+    const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
     return launch("norm_pair_long_kernel", norm_pair_long_kernel<VEC>,
-                  {dim3(p.tokens < most ? p.tokens : most), threads, 0, 1}, s, p);
+                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1}, s, p);
+}
+
+template <int XT> int dispatch_residual(const PairParams &p, cudaStream_t s) {
+    if (p.rt == FM_X_BF16) return dispatch_width<8, XT, FM_X_BF16>(p, s);
+    if (p.rt == FM_X_F16) return dispatch_width<8, XT, FM_X_F16>(p, s);
+    return dispatch_width<8, XT, FM_X_F32>(p, s);
+}
+
+template <int VEC> int dispatch_pair(const PairParams &p, cudaStream_t s) {
+    if constexpr (VEC != 8) {
+        return dispatch_width<VEC, PAIR_ANY, PAIR_ANY>(p, s);
+    } else {
+        if (p.xt == FM_X_BF16) return dispatch_residual<FM_X_BF16>(p, s);
+        if (p.xt == FM_X_F16) return dispatch_residual<FM_X_F16>(p, s);
+        return dispatch_residual<FM_X_F32>(p, s);
+    }
 }
 
 } // namespace
