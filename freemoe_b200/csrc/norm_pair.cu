@@ -27,7 +27,7 @@ struct PairParams {
     int32_t xt, rt, wt, gt, yt;
     PairGate gate_kind;
     uint32_t tokens, d;
-    float scale, res_scale, eps;
+    float scale, res_scale, eps, per_value; // per_value: 1 / d
 };
 
 // h of chunk c: `by` is the factor of the row (its first norm, the scale, its gate).
@@ -72,7 +72,7 @@ template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel
             }
             sum = team_sum<true>(sum, s_part[turn]);
             turn ^= 1u;
-            by *= rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+            by *= rsqrtf(sum * p.per_value + p.eps);
         }
         if (p.gate_kind == GATE_TOKEN) by *= load1(p.gate, p.gt, row * p.gs);
         float root = 0.0f;
@@ -87,7 +87,7 @@ template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel
             }
             sum = team_sum<true>(sum, s_part[turn]);
             turn ^= 1u;
-            root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+            root = rsqrtf(sum * p.per_value + p.eps);
         }
         // whole warps go round together: a scale's 16 lanes exchange inside
         for (uint32_t c0 = threadIdx.x & ~31u; c0 < chunks; c0 += n) {
@@ -107,28 +107,19 @@ template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel
     }
 }
 
-// A chunk as it was loaded: nothing waits for the loads before get().  VEC 8: of a type that is
-// known, in accesses of 16 bytes.  Otherwise of a type at run time (T is PAIR_ANY), in accesses of
-// two values or one, in the first words of their places.
+// A chunk as it was loaded: nothing waits for the loads before get().  VEC 8: accesses of 16
+// bytes, of a type that is known; otherwise (T is PAIR_ANY) of a type at run time, accesses of two
+// values or one in the first words of their places.
 constexpr int PAIR_ANY = -1;
 template <int VEC, int T> struct PairChunk {
     uint32_t w[T == PAIR_ANY || T == FM_X_F32 ? 8 : 4];
     __device__ __forceinline__ void load(const void *p, int32_t t, int64_t row, uint32_t c, uint32_t d) {
         if constexpr (VEC == 8) {
-            constexpr int N = x_size(T) / 2;
-            const uint4 *at = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + (row + c * 8) * x_size(T));
-            uint4 q[N] = {};
-            if (c * 8 < d) {
+            Raw8 q{};
+            if (c * 8 < d) q = raw8_load(p, T, row + c * 8);
+            const uint32_t all[8] = {q.a.x, q.a.y, q.a.z, q.a.w, q.b.x, q.b.y, q.b.z, q.b.w};
 #pragma unroll
-                for (int i = 0; i < N; ++i) q[i] = at[i];
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                w[4 * i] = q[i].x;
-                w[4 * i + 1] = q[i].y;
-                w[4 * i + 2] = q[i].z;
-                w[4 * i + 3] = q[i].w;
-            }
+            for (uint32_t i = 0; i < sizeof(w) / 4; ++i) w[i] = all[i];
         } else {
             const char *base = static_cast<const char *>(p) + row * x_size(t);
 #pragma unroll
@@ -152,8 +143,9 @@ template <int VEC, int T> struct PairChunk {
     }
     __device__ __forceinline__ void get(int32_t t, float (&v)[8]) const {
         if constexpr (VEC == 8) {
-            constexpr int B = T == FM_X_F32 ? 4 : 0; // (raw8_unpack looks at the second four with f32 only)
-            raw8_unpack(Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[B], w[B + 1], w[B + 2], w[B + 3])}, T, v);
+            constexpr int B = sizeof(w) == 32 ? 4 : 0; // (raw8_unpack looks at the second four with f32 only)
+            raw8_unpack(Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[B], w[B + 1], w[B + 2], w[B + 3])},
+                        T, v);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j += VEC) {
@@ -169,14 +161,32 @@ template <int VEC, int T> struct PairChunk {
     }
 };
 
+// The sum over a team, for warps that come in fours (the others' places hold zeros): every thread
+// adds up the partial sums itself.  (By shuffles they are another chain of five.)
+template <bool CTA> __device__ __forceinline__ float pair_sum(float v, float4 *s_part) {
+    v = warp_sum(v);
+    if constexpr (CTA) {
+        if ((threadIdx.x & 31u) == 0) reinterpret_cast<float *>(s_part)[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0f;
+        for (uint32_t i = 0; i * 128 < blockDim.x; ++i) {
+            const float4 q = s_part[i];
+            v += (q.x + q.y) + (q.z + q.w);
+        }
+    }
+    return v;
+}
+
 // A team (see norm_rows.cuh) a row, whose values stay in registers between the two norms;
-// the next row is on its way meanwhile.  The weights wait in shared memory as f32, the first
+// the next row is on its way meanwhile (FULL: and a gate of the row's own).  The weights wait in shared memory as f32, the first
 // one with the scale and a gate by channels in it.
-template <int VEC, int XT, int RT, bool CTA, int ITER, int MOST>
-__global__ void __launch_bounds__(MOST) norm_pair_kernel(const PairParams p) {
+template <int VEC, int XT, int RT, bool FULL, bool CTA, int ITER, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 512 && VEC == 8 && RT != FM_X_F32 ? 2 : 1) norm_pair_kernel(const PairParams p) {
     const uint32_t nt = CTA ? blockDim.x : 32u, teams = CTA ? 1u : blockDim.x / 32;
-    extern __shared__ float4 s_w[]; // chunk c: w1 in s_w[2 c], s_w[2 c + 1], w2 behind all of w1
-    __shared__ float s_part[2][32];
+    // chunk c's first four values of w1 in s_w[c], the others, then w2's, `all` further each: lanes side
+    // by side (with a chunk's eight together LDS takes twice as long, and 8192 x 4096 48 us)
+    extern __shared__ float4 s_w[];
+    __shared__ float4 s_part[2][8];
     const uint32_t c0 = CTA ? threadIdx.x : threadIdx.x % 32, all = nt * ITER;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * teams;
     after_stream();
@@ -202,73 +212,73 @@ __global__ void __launch_bounds__(MOST) norm_pair_kernel(const PairParams p) {
         if (p.gate_kind == GATE_CHANNEL) load_chunk<VEC>(p.gate, p.gt, 0, c, p.d, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] *= p.gate_kind == GATE_CHANNEL ? g[j] * p.scale : p.scale;
-        s_w[2 * c] = make_float4(w[0], w[1], w[2], w[3]);
-        s_w[2 * c + 1] = make_float4(w[4], w[5], w[6], w[7]);
+        s_w[c] = make_float4(w[0], w[1], w[2], w[3]);
+        s_w[all + c] = make_float4(w[4], w[5], w[6], w[7]);
         if (!p.y) continue;
         load_chunk<VEC>(p.w2, p.wt, 0, c, p.d, w);
-        s_w[2 * (all + c)] = make_float4(w[0], w[1], w[2], w[3]);
-        s_w[2 * (all + c) + 1] = make_float4(w[4], w[5], w[6], w[7]);
+        s_w[2 * all + c] = make_float4(w[0], w[1], w[2], w[3]);
+        s_w[3 * all + c] = make_float4(w[4], w[5], w[6], w[7]);
     }
+    if (threadIdx.x < 16) s_part[threadIdx.x / 8][threadIdx.x % 8] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __syncthreads();
     uint32_t turn = 0; // of the two buffers of partial sums: a thread that is ahead by a sum writes the other
     for (; row < p.tokens; row += step) {
         float h[ITER][8];
-        PairChunk<VEC, RT> mine[ITER];
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            x[i].get(p.xt, h[i]);
-            mine[i] = r[i];
+        for (int i = 0; i < ITER; ++i) x[i].get(p.xt, h[i]);
+        PairChunk<VEC, RT> g[FULL ? ITER : 1];
+        if constexpr (FULL) {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) g[i].load(p.gate, p.gt, row * p.gs, c0 + i * nt, p.d);
         }
-        if (row + step < p.tokens) load(row + step);
         float by = 1.0f;
         if (p.w1) {
-            float sum = 0.0f;
+            uint64_t sums = 0;
 #pragma unroll
-            for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-            sum = team_sum<CTA>(sum, s_part[turn]);
+            for (int i = 0; i < ITER; ++i) sums = squares8(h[i], sums);
+            const float sum = pair_sum<CTA>(both(sums), s_part[turn]);
             turn ^= 1u;
-            by = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+            by = rsqrtf(sum * p.per_value + p.eps);
         }
         if (p.gate_kind == GATE_TOKEN) by *= load1(p.gate, p.gt, row * p.gs);
-        float sum = 0.0f;
+        uint64_t sums = 0;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const uint32_t c = c0 + i * nt;
-            const float4 wa = s_w[2 * c], wb = s_w[2 * c + 1];
+            const float4 wa = s_w[c], wb = s_w[all + c];
             const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
             float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * by * w[j];
-            if (p.gate_kind == GATE_FULL) {
+            mul8(h[i], by);
+            mul8(h[i], w);
+            if constexpr (FULL) {
+                g[i].get(p.gt, v);
+                mul8(h[i], v);
+            } else if (p.gate_kind == GATE_FULL) {
                 load_chunk<VEC>(p.gate, p.gt, row * p.gs, c, p.d, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] *= v[j];
+                mul8(h[i], v);
             }
-            mine[i].get(p.rt, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                h[i][j] = fmaf(v[j], p.res_scale, h[i][j]);
-                sum = fmaf(h[i][j], h[i][j], sum);
-            }
+            r[i].get(p.rt, v);
+            add8(h[i], v, p.res_scale);
+            sums = squares8(h[i], sums);
         }
         if (p.res_out) {
 #pragma unroll
             for (int i = 0; i < ITER; ++i)
                 store_chunk<VEC>(p.res_out, RT == PAIR_ANY ? p.rt : RT, row * p.rs, c0 + i * nt, p.d, h[i]);
         }
+        // (right after this row's values were taken the loads cost more than they hide: 8192 x 4096 51 us, 46 here)
+        if (row + step < p.tokens) load(row + step);
         if (!p.y) continue;
-        sum = team_sum<CTA>(sum, s_part[turn]);
+        const float sum = pair_sum<CTA>(both(sums), s_part[turn]);
         turn ^= 1u;
-        const float root = rsqrtf(sum / static_cast<float>(p.d) + p.eps);
+        const float root = rsqrtf(sum * p.per_value + p.eps);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const uint32_t c = c0 + i * nt;
-            const float4 wa = s_w[2 * (all + c)], wb = s_w[2 * (all + c) + 1];
+            const float4 wa = s_w[2 * all + c], wb = s_w[3 * all + c];
             const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * root * w[j];
+            mul8(h[i], root);
+            mul8(h[i], w);
             if (p.yt == FM_X_E4M3)
                 store_e4m3<VEC>(p, row, c, h[i]);
             else if (p.yt == FM_X_F32)
@@ -281,9 +291,9 @@ __global__ void __launch_bounds__(MOST) norm_pair_kernel(const PairParams p) {
     }
 }
 
-template <int VEC, int XT, int RT, bool CTA, int ITER, int MOST>
+template <int VEC, int XT, int RT, bool FULL, bool CTA, int ITER, int MOST>
 int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
-    auto kfn = norm_pair_kernel<VEC, XT, RT, CTA, ITER, MOST>;
+    auto kfn = norm_pair_kernel<VEC, XT, RT, FULL, CTA, ITER, MOST>;
     const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
     const uint32_t smem = (CTA ? threads : 32) * ITER * 64;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
@@ -301,20 +311,28 @@ int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
 // there are rows for half the threads of the GPU only (latency counts then).
-template <int VEC, int XT, int RT> int dispatch_width(const PairParams &p, cudaStream_t s) {
+template <int VEC, int XT, int RT, bool FULL = false> int dispatch_width(const PairParams &p, cudaStream_t s) {
     const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
     const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
-    if (p.d <= 256) return launch_pair<VEC, XT, RT, false, 1, 128>(p, 128, s);
-    if (p.d <= 1024) return launch_pair<VEC, XT, RT, false, 4, 128>(p, 128, s);
-    if (few && one <= 1024) return launch_pair<VEC, XT, RT, true, 1, 1024>(p, one, s);
-    if (two <= 512) return launch_pair<VEC, XT, RT, true, 2, 512>(p, two, s);
-    if (two <= 1024) return launch_pair<VEC, XT, RT, true, 2, 1024>(p, two, s);
+    if (p.d <= 256) return launch_pair<VEC, XT, RT, FULL, false, 1, 128>(p, 128, s);
+    if (p.d <= 1024) return launch_pair<VEC, XT, RT, FULL, false, 4, 128>(p, 128, s);
+    if (few && one <= 1024) return launch_pair<VEC, XT, RT, FULL, true, 1, 1024>(p, one, s);
+    if (two <= 512) return launch_pair<VEC, XT, RT, FULL, true, 2, 512>(p, two, s);
+    if (two <= 1024) return launch_pair<VEC, XT, RT, FULL, true, 2, 1024>(p, two, s);
     const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
     return launch("norm_pair_long_kernel", norm_pair_long_kernel<VEC>,
                   {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1}, s, p);
 }
 
+// A gate of x's shape has loads of its own where it is of the residual's type, 16 bits (8192 x 4096
+// in bf16: 57 us, 65 where they come when they are needed).
 template <int XT> int dispatch_residual(const PairParams &p, cudaStream_t s) {
+    if (p.gate_kind == GATE_FULL && p.gt == p.rt) {
+        if constexpr (XT != FM_X_F16)
+            if (p.rt == FM_X_BF16) return dispatch_width<8, XT, FM_X_BF16, true>(p, s);
+        if constexpr (XT != FM_X_BF16)
+            if (p.rt == FM_X_F16) return dispatch_width<8, XT, FM_X_F16, true>(p, s);
+    }
     if (p.rt == FM_X_BF16) return dispatch_width<8, XT, FM_X_BF16>(p, s);
     if (p.rt == FM_X_F16) return dispatch_width<8, XT, FM_X_F16>(p, s);
     return dispatch_width<8, XT, FM_X_F32>(p, s);
@@ -390,6 +408,7 @@ extern "C" int fmcuda_norm_add_norm(const fmcuda_norm_add_norm_args *a, void *st
     p.scale = a->scale;
     p.res_scale = a->residual_scale;
     p.eps = a->epsilon;
+    p.per_value = 1.0f / static_cast<float>(a->d_model);
     auto fits = [&](int64_t values, uint32_t bytes) {
         auto at = [&](const void *q) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; };
         auto row = [&](int64_t stride) { return a->tokens == 1 || stride % values == 0; };

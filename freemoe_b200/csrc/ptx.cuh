@@ -156,4 +156,34 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// Eight values at a time: a *= b, a *= the factor, a = a + b * the factor, sums of squares.
+__device__ __forceinline__ void mul8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), a[j], a[j + 1]);
+}
+__device__ __forceinline__ void mul8(float (&a)[8], float by) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(by, by)), a[j], a[j + 1]);
+}
+__device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8], float by) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        unpack_f32x2(fma_f32x2(pack_f32x2(b[j], b[j + 1]), pack_f32x2(by, by), pack_f32x2(a[j], a[j + 1])), a[j], a[j + 1]);
+}
+__device__ __forceinline__ uint64_t squares8(const float (&a)[8], uint64_t sums) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t two = pack_f32x2(a[j], a[j + 1]);
+        sums = fma_f32x2(two, two, sums);
+    }
+    return sums;
+}
+__device__ __forceinline__ float both(uint64_t sums) {
+    float a, b;
+    unpack_f32x2(sums, a, b);
+    return a + b;
+}
+
 } // namespace fmb
