@@ -25,6 +25,7 @@ namespace {
 constexpr uint32_t ROPE_THREADS = 256;
 constexpr uint32_t ROPE_MAX_AXES = 8;
 constexpr uint32_t ROPE_MAX_DIM = 1024, ROPE_TURNS = ROPE_MAX_DIM / 2, ROPE_BATCH = 8;
+constexpr uint32_t ROPE_START = 1; // what a CTA costs beside its tokens, in tokens
 
 struct RopeParams {
     const void *q, *k, *v;
@@ -46,8 +47,18 @@ struct RopeParams {
     int64_t axis_stride; // positions from axis to axis
 };
 
+// Where the cosine and sine of pair `pair` stand, `per` pairs an eight: lanes of consecutive eights read
+// two pairs each side by side.  (With an eight's pairs one after the other their 16-byte reads meet in
+// the same banks, four at a time.)
+__host__ __device__ __forceinline__ uint32_t rope_span(uint32_t half, uint32_t per) { return (half + per - 1) / per * per; }
+__device__ __forceinline__ uint32_t rope_place(uint32_t pair, uint32_t per, uint32_t eights) {
+    const uint32_t eight = pair / per, in = pair % per;
+    return in / 2 * (2 * eights) + 2 * eight + in % 2;
+}
+
 // The cosines of the CTA's tokens, and their rows of the cache (-1: a slot below zero or,
-// reported, past the cache); ends with the CTA's barrier.
+// reported, past the cache); ends with the CTA's barrier.  PER: pairs an eight, 0: in order.
+template <uint32_t PER>
 __device__ __forceinline__ void rope_tokens(const RopeParams &p, uint32_t t0, uint32_t n, float2 *s_turns,
                                             int64_t *s_row) {
     const uint32_t half = p.rot / 2;
@@ -65,7 +76,9 @@ __device__ __forceinline__ void rope_tokens(const RopeParams &p, uint32_t t0, ui
                              static_cast<double>(p.inv_freq[i - k * half]) * 0.15915494309189533577; // 1 / (2 pi)
         float sn, cs;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-        s_turns[i] = make_float2(cs * p.factor, sn * p.factor);
+        const uint32_t pair = i - k * half;
+        s_turns[PER ? k * rope_span(half, PER) + rope_place(pair, PER, (half + PER - 1) / PER) : i] =
+            make_float2(cs * p.factor, sn * p.factor);
     }
     if (threadIdx.x < n) {
         int64_t row = -1;
@@ -105,9 +118,11 @@ __device__ __forceinline__ uint4 rope_shuffle(uint4 v, uint32_t lane) {
 // Measured with 8192 tokens of 32 + 8 heads of 128, bf16, interleaved (201 MB, 31 us at the
 // measured copy rate): 37 us; U = 2 or 4, 39; an index over all of a token's eights with its
 // divisions, 44 (issue slots 65% busy); the cosines worked out by every thread for
-// itself, 64.  Bound by the loads under way: registers against warps.  HALVES: 42 us, from
-// f32 to bf16 (302 MB) 65 against 47; it reads twice the cosines for an eight and shuffles,
-// and what bounds it has not been profiled.
+// itself, 64.  Bound by the loads under way: registers against warps (the next token's loads
+// beside this one's, with 64 or 85 registers: 39 to 43).  HALVES: 37 us too, from f32 to bf16
+// (302 MB) 51, heads of 64 25 (101 MB; a third of the places for heads is empty).  Before the
+// cosines lay side by side (rope_place) and before batches left no part of a round idle, both
+// were 42 and 62, with L1 and shared memory 69% busy.
 enum { ROPE_INTER, ROPE_HALVES, ROPE_PAIRED };
 
 template <int LAYOUT, int IN, int OUT>
@@ -116,7 +131,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, LAYOUT == ROPE_PAIRED && IN == F
     constexpr bool INTER = LAYOUT == ROPE_INTER, PAIRED = LAYOUT == ROPE_PAIRED;
     constexpr int PAIRS = INTER ? 4 : 8, U = IN == FM_X_F32 || PAIRED ? 2 : 3;
     constexpr int SI = x_size(IN), SO = x_size(OUT);
-    __shared__ float2 s_turns[ROPE_TURNS];
+    __shared__ __align__(16) float2 s_turns[ROPE_TURNS];
     __shared__ int64_t s_row[ROPE_BATCH];
     const uint32_t t0 = blockIdx.x * p.batch, n = p.tokens - t0 < p.batch ? p.tokens - t0 : p.batch;
     const uint32_t half = p.rot / 2, at_once = blockDim.x / p.head_items; // heads at once
@@ -128,7 +143,9 @@ __global__ void __launch_bounds__(ROPE_THREADS, LAYOUT == ROPE_PAIRED && IN == F
     // HALVES: the lane with the partners, and whether they are the first of their pairs
     const bool second = item * 8 >= half;
     const uint32_t partner = (threadIdx.x & 31u) + (pair ? second ? 0u - half / 8 : half / 8 : 0u);
-    const float2 *my_turns = s_turns + (INTER ? item * 4 : LAYOUT == ROPE_HALVES && second ? ea - half : ea);
+    const uint32_t my_pair = INTER ? item * 4 : LAYOUT == ROPE_HALVES && second ? ea - half : ea;
+    const uint32_t spans = rope_span(half, PAIRS), quarter = 2 * (spans / PAIRS); // from two pairs to the next two
+    const float2 *my_turns = s_turns + 2 * (my_pair / PAIRS);
     after_stream();
     let_next();
     bool ready = false;
@@ -170,7 +187,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, LAYOUT == ROPE_PAIRED && IN == F
             }
         };
         load();
-        if (!ready) rope_tokens(p, t0, n, s_turns, s_row); // every thread's first round: its barrier
+        if (!ready) rope_tokens<PAIRS>(p, t0, n, s_turns, s_row); // every thread's first round: its barrier
         ready = true;
 #pragma unroll 1
         for (uint32_t k = 0; k < n; ++k) {
@@ -178,9 +195,13 @@ __global__ void __launch_bounds__(ROPE_THREADS, LAYOUT == ROPE_PAIRED && IN == F
             const int64_t row = s_row[k];
             float2 cs[PAIRS];
             if (pair) {
+                // (of the last interleaved eight some pairs are not turned, and their places hold anything)
 #pragma unroll
-                for (int j = 0; j < PAIRS; ++j)
-                    if (!INTER || item * 4 + j < half) cs[j] = my_turns[k * half + j];
+                for (int j = 0; j < PAIRS; j += 2) {
+                    const float4 two = *reinterpret_cast<const float4 *>(my_turns + k * spans + j / 2 * quarter);
+                    cs[j] = make_float2(two.x, two.y);
+                    cs[j + 1] = make_float2(two.z, two.w);
+                }
             }
 #pragma unroll
             for (int x = 0; x < U; ++x) {
@@ -254,7 +275,7 @@ template <bool INTER> __global__ void __launch_bounds__(ROPE_THREADS) rope_appen
     const int64_t t = blockIdx.x;
     after_stream();
     let_next();
-    rope_tokens(p, blockIdx.x, 1, s_turns, s_row);
+    rope_tokens<0>(p, blockIdx.x, 1, s_turns, s_row);
     const int64_t cache_row = s_row[0];
     const uint32_t half = p.rot / 2, turned = p.heads + p.kv_heads, head_items = p.dim - half;
     const uint32_t items = turned * head_items + p.kv_heads * p.dim;
@@ -432,12 +453,17 @@ int rope_append(const fmcuda_rope_append_args *a, const uint8_t *axis, uint32_t 
     uint32_t parts = sms / a->tokens;
     parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
     if (vec && a->tokens > sms * 4) {
-        // more than the GPU holds at once: several to a CTA, as many as its threads have
-        // cosines to work out
-        const uint32_t most = half ? ROPE_THREADS / half : ROPE_BATCH;
-        p.batch = (a->tokens + sms * 4 - 1) / (sms * 4);
-        p.batch = p.batch > most ? most : p.batch;
-        p.batch = p.batch < 1 ? 1 : p.batch > ROPE_BATCH ? ROPE_BATCH : p.batch;
+        // more than the GPU holds at once: several to a CTA, as many as their cosines have room for and as
+        // leave the least of the last round idle (four CTAs an SM hold 592 times the batch)
+        const uint32_t span = half ? rope_span(half, a->interleaved ? 4 : 8) : 1, room = ROPE_TURNS / span;
+        uint64_t least = ~0ull;
+        for (uint32_t n = 1; n <= ROPE_BATCH && n <= room; ++n) {
+            const uint64_t ctas = (a->tokens + n - 1) / n, rounds4 = (ctas + sms * 4 - 1) / (sms * 4);
+            if (rounds4 * (n + ROPE_START) <= least) {
+                least = rounds4 * (n + ROPE_START);
+                p.batch = n;
+            }
+        }
     }
     const Launch l{dim3((a->tokens + p.batch - 1) / p.batch, parts), threads, 0, 1};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
