@@ -37,7 +37,7 @@
 namespace fmb {
 namespace {
 
-constexpr uint32_t LP_MAX_TOP = 32, LP_GROUPS = 64, LP_LIST = 1024, LP_MAX_CLUSTER = 8, LP_THREADS = 512;
+constexpr uint32_t LP_MAX_TOP = 32, LP_GROUPS = 64, LP_LIST = 1024, LP_MAX_CLUSTER = 8, LP_THREADS = 512, LP_MANY = 256;
 constexpr float LP_LEAST = -200.0f; // 2^t is 0 from here down; a finite t keeps t 2^t a number
 
 struct LogProbParams {
@@ -83,14 +83,20 @@ struct Chunk {
 };
 __device__ __forceinline__ Chunk load_chunk32(const void *at) {
     Chunk r;
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
                  : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
                    "=r"(r.w[7])
                  : "l"(at));
     return r;
 }
 
-// Values of a 4-byte word; `V` of them.
+// The same for a chunk that is read a second time, of which single values are looked at again: kept in L1.
+__device__ __forceinline__ Chunk load_chunk32_again(const void *at) {
+    const uint4 a = __ldg(static_cast<const uint4 *>(at)), b = __ldg(static_cast<const uint4 *>(at) + 1);
+    return Chunk{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+
+// The two values of a 4-byte word.
 template <int T> __device__ __forceinline__ float2 two_of(uint32_t u) {
     if constexpr (T == FM_X_BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
     return __half22float2(*reinterpret_cast<const __half2 *>(&u));
@@ -310,7 +316,10 @@ struct LPShared {
     uint64_t list[LP_LIST];
     uint64_t first[LP_MAX_TOP]; // the first values of the row, or of the CTA's part of it
     float ref[LP_THREADS / 32], sum[LP_THREADS / 32], tsum[LP_THREADS / 32];
-    float all[3]; // ref, sum, tsum of the CTA
+    // what the cluster's CTAs send to the first one: their first values and their sums
+    uint64_t sent[LP_MAX_CLUSTER][LP_MAX_TOP];
+    uint32_t before[LP_MAX_CLUSTER][LP_MAX_TOP];
+    float sent_sums[3][LP_MAX_CLUSTER];
     uint32_t n, singles, columns;
     uint32_t single[LP_THREADS];  // chunks that are read again
     uint16_t column[LP_THREADS];  // threads whose chunks are all read again
@@ -327,14 +336,46 @@ __device__ __forceinline__ void rank_keys(const uint64_t *keys, uint32_t n, uint
     }
 }
 
+// The k first of the keys that the cluster's CTAs have sent, 32 places each, each in order (0: no more):
+// a key's place is its own in its list and what comes before it in the others.  A warp takes a list,
+// or half of what it is compared with, a lane a key.
+__device__ __forceinline__ void merge_lists(LPShared &s, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 31u, warps = blockDim.x / 32;
+    for (uint32_t w = threadIdx.x >> 5; w < 2 * LP_MAX_CLUSTER; w += warps) {
+        const uint32_t mine = w / 2;
+        const uint64_t key = s.sent[mine][lane];
+        if (!__any_sync(0xFFFFFFFFu, key != 0)) continue;
+        uint32_t before = w % 2 ? 0 : lane;
+#pragma unroll
+        for (uint32_t x = 0; x < LP_MAX_CLUSTER / 2; ++x) {
+            const uint32_t l = w % 2 * (LP_MAX_CLUSTER / 2) + x;
+            uint32_t n = 0; // of list l that come before; lists are no longer than 31 or full
+#pragma unroll
+            for (uint32_t step = 16; step > 0; step >>= 1)
+                if (s.sent[l][n + step - 1] > key) n += step;
+            n += s.sent[l][n] > key;
+            before += l == mine ? 0 : n;
+        }
+        if (key && before) atomicAdd(&s.before[mine][lane], before);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < LP_MAX_CLUSTER * 32; i += blockDim.x) {
+        const uint64_t key = s.sent[i / 32][i % 32];
+        const uint32_t at = s.before[i / 32][i % 32];
+        if (key && at < k) s.first[at] = key;
+    }
+    __syncthreads();
+}
+
 // The k first values of the CTA's part of a row, to s.first; `mine` is the key of the thread's
-// best chunk, and groups of `lanes` threads have put theirs to s.groups.
+// best chunk, and groups of 2^lanes_log2 threads have put theirs to s.groups.
 template <int T>
 __device__ __forceinline__ void select_top(const Row<T> &row, const Stream<T> &stream, uint64_t mine, uint64_t group,
-                                           uint32_t lanes, uint32_t k, uint32_t rank, uint32_t threads, LPShared &s) {
+                                           uint32_t lanes_log2, uint32_t k, uint32_t rank, uint32_t threads, LPShared &s) {
     constexpr uint32_t V = LP_VEC<T>;
     // the group that k - 1 others come before: its threads share the count
-    const uint32_t groups = blockDim.x / lanes, part = groups / lanes, from = threadIdx.x % lanes * part;
+    const uint32_t lanes = 1u << lanes_log2, part = blockDim.x >> (2 * lanes_log2);
+    const uint32_t from = (threadIdx.x & (lanes - 1)) * part;
     uint32_t before = 0;
 #pragma unroll 8
     for (uint32_t j = 0; j < part; ++j) before += s.groups[from + j] > group;
@@ -351,7 +392,8 @@ __device__ __forceinline__ void select_top(const Row<T> &row, const Stream<T> &s
             s.column[atomicAdd(&s.columns, 1u)] = static_cast<uint16_t>(threadIdx.x);
     }
     __syncthreads();
-    const uint32_t per = (row.whole + 2 + threads - 1) / threads, singles = s.singles, all = singles + s.columns * per;
+    const uint32_t singles = s.singles, columns = s.columns;
+    const uint32_t per = columns ? (row.whole + 2 + threads - 1) / threads : 1, all = singles + columns * per;
     // every value that does not come behind the bound, NaN too
     auto visit = [&](auto &&take) {
         for (uint32_t w = threadIdx.x; w < all; w += blockDim.x) {
@@ -364,7 +406,7 @@ __device__ __forceinline__ void select_top(const Row<T> &row, const Stream<T> &s
             }
             const uint32_t n = row.size_of(chunk), first = row.first_of(chunk);
             float v[V];
-            unpack<T>(chunk - 1 < row.whole ? load_chunk32(row.whole_at(chunk - 1)) : row.end(chunk), v);
+            unpack<T>(chunk - 1 < row.whole ? load_chunk32_again(row.whole_at(chunk - 1)) : row.end(chunk), v);
             const bool ties = chunk <= bound_chunk;
             uint32_t in = 0;
 #pragma unroll
@@ -420,7 +462,7 @@ __device__ __forceinline__ double log_of(float sum) {
 // do, 64 warps an SM are worth more than that (4096 rows of 128256 in bf16: 192 us with a chunk
 // a thread on its way and 32 registers, 200 with 40, 203 to 211 with two and 64).
 template <int T, bool FEW>
-__global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const LogProbParams p, uint32_t ranks) {
+__global__ void __launch_bounds__(FEW ? LP_THREADS : LP_MANY, FEW ? 2 : 8) logprobs_kernel(const LogProbParams p, uint32_t ranks) {
     __shared__ LPShared s;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
     const uint32_t rank = blockIdx.x % ranks, threads = blockDim.x * ranks;
@@ -430,16 +472,18 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
         s.n = s.singles = s.columns = 0;
     }
     if (threadIdx.x < LP_MAX_TOP) s.first[threadIdx.x] = 0;
+    if (ranks > 1) {
+        for (uint32_t i = threadIdx.x; i < LP_MAX_CLUSTER * LP_MAX_TOP; i += blockDim.x) {
+            s.sent[i / LP_MAX_TOP][i % LP_MAX_TOP] = 0;
+            s.before[i / LP_MAX_TOP][i % LP_MAX_TOP] = 0;
+        }
+        cluster_arrive();
+    }
     after_stream();
     let_next();
     const Row<T> row(p, r);
     const uint32_t me = rank * blockDim.x + threadIdx.x;
-    float given = 0.0f;
-    int32_t token = -1;
-    if (me == 0) {
-        token = p.tokens[r];
-        if (token >= 0 && static_cast<uint32_t>(token) < row.vocab) given = load1(row.at, T, static_cast<uint32_t>(token));
-    }
+    const int32_t token = me == 0 ? __ldg(p.tokens + r) : -1;
     // chunk 0 may be empty, and so may the last
     const uint32_t first = me || row.head ? me : threads, last = row.whole + (row.tail ? 1 : 0);
     Stream<T> stream(p, first <= last ? first : 0xFFFFFFFFu);
@@ -456,18 +500,36 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
         from += threads * 32ull;
         return x;
     };
-    constexpr int U = FEW ? 4 : 1;
-    for (; chunk < total; chunk += U * threads) {
-        Chunk x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load(chunk + u * threads);
-#pragma unroll
-        for (int u = 0; u < U; ++u) stream.add(p, x[u], chunk + u * threads + lane);
+    if constexpr (FEW) {
+        // two are added while the next two are on their way
+        Chunk x[2], y[2];
+        x[0] = load(chunk);
+        x[1] = load(chunk + threads);
+#pragma unroll 1
+        for (; chunk < total; chunk += 2 * threads) {
+            y[0] = load(chunk + 2 * threads);
+            y[1] = load(chunk + 3 * threads);
+            stream.add(p, x[0], chunk + lane);
+            stream.add(p, x[1], chunk + threads + lane);
+            x[0] = y[0];
+            x[1] = y[1];
+        }
+    } else {
+#pragma unroll 1
+        for (; chunk < total; chunk += threads) {
+            Chunk x = load(chunk);
+            stream.add(p, x, chunk + lane);
+        }
     }
 
+    // the best chunk, which may be read again, on its way to L1
+    if (FEW && p.top && stream.chunk - 1 < row.whole)
+        asm volatile("prefetch.global.L1 [%0];\n" ::"l"(row.whole_at(stream.chunk - 1)));
+    const bool known = static_cast<uint32_t>(token) < row.vocab; // (of the row's first thread)
+    const float given = known ? load1(row.at, T, static_cast<uint32_t>(token)) : 0.0f;
     Sums all = stream.sums();
     // threads a group, and the group's best chunk
-    const uint32_t lanes = blockDim.x > LP_GROUPS ? blockDim.x / LP_GROUPS : 1;
+    const uint32_t lanes_log2 = blockDim.x > LP_GROUPS ? 31 - __clz(blockDim.x / LP_GROUPS) : 0, lanes = 1u << lanes_log2;
     uint64_t mine = 0, group = 0;
     if (p.top) {
         group = mine = stream.chunk == 0xFFFFFFFFu ? 0 : key_of(code_of(stream.best), stream.chunk);
@@ -475,7 +537,7 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
             const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, group, o);
             group = other > group ? other : group;
         }
-        if (threadIdx.x % lanes == 0) s.groups[threadIdx.x / lanes] = group;
+        if ((threadIdx.x & (lanes - 1)) == 0) s.groups[threadIdx.x >> lanes_log2] = group;
     }
     all.move(warp_max(all.ref), p.c);
     all.sum = warp_sum(all.sum);
@@ -486,7 +548,7 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
         s.tsum[warp] = all.tsum;
     }
     __syncthreads();
-    if (p.top) select_top<T>(row, stream, mine, group, lanes, p.top, rank, threads, s);
+    if (p.top) select_top<T>(row, stream, mine, group, lanes_log2, p.top, rank, threads, s);
     if (ranks == 1 && warp) return;
     if (warp == 0) {
         const bool in = lane < warps;
@@ -496,31 +558,28 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
         all.move(warp_max(all.ref), p.c);
         all.sum = warp_sum(all.sum);
         all.tsum = warp_sum(all.tsum);
-        if (ranks > 1 && lane == 0) {
-            s.all[0] = all.ref;
-            s.all[1] = all.sum;
-            s.all[2] = all.tsum;
-        }
     }
     if (ranks > 1) {
-        cluster_sync();
-        if (rank == 0) {
-            for (uint32_t w = threadIdx.x; w < ranks * p.top; w += blockDim.x)
-                s.list[w] = cluster_load64(smem_u32(&s.first[w % p.top]), w / p.top);
-            if (warp == 0) {
-                const bool in = lane < ranks;
-                all.ref = in ? cluster_load(smem_u32(&s.all[0]), lane) : -FLT_MAX;
-                all.sum = in ? cluster_load(smem_u32(&s.all[1]), lane) : 0.0f;
-                all.tsum = in ? cluster_load(smem_u32(&s.all[2]), lane) : 0.0f;
-                all.move(warp_max(all.ref), p.c);
-                all.sum = warp_sum(all.sum);
-                all.tsum = warp_sum(all.tsum);
-            }
+        cluster_wait(); // all CTAs have begun, and the first one has cleared what they send to
+        if (threadIdx.x < p.top) cluster_store(smem_u32(&s.sent[rank][threadIdx.x]), 0, s.first[threadIdx.x]);
+        if (threadIdx.x == 0) {
+            cluster_store(smem_u32(&s.sent_sums[0][rank]), 0, all.ref);
+            cluster_store(smem_u32(&s.sent_sums[1][rank]), 0, all.sum);
+            cluster_store(smem_u32(&s.sent_sums[2][rank]), 0, all.tsum);
         }
-        cluster_sync(); // nobody leaves, and nothing of rank 0's is overwritten, while it is read
+        cluster_arrive();
+        cluster_wait();
         if (rank != 0) return;
-        rank_keys(s.list, ranks * p.top, p.top, s.first);
-        __syncthreads();
+        if (warp == 0) {
+            const bool in = lane < ranks;
+            all.ref = in ? s.sent_sums[0][lane] : -FLT_MAX;
+            all.sum = in ? s.sent_sums[1][lane] : 0.0f;
+            all.tsum = in ? s.sent_sums[2][lane] : 0.0f;
+            all.move(warp_max(all.ref), p.c);
+            all.sum = warp_sum(all.sum);
+            all.tsum = warp_sum(all.tsum);
+        }
+        if (p.top) merge_lists(s, p.top);
         if (warp) return;
     }
     // sum 0: a row of nothing but -inf
@@ -529,7 +588,7 @@ __global__ void __launch_bounds__(LP_THREADS, FEW ? 2 : 4) logprobs_kernel(const
         return all.sum == 0.0f ? -INFINITY : static_cast<float>(p.scale * (static_cast<double>(x) - all.ref) - log_sum);
     };
     if (lane == 0) {
-        if (token >= 0 && static_cast<uint32_t>(token) >= row.vocab) {
+        if (token >= 0 && !known) {
             raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
             p.logprobs[r] = NAN;
         } else {
@@ -598,7 +657,7 @@ extern "C" int fmcuda_token_logprobs(const fmcuda_token_logprobs_args *a, void *
     uint32_t ranks = 1, threads = 32;
     while (ranks < LP_MAX_CLUSTER && a->tokens * ranks * 2 <= sms && chunks >= ranks * 1024ull) ranks *= 2;
     auto few = [&](uint32_t n) { return static_cast<uint64_t>(a->tokens) * ranks * n <= sms * 1024; };
-    while ((threads < 256 && chunks > static_cast<uint64_t>(threads) * ranks * 4) ||
+    while ((threads < LP_MANY && chunks > static_cast<uint64_t>(threads) * ranks * 4) ||
            (threads < LP_THREADS && chunks > static_cast<uint64_t>(threads) * ranks && few(2 * threads)))
         threads *= 2;
     const Launch l{dim3(a->tokens * ranks), threads, 0, ranks};

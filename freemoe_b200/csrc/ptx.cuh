@@ -114,12 +114,20 @@ __device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-__device__ __forceinline__ uint64_t cluster_load64(uint32_t addr, uint32_t rank) {
+// The two halves of cluster_sync.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+// Stores to CTA `rank`'s shared memory; all CTAs of the cluster must be known to run.
+__device__ __forceinline__ uint32_t cluster_at(uint32_t addr, uint32_t rank) {
     uint32_t at;
-    uint64_t v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(at) : "memory");
-    return v;
+    return at;
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(cluster_at(addr, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(cluster_at(addr, rank)), "f"(v) : "memory");
 }
 
 // ---- arithmetic ---------------------------------------------------------------
