@@ -5,6 +5,9 @@
     y  = h + experts(norm(h))            add_rms_norm (adds the attention's output to the
                                          residual stream), router, moe_block / moe_prefill
 
+By its configuration the layer also has norms behind its blocks (norm_add_norm), positions of
+several axes, a window with first keys that stay visible (the pages between are freed), and an
+output head whose rows are scored (token_logprobs).
 A prompt goes through in chunks of any length, then token by token; the calls are the
 same.  Run as a program it takes prompts of ragged lengths through a layer in one chunk
 and in several, and prints how far the two are apart and what a decoding step costs:
@@ -39,6 +42,11 @@ class Config:
     rope_base: float = 10000.0
     epsilon: float = 1e-5
     window: int = 0
+    sinks: int = 0            # first keys that stay visible behind the window
+    sections: tuple = ()      # rotated pairs of each axis, where positions have several
+    block_norms: bool = False # norms behind the blocks too, with a gate by channels
+    block_scale: float = 1.0  # of a block's normed output
+    vocab: int = 0            # rows of an output head
 
 
 @dataclass
@@ -60,8 +68,12 @@ class Layer:
             parts = [hotpath.synth_weights(TYPE_Q4_K, rows, cols, seed + 100 + 3 * e + i, 0.05)
                      for i, (rows, cols) in enumerate(((c.ffn, c.d_model), (c.ffn, c.d_model), (c.d_model, c.ffn)))]
             layer.experts.append(torch.cat(parts))
-        layer.weights["norm_attention"] = torch.ones(c.d_model, device="cuda")
-        layer.weights["norm_experts"] = torch.ones(c.d_model, device="cuda")
+        for name in ("norm_attention", "norm_experts", "norm_head", "behind_attention", "behind_experts", "gate_attention",
+                     "gate_experts"):
+            layer.weights[name] = torch.ones(c.d_model, device="cuda")
+        if c.vocab:
+            head = hotpath.synth_weights(TYPE_Q8_0, c.vocab, c.d_model, seed + 50, 0.05)
+            layer.weights["head"] = (TYPE_Q8_0, head, c.vocab, c.d_model)
         return layer
 
     def product(self, name: str, x: torch.Tensor) -> torch.Tensor:
@@ -80,6 +92,16 @@ class Cache:
         self.table = torch.full((sequences, -(-max_len // c.page_size)), -1, dtype=torch.int32)
         self.lens = [0] * sequences
         self.free = list(range(pages))[::-1]
+        self.window, self.sinks, self.n_axes = c.window, c.sinks, len(c.sections)
+
+    def axes(self, positions: torch.Tensor) -> torch.Tensor:
+        """With several axes: every other 16 tokens are an image's, four to a row of it."""
+        if not self.n_axes:
+            return positions
+        image, inside = positions // 16 % 2 == 1, positions % 16
+        start = positions - inside
+        return torch.stack([torch.where(image, start + d, positions) for d in
+                            (0 * inside, inside // 4, inside % 4)[:self.n_axes]]).contiguous()
 
     def extend(self, new_tokens: list[int]):
         """Room for each sequence's new tokens; what the layer's calls need to know of them."""
@@ -91,10 +113,17 @@ class Cache:
                     self.table[b, page] = self.free.pop()
                 positions.append(p)
                 slots.append(int(self.table[b, page]) * self.page_size + row)
+            if self.window and self.sinks:
+                # what no row from here on sees is freed: behind the first keys, before the windows
+                gone = max(0, self.lens[b] - self.window + 1) // self.page_size
+                for i in range(-(-self.sinks // self.page_size), gone):
+                    if self.table[b, i] >= 0:
+                        self.free.append(int(self.table[b, i]))
+                        self.table[b, i] = -1
             self.lens[b] += n
             starts.append(starts[-1] + n)
         return {
-            "positions": torch.tensor(positions, dtype=torch.int32).cuda(),
+            "positions": self.axes(torch.tensor(positions, dtype=torch.int32).cuda()),
             "slots": torch.tensor(slots, dtype=torch.int64).cuda(),
             "page_table": self.table.cuda(),
             "q_start": torch.tensor(starts, dtype=torch.int32).cuda(),
@@ -111,16 +140,33 @@ def decoder_layer(layer: Layer, cache: Cache, x: torch.Tensor, step: dict, inv_f
     normed, _ = attention.add_rms_norm(x, w["norm_attention"], epsilon=c.epsilon)
     qkv = layer.product("qkv", normed).view(tokens, c.heads + 2 * c.kv_heads, c.head_dim)
     q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), dim=1)
+    axes = attention.rope_axes(c.sections) if c.sections else None
     q = attention.rope_append(q, k, v, step["positions"], inv_freq, cache.k, cache.v, step["slots"],
-                              attention_factor=attention_factor)
+                              attention_factor=attention_factor, axes=axes)
     o = attention.paged_attention(q, cache.k, cache.v, step["page_table"], step["q_start"], step["kv_len"],
-                                  max_q_len=step["max_q_len"], max_kv_len=step["max_kv_len"], window=c.window)
+                                  max_q_len=step["max_q_len"], max_kv_len=step["max_kv_len"], window=c.window,
+                                  sinks=c.sinks)
     o = layer.product("out", o.view(tokens, -1))
-    normed, h = attention.add_rms_norm(o, w["norm_experts"], residual=x, epsilon=c.epsilon, out_dtype=torch.bfloat16)
+    if c.block_norms:
+        normed, h = attention.norm_add_norm(o, w["behind_attention"], x, w["norm_experts"], gate=w["gate_attention"],
+                                            scale=c.block_scale, epsilon=c.epsilon, out_dtype=torch.bfloat16)
+    else:
+        normed, h = attention.add_rms_norm(o, w["norm_experts"], residual=x, epsilon=c.epsilon, out_dtype=torch.bfloat16)
     experts = hotpath.moe_block if tokens <= 64 else hotpath.moe_prefill
     y, ids, _ = experts(normed, layer.product("router", normed), layer.experts, top_k=c.top_k, ffn=c.ffn,
                         gate_type=TYPE_Q4_K, return_routing=True)
+    if c.block_norms:
+        _, out = attention.norm_add_norm(y, w["behind_experts"], h, None, gate=w["gate_experts"], scale=c.block_scale,
+                                         epsilon=c.epsilon)
+        return out, ids
     return (h.float() + y).to(torch.bfloat16), ids
+
+
+def score(layer: Layer, x: torch.Tensor, following: torch.Tensor, top: int = 5):
+    """The log probabilities of the tokens that follow the rows of the stream ``x``, the entropy, and the most
+    probable tokens."""
+    normed, _ = attention.add_rms_norm(x, layer.weights["norm_head"], epsilon=layer.config.epsilon)
+    return hotpath.token_logprobs(layer.product("head", normed), following, top=top)
 
 
 def run(config: Config, lens: list[int], steps: int = 4, chunk: int | None = None, seed: int = 0):
@@ -175,6 +221,12 @@ def main() -> None:
     end.record()
     torch.cuda.synchronize()
     print(f"a decoding step of 64 sequences behind 1000 keys: {begin.elapsed_time(end) / 20 * 1e3:.0f} us")
+    config = Config(window=100, sinks=8, sections=(8, 12, 12), block_norms=True, block_scale=0.5, vocab=32000)
+    (whole, _), layer = run(config, lens), Layer.synthetic(config)
+    following = torch.zeros(whole[0].shape[0], dtype=torch.int32, device="cuda")
+    logprobs, entropy, _, _ = score(layer, whole[0], following)
+    print(f"with norms behind the blocks, three axes and a window with first keys: mean log probability of a fixed token "
+          f"{float(logprobs.mean()):.2f}, mean entropy {float(entropy.mean()):.2f}")
 
 
 if __name__ == "__main__":
