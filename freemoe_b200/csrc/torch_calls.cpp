@@ -7,6 +7,8 @@
 // device), allocate the outputs on the current stream, and call the C entries,
 // whose addresses the Python package hands over (bind), so that there is one
 // library and one set of kernels.  Refusals are raised as the package's FmError.
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -77,6 +79,17 @@ struct Here {
     void *stream() const { return c10::cuda::getCurrentCUDAStream(device).stream(); }
 };
 
+// Outputs and workspaces on the current device, where the calls are (Here): from its allocator
+// directly, 0.4 us each and not 0.75 as by way of the dispatcher.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+    return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(),
+                                     c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+Tensor fresh_like(const Tensor &t) { // in memory too
+    return at::detail::empty_strided_generic(t.sizes(), t.strides(), c10::cuda::CUDACachingAllocator::get(),
+                                             c10::DispatchKeySet(c10::DispatchKey::CUDA), t.scalar_type());
+}
+
 void *at_of(const MaybeTensor &t) { return t ? t->data_ptr() : nullptr; }
 
 bool dense(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1; }
@@ -91,7 +104,7 @@ Tensor run_norm(const Tensor &x, const Tensor &weight, const MaybeTensor &residu
     fmcuda_rms_norm_args a{};
     if (residual) {
         // like the residual in memory too: the C entry takes one stride for both
-        h = at::empty_strided(residual->sizes(), residual->strides(), residual->options());
+        h = fresh_like(*residual);
         a.residual = residual->data_ptr();
         a.residual_out = h.data_ptr();
         a.residual_stride = residual->stride(0);
@@ -121,7 +134,7 @@ std::tuple<Tensor, MaybeTensor> add_rms_norm(const Tensor &x, const Tensor &weig
                                              double epsilon, std::optional<at::ScalarType> out_dtype) {
     need_rows(x);
     const Here here(x);
-    const Tensor y = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+    const Tensor y = fresh(x.sizes(), out_dtype.value_or(x.scalar_type()));
     const Tensor h = run_norm(x, weight, residual, epsilon, y, dtype_of(y), nullptr, here);
     return {y, residual ? MaybeTensor(h) : std::nullopt};
 }
@@ -130,8 +143,8 @@ std::tuple<Tensor, Tensor, MaybeTensor> add_rms_norm_fp8(const Tensor &x, const 
                                                          const MaybeTensor &residual, double epsilon) {
     need_rows(x);
     const Here here(x);
-    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-    const Tensor scales = at::empty({x.size(0), (x.size(1) + 127) / 128}, x.options().dtype(at::kFloat));
+    const Tensor codes = fresh(x.sizes(), at::kFloat8_e4m3fn);
+    const Tensor scales = fresh({x.size(0), (x.size(1) + 127) / 128}, at::kFloat);
     const Tensor h =
         run_norm(x, weight, residual, epsilon, codes, FM_X_E4M3, static_cast<float *>(scales.data_ptr()), here);
     return {codes, scales, residual ? MaybeTensor(h) : std::nullopt};
@@ -149,7 +162,7 @@ Tensor run_norm_pair(const Tensor &x, const MaybeTensor &post_weight, const Tens
          "the two weights have one type", FM_STATUS_INVALID_ARGUMENT);
     need(dense(x) && dense(residual), "norm inputs must be contiguous in their rows");
     // like the residual in memory too: the C entry takes one stride for both
-    const Tensor h = at::empty_strided(residual.sizes(), residual.strides(), residual.options());
+    const Tensor h = fresh_like(residual);
     fmcuda_norm_add_norm_args a{};
     if (gate) {
         const int64_t rows = gate->dim() == 2 ? gate->size(0) : 1;
@@ -192,7 +205,7 @@ std::tuple<MaybeTensor, Tensor> norm_add_norm(const Tensor &x, const MaybeTensor
     need_rows(x);
     const Here here(x);
     MaybeTensor y;
-    if (pre_weight) y = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+    if (pre_weight) y = fresh(x.sizes(), out_dtype.value_or(x.scalar_type()));
     const Tensor h =
         run_norm_pair(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon, y, nullptr, here);
     return {y, h};
@@ -204,8 +217,8 @@ std::tuple<Tensor, Tensor, Tensor> norm_add_norm_fp8(const Tensor &x, const Mayb
                                                      double epsilon) {
     need_rows(x);
     const Here here(x);
-    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-    const Tensor scales = at::empty({x.size(0), (x.size(1) + 127) / 128}, x.options().dtype(at::kFloat));
+    const Tensor codes = fresh(x.sizes(), at::kFloat8_e4m3fn);
+    const Tensor scales = fresh({x.size(0), (x.size(1) + 127) / 128}, at::kFloat);
     const Tensor h = run_norm_pair(x, post_weight, residual, pre_weight, gate, scale, residual_scale, epsilon, codes,
                                    static_cast<float *>(scales.data_ptr()), here);
     return {codes, scales, h};
@@ -266,7 +279,7 @@ Tensor rope_append(const Tensor &q, const MaybeTensor &k, const MaybeTensor &v, 
         a.n_pages = static_cast<uint32_t>(k_cache->size(0));
         a.page_size = static_cast<uint32_t>(k_cache->size(2));
     }
-    const Tensor out = at::empty(q.sizes(), q.options().dtype(kind));
+    const Tensor out = fresh(q.sizes(), kind);
     a.q = q.data_ptr();
     a.q_out = out.data_ptr();
     a.positions = static_cast<const int32_t *>(positions.data_ptr());
@@ -317,11 +330,11 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     need(page_table.size(1) * k_cache.size(2) >= max_kv_len, "page table is shorter than max_kv_len");
     need(q.stride(2) == 1 && k_cache.stride(3) == 1 && (page_table.size(1) <= 1 || page_table.stride(1) == 1),
          "q, caches and page_table must be contiguous in their last dimension");
-    const Tensor out = at::empty(q.sizes(), q.options());
+    const Tensor out = fresh(q.sizes(), q.scalar_type());
     Tensor lse;
     fmcuda_paged_attention_args a{};
     if (return_lse) {
-        lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+        lse = fresh({q.size(0), q.size(1)}, at::kFloat);
         a.lse = static_cast<float *>(lse.data_ptr());
     }
     a.q = q.data_ptr();
@@ -359,7 +372,7 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     if (!workspace) {
         check(entries.attention_bytes(&a, kept, &bytes));
         if (bytes) {
-            own = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+            own = fresh({static_cast<int64_t>(bytes)}, at::kByte);
             at = own.data_ptr();
         }
     }
@@ -378,9 +391,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, 
     need(dense(logits), "logits must be contiguous in their rows");
     need(top >= 0 && top <= logits.size(1), "top must not be negative or above the vocabulary",
          FM_STATUS_INVALID_ARGUMENT);
-    const auto f32 = logits.options().dtype(at::kFloat);
-    const Tensor chosen = at::empty({rows}, f32), entropy = at::empty({rows}, f32), best = at::empty({rows, top}, f32);
-    const Tensor ids = at::empty({rows, top}, logits.options().dtype(at::kInt));
+    const Tensor chosen = fresh({rows}, at::kFloat), entropy = fresh({rows}, at::kFloat);
+    const Tensor best = fresh({rows, top}, at::kFloat), ids = fresh({rows, top}, at::kInt);
     fmcuda_token_logprobs_args a{};
     a.logits = logits.data_ptr();
     a.token = static_cast<const int32_t *>(tokens.data_ptr());
