@@ -102,13 +102,7 @@ __device__ __forceinline__ void store_e4m3(const P &p, uint64_t row, uint32_t c,
     const float divisor = finite ? scale : 0.0f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(scale));
-    // two at a time; the same roundings
-    float z[8];
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const uint64_t x = pack_f32x2(v[j], v[j + 1]), inv2 = pack_f32x2(inv, inv), q = mul_f32x2(x, inv2);
-        unpack_f32x2(fma_f32x2(fma_f32x2(q, pack_f32x2(-divisor, -divisor), x), inv2, q), z[j], z[j + 1]);
-    }
+    auto code = [&](float x) { return quotient(x, divisor, inv); };
     uint8_t *y = static_cast<uint8_t *>(p.y) + row * p.ys;
     const uint32_t groups = (p.d + 127) / 128;
     if ((c & 15u) == 0 && (c >> 4) < groups) p.scales[row * groups + (c >> 4)] = scale;
@@ -117,13 +111,13 @@ __device__ __forceinline__ void store_e4m3(const P &p, uint64_t row, uint32_t c,
             uint32_t w[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                w[i] = e4m3x2(z[4 * i], z[4 * i + 1]) | e4m3x2(z[4 * i + 2], z[4 * i + 3]) << 16;
+                w[i] = e4m3x2(code(v[4 * i]), code(v[4 * i + 1])) | e4m3x2(code(v[4 * i + 2]), code(v[4 * i + 3])) << 16;
             *reinterpret_cast<uint2 *>(y + c * 8) = make_uint2(w[0], w[1]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const uint32_t e = value_at<VEC>(c, j), two = e4m3x2(z[j], z[j + 1]);
+            const uint32_t e = value_at<VEC>(c, j), two = e4m3x2(code(v[j]), code(v[j + 1]));
             if constexpr (VEC == 2) {
                 if (e < p.d) *reinterpret_cast<uint16_t *>(y + e) = static_cast<uint16_t>(two);
             } else {
