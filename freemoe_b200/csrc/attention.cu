@@ -91,6 +91,13 @@ AttnPlan attn_plan(const fmcuda_paged_attention_args &a, uint32_t sinks) {
         n.deal = items < static_cast<uint64_t>(sms) * (prompt ? 1 : DEAL_ITEMS) && n.pairs <= AP_MAX_PAIRS &&
                  keys_seen(a, sinks, AP_PAIR) > AP_KEYS * WHOLE_BLOCKS;
         n.ctas = !n.deal && items < sms ? static_cast<uint32_t>(items) : sms;
+        // with first keys single tiles may be items, on the SMs that sequences of few rows leave: a CTA
+        // a unit, or all (39 decoding sequences beside a chunk of 56 items 38 us, with 112 of single tiles 47)
+        const uint64_t beside = !n.rows ? 0 : n.cluster || n.units ? static_cast<uint64_t>(a.seqs) * a.kv_heads : sms;
+        if (sinks && !n.deal && beside < sms) {
+            n.singles = static_cast<uint32_t>(items * 2 < sms - beside ? items * 2 : sms - beside);
+            n.ctas = n.ctas > n.singles ? n.ctas : n.singles;
+        }
         if (n.deal) {
             n.ppart = take(static_cast<uint64_t>(n.ctas) * 2 * AP_PAIR * n.dp * 4);
             n.ppart_ml = take(static_cast<uint64_t>(n.ctas) * 2 * AP_PAIR * 8);

@@ -23,6 +23,7 @@ struct AttnPlan {
     uint32_t tiles;          // row tiles of a unit's sequence and head, at most
     bool deal;               // prompt kernel: blocks are dealt out, not items
     uint32_t pairs, ctas;    // its pairs of tiles (a bound), and its grid
+    uint32_t singles;        // CTAs that may take single tiles
     uint64_t prefix, part, part_ml, tail_rows, ppart, ppart_ml, tail, total; // workspace offsets
 };
 
@@ -88,6 +89,7 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
         pp.part_ml = reinterpret_cast<float2 *>(ws + n.ppart_ml);
         pp.tail = reinterpret_cast<int4 *>(ws + n.tail);
         pp.ctas = n.ctas;
+        pp.singles = n.singles;
         pp.rows_form = n.cluster ? AR_CLUSTER : n.units ? AR_UNIT : AR_RANGES;
         pp.rows_tiles = n.tiles;
         pp.rows_warps = unit_warps;

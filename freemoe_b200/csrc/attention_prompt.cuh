@@ -34,6 +34,10 @@
 // sequence are zeroed after the copy: their weights are zero, but what lies
 // there may be NaN.
 //
+// SINKS: where there are CTAs (pp.singles) for twice the items, whole ones are single tiles: a CTA's other tile
+// is empty, and its one tile does not wait for turns (a chunk of 510 rows, 28 heads on 4 key heads of
+// 64, window 1000 and 130 first keys, beside 7 decoding sequences 26 us, with pairs 31).
+//
 // SINKS: the first p.sinks keys stay visible behind the window.  A pair's blocks are then
 // counted without the gap between those of the first keys and those of its windows (`skip`
 // blocks from block `first` on), and a tile takes the ones before fe and those of [tb, te).
@@ -89,6 +93,7 @@ struct APParams {
     bool wide;         // rows of out lie and end on 32 bytes
     bool deal;         // blocks are dealt out, not items
     uint32_t max_pairs;
+    uint32_t singles;  // SINKS: CTAs that may take single tiles for items
     uint32_t ctas;     // CTAs of the prompt kernel; the others of attn_beside_kernel take few-row sequences
     ARForm rows_form;  // and how: a CTA a unit, a warp a unit, or even ranges
     uint32_t rows_tiles, rows_warps; // row tiles a unit's sequence and head; warps that a unit each takes
@@ -257,6 +262,7 @@ struct APWalk {
     uint64_t left;               // cost left; or items in all
     uint32_t round;              // dealt items
     uint32_t piece;              // blocks of a piece where each CTA has one piece of one item; else 0
+    bool single;                 // SINKS: items are single tiles
 };
 struct APSeg {
     AttnSeq s;
@@ -289,7 +295,9 @@ template <bool SINKS> __device__ __forceinline__ bool ap_next(const APParams &pp
                               (w.round & 1u ? pp.ctas - 1 - blockIdx.x : blockIdx.x);
         if (rank >= w.left) return false;
         ++w.round;
-        const uint64_t item = w.left - 1 - rank; // the longest tiles of a sequence are its last
+        const uint64_t last = w.left - 1 - rank; // the longest tiles of a sequence are its last
+        const uint64_t item = SINKS && w.single ? last / 2 : last;
+        if (SINKS) w.off = static_cast<uint32_t>(last & 1u); // which of the two tiles
         const uint32_t want = static_cast<uint32_t>(item / p.kv_heads);
         w.head = static_cast<uint32_t>(item - static_cast<uint64_t>(want) * p.kv_heads);
         uint32_t before = 0;
@@ -320,6 +328,7 @@ template <bool SINKS> __device__ __forceinline__ bool ap_next(const APParams &pp
         g.s = attn_seq(p, g.b, false);
         g.t0 = ap_tile(p, g.s, g.pair * AP_PAIR);
         g.t1 = ap_tile(p, g.s, g.pair * AP_PAIR + AP_TILE);
+        if (SINKS && !pp.deal && w.single) (w.off ? g.t0 : g.t1) = APTile{};
         const APSpan span = ap_span<SINKS>(p, g.t0, g.t1);
         g.first = span.first;
         g.skip = span.skip;
@@ -522,6 +531,10 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
         fence_proxy_async(); // the copies of keys come into the tables' place
     } else {
         walk.left = static_cast<uint64_t>(misc[2]) * p.kv_heads;
+        if (SINKS && walk.left * 2 <= pp.singles) {
+            walk.left *= 2;
+            walk.single = true;
+        }
         if (blockIdx.x >= walk.left) return;
     }
 
