@@ -298,7 +298,7 @@ template <bool SINKS> __device__ __forceinline__ bool ap_next(const APParams &pp
         const uint64_t last = w.left - 1 - rank; // the longest tiles of a sequence are its last
         const uint64_t item = SINKS && w.single ? last / 2 : last;
         if (SINKS) w.off = static_cast<uint32_t>(last & 1u); // which of the two tiles
-        const uint32_t want = static_cast<uint32_t>(item / p.kv_heads);
+        const uint32_t want = static_cast<uint32_t>(SINKS ? quotient(item, p.kv_heads) : item / p.kv_heads);
         w.head = static_cast<uint32_t>(item - static_cast<uint64_t>(want) * p.kv_heads);
         uint32_t before = 0;
         w.b = 0;
@@ -418,7 +418,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
         }
     } else if (threadIdx.x == 32) {
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 1);
+            mbar_init(&q_full[i], SINKS ? 4 : 1);
             mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
@@ -686,6 +686,10 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
 #pragma unroll
                 for (uint32_t t = 0; t < 2; ++t) {
                     if ((g->te[t] == g->tb[t] && !(SINKS && g->fe[t])) || !ok) continue;
+                    if (SINKS && k == 0) { // by the softmax warps
+                        ++n[t];
+                        continue;
+                    }
                     ok = ap_wait(&q_empty[t], (n[t] & 1u) ^ 1u, abort_flag, p.status);
                     if (!ok) break;
                     ++n[t];
@@ -714,7 +718,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     cp_async_wait<0>();
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&q_full[t]);
+                    if (lane < (SINKS ? 4 : 1)) mbar_arrive(&q_full[t]);
                 }
                 if (!ok) break;
                 release(k);
@@ -818,6 +822,27 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                 key_hi = hi > 0 ? static_cast<uint32_t>(hi) : 0;
                 key_lo = lo > 0 ? static_cast<uint32_t>(lo) : 0;
                 if (SINKS) first_hi = p.sinks < key_hi ? p.sinks : key_hi;
+            }
+            if (SINKS && k == 0 && blocks) {
+                // the first segment's Q, a thread its row: the softmax has nothing to do yet, and one warp
+                // takes 5000 cycles for a tile (later ones are on their way while a segment runs)
+                const bool live = tok < g->ql;
+                const int64_t from = static_cast<int64_t>((static_cast<uint64_t>(g->q0) + tok) * p.qt +
+                                                          (static_cast<uint64_t>(g->head) * p.group + (row - tok * p.group)) * p.qh);
+                const uint32_t base = smem_u32(smem + t * L::BLOCK) + r * 128;
+#pragma unroll
+                for (uint32_t piece = 0; piece < DP / 8; ++piece) {
+                    const bool in = live && piece * 8 < p.dim;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(
+                                     base + (piece >> 3) * L::HALF + (((piece & 7u) ^ (r & 7u)) << 4)),
+                                 "l"(static_cast<const uint16_t *>(p.q) + (in ? from + piece * 8 : 0)), "r"(in ? 16u : 0u)
+                                 : "memory");
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[t]);
             }
             const uint64_t token = static_cast<uint64_t>(g->q0) + tok;
             const uint32_t qhead = g->head * p.group + (row - tok * p.group);
