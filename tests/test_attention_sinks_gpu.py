@@ -157,6 +157,42 @@ def test_more_rows_than_keys(cuda):
         assert (out[:n - kv] == 0).all() and (lse[:n - kv] == -math.inf).all()
 
 
+def test_sequences_without_rows(cuda):
+    for lens in ([(0, 50), (1, 300), (0, 900), (130, 900), (0, 7)], [(0, 500), (1, 700), (0, 3)], [(0, 5)] * 200 + [(1, 400)]):
+        check(cuda, lens, 8, 2, 64, 16, 70, 20)
+
+
+def test_rows_behind_the_last_sequence_stay(cuda):
+    """Rows past q_start's end, a batch's padding, are neither read nor written."""
+    import ctypes as C
+
+    from freemoe_b200._lib import PagedAttentionArgs, check as ok, load
+
+    for lens in ([(1, 500), (1, 90)], [(150, 700), (1, 90)]):
+        b = Batch(lens, 8, 2, 64, 16, 100, 9)
+        used, tokens = b.starts[-1], b.starts[-1] + 300
+        want, _ = b.run()
+        q = torch.full((tokens, 8, 64), float("nan"), dtype=BF16, device="cuda")
+        q[:used] = b.q
+        out = torch.full((tokens, 8, 64), 7.0, dtype=BF16, device="cuda")
+        a = PagedAttentionArgs(
+            q=q.data_ptr(), k_cache=b.k_cache.data_ptr(), v_cache=b.v_cache.data_ptr(), out=out.data_ptr(),
+            page_table=b.table.data_ptr(), q_start=b.q_start.data_ptr(), kv_len=b.kv_len.data_ptr(), q_token_stride=512,
+            q_head_stride=64, out_token_stride=512, out_head_stride=64, cache_page_stride=b.k_cache.stride(0),
+            cache_head_stride=b.k_cache.stride(1), cache_row_stride=b.k_cache.stride(2), page_table_stride=b.table.stride(0),
+            dtype=1, seqs=len(lens), tokens=tokens, heads=8, kv_heads=2, head_dim=64, n_pages=b.k_cache.shape[0],
+            page_size=16, max_q_len=max(n for n, _ in lens), max_kv_len=max(kv for _, kv in lens), causal=1, window=100,
+            scale=b.scale)
+        need = C.c_uint64()
+        ok(load().fmcuda_paged_attention_sinks_workspace_bytes(C.byref(a), 9, C.byref(need)))
+        ws = torch.empty(max(1, need.value), dtype=torch.uint8, device="cuda")
+        ok(load().fmcuda_paged_attention_sinks(C.byref(a), 9, ws.data_ptr(), need.value,
+                                               torch.cuda.current_stream().cuda_stream))
+        assert cuda.device_status() == 0 and (out[used:] == 7).all()
+        off = (out[:used].float() - want.float()).abs()
+        assert (off <= 2 * 2.0 ** -8 * (want.float().abs() + 4)).all()  # cut otherwise, perhaps: the weights' rounding
+
+
 def test_sinks_that_add_nothing(cuda):
     """Where the window reaches the first keys, or covers all, the result is the window's; 0 is the call without them."""
     b = Batch([(130, 900), (1, 600)], 8, 2, 128, 16, 10000, 40)

@@ -186,6 +186,12 @@ def test_offsets_past_32_bits(cuda):
     assert (got[3][:-40] == got[3][0]).all()
 
 
+def test_a_very_large_vocabulary(cuda):
+    for dtype in (BF16, F32):
+        x = logits_of(2, (1 << 24) + 37, dtype)
+        hold(x, tokens_of(2, x.shape[1]), 32)
+
+
 def test_the_same_bits_each_time_on_any_stream_and_replayed(cuda):
     from freemoe_b200 import hotpath
 

@@ -214,19 +214,32 @@ def test_rows_far_apart(cuda):
     hold(x, w, tensor(3, 1024, seed=2), w)
 
 
-def test_captured_and_replayed(cuda):
+@pytest.mark.parametrize("tokens,d", [(40, 2048), (3000, 7000), (3, 40000), (1, 4096)])
+def test_captured_and_replayed(cuda, tokens, d):
     from freemoe_b200 import attention
 
-    x, res, w = tensor(40, 2048, dtype=BF16), tensor(40, 2048, dtype=BF16, seed=1), tensor(2048, seed=2)
-    attention.norm_add_norm(x, w, res, w)
+    x, res, w = tensor(tokens, d, dtype=BF16), tensor(tokens, d, dtype=BF16, seed=1), tensor(d, seed=2)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         y, h = attention.norm_add_norm(x, w, res, w)
     for seed in (5, 6):
-        x.copy_(tensor(40, 2048, dtype=BF16, seed=seed))
+        x.copy_(tensor(tokens, d, dtype=BF16, seed=seed))
         graph.replay()
         want = attention.norm_add_norm(x, w, res, w)
         assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+
+
+def test_a_very_wide_row(cuda):
+    """2^22 values: a thread adds 4096 of them, chunk by chunk of eight and the chunks in turn, which the bound on a sum's error
+    covers with (8 + 512 + 15) 2^-24 in place of 44 2^-24."""
+    from freemoe_b200 import attention
+
+    d = 1 << 22
+    x, res, w1, w2 = (tensor(2, d, seed=1), tensor(2, d, dtype=BF16, seed=2), tensor(d, seed=3), tensor(d, seed=4))
+    y, h = attention.norm_add_norm(x, w1, res, w2)
+    want_h, dh, want_y, dy = exact(x, w1, res, w2)
+    within(h, want_h, dh * (535 + 35) / 35)
+    within(y, want_y, dy * (535 + 40) / 35)
 
 
 def test_refusals(cuda):
