@@ -41,6 +41,8 @@
 // SINKS: the first p.sinks keys stay visible behind the window.  A pair's blocks are then
 // counted without the gap between those of the first keys and those of its windows (`skip`
 // blocks from block `first` on), and a tile takes the ones before fe and those of [tb, te).
+// A prompt of 8192, 32/8 heads of 128, window 2048, 16 first keys: 250 to 285 us by heat (0.85 to 0.97
+// PFLOP/s of the products that the mask leaves).
 //
 // A persistent CTA an SM.  Where there are many (pair of tiles, key head) items,
 // they go to the CTAs whole, the longest first, in rounds that run there and

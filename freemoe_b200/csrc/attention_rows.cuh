@@ -24,7 +24,8 @@
 // its range, and of the unit that goes on after it.
 //
 // SINKS: the first p.sinks keys stay visible behind the window.  A unit's steps are then those of
-// these keys and, after a gap that is neither read nor counted, those of the window.
+// these keys and, after a gap that is neither read nor counted, those of the window (64 sequences
+// of up to 32768 keys, window 4096, 64 first keys, 1.03 GB: 160 to 174 us, 90 to 98%).
 //
 // Measured, 8 key heads of 128: 64 sequences of up to 8192 keys (1.09 GB) 170 to 181 us by
 // machine, 94 to 99% of the rate of a copy; one sequence of 131071 keys and 4 key heads
