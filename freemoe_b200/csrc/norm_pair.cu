@@ -9,8 +9,8 @@
 // digits.
 //
 // Measured, 8192 rows of 4096: bf16 46 us (268 MB, 5.8 TB/s, 89% of the rate of a copy), to
-// e4m3 46, x and y in f32 57, a gate of x's shape 54; rows of 8192 89; rows of 4095 95 (accesses
-// of two bytes).  A row alone 3.3 us: a launch, the loads and two sums, one after the other.
+// e4m3 46, x and y in f32 57, a gate of x's shape 54; rows of 8192 89; rows of 4095 82 (accesses
+// of two bytes).  A row alone 3.1 us: a launch, the loads and two sums, one after the other.
 #include <cmath>
 #include <string>
 
@@ -116,8 +116,9 @@ template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel
 // values or one in the first words of their places.
 constexpr int PAIR_ANY = -1;
 template <int VEC, int T> struct PairChunk {
-    uint32_t w[T == PAIR_ANY || T == FM_X_F32 ? 8 : 4];
-    __device__ __forceinline__ void load(const void *p, int32_t t, int64_t row, uint32_t c, uint32_t d) {
+    uint32_t w[VEC != 8 || T == FM_X_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const void *p, int32_t type, int64_t row, uint32_t c, uint32_t d) {
+        const int32_t t = T == PAIR_ANY ? type : T;
         if constexpr (VEC == 8) {
             Raw8 q{};
             if (c * 8 < d) q = raw8_load(p, T, row + c * 8);
@@ -125,42 +126,61 @@ template <int VEC, int T> struct PairChunk {
 #pragma unroll
             for (uint32_t i = 0; i < sizeof(w) / 4; ++i) w[i] = all[i];
         } else {
+            // the type is asked for once, not at each value (1700 rows of 311 9.3 -> 7.0 us, 8192 of 4095 92 -> 82)
             const char *base = static_cast<const char *>(p) + row * x_size(t);
+            if (t == FM_X_F32) {
 #pragma unroll
-            for (int j = 0; j < 8; j += VEC) {
-                const uint32_t e = value_at<VEC>(c, j);
-                w[j] = 0;
-                if (VEC == 2) w[j + 1] = 0;
-                if (e >= d) continue;
-                const char *at = base + static_cast<uint64_t>(e) * x_size(t);
-                if (VEC == 2 && t == FM_X_F32) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                for (int j = 0; j < 8; j += VEC) {
+                    const uint32_t e = value_at<VEC>(c, j);
+                    const uint32_t *at = reinterpret_cast<const uint32_t *>(base) + e;
+                    uint2 v = make_uint2(0, 0);
+                    if (e < d) {
+                        if constexpr (VEC == 2)
+                            v = *reinterpret_cast<const uint2 *>(at);
+                        else
+                            v.x = *at;
+                    }
                     w[j] = v.x;
-                    w[j + 1] = v.y;
-                } else if (VEC == 2 || t == FM_X_F32) {
-                    w[j] = *reinterpret_cast<const uint32_t *>(at);
-                } else {
-                    w[j] = *reinterpret_cast<const uint16_t *>(at);
+                    if constexpr (VEC == 2) w[j + 1] = v.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j += VEC) {
+                    const uint32_t e = value_at<VEC>(c, j);
+                    const uint16_t *at = reinterpret_cast<const uint16_t *>(base) + e;
+                    w[j] = 0;
+                    if (e >= d) continue;
+                    if constexpr (VEC == 2)
+                        w[j] = *reinterpret_cast<const uint32_t *>(at);
+                    else
+                        w[j] = *at;
                 }
             }
         }
     }
-    __device__ __forceinline__ void get(int32_t t, float (&v)[8]) const {
+    __device__ __forceinline__ void get(int32_t type, float (&v)[8]) const {
+        const int32_t t = T == PAIR_ANY ? type : T;
         if constexpr (VEC == 8) {
             constexpr int B = sizeof(w) == 32 ? 4 : 0; // (raw8_unpack looks at the second four with f32 only)
             raw8_unpack(Raw8{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[B], w[B + 1], w[B + 2], w[B + 3])},
                         T, v);
         } else {
+            if (t == FM_X_F32) {
 #pragma unroll
-            for (int j = 0; j < 8; j += VEC) {
-                if constexpr (VEC == 2) {
-                    const float2 f = load2(&w[j], t, 0);
-                    v[j] = f.x;
-                    v[j + 1] = f.y;
-                } else {
-                    v[j] = load1(&w[j], t, 0);
-                }
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+            } else if (t == FM_X_BF16) {
+                values<__nv_bfloat16>(v);
+            } else {
+                values<__half>(v);
             }
+        }
+    }
+    template <typename H> __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; j += VEC) {
+            const H *h = reinterpret_cast<const H *>(&w[j]);
+            v[j] = static_cast<float>(h[0]);
+            if constexpr (VEC == 2) v[j + 1] = static_cast<float>(h[1]);
         }
     }
 };
@@ -180,6 +200,26 @@ template <bool CTA> __device__ __forceinline__ float pair_sum(float v, float4 *s
     }
     return v;
 }
+
+// A chunk of a weight, of a type at run time in each form.
+template <int VEC> struct PairWeight {
+    PairChunk<VEC == 8 ? 2 : VEC, PAIR_ANY> narrow;
+    Raw8 wide;
+    __device__ __forceinline__ void load(const void *p, int32_t t, uint32_t c, uint32_t d) {
+        if constexpr (VEC == 8) {
+            wide = Raw8{};
+            if (c * 8 < d) wide = raw8_load(p, t, c * 8);
+        } else {
+            narrow.load(p, t, 0, c, d);
+        }
+    }
+    __device__ __forceinline__ void get(int32_t t, float (&v)[8]) const {
+        if constexpr (VEC == 8)
+            raw8_unpack(wide, t, v);
+        else
+            narrow.get(t, v);
+    }
+};
 
 // A team (see norm_rows.cuh) a row, whose values stay in registers between the two norms;
 // the next row is on its way meanwhile (FULL: and a gate of the row's own).  The weights
@@ -220,12 +260,21 @@ __global__ void __launch_bounds__(MOST, MOST == 512 && VEC == 8 && RT != FM_X_F3
         for (int j = 0; j < 8; ++j) w[j] *= p.gate_kind == GATE_CHANNEL ? g[j] * p.scale : p.scale;
     };
     float w1[ONE ? ITER : 1][8], w2[ONE ? ITER : 1][8];
-    if constexpr (ONE) {
+    if constexpr (ONE) { // all loads, then their values (one row of 4096: 3.05 -> 2.9 us)
+        PairWeight<VEC> a, g, b;
+        if (p.w1) a.load(p.w1, p.wt, c0, p.d);
+        if (p.gate_kind == GATE_CHANNEL) g.load(p.gate, p.gt, c0, p.d);
+        if (p.y) b.load(p.w2, p.wt, c0, p.d);
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            first_weight(c0 + i * nt, w1[i]);
-            if (p.y) load_chunk<VEC>(p.w2, p.wt, 0, c0 + i * nt, p.d, w2[i]);
+        for (int j = 0; j < 8; ++j) w1[0][j] = 1.0f, w2[0][j] = p.scale;
+        if (p.w1) a.get(p.wt, w1[0]);
+        if (p.gate_kind == GATE_CHANNEL) {
+            g.get(p.gt, w2[0]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w2[0][j] *= p.scale;
         }
+        mul8(w1[0], w2[0]);
+        if (p.y) b.get(p.wt, w2[0]);
     }
     for (uint32_t c = threadIdx.x; !ONE && c < all; c += blockDim.x) {
         float w[8];
@@ -340,13 +389,30 @@ int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one and a row a CTA
 // where there are rows for half the threads of the GPU only (latency counts then: one row of 4096
-// 3.4 -> 3.2 us, 256 rows 4.5 -> 4.1; but 512 rows of 4096 6.6 -> 7.1, 1024 9.1 -> 12.1).
+// 3.4 -> 3.1 us, 256 rows 4.5 -> 4.1; but 512 rows of 4096 6.6 -> 7.1, 1024 9.1 -> 12.1).
 template <int VEC, int XT, int RT, bool FULL = false> int dispatch_width(const PairParams &p, cudaStream_t s) {
     const uint32_t chunks = (p.d + 127) / 128 * 16, one = (chunks + 31) / 32 * 32, two = ((chunks + 1) / 2 + 31) / 32 * 32;
     const bool few = static_cast<uint64_t>(p.tokens) * one <= static_cast<uint64_t>(device_sm_count()) * 1024;
     if (p.d <= 256) return launch_pair<VEC, XT, RT, FULL, false, false, 1, 128>(p, 128, s);
     if (p.d <= 1024) return launch_pair<VEC, XT, RT, FULL, false, false, 4, 128>(p, 128, s);
-    if (few && one <= 1024) return launch_pair<VEC, XT, RT, FULL, true, true, 1, 1024>(p, one, s);
+    if (few && one <= 1024) {
+        if constexpr (VEC != 8) {
+            // code that runs once comes from memory: that of one pair of types is shorter (a row of 4095
+            // in bf16 3.4 us, 5.1 with types at run time; with many rows they take the same time)
+            auto typed = [&](int32_t xt, int32_t rt) { return p.xt == xt && p.rt == rt; };
+            if (typed(FM_X_BF16, FM_X_BF16))
+                return launch_pair<VEC, FM_X_BF16, FM_X_BF16, FULL, true, true, 1, 1024>(p, one, s);
+            if (typed(FM_X_F32, FM_X_BF16))
+                return launch_pair<VEC, FM_X_F32, FM_X_BF16, FULL, true, true, 1, 1024>(p, one, s);
+            if (typed(FM_X_F16, FM_X_F16))
+                return launch_pair<VEC, FM_X_F16, FM_X_F16, FULL, true, true, 1, 1024>(p, one, s);
+            if (typed(FM_X_F32, FM_X_F16))
+                return launch_pair<VEC, FM_X_F32, FM_X_F16, FULL, true, true, 1, 1024>(p, one, s);
+            if (typed(FM_X_F32, FM_X_F32))
+                return launch_pair<VEC, FM_X_F32, FM_X_F32, FULL, true, true, 1, 1024>(p, one, s);
+        }
+        return launch_pair<VEC, XT, RT, FULL, true, true, 1, 1024>(p, one, s);
+    }
     if (two <= 512) return launch_pair<VEC, XT, RT, FULL, true, false, 2, 512>(p, two, s);
     if (two <= 1024) return launch_pair<VEC, XT, RT, FULL, true, false, 2, 1024>(p, two, s);
     const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
