@@ -322,9 +322,10 @@ std::tuple<Tensor, MaybeTensor> paged_attention(const Tensor &q, const Tensor &k
     need(page_table.scalar_type() == at::kInt && q_start.scalar_type() == at::kInt &&
              kv_len.scalar_type() == at::kInt && q_start.is_contiguous() && kv_len.is_contiguous(),
          "page_table, q_start and kv_len are int32", FM_STATUS_INVALID_ARGUMENT);
-    need(max_q_len >= 0 && max_kv_len >= 0 && window >= 0 && sinks >= 0, "lengths must not be negative", FM_STATUS_INVALID_ARGUMENT);
-    need(max_kv_len <= INT32_MAX && window <= UINT32_MAX && sinks <= UINT32_MAX && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
-             seqs < INT32_MAX && k_cache.size(0) <= INT32_MAX && k_cache.size(1) <= INT32_MAX &&
+    need(max_q_len >= 0 && max_kv_len >= 0 && window >= 0 && sinks >= 0, "lengths must not be negative",
+         FM_STATUS_INVALID_ARGUMENT);
+    need(max_kv_len <= INT32_MAX && window <= UINT32_MAX && sinks <= UINT32_MAX && q.size(0) <= INT32_MAX &&
+             q.size(1) <= INT32_MAX && seqs < INT32_MAX && k_cache.size(0) <= INT32_MAX && k_cache.size(1) <= INT32_MAX &&
              k_cache.size(2) <= INT32_MAX && q.size(2) <= INT32_MAX,
          "attention lengths out of range");
     need(page_table.size(1) * k_cache.size(2) >= max_kv_len, "page table is shorter than max_kv_len");
