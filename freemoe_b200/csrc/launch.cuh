@@ -18,9 +18,13 @@ struct Launch {
     uint32_t threads, smem;
     uint32_t cluster; // CTAs a cluster, 1: none
 };
+// A launch may have 48 KB without asking, a kernel's static share among them: from here on the limit
+// of the dynamic share is raised.
+constexpr uint32_t ASK_FOR_SMEM = 32 * 1024;
+
 template <typename... K, typename... A>
 int launch(const char *what, void (*kernel)(K...), const Launch &l, cudaStream_t s, const A &...args) {
-    if (l.smem > 48 * 1024) {
+    if (l.smem > ASK_FOR_SMEM) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(l.smem));
         if (e != cudaSuccess) return cuda_status(e, what);

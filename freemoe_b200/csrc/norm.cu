@@ -254,7 +254,7 @@ int launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
     if (want > grid) { // as many CTAs as the GPU holds; otherwise one a row
         int per_sm = 0;
-        if (smem > 48 * 1024) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (smem > ASK_FOR_SMEM) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
             (void)cudaGetLastError();
             per_sm = 1;

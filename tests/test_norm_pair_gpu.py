@@ -277,3 +277,14 @@ def test_refusals(cuda):
     refused(26, x.double(), w, r, w, fn=attention.norm_add_norm_fp8)
     y, h = attention.norm_add_norm(x[:0], w, r[:0], w)
     assert y.shape == h.shape == (0, 64)
+
+
+@pytest.mark.parametrize("x_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("res_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tokens", [5, 700])
+@pytest.mark.parametrize("d", [1026, 1537, 6001])
+def test_types_of_long_odd_rows(cuda, x_dtype, res_dtype, tokens, d):
+    x, res = tensor(tokens, d, dtype=x_dtype, seed=3), tensor(tokens, d, dtype=res_dtype, seed=5)
+    for w_dtype in (F32, BF16, F16):
+        w1, w2 = tensor(d, dtype=w_dtype, seed=1), tensor(d, dtype=w_dtype, seed=2)
+        hold(x, w1, res, w2, out=F16, gate=tensor(d, dtype=x_dtype, seed=4), scale=0.7)
