@@ -889,7 +889,8 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     top[c] = max2(top[c], __uint_as_float(x[c][31]));
                 }
                 const float high = max2(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
-                if (__any_sync(0xFFFFFFFFu, !(high <= m + 8.0f))) {
+                // rows behind the last query do not ask: their products with keys that were not read may be NaN
+                if (__any_sync(0xFFFFFFFFu, valid && !(high <= m + 8.0f))) {
                     const float to = max2(m, high);
                     const float f = m == -INFINITY ? 0.0f : exp2_approx(m - to);
                     m = to;
