@@ -98,22 +98,24 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
         if (!rc) rc = make_cache_map(&map_v, a, a.v_cache, pp.box_rows, pp.heads_first);
         if (!rc && n.rows)
             rc = launch("attn_beside_kernel", attn_beside_kernel<DP, BF16, SINKS>,
-                        {dim3(n.ctas + rows_ctas), AP_THREADS, AP_BESIDE_SMEM<DP>, 1}, s, map_k, map_v, pp);
+                        {dim3(n.ctas + rows_ctas), AP_THREADS, AP_BESIDE_SMEM<DP>, 1, AP_BESIDE_SMEM<DP>}, s, map_k,
+                        map_v, pp);
         else if (!rc)
             rc = launch("attn_prompt_kernel", attn_prompt_kernel<DP, BF16, SINKS>,
-                        {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, 1}, s, map_k, map_v, pp);
+                        {dim3(n.ctas), AP_THREADS, APrompt<DP>::SMEM, 1, APrompt<DP>::SMEM}, s, map_k, map_v, pp);
     } else if (n.cluster) {
         rc = launch("attn_cluster_kernel", attn_cluster_kernel<DP, BF16, SINKS>,
-                    {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, n.cluster}, s, p, n.tiles);
+                    {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, n.cluster, ARows<DP>::SMEM}, s, p, n.tiles);
     } else if (n.units) {
         rc = launch("attn_unit_kernel", attn_unit_kernel<DP, BF16, SINKS>,
-                    {dim3(rows_ctas), unit_warps * 32, ARows<DP>::RINGS / AR_WARPS * unit_warps, 1}, s, p, n.tiles);
+                    {dim3(rows_ctas), unit_warps * 32, ARows<DP>::RINGS / AR_WARPS * unit_warps, 1, ARows<DP>::RINGS}, s,
+                    p, n.tiles);
     } else {
-        rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16, SINKS>, {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, 1}, s,
-                    p);
+        rc = launch("attn_rows_kernel", attn_rows_kernel<DP, BF16, SINKS>,
+                    {dim3(rows_ctas), AR_THREADS, ARows<DP>::SMEM, 1, ARows<DP>::SMEM}, s, p);
     }
     if (!rc && n.prompt && n.deal)
-        rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1}, s, pp);
+        rc = launch("attn_join_kernel", attn_join_kernel<DP, BF16>, {dim3(n.ctas, AJ_SLICES), 256, 0, 1, 0}, s, pp);
     if (rc || !n.rows || n.cluster || n.units) return rc;
     const uint64_t most = static_cast<uint64_t>(a.max_q_len) * n.group, units = static_cast<uint64_t>(p.seqs) * p.kv_heads;
     const uint32_t rows = most < n.row_limit ? static_cast<uint32_t>(most) : n.row_limit;
@@ -121,12 +123,12 @@ int launch_attention(const fmcuda_paged_attention_args &a, const AttnPlan &n, co
     if (units * 16 <= p.workers) {
         const dim3 whole(static_cast<uint32_t>(units), rows), parts(static_cast<uint32_t>(units), rows * 2);
         if (units * rows * 2 <= static_cast<uint64_t>(device_sm_count())) // one such CTA an SM
-            return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 32, 5, 2>, {parts, 32 * 32, 0, 1}, s, p, false);
-        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 32, 5, 1>, {whole, 32 * 32, 0, 1}, s, p, false);
+            return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 32, 5, 2>, {parts, 32 * 32, 0, 1, 0}, s, p, false);
+        return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 32, 5, 1>, {whole, 32 * 32, 0, 1, 0}, s, p, false);
     }
     const bool by_worker = units * n.tiles > p.workers;
     const dim3 grid = by_worker ? dim3(p.workers, rows < AR_ROWS ? rows : AR_ROWS) : dim3(static_cast<uint32_t>(units), rows);
-    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 4, 2, 1>, {grid, 4 * 32, 0, 1}, s, p, by_worker);
+    return launch("attn_combine_kernel", attn_combine_kernel<DP, BF16, SINKS, 4, 2, 1>, {grid, 4 * 32, 0, 1, 0}, s, p, by_worker);
 }
 
 // By the plan's padded head width and the arguments' type.

@@ -17,17 +17,36 @@ struct Launch {
     dim3 grid;
     uint32_t threads, smem;
     uint32_t cluster; // CTAs a cluster, 1: none
+    uint32_t most;    // the most shared memory that any launch of this kernel asks for
 };
 // A launch may have 48 KB without asking, a kernel's static share among them: from here on the limit
 // of the dynamic share is raised.
 constexpr uint32_t ASK_FOR_SMEM = 32 * 1024;
 
+// The limit belongs to the kernel and not to the launch, and other host threads may be between
+// theirs and their launches: every launch that needs one sets the same, the most that any needs.
+template <typename... K> cudaError_t allow_smem(void (*kernel)(K...), const Launch &l) {
+    if (l.smem <= ASK_FOR_SMEM) return cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.most));
+}
+
+// CTAs of such launches that an SM holds.
+template <typename... K> uint32_t ctas_per_sm(void (*kernel)(K...), const Launch &l) {
+    int n = 0;
+    if (allow_smem(kernel, l) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, static_cast<int>(l.threads), l.smem) != cudaSuccess || n < 1) {
+        (void)cudaGetLastError();
+        n = 1;
+    }
+    return static_cast<uint32_t>(n);
+}
+
 template <typename... K, typename... A>
 int launch(const char *what, void (*kernel)(K...), const Launch &l, cudaStream_t s, const A &...args) {
-    if (l.smem > ASK_FOR_SMEM) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(l.smem));
-        if (e != cudaSuccess) return cuda_status(e, what);
+    const cudaError_t limit = allow_smem(kernel, l);
+    if (limit != cudaSuccess) {
+        (void)cudaGetLastError();
+        return cuda_status(limit, what);
     }
     cudaLaunchAttribute attrs[2]{};
     cudaLaunchConfig_t config{};

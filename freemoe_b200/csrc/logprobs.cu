@@ -668,7 +668,7 @@ extern "C" int fmcuda_token_logprobs(const fmcuda_token_logprobs_args *a, void *
     while ((threads < LP_MANY && chunks > static_cast<uint64_t>(threads) * ranks * 4) ||
            (threads < LP_THREADS && chunks > static_cast<uint64_t>(threads) * ranks && few(2 * threads)))
         threads *= 2;
-    const Launch l{dim3(a->tokens * ranks), threads, 0, ranks};
+    const Launch l{dim3(a->tokens * ranks), threads, 0, ranks, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->dtype == FM_X_F32) return launch_logprobs<FM_X_F32>(p, l, few(threads), s);
     if (a->dtype == FM_X_BF16) return launch_logprobs<FM_X_BF16>(p, l, few(threads), s);

@@ -250,18 +250,11 @@ template <int VEC, int IN, bool CTA, int ITER, int MOST>
 int launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
     auto kfn = add_rms_norm_kernel<VEC, IN, CTA, ITER, MOST>;
     const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
-    const uint32_t smem = (CTA ? threads : 32) * ITER * 32;
+    const uint32_t smem = (CTA ? threads : 32) * ITER * 32, most = (CTA ? MOST : 32) * ITER * 32;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
-    if (want > grid) { // as many CTAs as the GPU holds; otherwise one a row
-        int per_sm = 0;
-        if (smem > ASK_FOR_SMEM) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
-            (void)cudaGetLastError();
-            per_sm = 1;
-        }
-        grid *= static_cast<uint32_t>(per_sm);
-    }
-    return launch("add_rms_norm_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1}, s, p);
+    // more rows than SMs: as many CTAs as the GPU holds; otherwise one a row
+    if (want > grid) grid *= ctas_per_sm(kfn, {dim3(), threads, smem, 1, most});
+    return launch("add_rms_norm_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1, most}, s, p);
 }
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one where
@@ -276,7 +269,7 @@ template <int VEC, int IN> int dispatch_width(const NormParams &p, cudaStream_t 
     if (two <= 1024) return launch_norm<VEC, IN, true, 2, 1024>(p, two, s);
     const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
     return launch("add_rms_norm_long_kernel", add_rms_norm_long_kernel<VEC>,
-                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1}, s, p);
+                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1, 0}, s, p);
 }
 
 template <int VEC> int dispatch_norm(const NormParams &p, cudaStream_t s) {

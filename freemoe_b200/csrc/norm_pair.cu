@@ -371,20 +371,12 @@ template <int VEC, int XT, int RT, bool FULL, bool CTA, bool ONE, int ITER, int 
 int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
     auto kfn = norm_pair_kernel<VEC, XT, RT, FULL, CTA, ONE, ITER, MOST>;
     const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
-    const uint32_t smem = ONE ? 0 : (CTA ? threads : 32) * ITER * 64;
+    const uint32_t smem = ONE ? 0 : (CTA ? threads : 32) * ITER * 64, most = ONE ? 0 : (CTA ? MOST : 32) * ITER * 64;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
-    if (ONE) {
-        grid = want;
-    } else if (want > grid) { // as many CTAs as the GPU holds; otherwise one a row
-        int per_sm = 0;
-        if (smem > ASK_FOR_SMEM) cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kfn, threads, smem) != cudaSuccess || per_sm < 1) {
-            (void)cudaGetLastError();
-            per_sm = 1;
-        }
-        grid *= static_cast<uint32_t>(per_sm);
-    }
-    return launch("norm_pair_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1}, s, p);
+    if (ONE) grid = want;
+    // more rows than SMs: as many CTAs as the GPU holds; otherwise one a row
+    if (want > grid) grid *= ctas_per_sm(kfn, {dim3(), threads, smem, 1, most});
+    return launch("norm_pair_kernel", kfn, {dim3(want < grid ? want : grid), threads, smem, 1, most}, s, p);
 }
 
 // Short rows to warps, four a CTA; longer ones to CTAs, a thread two chunks, or one and a row a CTA
@@ -417,7 +409,7 @@ template <int VEC, int XT, int RT, bool FULL = false> int dispatch_width(const P
     if (two <= 1024) return launch_pair<VEC, XT, RT, FULL, true, false, 2, 1024>(p, two, s);
     const uint32_t most = static_cast<uint32_t>(device_sm_count()) * 2;
     return launch("norm_pair_long_kernel", norm_pair_long_kernel<VEC>,
-                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1}, s, p);
+                  {dim3(p.tokens < most ? p.tokens : most), 1024, 0, 1, 0}, s, p);
 }
 
 // A gate of x's shape has loads of its own where it is of the residual's type, 16 bits (8192 x 4096

@@ -465,7 +465,7 @@ int rope_append(const fmcuda_rope_append_args *a, const uint8_t *axis, uint32_t 
             }
         }
     }
-    const Launch l{dim3((a->tokens + p.batch - 1) / p.batch, parts), threads, 0, 1};
+    const Launch l{dim3((a->tokens + p.batch - 1) / p.batch, parts), threads, 0, 1, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!vec && a->interleaved) return launch("rope_append_any_kernel", rope_append_any_kernel<true>, l, s, p);
     if (!vec) return launch("rope_append_any_kernel", rope_append_any_kernel<false>, l, s, p);
