@@ -198,7 +198,10 @@ template <int TYPE, int NMAT, int EPI, int G>
 int launch_gg_inst(const GGemmParams &p, const CUtensorMap &map, uint32_t max_units, cudaStream_t s) {
     auto kfn = grouped_gemm_kernel<TYPE, NMAT, EPI, G>;
     const uint32_t smem = GGLayout<TYPE, NMAT>::smem_bytes(p.experts);
-    cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // the limit is the kernel's and not the launch's: for all numbers of experts, so that no other host
+    // thread lowers it before this launch
+    cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(GGLayout<TYPE, NMAT>::smem_bytes(GG_MAX_EXPERTS)));
     if (err != cudaSuccess) {
         (void)cudaGetLastError();
         return cuda_status(err, "grouped GEMM shared-memory attribute");

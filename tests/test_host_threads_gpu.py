@@ -81,12 +81,36 @@ class Decoding:
         return lib.fmcuda_paged_attention_sinks(C.byref(self.args), self.sinks, self.workspace.data_ptr(), self.bytes, stream)
 
 
+class Experts:
+    """The grouped products of a batch of tokens, whose tables grow with the experts."""
+
+    def __init__(self, experts, tokens=64, top_k=4, d=512, ffn=256):
+        from freemoe_b200 import TYPE_Q8_0, hotpath
+
+        g = torch.Generator(device="cuda").manual_seed(experts)
+        self.x = torch.randn(tokens, d, generator=g, device="cuda").bfloat16()
+        self.logits = torch.randn(tokens, experts, generator=g, device="cuda")
+        self.slot = torch.cat([hotpath.synth_weights(TYPE_Q8_0, rows, cols, i, 0.05)
+                               for i, (rows, cols) in enumerate(((ffn, d), (ffn, d), (d, ffn)))])
+        self.table, self.y = hotpath.slot_table([self.slot] * experts, "cuda"), torch.empty(tokens, d, device="cuda")
+        self.out = (self.y,)
+        part = hotpath.row_bytes(TYPE_Q8_0, d) * ffn
+        self.args = hotpath.moe_args(self.x, self.logits, self.table, experts=experts, top_k=top_k, d_model=d, ffn=ffn,
+                                     gate_type=TYPE_Q8_0, up_type=TYPE_Q8_0, down_type=TYPE_Q8_0, up_offset=part,
+                                     down_offset=2 * part, y=self.y)
+        self.workspace = torch.empty(hotpath.moe_prefill_workspace_bytes(tokens, experts, top_k, d, ffn),
+                                     dtype=torch.uint8, device="cuda")
+
+    def call(self, lib, stream):
+        return lib.fmcuda_moe_prefill(C.byref(self.args), None, self.workspace.data_ptr(), self.workspace.numel(), stream)
+
+
 @pytest.mark.parametrize("make", [
     lambda: (Norms(6144), Norms(8192)), lambda: (Norms(5120), Norms(7168)), lambda: (Norms(9216), Norms(16384)),
     lambda: (Norm(12288), Norm(16384)), lambda: (Norm(9216), Norm(12288)), lambda: (Decoding(40), Decoding(160)),
-    lambda: (Decoding(40, window=20, sinks=3), Decoding(160, window=20, sinks=3)),
+    lambda: (Decoding(40, window=20, sinks=3), Decoding(160, window=20, sinks=3)), lambda: (Experts(8), Experts(700)),
 ], ids=["norms 6144 8192", "norms 5120 7168", "norms 9216 16384", "norm 12288 16384", "norm 9216 12288", "decoding",
-        "decoding with first keys"])
+        "decoding with first keys", "experts"])
 def test_two_threads(cuda, make):
     lib, jobs = load(), make()
     streams = [torch.cuda.Stream() for _ in jobs]
