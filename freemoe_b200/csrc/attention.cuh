@@ -37,7 +37,7 @@ struct AttnSeq {
 
 __device__ __forceinline__ AttnSeq attn_seq(const AttnParams &p, uint32_t b, bool report) {
     AttnSeq s;
-    const int32_t q0 = __ldg(p.q_start + b), q1 = __ldg(p.q_start + b + 1), kl = __ldg(p.kv_len + b);
+    const int32_t q0 = p.q_start[b], q1 = p.q_start[b + 1], kl = p.kv_len[b];
     bool bad = false;
     s.q0 = static_cast<uint32_t>(q0);
     s.ql = static_cast<uint32_t>(q1 - q0);

@@ -623,7 +623,7 @@ __device__ __forceinline__ void ap_chunks(const CUtensorMap &map_k, const CUtens
                     if (live) {
                         const uint32_t at = key / p.page_size;
                         row = static_cast<int32_t>(key - at * p.page_size);
-                        page = __ldg(p.table + g.b * p.tb + at);
+                        page = p.table[g.b * p.tb + at];
                         if (page < 0 || static_cast<uint32_t>(page) >= p.n_pages) {
                             raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
                             page = -1; // outside the tensor map: the box is filled with zeros

@@ -326,7 +326,7 @@ __device__ __forceinline__ int64_t ar_key_at(const AttnParams &p, const AttnSeq 
     const uint32_t key = key_first + (lane & (ar_keys(DP) - 1));
     if ((key < s.lo && !(SINKS && key < p.sinks)) || key >= s.kl) return -1;
     const uint32_t page = key / p.page_size;
-    const int32_t id = __ldg(p.table + b * p.tb + page);
+    const int32_t id = p.table[b * p.tb + page];
     if (id < 0 || static_cast<uint32_t>(id) >= p.n_pages) {
         raise_device_status(p.status, FM_STATUS_INVALID_ARGUMENT);
         return -1;

@@ -3,7 +3,9 @@
 // earlier work of the stream done, as it would after an ordinary launch, but its CTAs are
 // already there (an ordinary launch costs one to two microseconds between two kernels,
 // as much as some of these kernels take).  let_next() lets the next launch of this kind
-// come; without it that one begins when this kernel ends.
+// come; without it that one begins when this kernel ends.  Such kernels read memory by ordinary
+// loads: read-only ones (ld.global.nc, __ldg) promise data that nobody writes from the kernel's
+// begin on, which is before after_stream(), and may be moved there.
 #pragma once
 
 #include "common.cuh"

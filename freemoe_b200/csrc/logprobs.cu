@@ -86,9 +86,10 @@ template <int T> constexpr int LP_VEC = 32 / static_cast<int>(x_size(T)); // val
 struct Chunk {
     uint32_t w[8];
 };
+// (Not by read-only loads, here and below: the kernel begins while the one that writes the logits may still run.)
 __device__ __forceinline__ Chunk load_chunk32(const void *at) {
     Chunk r;
-    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
                  : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
                    "=r"(r.w[7])
                  : "l"(at));
@@ -97,7 +98,7 @@ __device__ __forceinline__ Chunk load_chunk32(const void *at) {
 
 // The same for a chunk that is read a second time, of which single values are looked at again: kept in L1.
 __device__ __forceinline__ Chunk load_chunk32_again(const void *at) {
-    const uint4 a = __ldg(static_cast<const uint4 *>(at)), b = __ldg(static_cast<const uint4 *>(at) + 1);
+    const uint4 a = *static_cast<const uint4 *>(at), b = static_cast<const uint4 *>(at)[1];
     return Chunk{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
 
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(FEW ? LP_THREADS : LP_MANY, FEW ? 2 : 8)
     let_next();
     const Row<T> row(p, r);
     const uint32_t me = rank * blockDim.x + threadIdx.x;
-    const int32_t token = me == 0 ? __ldg(p.tokens + r) : -1;
+    const int32_t token = me == 0 ? p.tokens[r] : -1;
     // chunk 0 may be empty, and so may the last
     const uint32_t first = me || row.head ? me : threads, last = row.whole + (row.tail ? 1 : 0);
     Stream<T> stream(p, first <= last ? first : 0xFFFFFFFFu);
