@@ -249,7 +249,7 @@ template <int VEC> __global__ void __launch_bounds__(1024) add_rms_norm_long_ker
 template <int VEC, int IN, bool CTA, int ITER, int MOST>
 int launch_norm(const NormParams &p, uint32_t threads, cudaStream_t s) {
     auto kfn = add_rms_norm_kernel<VEC, IN, CTA, ITER, MOST>;
-    const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
+    const uint32_t teams = CTA ? 1 : threads / 32, want = p.tokens / teams + (p.tokens % teams ? 1 : 0);
     const uint32_t smem = (CTA ? threads : 32) * ITER * 32, most = (CTA ? MOST : 32) * ITER * 32;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
     // more rows than SMs: as many CTAs as the GPU holds; otherwise one a row

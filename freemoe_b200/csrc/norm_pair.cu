@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(MOST, MOST == 512 && VEC == 8 && RT != FM_X_F3
 template <int VEC, int XT, int RT, bool FULL, bool CTA, bool ONE, int ITER, int MOST>
 int launch_pair(const PairParams &p, uint32_t threads, cudaStream_t s) {
     auto kfn = norm_pair_kernel<VEC, XT, RT, FULL, CTA, ONE, ITER, MOST>;
-    const uint32_t teams = CTA ? 1 : threads / 32, want = (p.tokens + teams - 1) / teams;
+    const uint32_t teams = CTA ? 1 : threads / 32, want = p.tokens / teams + (p.tokens % teams ? 1 : 0);
     const uint32_t smem = ONE ? 0 : (CTA ? threads : 32) * ITER * 64, most = ONE ? 0 : (CTA ? MOST : 32) * ITER * 64;
     uint32_t grid = static_cast<uint32_t>(device_sm_count());
     if (ONE) grid = want;
