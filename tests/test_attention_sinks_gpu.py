@@ -258,3 +258,31 @@ def test_refusals(cuda):
     refused(8, sinks=1 << 32)
     refused(26, causal=False)
     refused(26, workspace=torch.empty(0, dtype=torch.uint8), window=100)
+
+
+@pytest.mark.parametrize("sinks", [900, 901, (1 << 31) - 1, 1 << 31, (1 << 32) - 1])
+@pytest.mark.parametrize("window", [1, 7, 128])
+def test_more_first_keys_than_keys(cuda, sinks, window):
+    """All of a sequence's keys, however many more are asked for: against 64 bits, no key lost or counted twice
+    (one of 900 moves the log-sum-exp by 1e-3, 20 times what is allowed)."""
+    b = Batch([(130, 900), (1, 600), (900, 900)], 8, 2, 128, 16, 10000, 40, seed=1)
+    out, lse = b.run(window=window, sinks=sinks)
+    assert cuda.device_status() == 0
+    b.window, b.sinks = window, sinks
+    hold(b, out, lse)
+    d = Batch([(1, 900), (1, 600)], 8, 2, 64, 16, 10000, 40, F16, seed=2)
+    out, lse = d.run(window=window, sinks=sinks)
+    d.window, d.sinks = window, sinks
+    hold(d, out, lse)
+
+
+@pytest.mark.parametrize("lens", [[(1, 500), (1, 90)], [(150, 700), (1, 90)], [(0, 30), (40, 40)]])
+def test_padded_batches(cuda, lens):
+    """Rows behind the last sequence change nothing: the others against 64 bits."""
+    b = Batch(lens, 8, 2, 64, 16, 100, 9)
+    used = b.starts[-1]
+    b.q = torch.cat([b.q, torch.full((300, 8, 64), float("nan"), dtype=BF16, device="cuda")])
+    out, lse = b.run()
+    assert cuda.device_status() == 0
+    b.q = b.q[:used]
+    hold(b, out[:used], lse[:used])
