@@ -55,6 +55,7 @@ class Layer:
     config: Config
     weights: dict = field(default_factory=dict)
     experts: list = field(default_factory=list)
+    axes: torch.Tensor | None = None  # of the rotated pairs, where positions have several
 
     @classmethod
     def synthetic(cls, config: Config, seed: int = 0) -> "Layer":
@@ -71,6 +72,7 @@ class Layer:
         for name in ("norm_attention", "norm_experts", "norm_head", "behind_attention", "behind_experts", "gate_attention",
                      "gate_experts"):
             layer.weights[name] = torch.ones(c.d_model, device="cuda")
+        layer.axes = attention.rope_axes(c.sections) if c.sections else None
         if c.vocab:
             head = hotpath.synth_weights(TYPE_Q8_0, c.vocab, c.d_model, seed + 50, 0.05)
             layer.weights["head"] = (TYPE_Q8_0, head, c.vocab, c.d_model)
@@ -140,9 +142,8 @@ def decoder_layer(layer: Layer, cache: Cache, x: torch.Tensor, step: dict, inv_f
     normed, _ = attention.add_rms_norm(x, w["norm_attention"], epsilon=c.epsilon)
     qkv = layer.product("qkv", normed).view(tokens, c.heads + 2 * c.kv_heads, c.head_dim)
     q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), dim=1)
-    axes = attention.rope_axes(c.sections) if c.sections else None
     q = attention.rope_append(q, k, v, step["positions"], inv_freq, cache.k, cache.v, step["slots"],
-                              attention_factor=attention_factor, axes=axes)
+                              attention_factor=attention_factor, axes=layer.axes)
     o = attention.paged_attention(q, cache.k, cache.v, step["page_table"], step["q_start"], step["kv_len"],
                                   max_q_len=step["max_q_len"], max_kv_len=step["max_kv_len"], window=c.window,
                                   sinks=c.sinks)

@@ -143,3 +143,15 @@ def test_two_streams_at_once(cuda):
         for a, b in zip(want, got):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert cuda.device_status() == 0
+
+
+def test_the_axes_are_worked_out_once(cuda, monkeypatch):
+    """A layer has the axes of its pairs at hand: its calls make no copy from the host for them."""
+    import decoder_layer as example
+
+    config = layer_config()
+    layer, cache = example.Layer.synthetic(config), example.Cache(config, 8, 1, 100)
+    inv_freq, _ = example.attention.rope_frequencies(config.head_dim)
+    x = torch.randn(3, config.d_model, device="cuda").to(BF16)
+    monkeypatch.setattr(example.attention, "rope_axes", lambda *a, **k: pytest.fail("worked out in a call"))
+    example.decoder_layer(layer, cache, x, cache.extend([3]), inv_freq)
