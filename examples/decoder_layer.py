@@ -69,9 +69,10 @@ class Layer:
             parts = [hotpath.synth_weights(TYPE_Q4_K, rows, cols, seed + 100 + 3 * e + i, 0.05)
                      for i, (rows, cols) in enumerate(((c.ffn, c.d_model), (c.ffn, c.d_model), (c.d_model, c.ffn)))]
             layer.experts.append(torch.cat(parts))
+        g = torch.Generator(device="cuda").manual_seed(seed + 1000)
         for name in ("norm_attention", "norm_experts", "norm_head", "behind_attention", "behind_experts", "gate_attention",
                      "gate_experts"):
-            layer.weights[name] = torch.ones(c.d_model, device="cuda")
+            layer.weights[name] = 1 + 0.1 * torch.randn(c.d_model, generator=g, device="cuda")
         layer.axes = attention.rope_axes(c.sections) if c.sections else None
         if c.vocab:
             head = hotpath.synth_weights(TYPE_Q8_0, c.vocab, c.d_model, seed + 50, 0.05)

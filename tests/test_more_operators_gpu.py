@@ -155,3 +155,78 @@ def test_the_axes_are_worked_out_once(cuda, monkeypatch):
     x = torch.randn(3, config.d_model, device="cuda").to(BF16)
     monkeypatch.setattr(example.attention, "rope_axes", lambda *a, **k: pytest.fail("worked out in a call"))
     example.decoder_layer(layer, cache, x, cache.extend([3]), inv_freq)
+
+
+def rms(x, w, epsilon):
+    x = x.double()
+    return x / torch.sqrt((x * x).mean(-1, keepdim=True) + epsilon) * w.double()
+
+
+def plain_layer(layer, x, inv_freq, swap={}):
+    """One sequence from its begin through the layer in plain torch, in 64 bits but for the products and the
+    experts, which are the layer's own, and with the roundings that it makes."""
+    import decoder_layer as example
+
+    from freemoe_b200 import TYPE_Q4_K, hotpath
+
+    c, n = layer.config, x.shape[0]
+    w = {name: layer.weights[swap.get(name, name)] for name in layer.weights}
+    qkv = layer.product("qkv", rms(x, w["norm_attention"], c.epsilon).to(BF16)).view(n, c.heads + 2 * c.kv_heads, c.head_dim)
+    q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), dim=1)
+    positions = example.Cache(c, 1, 1, n).axes(torch.arange(n, dtype=torch.int32, device="cuda"))
+    positions = positions if c.sections else positions[None]
+    axis = sum(([a] * pairs for a, pairs in enumerate(c.sections)), []) or [0] * (c.head_dim // 2)
+    angle = torch.stack([positions[a].double() * f for a, f in zip(axis, inv_freq.double())], -1)[:, None]
+
+    def turn(t):
+        a, b = t.double().split(c.head_dim // 2, -1)
+        return torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1).to(BF16).double()
+
+    group = c.heads // c.kv_heads
+    q, k, v = turn(q), turn(k).repeat_interleave(group, 1), v.to(BF16).double().repeat_interleave(group, 1)
+    at = torch.arange(n, device="cuda")
+    seen = at <= at[:, None]
+    if c.window:
+        seen &= (at > at[:, None] - c.window) | (at < c.sinks)
+    s = (torch.einsum("qhd,khd->hqk", q, k) / c.head_dim ** 0.5).masked_fill(~seen, float("-inf"))
+    o = layer.product("out", torch.einsum("hqk,khd->qhd", s.softmax(-1), v).reshape(n, -1).to(BF16)).double()
+    if c.block_norms:
+        h = x.double() + c.block_scale * w["gate_attention"].double() * rms(o, w["behind_attention"], c.epsilon)
+    else:
+        h = x.double() + o
+    normed, h = rms(h, w["norm_experts"], c.epsilon).to(BF16), h.to(BF16).double()
+    experts = hotpath.moe_block if n <= 64 else hotpath.moe_prefill
+    y, ids, _ = experts(normed, layer.product("router", normed), layer.experts, top_k=c.top_k, ffn=c.ffn,
+                        gate_type=TYPE_Q4_K, return_routing=True)
+    if c.block_norms:
+        return h + c.block_scale * w["gate_experts"].double() * rms(y, w["behind_experts"], c.epsilon), ids
+    return h + y.double(), ids
+
+
+@pytest.mark.parametrize("change", [{}, {"block_norms": False}, {"sections": (), "window": 0, "sinks": 0},
+                                    {"block_scale": -0.3, "sections": (20, 12), "page_size": 8}])
+@pytest.mark.parametrize("n", [5, 200])
+def test_a_layer_against_plain_torch(cuda, change, n):
+    """Each weight and gate where it belongs: the layer's roundings are those of the header, and each of them is
+    made in the plain form too, so that the two differ by the softmax weights' and by ties that fall otherwise."""
+    import decoder_layer as example
+
+    config = layer_config(**change)
+    layer, cache = example.Layer.synthetic(config, 7), example.Cache(config, 40, 1, 300)
+    inv_freq, _ = example.attention.rope_frequencies(config.head_dim)
+    x = torch.randn(n, config.d_model, generator=torch.Generator("cuda").manual_seed(9), device="cuda").to(BF16)
+    got, took = example.decoder_layer(layer, cache, x, cache.extend([n]), inv_freq)
+    assert cuda.device_status() == 0
+
+    def off(**swap):
+        want, ids = plain_layer(layer, x, inv_freq, swap)
+        same = (took == ids).all(1)
+        return float((got.double() - want)[same].norm() / want[same].norm()), float(same.float().mean())
+
+    distance, same = off()
+    assert distance < 4 * 2.0 ** -8 and same >= 0.95
+    names = ["norm_attention", "norm_experts"]
+    if config.block_norms:
+        names += ["behind_attention", "behind_experts", "gate_attention", "gate_experts"]
+    for name in names:  # another one in its place is seen
+        assert off(**{name: "norm_head"})[0] > 2 * distance, name
