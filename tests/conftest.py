@@ -17,6 +17,12 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100a) GPU")
 
 
+def pytest_collection_modifyitems(items):
+    """What runs the reference's engine comes last: where that is not built (its sources are not there)
+    a session that stops at the first failure has run all else."""
+    items.sort(key=lambda item: hasattr(getattr(item, "module", None), "ENGINE"))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.oracle import Oracle
