@@ -149,7 +149,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
 
     ``positions`` int32 [tokens]; ``inv_freq`` f32, one per rotated pair.  With ``axes``
     (:func:`rope_axes`: uint8, the axis of each pair) positions are int32 [axes, tokens],
-    time, height and width say (``fmcuda_rope_append_axes``)."""
+    time, height and width say, a row of its own for each (not expanded over the axes)
+    (``fmcuda_rope_append_axes``)."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return _calls.rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, interleaved,

@@ -41,8 +41,9 @@
 // SINKS: the first p.sinks keys stay visible behind the window.  A pair's blocks are then
 // counted without the gap between those of the first keys and those of its windows (`skip`
 // blocks from block `first` on), and a tile takes the ones before fe and those of [tb, te).
-// A prompt of 8192, 32/8 heads of 128, window 2048, 16 first keys: 250 to 285 us by heat (0.85 to 0.97
-// PFLOP/s of the products that the mask leaves).
+// A prompt of 8192, 32/8 heads of 128, window 2048, 16 first keys: 250 to 294 us by machine and heat (0.82
+// to 0.97 PFLOP/s of the products that the mask leaves); heads of 64 213 to 232 (0.52 to 0.57; their
+// exponentials alone are 102 us).
 //
 // A persistent CTA an SM.  Where there are many (pair of tiles, key head) items,
 // they go to the CTAs whole, the longest first, in rounds that run there and

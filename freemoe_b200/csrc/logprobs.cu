@@ -27,10 +27,11 @@
 // A CTA takes a row; where rows are few a cluster does, whose CTAs send their sums and first
 // values to one of them.
 //
-// Measured: 4096 rows of 128256, bf16, 5 alternatives (1.05 GB) 193 to 207 us by machine and
-// heat, 77 to 83% of the rate of a copy (exponentials 60% busy, issue slots 65%); without
-// alternatives 180; 2048 rows in f32 171 to 180.  333 rows of 32003, f16, 32 alternatives 15 us,
-// of which the selection is 4; one row of 151936 in f32, 20 alternatives, 8.2 us, latency.
+// Measured: 4096 rows of 128256, bf16, 5 alternatives (1.05 GB) 193 to 240 us by machine and
+// heat, 67 to 83% of the rate of a copy (exponentials 60% busy, issue slots 65%); without
+// alternatives 180 to 205; 2048 rows in f32 171 to 184.  333 rows of 32003, f16, 32 alternatives,
+// half of them ruled out 15 us, of which the selection is 4, and 18 with none ruled out; one row of
+// 151936 in f32, 20 alternatives, 8.4 us, latency.
 #include <cfloat>
 #include <cmath>
 #include <string>
@@ -455,8 +456,8 @@ __device__ __forceinline__ void select_top(const Row<T> &row, const Stream<T> &s
     __syncthreads();
 }
 
-// The logarithm of a sum, as that of its exponent and of a value near 1: f32 for the latter
-// is exact to 2^-26.
+// The logarithm of a sum, as that of its exponent and of a value in [3/4, 3/2): f32 for the latter,
+// which stays below 0.41, is off by at most 2^-25 (one unit of logf).
 __device__ __forceinline__ double log_of(float sum) {
     const int k = static_cast<int>(__float_as_uint(sum) - 0x3F400000u) >> 23; // sum / 2^k in [3/4, 3/2)
     const float near = __uint_as_float(__float_as_uint(sum) - (static_cast<uint32_t>(k) << 23));

@@ -9,8 +9,9 @@
 // digits.
 //
 // Measured, 8192 rows of 4096: bf16 46 us (268 MB, 5.8 TB/s, 89% of the rate of a copy), to
-// e4m3 46, x and y in f32 57, a gate of x's shape 54; rows of 8192 89; rows of 4095 82 (accesses
-// of two bytes).  A row alone 3.1 us: a launch, the loads and two sums, one after the other.
+// e4m3 46, x in f32 58 (336 MB), x and y in f32 77 (403 MB), a gate of x's shape 54; rows of 8192
+// 88; rows of 4095 82 (accesses of two bytes).  A row alone 3.1 us: a launch, the loads and two
+// sums, one after the other.
 #include <cmath>
 #include <string>
 
@@ -56,7 +57,9 @@ __device__ __forceinline__ void pair_h(const PairParams &p, uint64_t row, uint32
     for (int j = 0; j < 8; ++j) h[j] = fmaf(v[j], p.res_scale, h[j]);
 }
 
-// Rows longer than the registers of a CTA hold: read three times, the second and third from L2.
+// Rows longer than the registers of a CTA hold (16384 values): read three times, the second and third
+// from L2.  1024 rows of 32768 in bf16 101 us (134 MB; 2048 rows of 16384, in registers, 54); one of
+// 131072 44.
 template <int VEC> __global__ void __launch_bounds__(1024) norm_pair_long_kernel(const PairParams p) {
     __shared__ float s_part[2][32];
     const uint32_t chunks = ((p.d + 127) / 128) * 16, n = blockDim.x;
@@ -390,7 +393,8 @@ template <int VEC, int XT, int RT, bool FULL = false> int dispatch_width(const P
     if (few && one <= 1024) {
         if constexpr (VEC != 8) {
             // code that runs once comes from memory: that of one pair of types is shorter (a row of 4095
-            // in bf16 3.4 us, 5.1 with types at run time; with many rows they take the same time)
+            // in bf16 3.0 us; with many rows they take the same time).  The pairs here are a stream and its
+            // block in one type, and a block in f32; the other four have types at run time, 4.4 to 4.9 us.
             auto typed = [&](int32_t xt, int32_t rt) { return p.xt == xt && p.rt == rt; };
             if (typed(FM_X_BF16, FM_X_BF16))
                 return launch_pair<VEC, FM_X_BF16, FM_X_BF16, FULL, true, true, 1, 1024>(p, one, s);

@@ -120,7 +120,8 @@ __device__ __forceinline__ uint4 rope_shuffle(uint4 v, uint32_t lane) {
 // divisions, 44 (issue slots 65% busy); the cosines worked out by every thread for
 // itself, 64.  Bound by the loads under way: registers against warps (the next token's loads
 // beside this one's, with 64 or 85 registers: 39 to 43).  HALVES: 37 us too, from f32 to bf16
-// (302 MB) 51, heads of 64 25 (101 MB; a third of the places for heads is empty).  Before the
+// (302 MB) 51, heads of 64 25 (101 MB; 48 heads have half of the 96 places).  PAIRED: heads of 80 35
+// (126 MB), from f32 57 (189 MB).  Before the
 // cosines lay side by side (rope_place) and before batches left no part of a round idle, both
 // were 42 and 62, with L1 and shared memory 69% busy.
 enum { ROPE_INTER, ROPE_HALVES, ROPE_PAIRED };
@@ -454,7 +455,8 @@ int rope_append(const fmcuda_rope_append_args *a, const uint8_t *axis, uint32_t 
     parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
     if (vec && a->tokens > sms * 4) {
         // more than the GPU holds at once: several to a CTA, as many as their cosines have room for and as
-        // leave the least of the last round idle (four CTAs an SM hold 592 times the batch)
+        // leave the least of the last round idle (four CTAs an SM hold 592 times the batch; PAIRED from f32
+        // has two, and another batch there has not been measured)
         const uint32_t span = half ? rope_span(half, a->interleaved ? 4 : 8) : 1, room = ROPE_TURNS / span;
         uint64_t least = ~0ull;
         for (uint32_t n = 1; n <= ROPE_BATCH && n <= room; ++n) {
