@@ -1,8 +1,8 @@
 """Norms of as many rows as a call can have: 2^32 - 1, in teams of four a CTA.
 
-Tolerance: rows of one value x = 0.5, w = 1.5, epsilon 0 in f32 and r = 0.25 in bf16 arithmetic that
-is exact but for the root: y = sign(x) w is rounded from a product within 4 * 2^-24 of it, to bf16
-exactly 1.5.
+Rows of one value, without epsilon: y = sign(x) w, here +-1.5, and h = r + y.  The root is within 2
+units of f32 and the two products within half a unit each, so that y is within 2^-21 of +-1.5 and h of
+1.75 and -1, which round to just these in bf16: equal, no tolerance.
 """
 from __future__ import annotations
 

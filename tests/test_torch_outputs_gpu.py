@@ -110,3 +110,16 @@ def test_deterministic_algorithms_fill_fresh_memory(cuda):
             assert torch.equal(out[:5], want[0][:5]) and torch.equal(lse[:5], want[1][:5])
     finally:
         torch.use_deterministic_algorithms(False)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_calls_with_deterministic_algorithms(cuda, name):
+    call, _ = calls()[name]
+    want = tensors(call())
+    torch.use_deterministic_algorithms(True)
+    try:
+        got = tensors(call())
+    finally:
+        torch.use_deterministic_algorithms(False)
+    for a, b in zip(want, got):
+        assert a.stride() == b.stride() and torch.equal(a.float(), b.float())
